@@ -42,6 +42,12 @@ typedef enum {
   TPP_ACT_RELU = 3       /* csrc/activation/activation.cuh:59-67 (ReluHalf)  */
 } tpp_act;
 
+/* Element codes of an 8-bit KV cache (0 where a cache holds 16-bit values) */
+typedef enum {
+  TPP_CODE_E4M3 = 1, /* OCP float8 e4m3fn */
+  TPP_CODE_INT8 = 2
+} tpp_code;
+
 #define TPP_OK 0
 #define TPP_E_INVALID (-1)     /* bad pointer / shape / stride argument     */
 #define TPP_E_UNSUPPORTED (-2) /* dtype or shape the kernels do not handle  */
@@ -160,6 +166,54 @@ int tpp_qk_norm_rope(void *q, int64_t q_stride, void *k, int64_t k_stride,
                      const void *q_norm_w, const void *k_norm_w, const void *cos,
                      const void *sin, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D,
                      float eps_q, float eps_k, int dtype, int cs_dtype, void *stream);
+
+/* RoPE at given positions: q [B, S, Hq, D] and k [B, S, Hk, D] (Hk = 0: none)
+ * through {batch, token, head} strides, last dim contiguous, in one launch; the
+ * outputs may be the inputs (same pointers and strides: in place). Token (b, s)
+ * is rotated at positions[b * pos_stride + s] (int32, or int64 with pos_is_64):
+ * pair j by the angle position * inv_freq[j] (fp64 [R / 2], radians a
+ * position), cos and sin times `factor`. The first R elements of a head are
+ * paired (2j, 2j + 1) if `interleaved`, else (j, j + R / 2); the others, and
+ * every token at a negative position, are copied. D and R even, R <= D. fp32
+ * math on fp64-reduced angles, one rounding. Next to rope_apply_half2_dual
+ * (csrc/dlops/qkrope/qkrope.cuh:69-93), which knows rows 0 .. S - 1 of a table
+ * only. */
+int tpp_rope_at(const void *q, const void *k, void *q_out, void *k_out,
+                const int64_t *q_strides, const int64_t *k_strides,
+                const int64_t *qo_strides, const int64_t *ko_strides,
+                const void *positions, int64_t pos_stride, int pos_is_64,
+                const double *inv_freq, float factor, int64_t B, int64_t S,
+                int64_t Hq, int64_t Hk, int64_t D, int64_t R, int interleaved,
+                int dtype, void *stream);
+
+/* ---- 8-bit KV cache -------------------------------------------------------- */
+
+/* Writes k and v [B, S, H, D] ({batch, token, head} strides, last dim
+ * contiguous, rows 16-byte aligned) into a cache of codes [B, H, Lmax, D]
+ * ({batch, head} strides, rows contiguous) and exponent bytes [B, H, Lmax]
+ * ({batch, head} strides): a row is its codes times 2^(byte - 127), the least
+ * power of two that holds it, each code the nearest (ties to even). Token s of
+ * sequence b goes to positions[b] + s (positions NULL: start + s) where that is
+ * in [0, Lmax) and s < counts[b] (counts NULL: all); other rows keep what they
+ * hold. A row with an infinity or NaN is stored as NaN (byte 255). code a
+ * tpp_code, D in {64, 128, 256}. Next to KVCache.update
+ * (torchpp/llmops/kvcache.py:50-108), which keeps 16-bit values. */
+int tpp_kv_quant_append(const void *k, const void *v, const int64_t *k_strides,
+                        const int64_t *v_strides, void *k_codes, void *v_codes,
+                        void *k_exps, void *v_exps, const int64_t *code_strides,
+                        const int64_t *exp_strides, const int32_t *positions,
+                        int64_t start, const int32_t *counts, int64_t B, int64_t S,
+                        int64_t H, int64_t D, int64_t Lmax, int code, int dtype,
+                        void *stream);
+
+/* The first `len` rows of every head of such a cache as values of `dtype`:
+ * k_out, v_out [B, H, len, D] contiguous. One rounding (none in bfloat16);
+ * float16 is limited to +-65504. */
+int tpp_kv_quant_read(const void *k_codes, const void *v_codes, const void *k_exps,
+                      const void *v_exps, const int64_t *code_strides,
+                      const int64_t *exp_strides, void *k_out, void *v_out,
+                      int64_t B, int64_t H, int64_t len, int64_t D, int64_t Lmax,
+                      int code, int dtype, void *stream);
 
 /* ---- linear layers ------------------------------------------------------- */
 
@@ -457,6 +511,34 @@ int tpp_attn_decode_oproj_sync_errors(void *workspace, int *out, void *stream);
  * counterpart in the reference. */
 int tpp_decode_force_sync_error(void *workspace, int kernel, void *stream);
 
+/* Attention of T drafted tokens per sequence (1 to 64) over a KV cache that
+ * holds their keys and values behind the context's: q, o [B, T, Hq, D]
+ * ({batch, token, head} strides), caches [B, Hkv, Lmax, D] ({batch, head,
+ * position} strides), all with a contiguous last dim. Token t sees the keys
+ * below seqlens[b] (the context, without the drafted tokens) and key seqlens[b]
+ * + i for each i that is t or an ancestor of t by `parents` [B, T] (int32; an
+ * earlier token, or -1: the context; any other value is padding and sees
+ * nothing, nor do its children; NULL: a chain). Lengths are limited to [0,
+ * Lmax]; a token whose own key would lie past Lmax sees nothing. Rows that see
+ * nothing are 0. code 0:
+ * caches of `dtype`; a tpp_code: 8-bit codes with k_exps / v_exps [B, Hkv, Lmax]
+ * as written by tpp_kv_quant_append. softmax_scale <= 0 means 1/sqrt(D). D <=
+ * 256. Next to flash_attn_func with Sq = 1 over the cache prefix
+ * (torchpp/attention/gqa.py:117-128). */
+int tpp_tree_attn(const void *q, const void *k, const void *v, void *o,
+                  const void *k_exps, const void *v_exps, const int64_t *q_strides,
+                  const int64_t *k_strides, const int64_t *v_strides,
+                  const int64_t *exp_strides, const int64_t *o_strides,
+                  const int32_t *seqlens, const int32_t *parents, int64_t B,
+                  int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t Lmax,
+                  float softmax_scale, int code, int dtype, void *workspace,
+                  size_t ws_bytes, void *stream);
+
+/* Workspace bytes of tpp_tree_attn (16-byte aligned, no initialisation; 0:
+ * none). */
+size_t tpp_tree_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                    int64_t D, int64_t Lmax, int code);
+
 /* ---- sampling ------------------------------------------------------------ */
 
 /* Greedy sampling: out[b] = argmax_n x[b, n] for x [B, ldx] (first index of
@@ -464,6 +546,37 @@ int tpp_decode_force_sync_error(void *workspace, int kernel, void *stream);
  * LLMInference.sample_greedy (torchpp/llmops/llm.py:181-186). */
 int tpp_argmax_rows(const void *x, int64_t *out, int64_t B, int64_t N,
                     int64_t ldx, int dtype, void *stream);
+
+/* Workspace bytes of tpp_verify_draft (8-byte aligned, no initialisation). */
+size_t tpp_verify_draft_workspace_size(int64_t B, int64_t V);
+
+/* Verification of T drafted tokens (1 to 64) per sequence against the target's
+ * probabilities. target_probs [B, T + 1, V] and draft_probs [B, T, V] of
+ * `dtype` (fp32, fp16 or bf16) through {batch, row} strides, last dim
+ * contiguous; row 0 of target_probs follows the context, row t + 1 drafted
+ * token t. A mass that is not finite or not above 0 counts as 0. uniforms
+ * [B, T + 1] fp32 in [0, 1). draft_tokens [B, T]; a token outside [0, V) is
+ * padding and never accepted.
+ *  - draft_probs given (a chain, parents NULL): token i stays while u_i q_i <
+ *    p_i; the next token is drawn from max(p - q, 0) at the first that does
+ *    not, from p behind the last or at padding.
+ *  - no draft_probs (tokens chosen without a draw), parents [B, T] as in
+ *    tpp_tree_attn or NULL for a chain: at each node, from the context down,
+ *    the child c with below(c) <= u_depth < below(c) + p(c) stays, below(c)
+ *    the mass of its earlier siblings (a token that an earlier sibling has
+ *    counts as none); the next token is drawn from p without the children of
+ *    the node where none stays.
+ * The next token is the first index at which the running sum of those weights
+ * passes u_T times their sum, from the whole row if they have no mass, -1 if
+ * that has none; sums are fp64. accepted [B]: how many tokens stay; path [B, T]:
+ * their indices in order, then -1; next_token [B]. Next to the samplers of
+ * torchpp/llmops/llm.py:114-186. */
+int tpp_verify_draft(const int64_t *draft_tokens, const int32_t *parents,
+                     const void *target_probs, const int64_t *target_strides,
+                     const void *draft_probs, const int64_t *draft_strides,
+                     const float *uniforms, int32_t *accepted, int32_t *path,
+                     int64_t *next_token, int64_t B, int64_t T, int64_t V,
+                     int dtype, void *workspace, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -987,9 +987,260 @@ int64_t attn_decode_sync_errors(at::Tensor like) {
   return any;
 }
 
+// ---- rotary embedding at positions, 8-bit cache, tree attention, verification
+void check_same_device(const at::Tensor &like, std::initializer_list<const at::Tensor *> ts) {
+  for (const at::Tensor *t : ts)
+    if (t->defined())
+      TORCH_CHECK(t->device() == like.device(), "all tensors must be on one device (", like.device(),
+                  " and ", t->device(), ")");
+}
+at::Tensor or_none(const c10::optional<at::Tensor> &t) {
+  return t.has_value() && t->defined() ? *t : at::Tensor();
+}
+
+std::vector<at::Tensor> rope_at(at::Tensor q, c10::optional<at::Tensor> k_opt, at::Tensor positions,
+                                at::Tensor inv_freq, bool interleaved, double attention_factor,
+                                bool inplace) {
+  const at::Tensor k = or_none(k_opt);
+  TORCH_CHECK(q.is_cuda(), "q must be on CUDA");
+  check_same_device(q, {&k, &positions, &inv_freq});
+  TORCH_CHECK(q.dim() == 4, "q must be 4D [batch, seq_len, heads, head_dim]");
+  const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
+  for (const at::Tensor *t : std::initializer_list<const at::Tensor *>{&q, &k}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(is_half_or_bf16(*t) && t->scalar_type() == q.scalar_type(),
+                "q and k must be float16 or bfloat16, of one dtype");
+    TORCH_CHECK(t->dim() == 4 && t->size(0) == B && t->size(1) == S && t->size(3) == D,
+                "q and k must be [B, S, H, D] with the same B, S and D");
+    TORCH_CHECK(t->numel() == 0 || t->stride(3) == 1, "q and k must have a contiguous last dimension");
+    TORCH_CHECK(t->size(2) > 0, "q and k must have at least one head");
+    if (inplace)
+      for (int i = 0; i < 3; ++i)
+        TORCH_CHECK(t->size(i) <= 1 || t->stride(i) >= D, "in place: rows of q or k overlap");
+  }
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+              "positions must be int32 or int64");
+  TORCH_CHECK((positions.dim() == 1 && positions.size(0) == S) ||
+                  (positions.dim() == 2 && positions.size(0) == B && positions.size(1) == S),
+              "positions must be [B, S] or [S]");
+  if (positions.numel() && positions.stride(-1) != 1) positions = positions.contiguous();
+  TORCH_CHECK(inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 && inv_freq.is_contiguous(),
+              "inv_freq must be a contiguous float64 vector of rotary_dim / 2 frequencies");
+  const int64_t R = 2 * inv_freq.size(0);
+  TORCH_CHECK(R >= 2 && R <= D && D % 2 == 0, "rotary_dim ", R, " does not fit head_dim ", D);
+  c10::DeviceGuard g(q.device());
+  at::Tensor qo = inplace ? q : torch::empty(q.sizes(), q.options()), ko;
+  if (k.defined()) ko = inplace ? k : torch::empty(k.sizes(), k.options());
+  if (q.numel() == 0) return {qo, ko};
+  auto str = [](const at::Tensor &t) { return std::vector<int64_t>{t.stride(0), t.stride(1), t.stride(2)}; };
+  const auto qs = str(q), qos = str(qo);
+  std::vector<int64_t> ks, kos;
+  if (k.defined()) ks = str(k), kos = str(ko);
+  check_rc(tpp_rope_at(q.data_ptr(), k.defined() ? k.data_ptr() : nullptr, qo.data_ptr(),
+                       k.defined() ? ko.data_ptr() : nullptr, qs.data(), ks.data(), qos.data(),
+                       kos.data(), positions.data_ptr(), positions.dim() == 2 ? positions.stride(0) : 0,
+                       positions.scalar_type() == at::kLong, inv_freq.data_ptr<double>(),
+                       (float)attention_factor, B, S, q.size(2), k.defined() ? k.size(2) : 0, D, R,
+                       interleaved, dtype_code(q), cur_stream(q)),
+           "rope_at");
+  return {qo, ko};
+}
+
+int code_of(const at::Tensor &codes) {
+  if (codes.scalar_type() == at::kFloat8_e4m3fn) return TPP_CODE_E4M3;
+  if (codes.scalar_type() == at::kChar) return TPP_CODE_INT8;
+  return -1;
+}
+
+// codes [B, H, L, D] and exponents [B, H, L] of K and V, of one layout
+int check_codes(const at::Tensor &kc, const at::Tensor &vc, const at::Tensor &ke, const at::Tensor &ve,
+                int64_t B) {
+  TORCH_CHECK(kc.is_cuda(), "cache codes must be on CUDA");
+  check_same_device(kc, {&vc, &ke, &ve});
+  const int code = code_of(kc);
+  TORCH_CHECK(code > 0 && vc.scalar_type() == kc.scalar_type(),
+              "cache codes must be float8_e4m3fn or int8, of one dtype");
+  TORCH_CHECK(ke.scalar_type() == at::kByte && ve.scalar_type() == at::kByte, "cache exponents must be uint8");
+  TORCH_CHECK(kc.dim() == 4 && vc.sizes() == kc.sizes() && vc.strides() == kc.strides(),
+              "cache codes must be [B, Hkv, L, D], K and V of one layout");
+  TORCH_CHECK(ke.dim() == 3 && ve.sizes() == ke.sizes() && ve.strides() == ke.strides() &&
+                  ke.size(0) == kc.size(0) && ke.size(1) == kc.size(1) && ke.size(2) == kc.size(2),
+              "cache exponents must be [B, Hkv, L], K and V of one layout");
+  TORCH_CHECK(kc.size(0) == B, "batch size mismatch");
+  TORCH_CHECK(kc.numel() == 0 || (kc.stride(3) == 1 && kc.stride(2) == kc.size(3) && ke.stride(2) == 1),
+              "cache rows must be contiguous along positions");
+  return code;
+}
+
+const int32_t *int32_b(const at::Tensor &t, int64_t B, const char *what) {
+  if (!t.defined()) return nullptr;
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.numel() == B && t.is_contiguous(), what,
+              " must be a contiguous CUDA int32 tensor [B]");
+  return t.data_ptr<int32_t>();
+}
+
+void kv_quant_append(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor vc, at::Tensor ke,
+                     at::Tensor ve, c10::optional<at::Tensor> positions, int64_t start,
+                     c10::optional<at::Tensor> counts) {
+  check_bshd(k, "k");
+  check_bshd(v, "v");
+  TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "k and v differ");
+  const int64_t B = k.size(0), S = k.size(1), H = k.size(2), D = k.size(3);
+  const int code = check_codes(kc, vc, ke, ve, B);
+  TORCH_CHECK(kc.size(1) == H && kc.size(3) == D, "cache shape mismatch");
+  const at::Tensor pos = or_none(positions), cnt = or_none(counts);
+  check_same_device(k, {&v, &kc, &pos, &cnt});
+  c10::DeviceGuard g(k.device());
+  const int64_t ks[3] = {k.stride(0), k.stride(1), k.stride(2)}, vs[3] = {v.stride(0), v.stride(1), v.stride(2)};
+  const int64_t cs[2] = {kc.stride(0), kc.stride(1)}, es[2] = {ke.stride(0), ke.stride(1)};
+  const int32_t *pp = int32_b(pos, B, "positions"), *cp = int32_b(cnt, B, "counts");
+  if (k.numel() == 0) return;
+  check_rc(tpp_kv_quant_append(k.data_ptr(), v.data_ptr(), ks, vs, kc.data_ptr(), vc.data_ptr(),
+                               ke.data_ptr(), ve.data_ptr(), cs, es, pp, start, cp, B, S, H, D,
+                               kc.size(2), code, dtype_code(k), cur_stream(k)),
+           "kv_quant_append");
+}
+
+std::vector<at::Tensor> kv_quant_read(at::Tensor kc, at::Tensor vc, at::Tensor ke, at::Tensor ve,
+                                      int64_t length, bool bf16) {
+  TORCH_CHECK(kc.dim() == 4, "cache codes must be [B, Hkv, L, D]");
+  const int64_t B = kc.size(0), H = kc.size(1), D = kc.size(3);
+  const int code = check_codes(kc, vc, ke, ve, B);
+  TORCH_CHECK(length >= 0 && length <= kc.size(2), "length ", length, " of a cache of ", kc.size(2));
+  c10::DeviceGuard g(kc.device());
+  const auto opt = kc.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+  auto k = torch::empty({B, H, length, D}, opt), v = torch::empty({B, H, length, D}, opt);
+  if (k.numel() == 0) return {k, v};
+  const int64_t cs[2] = {kc.stride(0), kc.stride(1)}, es[2] = {ke.stride(0), ke.stride(1)};
+  check_rc(tpp_kv_quant_read(kc.data_ptr(), vc.data_ptr(), ke.data_ptr(), ve.data_ptr(), cs, es,
+                             k.data_ptr(), v.data_ptr(), B, H, length, D, kc.size(2), code,
+                             bf16 ? TPP_BF16 : TPP_F16, cur_stream(kc)),
+           "kv_quant_read");
+  return {k, v};
+}
+
+at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor seqlens,
+                          c10::optional<at::Tensor> parents_opt, c10::optional<at::Tensor> k_exps,
+                          c10::optional<at::Tensor> v_exps, double softmax_scale,
+                          c10::optional<at::Tensor> out) {
+  check_bshd(q, "q");
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3);
+  const at::Tensor parents = or_none(parents_opt), ke = or_none(k_exps), ve = or_none(v_exps);
+  check_same_device(q, {&kc, &vc, &seqlens, &parents, &ke, &ve});
+  TORCH_CHECK(kc.dim() == 4 && vc.sizes() == kc.sizes(), "caches must be [B, Hkv, L, D]");
+  TORCH_CHECK(kc.size(0) == B && kc.size(3) == D, "cache shape mismatch");
+  const int64_t Hkv = kc.size(1), Lmax = kc.size(2);
+  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0, "number of query heads must be divisible by KV heads");
+  int code = 0;
+  int64_t es[2] = {0, 0};
+  if (kc.scalar_type() == q.scalar_type()) {
+    TORCH_CHECK(vc.scalar_type() == q.scalar_type(), "cache dtype must match q");
+    TORCH_CHECK(!ke.defined() && !ve.defined(), "a cache of values has no exponents");
+    TORCH_CHECK(kc.stride(3) == 1 && vc.stride(3) == 1, "caches must have a contiguous last dim");
+  } else {
+    TORCH_CHECK(code_of(kc) > 0, "caches must have q's dtype, or hold float8_e4m3fn or int8 codes");
+    TORCH_CHECK(ke.defined() && ve.defined(), "a cache of codes needs k_exps and v_exps");
+    code = check_codes(kc, vc, ke, ve, B);
+    es[0] = ke.stride(0), es[1] = ke.stride(1);
+  }
+  const int32_t *sl = int32_b(seqlens, B, "seqlens");
+  const int32_t *par = nullptr;
+  if (parents.defined()) {
+    TORCH_CHECK(parents.scalar_type() == at::kInt && parents.dim() == 2 && parents.size(0) == B &&
+                    parents.size(1) == T && parents.is_contiguous(),
+                "parents must be a contiguous int32 tensor [B, T]");
+    par = parents.data_ptr<int32_t>();
+  }
+  c10::DeviceGuard g(q.device());
+  at::Tensor o;
+  if (out.has_value() && out->defined()) {
+    o = *out;
+    TORCH_CHECK(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device() &&
+                    (o.numel() == 0 || o.stride(3) == 1),
+                "out must match q");
+  } else {
+    o = torch::empty(q.sizes(), q.options());
+  }
+  if (q.numel() == 0) return o;
+  const size_t wsb = tpp_tree_attn_workspace_size(B, T, Hq, Hkv, D, Lmax, code);
+  at::Tensor ws; // this call's own, from the caching allocator
+  if (wsb) ws = torch::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+  const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)}, os[3] = {o.stride(0), o.stride(1), o.stride(2)};
+  const int64_t ks[3] = {kc.stride(0), kc.stride(1), kc.stride(2)}, vs[3] = {vc.stride(0), vc.stride(1), vc.stride(2)};
+  check_rc(tpp_tree_attn(q.data_ptr(), kc.data_ptr(), vc.data_ptr(), o.data_ptr(),
+                         code ? ke.data_ptr() : nullptr, code ? ve.data_ptr() : nullptr, qs, ks, vs, es, os,
+                         sl, par, B, T, Hq, Hkv, D, Lmax, (float)softmax_scale, code, dtype_code(q),
+                         wsb ? ws.data_ptr() : nullptr, wsb, cur_stream(q)),
+           "tree_attention");
+  return o;
+}
+
+std::vector<at::Tensor> verify_draft(at::Tensor tokens, at::Tensor target, at::Tensor uniforms,
+                                     c10::optional<at::Tensor> draft_opt,
+                                     c10::optional<at::Tensor> parents_opt) {
+  TORCH_CHECK(target.is_cuda() && target.dim() == 3, "target_probs must be a CUDA tensor [B, T + 1, V]");
+  const at::Tensor draft = or_none(draft_opt), parents = or_none(parents_opt);
+  check_same_device(target, {&tokens, &uniforms, &draft, &parents});
+  TORCH_CHECK(tokens.dim() == 2 && tokens.scalar_type() == at::kLong, "draft_tokens must be int64 [B, T]");
+  const int64_t B = tokens.size(0), T = tokens.size(1), V = target.size(2);
+  TORCH_CHECK(dtype_code(target) >= 0, "target_probs must be float32, float16 or bfloat16");
+  TORCH_CHECK(target.size(0) == B && target.size(1) == T + 1, "target_probs must be [B, T + 1, V]");
+  TORCH_CHECK(V > 0 && T > 0, "invalid shapes");
+  TORCH_CHECK(target.numel() == 0 || target.stride(2) == 1, "target_probs must have a contiguous last dim");
+  if (draft.defined()) {
+    TORCH_CHECK(!parents.defined(), "draft_probs go with a chain, not with a tree (parents)");
+    TORCH_CHECK(draft.scalar_type() == target.scalar_type() && draft.dim() == 3 && draft.size(0) == B &&
+                    draft.size(1) == T && draft.size(2) == V && (draft.numel() == 0 || draft.stride(2) == 1),
+                "draft_probs must be [B, T, V] of target_probs' dtype with a contiguous last dim");
+  }
+  TORCH_CHECK(uniforms.scalar_type() == at::kFloat && uniforms.dim() == 2 && uniforms.size(0) == B &&
+                  uniforms.size(1) == T + 1,
+              "uniforms must be float32 [B, T + 1]");
+  if (parents.defined())
+    TORCH_CHECK(parents.scalar_type() == at::kInt && parents.dim() == 2 && parents.size(0) == B &&
+                    parents.size(1) == T,
+                "parents must be int32 [B, T]");
+  c10::DeviceGuard g(target.device());
+  tokens = tokens.contiguous();
+  uniforms = uniforms.contiguous();
+  const at::Tensor par = parents.defined() ? parents.contiguous() : parents;
+  const auto i32 = target.options().dtype(at::kInt);
+  auto accepted = torch::empty({B}, i32), path = torch::empty({B, T}, i32),
+       next = torch::empty({B}, target.options().dtype(at::kLong));
+  if (B == 0) return {accepted, path, next};
+  const size_t wsb = tpp_verify_draft_workspace_size(B, V);
+  auto ws = torch::empty({(int64_t)wsb}, target.options().dtype(at::kByte));
+  const int64_t ps[2] = {target.stride(0), target.stride(1)};
+  int64_t qs[2] = {0, 0};
+  if (draft.defined()) qs[0] = draft.stride(0), qs[1] = draft.stride(1);
+  check_rc(tpp_verify_draft(tokens.data_ptr<int64_t>(), par.defined() ? par.data_ptr<int32_t>() : nullptr,
+                            target.data_ptr(), ps, draft.defined() ? draft.data_ptr() : nullptr, qs,
+                            uniforms.data_ptr<float>(), accepted.data_ptr<int32_t>(),
+                            path.data_ptr<int32_t>(), next.data_ptr<int64_t>(), B, T, V,
+                            dtype_code(target), ws.data_ptr(), wsb, cur_stream(target)),
+           "verify_draft");
+  return {accepted, path, next};
+}
+
 } // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("rope_at", &rope_at, "RoPE of q and k [B, S, H, D] at given positions", py::arg("q"), py::arg("k"),
+        py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false,
+        py::arg("attention_factor") = 1.0, py::arg("inplace") = false);
+  m.def("kv_quant_append", &kv_quant_append, "write k and v into a cache of 8-bit codes", py::arg("k"),
+        py::arg("v"), py::arg("k_codes"), py::arg("v_codes"), py::arg("k_exps"), py::arg("v_exps"),
+        py::arg("positions"), py::arg("start") = 0, py::arg("counts") = py::none());
+  m.def("kv_quant_read", &kv_quant_read, "decode the first rows of a cache of 8-bit codes",
+        py::arg("k_codes"), py::arg("v_codes"), py::arg("k_exps"), py::arg("v_exps"), py::arg("length"),
+        py::arg("bf16"));
+  m.def("tree_attention", &tree_attention, "attention of drafted tokens over a KV cache", py::arg("q"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("seqlens"), py::arg("parents") = py::none(),
+        py::arg("k_exps") = py::none(), py::arg("v_exps") = py::none(), py::arg("softmax_scale") = 0.0,
+        py::arg("out") = py::none());
+  m.def("verify_draft", &verify_draft, "which drafted tokens stay, and the next token",
+        py::arg("draft_tokens"), py::arg("target_probs"), py::arg("uniforms"),
+        py::arg("draft_probs") = py::none(), py::arg("parents") = py::none());
   m.def("attn_decode_oproj", &attn_decode_oproj,
         "decode attention (fused QK-norm + RoPE + KV append) then the output projection and the "
         "residual add, in place on residual; returns the attention output",

@@ -3,9 +3,14 @@
 rope_apply / qkrope_apply keep the reference signatures and return new
 tensors; `rope_apply_` is the in-place variant. The kernels accept fp16 and
 bf16 inputs with fp16, bf16 or fp32 cos/sin tables, and qkrope_apply allows
-fewer K heads than Q heads (GQA).
+fewer K heads than Q heads (GQA). rope_apply_at rotates every token at a
+position of its own (drafted trees, far contexts) from frequencies that
+rope_frequencies makes, in either pair layout and over part of a head.
 """
 from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
 
 import torch
 
@@ -41,3 +46,67 @@ def compute_rope_params(head_dim, theta_base, context_length, device="cuda",
     ang = torch.outer(pos, inv_freq)
     ang = torch.cat([ang, ang], dim=1)
     return ang.cos().to(out_dtype).contiguous(), ang.sin().to(out_dtype).contiguous()
+
+
+def rope_frequencies(rotary_dim: int, theta_base: float = 10000.0, scaling: Optional[str] = None,
+                     factor: float = 1.0, original_context: int = 0, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0, device="cuda") -> Tuple[torch.Tensor, float]:
+    """(inv_freq fp64 [rotary_dim / 2] in radians a position, attention factor)
+    for rope_apply_at. Pair j turns by theta^(-2j / rotary_dim) a position;
+    `scaling` stretches that by `factor` for contexts longer than the trained:
+      "linear"  every frequency divided by factor (position interpolation)
+      "ntk"     theta * factor^(R / (R - 2)): the slowest pair is divided by
+                factor, the fastest kept
+      "yarn"    pairs that turn more than beta_fast times over original_context
+                kept, those that turn less than beta_slow times divided by
+                factor, a linear ramp over j between; attention factor
+                0.1 ln(factor) + 1
+    In fp64: an fp32 frequency is off by 0.06 rad at position 10^6."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling: {scaling}")
+    if factor < 1.0:
+        raise ValueError(f"factor must be at least 1, got {factor}")
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("ntk scaling needs a rotary_dim of 4 at least")
+        theta_base = theta_base * factor ** (rotary_dim / (rotary_dim - 2))
+    j = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    freq = float(theta_base) ** (-2.0 * j / rotary_dim)
+    attention_factor = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if original_context < 1:
+            raise ValueError("yarn scaling needs original_context, the trained context length")
+
+        def pair(turns):  # the pair that turns so often over the trained context
+            return (rotary_dim * math.log(original_context / (turns * 2 * math.pi))
+                    / (2 * math.log(theta_base)))
+
+        low = max(math.floor(pair(beta_fast)), 0)
+        high = min(math.ceil(pair(beta_slow)), rotary_dim - 1)
+        keep = 1.0 - ((j - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        freq = freq / factor * (1.0 - keep) + freq * keep
+        attention_factor = 0.1 * math.log(factor) + 1.0
+    return freq.to(device), attention_factor
+
+
+def rope_apply_at(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                  inv_freq: torch.Tensor, interleaved: bool = False,
+                  attention_factor: float = 1.0):
+    """Rotary embedding of q [B, S, Hq, D] and k [B, S, Hk, D] (or None) at
+    positions [B, S] or [S] (int32 or int64), in one launch; new contiguous
+    tensors. The first 2 * len(inv_freq) elements of a head turn, in pairs
+    (j, j + R/2) or, interleaved, (2j, 2j + 1); the rest, and tokens at negative
+    positions (padding), are copied. inv_freq as from rope_frequencies. q and k
+    may be views of a fused projection (any strides, contiguous last dim)."""
+    return tuple(_C.rope_at(q, k, positions, inv_freq, interleaved, attention_factor, False))
+
+
+def rope_apply_at_(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                   inv_freq: torch.Tensor, interleaved: bool = False,
+                   attention_factor: float = 1.0):
+    """rope_apply_at in place; returns (q, k)."""
+    return tuple(_C.rope_at(q, k, positions, inv_freq, interleaved, attention_factor, True))
