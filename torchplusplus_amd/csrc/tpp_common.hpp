@@ -273,6 +273,15 @@ template <int OFF, typename V> __device__ __forceinline__ V lds_read_b128(unsign
   asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(OFF));
   return r;
 }
+// Eight-bit form: within each 16 lanes, lane l gets the byte l % 8 of what lanes
+// l / 8, l / 8 + 2, .. l / 8 + 14 point at, i.e. pointing lane c + 2 r at V[k_r][d0
+// + 8 c] gives lane l the eight V[k_0 .. k_7][d0 + l].
+template <int OFF> __device__ __forceinline__ u32x2 lds_read_tr8(unsigned addr) {
+  static_assert(OFF >= 0 && OFF < 65536, "ds offset is 16 bits");
+  u32x2 r;
+  asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(OFF));
+  return r;
+}
 // s_waitcnt lgkmcnt(N) that also redefines the results in v, which are
 // complete once at most N LDS reads are outstanding: uses of v after it see
 // the loaded data (the tie keeps the compiler from copying a register the
@@ -309,6 +318,39 @@ __device__ __forceinline__ void static_for_impl(F &&f, std::integer_sequence<int
 }
 template <int N, typename F> __device__ __forceinline__ void static_for(F &&f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// ---- attention tiles and splits (attention.hip, tree_attention.hip) ----------
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32x32(typename VecT<T>::v8 a, typename VecT<T>::v8 b,
+                                            f32x16 c) {
+  if constexpr (__is_same(T, bf16))
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// V tiles are stored row-major like K ([key][16-byte unit]) and read as
+// MFMA operands with ds_read_b64_tr_b16, whose 16-lane groups return lane
+// 4a+b the b-th 16-bit element of the words lanes a, a+4, a+8, a+12 point at:
+// pointing lane a'+4c' at V[k0 + c'][d0 + 4a'] gives lane l of the group
+// V[k0 + 0..3][d0 + l]. Unit u of key row r is stored at u ^ vswz(r): the
+// 32 lanes one read cycle serves (4 keys x 32 columns) then hit distinct
+// banks (D = 128: 256-byte rows, XOR 4*(r%4); D = 64: 128-byte rows, two
+// per bank row, XOR 4*((r/2)%2)).
+template <int D> __device__ __forceinline__ int vswz(int r) {
+  if constexpr (D == 128) return 4 * (r & 3);
+  else return 4 * ((r >> 1) & 1);
+}
+
+// x / n as a multiply by inv = 2^32 / n rounded up (0 for n = 1), exact for
+// x * n < 2^32. A decode attention block's first loads wait for its split and sequence:
+// two integer divisions there (~60 dependent instructions) cost 0.2 us.
+__host__ __device__ inline unsigned inv_of(int n) {
+  return n > 1 ? (unsigned)((1ULL << 32) / (unsigned)n + 1) : 0u;
+}
+__host__ __device__ inline int div_inv(unsigned x, unsigned inv) {
+  return inv ? (int)(((uint64_t)x * inv) >> 32) : (int)x;
 }
 
 } // namespace tpp
