@@ -28,9 +28,12 @@ struct TreeArgs {
 
 // Bit i of the result: this lane's token (lane index < T) sees drafted token
 // i. Ancestors by doubling: after step s a lane holds those up to 2^s levels up.
-__device__ __forceinline__ unsigned long long tree_bits(const TreeArgs &p, int b, int L) {
+__device__ __forceinline__ int tree_parent(const TreeArgs &p, int b) {
   const int lane = lane_id();
-  int up = lane < p.T ? (p.parents ? p.parents[(int64_t)b * p.T + lane] : lane - 1) : -2;
+  return lane >= p.T ? -2 : p.parents ? p.parents[(int64_t)b * p.T + lane] : lane - 1;
+}
+__device__ __forceinline__ unsigned long long tree_bits(const TreeArgs &p, int up, int L) {
+  const int lane = lane_id();
   int none = up < -1 || up >= lane;
   if (none) up = -1;
   unsigned lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
@@ -67,7 +70,7 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
   const int lane = lane_id(), t = blockIdx.x % p.T, h = blockIdx.x / p.T, b = blockIdx.y;
   const int hk = h / p.G;
   const int L = min(max(p.seqlens[b], 0), p.Lmax);
-  const unsigned long long bits = tree_bits(p, b, L);
+  const unsigned long long bits = tree_bits(p, tree_parent(p, b), L);
   const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)bits, t);
   const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(bits >> 32), t);
   const unsigned long long see = ((unsigned long long)hi << 32) | lo;
@@ -108,46 +111,54 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
 // Head sizes 64 and 128, 16-byte rows: on the matrix cores.
 //
 // The T G query rows of a KV head (row = token * G + head of the group) are the
-// columns of S^T = K Q^T and of O^T = V^T P^T (32x32x16; a lane owns one query
-// row, so the softmax needs one exchange, with lane ^ 32). A block is 4 waves
-// over NQ tiles of 32 rows and one split of the sequence's keys; each wave
-// streams its own tiles of KT keys (8 KB of K) by LDS-DMA into a private slot:
-// no barrier in the loop, the next K tile is requested once this one's
-// fragments are in registers, the next V tile after this one's. Waves are
-// merged through LDS, splits by tree_merge_kernel (a second launch: the splits'
-// arrival counters would have to be shared by calls, which two replayed graphs
-// may not do).
+// columns of S^T = K Q^T and of O^T = V^T P^T (16x16x32), NC groups of 16 a
+// block; the four lanes with equal lane % 16 share a query row, so the softmax
+// needs two exchanges. A block is 4 waves over one split of the sequence's keys;
+// each wave streams its own tiles of KT keys (8 KB of K) by LDS-DMA into a
+// private slot: no barrier in the loop, the next K tile is requested once this
+// one's fragments are in registers, the next V tile after this one's. Waves are
+// merged through LDS, splits by tree_merge_kernel (a second launch: arrival
+// counters would have to be shared by calls, which two replayed graphs may not
+// do).
+//
+// Key order: S^T gives lane quarter u the keys 16 st + 4 u + i (i = 0 .. 3) of
+// tile st. The product with V takes them as its K index 8 u + j of step c: j < 4
+// from st = 2 c, the others from st = 2 c + 1, so P never leaves its registers,
+// and the transposing LDS reads of V fetch rows in that order.
 //
 // Codes stay codes up to the registers: a tile of codes has half the bytes and
 // twice the keys. K fragments become T (exact: e4m3 and int8 values fit both
 // types), V fragments bfloat16; the exponents are applied to the scores and to
-// the probabilities, 2 x 16 a lane and 32 keys, where scaling the operands would
-// take 4 D / 64 times as many. P of a coded cache is rounded to bfloat16 (its
-// range holds p 2^e, fp16's does not), else to T, in fp16 times 2^15 so that
-// weights down to 2^-39 of the largest are kept; each weight is off by 2^-9 (fp16:
-// 2^-12) at most, the sum of weights is kept in fp32 from the unrounded ones.
+// the probabilities. P is the sum of two values of V's type (16 bits of it in
+// bfloat16, 22 in fp16, there times 2^15 so that weights down to 2^-39 of the
+// largest count): one would be off by 2^-9, more than the output's rounding in
+// fp16. The sum of weights is kept in fp32.
 // ---------------------------------------------------------------------------
 template <int KIND, int D> struct TreeTile {
   static constexpr int ROWB = D * (KIND ? 1 : 2);  // bytes of a row
   static constexpr int KT = ROWB == 256 ? 32 : 64; // keys of a tile
   static constexpr int UPR = ROWB / 16, TILEB = KT * ROWB;
-  // 16-byte unit u of row r is stored at u ^ ksw(r) in a K tile (so that 8
-  // lanes reading one unit of 8 rows hit distinct banks), at u ^ vsw(r) in a V
-  // tile (distinct banks for the transposing reads)
-  static __device__ __forceinline__ int ksw(int r) {
-    return UPR == 4 ? (r ^ (r >> 2)) & 3 : r & (UPR - 1);
-  }
+  // 16-byte unit u of row r is stored at u ^ ksw(r) in a K tile: 16 lanes that
+  // read one unit of 16 rows hit all 64 banks
+  static __device__ __forceinline__ int ksw(int r) { return (r / (16 / UPR)) & (UPR - 1); }
+  // and at u ^ vsw(r) in a V tile: so do 32 lanes of a transposing read (8 rows
+  // of two units, or rows r .. r + 7 and r + 16 .. r + 23 of one)
   static __device__ __forceinline__ int vsw(int r) {
-    if constexpr (KIND == 0) return vswz<D>(r);
-    else return D == 128 ? 2 * ((r >> 1) & 3) : 2 * ((r >> 2) & 1);
+    if constexpr (KIND == 0) return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+    else return D == 128 ? ((r >> 1) & 3) | ((r >> 2) & 4) : ((r >> 2) & 1) | ((r >> 3) & 2);
   }
 };
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16x16(typename VecT<T>::v8 a, typename VecT<T>::v8 b, f32x4 c) {
+  if constexpr (__is_same(T, bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
 
 // eight codes as values of type T
 template <typename T, int KIND>
 __device__ __forceinline__ typename VecT<T>::v8 codes8(unsigned a, unsigned b) {
   typedef typename VecT<T>::v8 V8;
-  u32x4 r;
   if constexpr (KIND == TPP_CODE_E4M3) {
     auto two = [](unsigned c, auto hi) {
       if constexpr (__is_same(T, bf16))
@@ -155,6 +166,7 @@ __device__ __forceinline__ typename VecT<T>::v8 codes8(unsigned a, unsigned b) {
       else
         return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, decltype(hi)::value));
     };
+    u32x4 r;
     r[0] = two(a, std::false_type{}), r[1] = two(a, std::true_type{});
     r[2] = two(b, std::false_type{}), r[3] = two(b, std::true_type{});
     return __builtin_bit_cast(V8, r);
@@ -167,360 +179,326 @@ __device__ __forceinline__ typename VecT<T>::v8 codes8(unsigned a, unsigned b) {
 }
 // 2^(e - 127) for byte I of w (255: infinity, which codes of 0 make a NaN)
 template <int I> __device__ __forceinline__ float exp_of(unsigned w) {
-  return __uint_as_float((I == 3 ? w >> 1 : w << (23 - 8 * I)) & 0x7f800000u);
+  return __uint_as_float(((w >> (8 * I)) & 0xffu) << 23);
 }
 
-template <typename T, int KIND, int D, int NQ>
-__global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void tree_tile_kernel(TreeArgs p, float *__restrict__ ws_o,
-                                                        float *__restrict__ ws_ml, int nsplit,
-                                                        unsigned nsplit_inv, unsigned hkv_inv,
-                                                        unsigned g_inv, int by_xcd) {
+// Eight probabilities, a's then b's, as the sum of two values of type PT each,
+// both cut and not rounded, so that lo is what hi leaves.
+template <typename PT>
+__device__ __forceinline__ void two_parts(const f32x4 &a, const f32x4 &b, typename VecT<PT>::v8 &hi,
+                                          typename VecT<PT>::v8 &lo) {
+  u32x4 h, l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float x = j < 2 ? a[2 * j] : b[2 * j - 4], y = j < 2 ? a[2 * j + 1] : b[2 * j - 3];
+    if constexpr (__is_same(PT, bf16)) { // a bfloat16 is the upper half of a float
+      h[j] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+      const float rx = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+      const float ry = y - __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+      l[j] = __builtin_amdgcn_perm(__float_as_uint(ry), __float_as_uint(rx), 0x07060302u);
+    } else {
+      const auto t = __builtin_amdgcn_cvt_pkrtz(x, y);
+      h[j] = __builtin_bit_cast(unsigned, t);
+      l[j] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(x - (float)t[0], y - (float)t[1]));
+    }
+  }
+  hi = __builtin_bit_cast(typename VecT<PT>::v8, h), lo = __builtin_bit_cast(typename VecT<PT>::v8, l);
+}
+
+// the largest over lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float quarter_max(float v) {
+  const unsigned u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned w = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto c = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+
+// One wave's part: NC groups of 16 query rows and what they have summed up.
+template <typename T, int KIND, int D, int NC> struct TreeWave {
   typedef typename VecT<T>::v8 V8;
   typedef std::conditional_t<KIND == 0, T, bf16> PT; // type of P and V operands
   typedef typename VecT<PT>::v8 P8;
   typedef TreeTile<KIND, D> TT;
-  constexpr int KT = TT::KT, NB = KT / 32, NW = 4, STRIDE = NW * KT, ROWB = TT::ROWB, UPR = TT::UPR;
-  constexpr int KPI = 64 / UPR, NDMA = KT / KPI, EX = KIND ? 1 : 0, NT = D / 32, C4 = D / 4;
-  static_assert(2 * TT::TILEB >= 32 * D * 4 && (KIND == 0 || NB == 2), "a wave's rows fit its tiles");
-  __shared__ __attribute__((aligned(16))) char smem[NW * 2 * TT::TILEB];
-  __shared__ __attribute__((aligned(16))) unsigned s_e[NW][64];
-  __shared__ float s_m[NW][32], s_l[NW][32];
-  constexpr float kUp = KIND == 0 && !__is_same(T, bf16) ? 15.f : 0.f;
+  static constexpr int KT = TT::KT, ROWB = TT::ROWB, UPR = TT::UPR, EB = KIND ? 1 : 2, EX = KIND ? 1 : 0;
+  static constexpr int NST = KT / 16, NX = ROWB / 64, NCS = KT / 32, NT = D / 16;
+  static constexpr float kUp = KIND == 0 && !__is_same(T, bf16) ? 15.f : 0.f; // P times 2^15
 
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = lane >> 5, ql = lane & 31;
-  const int pair = by_xcd ? blockIdx.z * 8 + (blockIdx.x & 7) : blockIdx.z;
-  const int qt = by_xcd ? blockIdx.x >> 3 : blockIdx.x, split = blockIdx.y;
-  const int b = div_inv(pair, hkv_inv), hk = pair - b * p.Hkv;
-  const int L = min(max(p.seqlens[b], 0), p.Lmax), end = min(L + p.T, p.Lmax);
-  const int nbatch = (int)((unsigned)(end + STRIDE - 1) / (unsigned)STRIDE);
-  const int per = div_inv((unsigned)(nbatch + nsplit - 1), nsplit_inv);
-  const int64_t c0 = (int64_t)split * per * STRIDE;
-  if (c0 >= end) return;
-  const int k_end = (int)(c0 + (int64_t)per * STRIDE < end ? c0 + (int64_t)per * STRIDE : end);
-  const int first = (int)c0 + w * KT;
-  const int n = first < k_end ? (k_end - first + STRIDE - 1) / STRIDE : 0; // this wave's tiles
+  V8 qf[NC][D / 32];
+  unsigned long long see[NC];
+  f32x4 o[NC][NT];
+  float m[NC], l[NC];
+  unsigned ko[NX], vo[NT], ea;
+  int t[NC];
 
-  constexpr int EB = KIND ? 1 : 2;
-  const char *ks = (const char *)p.k + ((int64_t)b * p.k_s[0] + (int64_t)hk * p.k_s[1]) * EB;
-  const char *vs = (const char *)p.v + ((int64_t)b * p.v_s[0] + (int64_t)hk * p.v_s[1]) * EB;
-  const int64_t eb = (int64_t)b * p.e_s[0] + (int64_t)hk * p.e_s[1];
-  const int dkey = lane / UPR, dslot = lane % UPR;
-  char *const ring = smem + w * (2 * TT::TILEB);
-  // exponents of a tile as the lanes of half h read them: 8 dwords of K (scores
-  // 32 st + 8 g + 4 h .. + 3 in dword 4 st + g), 8 of V 64 bytes on
-  const uint8_t *es = nullptr;
-  int edw = 0;
-  if constexpr (KIND != 0) {
-    es = (lane & 16 ? p.ve : p.ke) + eb;
-    edw = 4 * (((lane >> 2) & 1) * 8 + (lane & 3) * 2 + ((lane >> 3) & 1));
-  }
-  auto issue = [&](bool kt, int base) {
-    const char *src = kt ? ks : vs;
-    const int64_t ss = (kt ? p.k_s[2] : p.v_s[2]) * EB;
+  // query rows row[i] (clamped by the caller), asked for
+  __device__ __forceinline__ void ask(const TreeArgs &p, int b, int hk, unsigned g_inv, const int (&row)[NC]) {
+    const int u4 = lane_id() >> 4;
 #pragma unroll
-    for (int j = 0; j < NDMA; ++j) {
-      const int key = j * KPI + dkey;
-      const int ch = dslot ^ (kt ? TT::ksw(key) : TT::vsw(key));
-      __builtin_amdgcn_global_load_lds((const void *)(src + (int64_t)min(base + key, end - 1) * ss + ch * 16),
-                                       (__attribute__((address_space(3))) void *)(ring + (kt ? 0 : TT::TILEB) + j * 1024),
-                                       16, 0, kCpolNT);
+    for (int i = 0; i < NC; ++i) {
+      t[i] = div_inv((unsigned)row[i], g_inv);
+      const T *qp = row_of((const T *)p.q, p.q_s, p, b, hk, row[i], t[i]);
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) // codes: a 16-byte read holds both steps of 64 elements
+        qf[i][k] = *reinterpret_cast<const V8 *>(qp + (KIND ? (k / 2) * 64 + u4 * 16 + (k & 1) * 8 : k * 32 + u4 * 8));
     }
-    if constexpr (KIND != 0)
-      if (kt) // (lanes 32 - 63 repeat 0 - 31)
-        __builtin_amdgcn_global_load_lds((const void *)(es + min(base + edw, p.Lmax - 4)),
-                                         (__attribute__((address_space(3))) void *)s_e[w], 4, 0, 0);
-  };
-  if (n > 0) {
-    issue(true, first);
-    issue(false, first);
   }
-
-  // this lane's query row of each tile: its fragments, and what it sees
-  const unsigned long long bits = tree_bits(p, b, L);
-  const int rows = p.T * p.G;
-  V8 qf[NQ][D / 16];
-  unsigned long long see[NQ];
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const int r = min((qt * NQ + i) * 32 + ql, rows - 1);
-    const int t = div_inv((unsigned)r, g_inv), g = r - t * p.G;
-    see[i] = ((unsigned long long)(unsigned)__shfl((int)(bits >> 32), t, kWave) << 32) |
-             (unsigned)__shfl((int)bits, t, kWave);
-    const T *qp = (const T *)p.q + (int64_t)b * p.q_s[0] + (int64_t)t * p.q_s[1] + (int64_t)(hk * p.G + g) * p.q_s[2];
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) // codes: a 16-byte read holds both steps of 32 elements
-      qf[i][k] = *reinterpret_cast<const V8 *>(qp + (KIND ? (k / 2) * 32 + h * 16 + (k & 1) * 8 : k * 16 + h * 8));
+  template <typename E>
+  static __device__ __forceinline__ E *row_of(E *base, const int64_t (&st)[3], const TreeArgs &p, int b, int hk,
+                                              int row, int tok) {
+    return base + (int64_t)b * st[0] + (int64_t)tok * st[1] + (int64_t)(hk * p.G + row - tok * p.G) * st[2];
   }
-  // waited for here (with the first tiles): no wait for them inside the loop
+  // The rows have come, the first tiles are in flight: no wait for the rows
+  // inside the loop. LDS addresses of a tile's K and V and of its exponents.
+  __device__ __forceinline__ void begin(unsigned long long bits, unsigned kbase, unsigned vbase, unsigned ebase) {
+    const int lane = lane_id(), u4 = lane >> 4, l16 = lane & 15;
 #pragma unroll
-  for (int i = 0; i < NQ; ++i)
+    for (int i = 0; i < NC; ++i) {
+      see[i] = ((unsigned long long)(unsigned)__shfl((int)(bits >> 32), t[i], kWave) << 32) |
+               (unsigned)__shfl((int)bits, t[i], kWave);
+      m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) asm volatile("" ::"v"(qf[i][k]));
-
-  f32x16 o[NQ][NT];
-  float m_run[NQ], l_run[NQ];
+      for (int k = 0; k < D / 32; ++k) asm volatile("" ::"v"(qf[i][k]));
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    m_run[i] = -INFINITY, l_run[i] = 0.f;
+      for (int tt = 0; tt < NT; ++tt) o[i][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    ea = ebase + u4 * 16;
 #pragma unroll
-    for (int tt = 0; tt < NT; ++tt)
+    for (int x = 0; x < NX; ++x) ko[x] = kbase + (unsigned)((l16 * UPR + ((4 * x + u4) ^ TT::ksw(l16))) * 16);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[i][tt][r] = 0.f;
-  }
-  const float c2 = p.scale_log2;
-  const unsigned base0 = (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)ring;
-  const unsigned ebase = (unsigned)(uintptr_t)(const __attribute__((address_space(3))) unsigned *)s_e[w] + h * 32;
-  const int grp = lane >> 4;
-  unsigned vo[NT];
-#pragma unroll
-  for (int tt = 0; tt < NT; ++tt) {
-    if constexpr (KIND == 0) {
-      const int a4 = lane & 3, kl = 4 * (grp >> 1) + ((lane >> 2) & 3), d0 = tt * 32 + 16 * (grp & 1) + 4 * a4;
-      vo[tt] = base0 + TT::TILEB + kl * ROWB + (((d0 >> 3) ^ TT::vsw(kl)) << 4) + ((d0 & 7) << 1);
-    } else {
-      const int rr = (lane >> 1) & 7, kl = 8 * (rr >> 2) + 4 * (grp >> 1) + (rr & 3);
-      vo[tt] = base0 + TT::TILEB + kl * ROWB + (((2 * tt + (grp & 1)) ^ TT::vsw(kl)) << 4) + 8 * (lane & 1);
+    for (int tt = 0; tt < NT; ++tt) {
+      if constexpr (KIND == 0) { // lane a + 4 r at row 4 u + r, element 16 tt + 4 a
+        const int kl = 4 * u4 + ((lane >> 2) & 3), a = lane & 3;
+        vo[tt] = vbase + kl * ROWB + (((2 * tt) ^ TT::vsw(kl)) << 4) + 8 * a;
+      } else { // lane a + 2 r at row 4 u + r (r < 4) or 16 + 4 u + r - 4, byte 16 tt + 8 a
+        const int rr = (lane >> 1) & 7, kl = 16 * (rr >> 2) + 4 * u4 + (rr & 3);
+        vo[tt] = vbase + kl * ROWB + ((tt ^ TT::vsw(kl)) << 4) + 8 * (lane & 1);
+      }
     }
   }
 
-  for (int it = 0; it < n; ++it) {
-    const int kb = first + it * STRIDE;
-    const bool more = it + 1 < n, edge = kb + KT > L;
-    vm_wait<NDMA>(); // this tile's K (and exponents) landed, its V may be in flight
-    f32x16 s[NQ][NB];
+  // One tile, keys kb .. kb + KT - 1, `off` bytes on in the ring (its exponents
+  // eoff). after_k / after_v: its K / V fragments are in registers; wait_v: until
+  // its V has landed.
+  template <typename AK, typename WV, typename AV>
+  __device__ __forceinline__ void step(const TreeArgs &p, int kb, int L, unsigned off, unsigned eoff, AK after_k,
+                                       WV wait_v, AV after_v) {
+    const int u4 = lane_id() >> 4;
+    const bool edge = kb + KT > L;
+    const float c2 = p.scale_log2;
+    f32x4 s[NC][NST];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i)
+    for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int st = 0; st < NB; ++st)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[i][st][r] = 0.f;
-    u32x4 ex[4];
-    if constexpr (KIND == 0) {
-      constexpr int KS = D / 16, NS = KS * NB / 2;
-      V8 kr[3][2];
-      auto kfrag = [&](auto ii) {
-        constexpr int x = decltype(ii)::value;
-        static_for<2>([&](auto jj) {
-          constexpr int j = decltype(jj)::value, k = NB == 2 ? x : 2 * x + j;
-          const unsigned a = base0 + (unsigned)((ql * UPR + ((k * 2 + h) ^ TT::ksw(ql))) * 16);
-          kr[x % 3][j] = lds_read_b128<(NB == 2 ? j : 0) * 32 * ROWB, V8>(a);
-        });
-      };
-      kfrag(std::integral_constant<int, 0>{});
-      kfrag(std::integral_constant<int, 1>{});
-      static_for<NS>([&](auto ii) {
-        constexpr int x = decltype(ii)::value;
-        if constexpr (x + 2 < NS) kfrag(std::integral_constant<int, x + 2>{});
-        lds_wait_tied<(x + 2 < NS ? 2 : NS - 1 - x) * 2>(kr[x % 3]);
-        if constexpr (x == NS - 1) { // every K fragment is in registers
-          asm volatile("" ::: "memory");
-          if (more) issue(true, kb + STRIDE);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < NQ; ++i)
-            s[i][j % NB] = mfma32x32<T>(kr[x % 3][j], qf[i][NB == 2 ? x : 2 * x + j], s[i][j % NB]);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int st = 0; st < NST; ++st) s[i][st] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 kr[NX][NST], ex[2];
+    static_for<NX>([&](auto xx) {
+      constexpr int x = decltype(xx)::value;
+      static_for<NST>([&](auto tt) {
+        constexpr int st = decltype(tt)::value;
+        kr[x][st] = lds_read_b128<st * 16 * ROWB, u32x4>(ko[x] + off);
       });
-    } else {
-      constexpr int NP = D / 32; // 16-byte reads: two steps of a half's 8 elements
-      u32x4 kr[NP][2];
-      static_for<NP>([&](auto ii) {
-        constexpr int x = decltype(ii)::value;
-        const unsigned a = base0 + (unsigned)((ql * UPR + ((2 * x + h) ^ TT::ksw(ql))) * 16);
-        kr[x][0] = lds_read_b128<0, u32x4>(a);
-        kr[x][1] = lds_read_b128<32 * ROWB, u32x4>(a);
-      });
-      ex[0] = lds_read_b128<0, u32x4>(ebase), ex[1] = lds_read_b128<16, u32x4>(ebase);
-      ex[2] = lds_read_b128<64, u32x4>(ebase), ex[3] = lds_read_b128<80, u32x4>(ebase);
-      static_for<NP>([&](auto ii) {
-        constexpr int x = decltype(ii)::value;
-        lds_wait_tied<2 * (NP - 1 - x) + 4>(kr[x]);
-        if constexpr (x == NP - 1) {
-          lds_wait_tied<0>(ex);
-          asm volatile("" ::: "memory");
-          if (more) issue(true, kb + STRIDE);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (KIND != 0) ex[0] = lds_read_b128<0, u32x4>(ea + eoff), ex[1] = lds_read_b128<64, u32x4>(ea + eoff);
+    static_for<NX>([&](auto xx) {
+      constexpr int x = decltype(xx)::value;
+      lds_wait_tied<(NX - 1 - x) * NST + 2 * EX>(kr[x]);
+      if constexpr (x == NX - 1) { // every K fragment is in registers
+        if constexpr (KIND != 0) lds_wait_tied<0>(ex);
+        asm volatile("" ::: "memory");
+        after_k();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // (products into one accumulator are kept apart: back to back each would
+      // wait for the one ahead)
+      if constexpr (KIND == 0) {
+#pragma unroll
+        for (int st = 0; st < NST; ++st)
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+            s[i][st] = mfma16x16<T>(__builtin_bit_cast(V8, kr[x][st]), qf[i][x], s[i][st]);
+      } else {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int st = 0; st < 2; ++st) {
+          for (int st = 0; st < NST; ++st) {
             const V8 f = codes8<T, KIND>(kr[x][st][2 * u], kr[x][st][2 * u + 1]);
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) s[i][st] = mfma32x32<T>(f, qf[i][2 * x + u], s[i][st]);
+            for (int i = 0; i < NC; ++i) s[i][st] = mfma16x16<T>(f, qf[i][2 * x + u], s[i][st]);
           }
-        __builtin_amdgcn_sched_barrier(0);
-      });
-    }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
 
-    P8 pb[NQ][2 * NB];
+    P8 hi[NC][NCS], lo[NC][NCS];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
+    for (int i = 0; i < NC; ++i) {
       if constexpr (KIND != 0)
-#pragma unroll
-        for (int st = 0; st < NB; ++st)
-          static_for<16>([&](auto rr) {
-            constexpr int r = decltype(rr)::value;
-            s[i][st][r] *= exp_of<r % 4>(ex[st][r / 4]);
-          });
-      unsigned keep[NB]; // bit 8 g + e: score register 4 g + e
+        static_for<16>([&](auto rr) {
+          constexpr int r = decltype(rr)::value;
+          s[i][r / 4][r % 4] *= exp_of<r % 4>(ex[0][r / 4]);
+        });
+      unsigned keep[NCS]; // bit 16 (st % 2) + e: score e of tile st
       if (edge) {
         const unsigned ninf = __float_as_uint(-INFINITY);
 #pragma unroll
-        for (int st = 0; st < NB; ++st) {
-          const int rel = kb + 32 * st - L;
+        for (int c = 0; c < NCS; ++c) {
+          const int rel = kb + 32 * c - L;
           const unsigned k32 = rel >= 64 ? 0u
                                : rel >= 0 ? (unsigned)(see[i] >> rel)
                                : rel > -32 ? ((unsigned)see[i] << -rel) | ((1u << -rel) - 1u)
                                            : ~0u;
-          keep[st] = k32 >> (4 * h);
+          keep[c] = k32 >> (4 * u4);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const unsigned bm = (unsigned)__builtin_amdgcn_sbfe((int)keep[st], (r >> 2) * 8 + (r & 3), 1);
-            s[i][st][r] = __uint_as_float((__float_as_uint(s[i][st][r]) & bm) | (ninf & ~bm));
+          for (int r = 0; r < 8; ++r) {
+            const unsigned bm = (unsigned)__builtin_amdgcn_sbfe((int)keep[c], (r >> 2) * 16 + (r & 3), 1);
+            float &x = reinterpret_cast<float *>(&s[i][2 * c + (r >> 2)])[r & 3];
+            x = __uint_as_float((__float_as_uint(x) & bm) | (ninf & ~bm));
           }
         }
       }
-      float mx[4] = {s[i][0][0], s[i][0][1], s[i][0][2], s[i][0][3]};
+      float mt = -INFINITY;
 #pragma unroll
-      for (int st = 0; st < NB; ++st)
-#pragma unroll
-        for (int r = st == 0 ? 4 : 0; r < 16; ++r) mx[r & 3] = fmaxf(mx[r & 3], s[i][st][r]);
-      float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
-      mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-      const bool move = mt > m_run[i];
-      const float m_new = move ? mt : m_run[i];
+      for (int st = 0; st < NST; ++st)
+        mt = fmaxf(mt, fmaxf(fmaxf(s[i][st][0], s[i][st][1]), fmaxf(s[i][st][2], s[i][st][3])));
+      mt = quarter_max(mt);
+      const bool move = mt > m[i];
+      const float m_new = move ? mt : m[i];
       const float mc = m_new == -INFINITY ? 0.f : m_new * c2;
-      const float alpha = move ? __builtin_amdgcn_exp2f(m_run[i] * c2 - mc) : 1.f;
+      const float alpha = move ? __builtin_amdgcn_exp2f(m[i] * c2 - mc) : 1.f;
       float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int st = 0; st < NB; ++st)
+      for (int st = 0; st < NST; ++st)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
+        for (int r = 0; r < 4; ++r) {
           const float e = __builtin_amdgcn_exp2f(fmaf(s[i][st][r], c2, kUp - mc));
           s[i][st][r] = e;
-          ps[r & 3] += e;
+          ps[r] += e;
         }
-      l_run[i] = l_run[i] * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-      m_run[i] = m_new;
+      l[i] = l[i] * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
+      m[i] = m_new;
       if (__any(move)) {
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][tt][r] *= alpha;
+          for (int r = 0; r < 4; ++r) o[i][tt][r] *= alpha;
       }
       if constexpr (KIND != 0) {
-#pragma unroll
-        for (int st = 0; st < NB; ++st)
-          static_for<16>([&](auto rr) {
-            constexpr int r = decltype(rr)::value;
-            s[i][st][r] *= exp_of<r % 4>(ex[2 + st][r / 4]);
-          });
+        static_for<16>([&](auto rr) {
+          constexpr int r = decltype(rr)::value;
+          s[i][r / 4][r % 4] *= exp_of<r % 4>(ex[1][r / 4]);
+        });
         if (edge) { // a masked row of NaN: 0 times infinity above
 #pragma unroll
-          for (int st = 0; st < NB; ++st)
+          for (int c = 0; c < NCS; ++c)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[i][st][r] = __uint_as_float(__float_as_uint(s[i][st][r]) &
-                                            (unsigned)__builtin_amdgcn_sbfe((int)keep[st], (r >> 2) * 8 + (r & 3), 1));
+            for (int r = 0; r < 8; ++r) {
+              float &x = reinterpret_cast<float *>(&s[i][2 * c + (r >> 2)])[r & 3];
+              x = __uint_as_float(__float_as_uint(x) &
+                                  (unsigned)__builtin_amdgcn_sbfe((int)keep[c], (r >> 2) * 16 + (r & 3), 1));
+            }
         }
       }
 #pragma unroll
-      for (int c = 0; c < 2 * NB; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pb[i][c][j] = from_f32<PT>(s[i][c >> 1][(c & 1) * 8 + j]);
+      for (int c = 0; c < NCS; ++c) two_parts<PT>(s[i][2 * c], s[i][2 * c + 1], hi[i][c], lo[i][c]);
     }
 
-    // this tile's V landed (the next K may be in flight)
-    if (more) vm_wait<NDMA + EX>();
-    else vm_wait<0>();
-    constexpr int R = KIND ? NT : 2 * NT;
+    wait_v();
+    constexpr int R = KIND ? 4 : 8, NG = NCS * NT / 4; // four d tiles of a step at a time
     typedef std::conditional_t<KIND == 0, s16x4, u32x2> VR;
     VR vr[2][R];
-    auto vfrag = [&](auto cc) {
-      constexpr int c = decltype(cc)::value;
+    auto vfrag = [&](auto gg) {
+      constexpr int g = decltype(gg)::value, c = g / (NT / 4), t0 = 4 * (g % (NT / 4));
 #pragma unroll
-      for (int tt = 0; tt < NT; ++tt) {
+      for (int j = 0; j < 4; ++j) {
         if constexpr (KIND == 0) {
-          vr[c % 2][2 * tt] = lds_read_tr16<c * 16 * ROWB>(vo[tt]);
-          vr[c % 2][2 * tt + 1] = lds_read_tr16<c * 16 * ROWB + 8 * ROWB>(vo[tt]);
+          vr[g % 2][2 * j] = lds_read_tr16<c * 32 * ROWB>(vo[t0 + j] + off);
+          vr[g % 2][2 * j + 1] = lds_read_tr16<c * 32 * ROWB + 16 * ROWB>(vo[t0 + j] + off);
         } else {
-          vr[c % 2][tt] = lds_read_tr8<c * 16 * ROWB>(vo[tt]);
+          vr[g % 2][j] = lds_read_tr8<c * 32 * ROWB>(vo[t0 + j] + off);
         }
       }
     };
     vfrag(std::integral_constant<int, 0>{});
-    static_for<2 * NB>([&](auto cc) {
-      constexpr int c = decltype(cc)::value;
-      if constexpr (c + 1 < 2 * NB) vfrag(std::integral_constant<int, c + 1>{});
-      lds_wait_tied<(c + 1 < 2 * NB ? R : 0)>(vr[c % 2]);
-      if constexpr (c + 1 == 2 * NB) {
+    static_for<NG>([&](auto gg) {
+      constexpr int g = decltype(gg)::value, c = g / (NT / 4), t0 = 4 * (g % (NT / 4));
+      if constexpr (g + 1 < NG) vfrag(std::integral_constant<int, g + 1>{});
+      lds_wait_tied<(g + 1 < NG ? R : 0)>(vr[g % 2]);
+      if constexpr (g + 1 == NG) {
         asm volatile("" ::: "memory");
-        if (more) issue(false, kb + STRIDE);
+        after_v();
       }
       __builtin_amdgcn_sched_barrier(0);
+      constexpr int JG = NC == 1 ? 4 : 2;
 #pragma unroll
-      for (int tt = 0; tt < NT; ++tt) {
-        P8 f;
-        if constexpr (KIND == 0) {
-          typedef short s16x8 __attribute__((ext_vector_type(8)));
-          const s16x8 r12 = __builtin_shufflevector(vr[c % 2][2 * tt], vr[c % 2][2 * tt + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-          f = __builtin_bit_cast(P8, r12);
-        } else {
-          f = codes8<PT, KIND>(vr[c % 2][tt][0], vr[c % 2][tt][1]);
+      for (int j0 = 0; j0 < 4; j0 += JG) {
+        P8 f[JG];
+#pragma unroll
+        for (int j = 0; j < JG; ++j) {
+          if constexpr (KIND == 0) {
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            const s16x8 r12 = __builtin_shufflevector(vr[g % 2][2 * (j0 + j)], vr[g % 2][2 * (j0 + j) + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+            f[j] = __builtin_bit_cast(P8, r12);
+          } else {
+            f[j] = codes8<PT, KIND>(vr[g % 2][j0 + j][0], vr[g % 2][j0 + j][1]);
+          }
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i][t0 + j0 + j] = mfma16x16<PT>(f[j], lo[i][c], o[i][t0 + j0 + j]);
         }
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) o[i][tt] = mfma32x32<PT>(f, pb[i][c], o[i][tt]);
+        for (int j = 0; j < JG; ++j)
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i][t0 + j0 + j] = mfma16x16<PT>(f[j], hi[i][c], o[i][t0 + j0 + j]);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
   }
 
-  // The wave's rows, then the block's: row ql's chunk c of 4 values at c ^ ql
-  f32x4 *const part = reinterpret_cast<f32x4 *>(ring);
-  const int live = (int)((unsigned)(nbatch + per - 1) / (unsigned)per);
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const int r0 = (qt * NQ + i) * 32;
-    if (r0 >= rows) break; // all waves
-    if (i) __syncthreads();
+  // l, m (times the scale) over the four lanes of a row; rows that see nothing
+  // have none. True where a sum is not finite.
+  __device__ __forceinline__ bool end(const TreeArgs &p) {
     bool odd = false;
-    float l = l_run[i] + __shfl_xor(l_run[i], 32, kWave), m = m_run[i];
-    if (!see[i]) l = 0.f, m = -INFINITY;
 #pragma unroll
-    for (int tt = 0; tt < NT; ++tt)
+    for (int i = 0; i < NC; ++i) {
+      l[i] += __shfl_xor(l[i], 16, kWave);
+      l[i] += __shfl_xor(l[i], 32, kWave);
+      if (!see[i]) l[i] = 0.f, m[i] = -INFINITY;
 #pragma unroll
-      for (int rg = 0; rg < 4; ++rg) {
-        f32x4 v;
+      for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = see[i] ? o[i][tt][rg * 4 + e] : 0.f;
-          odd |= !(fabsf(v[e]) < INFINITY);
+          if (!see[i]) o[i][tt][e] = 0.f;
+          odd |= !(fabsf(o[i][tt][e]) < INFINITY);
         }
-        part[ql * C4 + ((tt * 8 + rg * 2 + h) ^ (ql & (C4 - 1)))] = v;
-      }
-    if (h == 0) s_m[w][ql] = m == -INFINITY ? m : m * c2, s_l[w][ql] = l;
-    // A row behind the context that is not finite, times a weight of 0, is a
-    // NaN in the products of those that do not see it: a wave with such a tile
-    // and a sum that is not finite sums again, over what each row sees.
-    if (n > 0 && first + (n - 1) * STRIDE + KT > L && __any(odd)) {
-      for (int q = 0; q < 32 && r0 + q < rows; ++q) {
+    }
+    return odd;
+  }
+  __device__ __forceinline__ float top(const TreeArgs &p, int i) const {
+    return m[i] == -INFINITY ? -INFINITY : m[i] * p.scale_log2;
+  }
+
+  // A row behind the context that is not finite, times a weight of 0, is a NaN in
+  // the products of those that do not see it. A wave that had such a tile and has
+  // a sum that is not finite sums again, key by key over what each row sees: its
+  // n tiles from key `first`, `stride` apart, up to k_end. put(i, q, d, x): the
+  // sum of element d of row q of group i.
+  template <typename PUT>
+  __device__ __forceinline__ void again(const TreeArgs &p, int b, int hk, const char *ks, const char *vs, int64_t eb,
+                                        int first, int stride, int n, int k_end, int L, unsigned g_inv,
+                                        const int (&row0)[NC], int rows, PUT put) const {
+    const int lane = lane_id();
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      for (int q = 0; q < 16 && row0[i] + q < rows; ++q) {
         const unsigned long long sq = ((unsigned long long)(unsigned)__shfl((int)(see[i] >> 32), q, kWave) << 32) |
                                       (unsigned)__shfl((int)see[i], q, kWave);
-        if (!sq) continue;
-        const int t = div_inv((unsigned)(r0 + q), g_inv), g = r0 + q - t * p.G;
-        const T *qp = (const T *)p.q + (int64_t)b * p.q_s[0] + (int64_t)t * p.q_s[1] + (int64_t)(hk * p.G + g) * p.q_s[2];
-        const float mq = __shfl(m_run[i], q, kWave), mc = mq == -INFINITY ? 0.f : mq * c2;
+        const float mq = __shfl(m[i], q, kWave), mc = mq == -INFINITY ? 0.f : mq * p.scale_log2;
+        const T *qp = row_of((const T *)p.q, p.q_s, p, b, hk, row0[i] + q, div_inv((unsigned)(row0[i] + q), g_inv));
         float acc[D / 64];
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) acc[c] = 0.f;
-        for (int it = 0; it < n; ++it)
-          for (int j = first + it * STRIDE; j < min(first + it * STRIDE + KT, k_end); ++j) {
+        for (int it = 0; it < n && sq; ++it)
+          for (int j = first + it * stride; j < min(first + it * stride + KT, k_end); ++j) {
             if (j >= L && !((sq >> (j - L)) & 1)) continue;
             const char *kr = ks + (int64_t)j * p.k_s[2] * EB, *vr = vs + (int64_t)j * p.v_s[2] * EB;
             const float fk = KIND ? exp_scale(p.ke, eb + j) : 1.f, fv = KIND ? exp_scale(p.ve, eb + j) : 1.f;
@@ -528,80 +506,370 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void tree_tile_kernel(TreeArg
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
               sd += to_f32(qp[c * 64 + lane]) * cache_value<T, KIND>(kr, c * 64 + lane, fk);
-            const float e = __builtin_amdgcn_exp2f(fmaf(wave_sum(sd), c2, kUp - mc));
+            const float e = __builtin_amdgcn_exp2f(fmaf(wave_sum(sd), p.scale_log2, kUp - mc));
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) acc[c] += e * cache_value<T, KIND>(vr, c * 64 + lane, fv);
           }
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const int d = c * 64 + lane;
-          reinterpret_cast<float *>(part + q * C4 + ((d / 4) ^ (q & (C4 - 1))))[d % 4] = acc[c];
-        }
+        for (int c = 0; c < D / 64; ++c) put(i, q, c * 64 + lane, acc[c]);
+      }
+  }
+};
+
+// The caller's block: its pair, and the keys of its split in whole batches of
+// `stride` keys (none: c0 >= end).
+struct TreeBlock {
+  int pair, b, hk, qt, split, L, end, live;
+  int64_t c0, c1;
+};
+template <int STRIDE>
+__device__ __forceinline__ void tree_split(const TreeArgs &p, int nsplit, unsigned nsplit_inv, TreeBlock &k) {
+  k.L = min(max(p.seqlens[k.b], 0), p.Lmax), k.end = min(k.L + p.T, p.Lmax);
+  const int nbatch = (int)((unsigned)(k.end + STRIDE - 1) / (unsigned)STRIDE);
+  const int per = div_inv((unsigned)(nbatch + nsplit - 1), nsplit_inv);
+  k.live = (int)((unsigned)(nbatch + per - 1) / (unsigned)per);
+  k.c0 = (int64_t)k.split * per * STRIDE;
+  k.c1 = k.c0 + (int64_t)per * STRIDE < k.end ? k.c0 + (int64_t)per * STRIDE : k.end;
+}
+__device__ __forceinline__ TreeBlock tree_block(const TreeArgs &p, unsigned hkv_inv, int by_xcd) {
+  TreeBlock k; // blocks of a pair on one XCD where pairs divide by them
+  k.pair = by_xcd ? blockIdx.z * 8 + (blockIdx.x & 7) : blockIdx.z;
+  k.qt = by_xcd ? blockIdx.x >> 3 : blockIdx.x, k.split = blockIdx.y;
+  k.b = div_inv(k.pair, hkv_inv), k.hk = k.pair - k.b * p.Hkv;
+  return k;
+}
+
+// A wave's LDS-DMA of tile units j0 .. j0 + N - 1 (1 KB each) of K or V. Byte
+// offsets of this lane's units from the tile's first row: a tile whose keys all
+// exist is one uniform address and these. Else keys past the last read its row
+// (masked).
+template <int KIND, int D, int N, int POL> struct TreeDma {
+  typedef TreeTile<KIND, D> TT;
+  static constexpr int EB = KIND ? 1 : 2, KPI = 64 / TT::UPR;
+  unsigned off[N];
+  int j0;
+  bool kt;
+  __device__ __forceinline__ int unit(int j) const {
+    const int key = (j0 + j) * KPI + lane_id() / TT::UPR;
+    return (lane_id() % TT::UPR) ^ (kt ? TT::ksw(key) : TT::vsw(key));
+  }
+  __device__ __forceinline__ void begin(bool k, int first_unit, int64_t stride) {
+    kt = k, j0 = first_unit;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      off[j] = (unsigned)(((j0 + j) * KPI + lane_id() / TT::UPR) * (int)stride * EB + (unit(j) << 4));
+  }
+  __device__ __forceinline__ void issue(const char *rows, int64_t stride, int base, int end, char *dst) const {
+    const char *src = rows + (int64_t)base * stride * EB;
+    if (base + TT::KT <= end) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        __builtin_amdgcn_global_load_lds((const void *)(src + off[j]),
+                                         (__attribute__((address_space(3))) void *)(dst + (j0 + j) * 1024), 16, 0, POL);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int key = (j0 + j) * KPI + lane_id() / TT::UPR;
+        __builtin_amdgcn_global_load_lds(
+            (const void *)(src + (int64_t)min(key, end - 1 - base) * stride * EB + (unit(j) << 4)),
+            (__attribute__((address_space(3))) void *)(dst + (j0 + j) * 1024), 16, 0, POL);
       }
     }
-    __syncthreads();
-    for (int idx = tid; idx < 32 * C4; idx += 64 * NW) {
-      const int row = idx / C4, c = idx % C4, r = r0 + row;
-      if (r >= rows) break;
-      float mx = -INFINITY;
+  }
+};
+// The exponents of a tile as the lanes read them: quarter u's four dwords (keys
+// 16 st + 4 u .. + 3 in dword st) of K at 16 u, of V 64 bytes on (lanes 32 - 63
+// repeat 0 - 31).
+__device__ __forceinline__ void issue_exps(const TreeArgs &p, int64_t eb, int base, unsigned *dst) {
+  const int lane = lane_id(), at = 16 * (lane & 3) + 4 * ((lane >> 2) & 3);
+  __builtin_amdgcn_global_load_lds((const void *)((lane & 16 ? p.ve : p.ke) + eb + min(base + at, p.Lmax - 4)),
+                                   (__attribute__((address_space(3))) void *)dst, 4, 0, 0);
+}
+template <typename P> __device__ __forceinline__ unsigned lds_addr(P *x) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)x;
+}
+
+// Up to 32 rows a block: the four waves share the rows and split the keys.
+template <typename T, int KIND, int D, int NC>
+__global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs p, float *__restrict__ ws_o,
+                                                           float *__restrict__ ws_ml, int nsplit,
+                                                           unsigned nsplit_inv, unsigned hkv_inv,
+                                                           unsigned g_inv, int by_xcd) {
+  typedef TreeTile<KIND, D> TT;
+  typedef TreeWave<T, KIND, D, NC> W;
+  constexpr int KT = TT::KT, NW = 4, STRIDE = NW * KT, NDMA = TT::TILEB / 1024, C4 = D / 4, ROWS = 16 * NC;
+  static_assert(2 * TT::TILEB >= ROWS * D * 4 && (KIND == 0 || KT == 64), "a wave's rows fit its tiles");
+  __shared__ __attribute__((aligned(16))) char smem[NW * 2 * TT::TILEB];
+  __shared__ __attribute__((aligned(16))) unsigned s_e[NW][64];
+  __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int u4 = lane >> 4, l16 = lane & 15;
+  TreeBlock k = tree_block(p, hkv_inv, by_xcd);
+  // what no length has a part in is asked for first: loads return in order, so a
+  // load behind the first tiles would wait for them
+  const int up = tree_parent(p, k.b);
+  const int rows = p.T * p.G;
+  W wv;
+  int row0[NC], row[NC];
 #pragma unroll
-      for (int ww = 0; ww < NW; ++ww) mx = fmaxf(mx, s_m[ww][row]);
-      const float mu = mx == -INFINITY ? 0.f : mx;
-      float ls = 0.f;
-      f32x4 os = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < NC; ++i) row0[i] = k.qt * ROWS + i * 16, row[i] = min(row0[i] + l16, rows - 1);
+  wv.ask(p, k.b, k.hk, g_inv, row);
+  tree_split<STRIDE>(p, nsplit, nsplit_inv, k);
+  if (k.c0 >= k.end) return;
+  const int first = (int)k.c0 + w * KT, k_end = (int)k.c1;
+  const int n = first < k_end ? (k_end - first + STRIDE - 1) / STRIDE : 0; // this wave's tiles
+
+  const char *ks = (const char *)p.k + ((int64_t)k.b * p.k_s[0] + (int64_t)k.hk * p.k_s[1]) * W::EB;
+  const char *vs = (const char *)p.v + ((int64_t)k.b * p.v_s[0] + (int64_t)k.hk * p.v_s[1]) * W::EB;
+  const int64_t eb = (int64_t)k.b * p.e_s[0] + (int64_t)k.hk * p.e_s[1];
+  char *const ring = smem + w * (2 * TT::TILEB);
+  TreeDma<KIND, D, NDMA, kCpolNT> dk, dv;
+  dk.begin(true, 0, p.k_s[2]);
+  dv.begin(false, 0, p.v_s[2]);
+  auto issue_k = [&](int base) {
+    dk.issue(ks, p.k_s[2], base, k.end, ring);
+    if constexpr (KIND != 0) issue_exps(p, eb, base, s_e[w]);
+  };
+  auto issue_v = [&](int base) { dv.issue(vs, p.v_s[2], base, k.end, ring + TT::TILEB); };
+  if (n > 0) {
+    issue_k(first);
+    issue_v(first);
+  }
+  wv.begin(tree_bits(p, up, k.L), lds_addr(ring), lds_addr(ring) + TT::TILEB, lds_addr(s_e[w]));
+  for (int it = 0; it < n; ++it) {
+    const int kb = first + it * STRIDE;
+    const bool more = it + 1 < n;
+    vm_wait<NDMA>(); // this tile's K (and exponents) landed, its V may be in flight
+    wv.step(p, kb, k.L, 0, 0,
+            [&] { if (more) issue_k(kb + STRIDE); },
+            [&] { // the next K may be in flight
+              if (more) vm_wait<NDMA + W::EX>();
+              else vm_wait<0>();
+            },
+            [&] { if (more) issue_v(kb + STRIDE); });
+  }
+
+  // The wave's rows, then the block's: chunk c (4 values) of row r at c ^ r
+  f32x4 *const part = reinterpret_cast<f32x4 *>(ring);
+  const bool odd = wv.end(p);
 #pragma unroll
-      for (int ww = 0; ww < NW; ++ww) {
-        const float cf = __builtin_amdgcn_exp2f(s_m[ww][row] - mu);
-        ls += s_l[ww][row] * cf;
-        const f32x4 pr = reinterpret_cast<const f32x4 *>(smem + ww * (2 * TT::TILEB))[row * C4 + (c ^ (row & (C4 - 1)))];
+  for (int i = 0; i < NC; ++i) {
+    const int r = i * 16 + l16;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) os[e] += pr[e] * cf;
-      }
-      if (live == 1) {
-        const int t = div_inv((unsigned)r, g_inv), g = r - t * p.G;
-        T *op = (T *)p.o + (int64_t)b * p.o_s[0] + (int64_t)t * p.o_s[1] + (int64_t)(hk * p.G + g) * p.o_s[2];
-        typename VecT<T>::v4 ov;
-        const float inv = ls != 0.f ? 1.f / ls : 0.f; // (NaN stays NaN)
+    for (int tt = 0; tt < W::NT; ++tt) part[r * C4 + ((tt * 4 + u4) ^ (r & (C4 - 1)))] = wv.o[i][tt];
+    if (u4 == 0) s_m[w][r] = wv.top(p, i), s_l[w][r] = wv.l[i];
+  }
+  if (n > 0 && first + (n - 1) * STRIDE + KT > k.L && __any(odd))
+    wv.again(p, k.b, k.hk, ks, vs, eb, first, STRIDE, n, k_end, k.L, g_inv, row0, rows, [&](int i, int q, int d, float x) {
+      const int r = i * 16 + q;
+      reinterpret_cast<float *>(part + r * C4 + ((d / 4) ^ (r & (C4 - 1))))[d % 4] = x;
+    });
+  __syncthreads();
+  for (int idx = tid; idx < ROWS * C4; idx += 64 * NW) {
+    const int q = idx / C4, c = idx % C4, r = row0[0] + q;
+    if (r >= rows) break;
+    float mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
-        *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
-      } else {
-        const int64_t slot = ((int64_t)pair * rows + r) * nsplit + split;
-        *reinterpret_cast<f32x4 *>(ws_o + slot * D + c * 4) = os;
-        if (c == 0) ws_ml[slot * 2] = mx, ws_ml[slot * 2 + 1] = ls;
-      }
+    for (int ww = 0; ww < NW; ++ww) mx = fmaxf(mx, s_m[ww][q]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float ls = 0.f;
+    f32x4 os = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ww = 0; ww < NW; ++ww) {
+      const float cf = __builtin_amdgcn_exp2f(s_m[ww][q] - mu);
+      ls += s_l[ww][q] * cf;
+      const f32x4 pr = reinterpret_cast<const f32x4 *>(smem + ww * (2 * TT::TILEB))[q * C4 + (c ^ (q & (C4 - 1)))];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) os[e] += pr[e] * cf;
+    }
+    if (k.live == 1) {
+      T *op = W::row_of((T *)p.o, p.o_s, p, k.b, k.hk, r, div_inv((unsigned)r, g_inv));
+      typename VecT<T>::v4 ov;
+      const float inv = ls != 0.f ? 1.f / ls : 0.f; // (NaN stays NaN)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
+      *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
+    } else {
+      const int64_t slot = ((int64_t)k.pair * rows + r) * nsplit + k.split;
+      *reinterpret_cast<f32x4 *>(ws_o + slot * D + c * 4) = os;
+      if (c == 0) ws_ml[slot * 2] = mx, ws_ml[slot * 2 + 1] = ls;
     }
   }
 }
 
-// The splits of every row: D / 4 lanes a row.
-template <typename T, int D, int STRIDE>
+// More rows: the four waves share the tiles of the split's keys, each with rows
+// of its own (up to two groups of 16), in a ring of four tiles: one barrier a
+// tile, after which the slot of the tile before last is asked for anew. With
+// waves that stream their own tiles, 264 rows over 32700 e4m3 keys moved 9 times
+// the cache through the L1s and took 122 us where the DMA alone took 44.
+template <typename T, int KIND, int D>
+__global__ __launch_bounds__(256, 2) void tree_rows_kernel(TreeArgs p, float *__restrict__ ws_o,
+                                                           float *__restrict__ ws_ml, int nsplit,
+                                                           unsigned nsplit_inv, unsigned hkv_inv,
+                                                           unsigned g_inv, int by_xcd, int groups) {
+  typedef TreeTile<KIND, D> TT;
+  constexpr int KT = TT::KT, NW = 4, ST = 4, N = TT::TILEB / 1024 / NW, EX = KIND ? 1 : 0, PER = 2 * N + EX;
+  __shared__ __attribute__((aligned(16))) char smem[ST * 2 * TT::TILEB];
+  __shared__ __attribute__((aligned(16))) unsigned s_e[ST][64];
+
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  TreeBlock k = tree_block(p, hkv_inv, by_xcd);
+  const int up = tree_parent(p, k.b);
+  const int rows = p.T * p.G;
+
+  // rows 16 (qt groups + w + 4 i) .. of this wave, i < nc
+  auto run = [&](auto ncc) {
+    constexpr int NC = decltype(ncc)::value;
+    typedef TreeWave<T, KIND, D, NC> W;
+    W wv;
+    int row0[NC], row[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      row0[i] = (k.qt * groups + w + 4 * i) * 16, row[i] = min(row0[i] + (lane & 15), rows - 1);
+    wv.ask(p, k.b, k.hk, g_inv, row);
+    tree_split<KT>(p, nsplit, nsplit_inv, k);
+    if (k.c0 >= k.end) return; // the whole block
+    const int first = (int)k.c0, k_end = (int)k.c1, n = (k_end - first + KT - 1) / KT;
+    const char *ks = (const char *)p.k + ((int64_t)k.b * p.k_s[0] + (int64_t)k.hk * p.k_s[1]) * W::EB;
+    const char *vs = (const char *)p.v + ((int64_t)k.b * p.v_s[0] + (int64_t)k.hk * p.v_s[1]) * W::EB;
+    const int64_t eb = (int64_t)k.b * p.e_s[0] + (int64_t)k.hk * p.e_s[1];
+    TreeDma<KIND, D, N, 0> dk, dv;
+    dk.begin(true, w * N, p.k_s[2]);
+    dv.begin(false, w * N, p.v_s[2]);
+    auto issue = [&](int it) { // (every wave brings the exponents: the same bytes)
+      char *const slot = smem + (it & (ST - 1)) * (2 * TT::TILEB);
+      dk.issue(ks, p.k_s[2], first + it * KT, k.end, slot);
+      if constexpr (KIND != 0) issue_exps(p, eb, first + it * KT, s_e[it & (ST - 1)]);
+      dv.issue(vs, p.v_s[2], first + it * KT, k.end, slot + TT::TILEB);
+    };
+    for (int it = 0; it < ST - 1; ++it)
+      if (it < n) issue(it);
+    wv.begin(tree_bits(p, up, k.L), lds_addr(smem), lds_addr(smem) + TT::TILEB, lds_addr(s_e[0]));
+    for (int it = 0; it < n; ++it) {
+      if (it + 2 < n) vm_wait<2 * PER>(); // this wave's part of tile `it` landed
+      else if (it + 1 < n) vm_wait<PER>();
+      else vm_wait<0>();
+      lds_barrier(); // everybody's part, and everybody is done with tile it - 1
+      if (it + 3 < n) issue(it + 3);
+      wv.step(p, first + it * KT, k.L, (it & (ST - 1)) * (2 * TT::TILEB), (it & (ST - 1)) * 256, [] {}, [] {}, [] {});
+    }
+    const bool odd = wv.end(p);
+    auto put = [&](int i, int q, int d, auto x, float l) { // x: one value or four
+      constexpr int M = sizeof(x) / 4;
+      const int r = row0[i] + q;
+      if (k.live == 1) {
+        T *op = W::row_of((T *)p.o, p.o_s, p, k.b, k.hk, r, div_inv((unsigned)r, g_inv)) + d;
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        if constexpr (M == 4) {
+          typename VecT<T>::v4 ov;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(x[e] * inv);
+          *reinterpret_cast<typename VecT<T>::v4 *>(op) = ov;
+        } else {
+          *op = from_f32<T>(x * inv);
+        }
+      } else {
+        *reinterpret_cast<decltype(x) *>(ws_o + (((int64_t)k.pair * rows + r) * nsplit + k.split) * D + d) = x;
+      }
+    };
+    const bool redo = first + n * KT > k.L && __any(odd);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int q = lane & 15, u4 = lane >> 4;
+      if (row0[i] + q >= rows) continue;
+      if (!redo)
+#pragma unroll
+        for (int tt = 0; tt < W::NT; ++tt) put(i, q, tt * 16 + u4 * 4, wv.o[i][tt], wv.l[i]);
+      if (u4 == 0 && k.live > 1) {
+        const int64_t slot = ((int64_t)k.pair * rows + row0[i] + q) * nsplit + k.split;
+        ws_ml[slot * 2] = wv.top(p, i), ws_ml[slot * 2 + 1] = wv.l[i];
+      }
+    }
+    if (redo)
+      wv.again(p, k.b, k.hk, ks, vs, eb, first, KT, n, k_end, k.L, g_inv, row0, rows,
+               [&](int i, int q, int d, float x) { put(i, q, d, x, __shfl(wv.l[i], q, kWave)); });
+  };
+  // a block's last groups may leave waves with one, or none: those bring their
+  // part of the tiles all the same (as one group, of rows past the last)
+  const int have = min(groups, (rows + 15) / 16 - k.qt * groups);
+  if (w + 4 < have) run(std::integral_constant<int, 2>{});
+  else run(std::integral_constant<int, 1>{});
+}
+
+// The splits of every row, which are runs of batches of 2^lstride keys. Four groups
+// of D / 4 lanes share a row's splits, each 16 splits' loads at once and before the
+// sequence's length has come (slots that no split wrote are read and not used): a
+// chain of length, maxima and sums would be three trips to memory, twice the
+// launch's time.
+template <typename T, int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, const float *__restrict__ ws_o,
                                                          const float *__restrict__ ws_ml, int nsplit,
-                                                         unsigned nsplit_inv, unsigned g_inv) {
-  constexpr int C4 = D / 4, RPB = 256 / C4;
-  const int rows = p.T * p.G, r = blockIdx.x * RPB + threadIdx.x / C4, c = threadIdx.x % C4;
+                                                         unsigned nsplit_inv, unsigned g_inv, int lstride) {
+  constexpr int C4 = D / 4, SG = 4, U = 4, RPB = 256 / (C4 * SG);
+  __shared__ f32x4 s_o[RPB][SG][C4];
+  __shared__ float s_m[RPB][SG], s_l[RPB][SG];
+  const int rb = threadIdx.x / (C4 * SG), sg = threadIdx.x / C4 % SG, c = threadIdx.x % C4;
+  const int rows = p.T * p.G, r = min(blockIdx.x * RPB + rb, rows - 1);
   const int hk = blockIdx.y, b = blockIdx.z;
-  if (r >= rows) return;
-  const int L = min(max(p.seqlens[b], 0), p.Lmax), end = min(L + p.T, p.Lmax);
-  const int nbatch = (int)((unsigned)(end + STRIDE - 1) / (unsigned)STRIDE);
+  const int64_t slot = (((int64_t)b * p.Hkv + hk) * rows + r) * nsplit;
+  const int len = p.seqlens[b];
+  f32x4 pr[U];
+  float m[U], l[U];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int64_t at = slot + min(s0 + j * SG + sg, nsplit - 1);
+      m[j] = ws_ml[at * 2], l[j] = ws_ml[at * 2 + 1];
+      pr[j] = *reinterpret_cast<const f32x4 *>(ws_o + at * D + c * 4);
+    }
+  };
+  load(0);
+  const int L = min(max(len, 0), p.Lmax), end = min(L + p.T, p.Lmax);
+  const int nbatch = (int)(((unsigned)end + (1u << lstride) - 1) >> lstride);
   const int per = div_inv((unsigned)(nbatch + nsplit - 1), nsplit_inv);
   const int live = (int)((unsigned)(nbatch + per - 1) / (unsigned)per);
   if (live == 1) return; // written by the tile kernel
-  const int64_t slot = (((int64_t)b * p.Hkv + hk) * rows + r) * nsplit;
-  float mx = -INFINITY;
-#pragma unroll 8
-  for (int s = 0; s < live; ++s) mx = fmaxf(mx, ws_ml[(slot + s) * 2]);
-  const float mu = mx == -INFINITY ? 0.f : mx;
-  float ls = 0.f;
+  float mx = -INFINITY, ls = 0.f;
   f32x4 os = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = 0; s < live; ++s) {
-    const float cf = __builtin_amdgcn_exp2f(ws_ml[(slot + s) * 2] - mu);
-    ls += ws_ml[(slot + s) * 2 + 1] * cf;
-    const f32x4 pr = *reinterpret_cast<const f32x4 *>(ws_o + (slot + s) * D + c * 4);
+  for (int s0 = 0; s0 < live; s0 += U * SG) {
+    if (s0) load(s0);
+    float mn = mx;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) os[e] += pr[e] * cf;
+    for (int j = 0; j < U; ++j) {
+      if (s0 + j * SG + sg >= live) m[j] = -INFINITY;
+      mn = fmaxf(mn, m[j]);
+    }
+    const float mu = mn == -INFINITY ? 0.f : mn, a = __builtin_amdgcn_exp2f(mx - mu);
+    ls *= a;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) os[e] *= a;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (s0 + j * SG + sg >= live) break; // (what such a slot holds may be anything)
+      const float cf = __builtin_amdgcn_exp2f(m[j] - mu);
+      ls += l[j] * cf;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) os[e] += pr[j][e] * cf;
+    }
+    mx = mn;
+  }
+  s_o[rb][sg][c] = os;
+  if (c == 0) s_m[rb][sg] = mx, s_l[rb][sg] = ls;
+  __syncthreads();
+  if (sg || blockIdx.x * RPB + rb >= rows) return;
+  float mt = mx;
+#pragma unroll
+  for (int g = 1; g < SG; ++g) mt = fmaxf(mt, s_m[rb][g]);
+  const float mu = mt == -INFINITY ? 0.f : mt;
+  ls = 0.f;
+  os = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < SG; ++g) {
+    const float cf = __builtin_amdgcn_exp2f(s_m[rb][g] - mu);
+    ls += s_l[rb][g] * cf;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) os[e] += s_o[rb][g][c][e] * cf;
   }
   const int t = div_inv((unsigned)r, g_inv), g = r - t * p.G;
   T *op = (T *)p.o + (int64_t)b * p.o_s[0] + (int64_t)t * p.o_s[1] + (int64_t)(hk * p.G + g) * p.o_s[2];
@@ -612,20 +880,24 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, const float
   *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
 }
 
-// How a call is cut: query tiles a block, blocks a pair, splits of the keys.
+// How a call is cut: groups of 16 query rows a block (nc: of a wave that shares
+// them with the other three; 0: the waves' own), blocks a pair, splits of the keys
+// in batches of 2^lstride.
 struct TreePlan {
-  int nq, qtiles, nsplit;
+  int nc, groups, qtiles, nsplit, lstride;
 };
 static TreePlan tree_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t Lmax, int code) {
-  TreePlan pl = {0, 0, 0};
+  TreePlan pl = {0, 0, 0, 0, 0};
   if (D != 64 && D != 128) return pl;
-  const int64_t rows = T * (Hq / Hkv);
-  pl.nq = rows > 32 ? 2 : 1;
-  pl.qtiles = (int)((rows + 32 * pl.nq - 1) / (32 * pl.nq));
-  const int kt = D * (code ? 1 : 2) == 256 ? 32 : 64;
-  const int64_t most = (Lmax + 4 * kt - 1) / (4 * kt), blocks = B * Hkv * pl.qtiles;
+  const int64_t groups = (T * (Hq / Hkv) + 15) / 16;
+  pl.nc = groups > 2 ? 0 : (int)groups;
+  pl.qtiles = groups > 2 ? (int)((groups + 7) / 8) : 1;
+  pl.groups = (int)((groups + pl.qtiles - 1) / pl.qtiles);
+  const int lkt = D * (code ? 1 : 2) == 256 ? 5 : 6;
+  pl.lstride = pl.nc ? lkt + 2 : lkt;
+  const int64_t most = (Lmax + (4 << lkt) - 1) >> (lkt + 2), blocks = B * Hkv * pl.qtiles;
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  int64_t ns = (2 * (int64_t)cus + blocks - 1) / blocks;
+  int64_t ns = 2 * (int64_t)cus / blocks; // two blocks a CU are resident
   if (ns > most) ns = most;
   pl.nsplit = (int)(ns > 256 ? 256 : ns < 1 ? 1 : ns);
   return pl;
@@ -681,6 +953,8 @@ extern "C" int tpp_tree_attn(const void *q, const void *k, const void *v, void *
     low_o |= (uint64_t)(a.o_s[i] * 2);
   }
   bool tiles = (D == 64 || D == 128) && !(low & 15) && !(low_o & 7) && B * Hkv <= 65535;
+  // (a tile's rows by 32-bit byte offsets)
+  for (int64_t r : {a.k_s[2], a.v_s[2]}) tiles = tiles && r >= 0 && r < (1 << 23);
   if (code)
     tiles = tiles && Lmax % 4 == 0 &&
             !(((uint64_t)(uintptr_t)k_exps | (uint64_t)(uintptr_t)v_exps | (uint64_t)a.e_s[0] | (uint64_t)a.e_s[1]) & 3);
@@ -705,25 +979,25 @@ extern "C" int tpp_tree_attn(const void *q, const void *k, const void *v, void *
   const dim3 grid(by_xcd ? 8 * pl.qtiles : pl.qtiles, pl.nsplit, (unsigned)(by_xcd ? pairs / 8 : pairs));
   const unsigned ninv = inv_of(pl.nsplit), hinv = inv_of((int)Hkv), ginv = inv_of(a.G);
   return TPP_DISPATCH_HALF(dtype, [&] {
-    auto go = [&](auto kd, auto dd, auto nn) {
-      constexpr int KIND = decltype(kd)::value, DD = decltype(dd)::value, NQ = decltype(nn)::value;
-      tree_tile_kernel<T, KIND, DD, NQ><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd);
+    auto by_d = [&](auto kd, auto dd) {
+      constexpr int KIND = decltype(kd)::value, DD = decltype(dd)::value;
+      if (pl.nc == 0)
+        tree_rows_kernel<T, KIND, DD><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, pl.groups);
+      else if (pl.nc == 1)
+        tree_tile_kernel<T, KIND, DD, 1><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd);
+      else
+        tree_tile_kernel<T, KIND, DD, 2><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd);
       if (pl.nsplit > 1)
-        tree_merge_kernel<T, DD, 4 * TreeTile<KIND, DD>::KT>
-              <<<dim3((unsigned)((rows + 1024 / DD - 1) / (1024 / DD)), (unsigned)Hkv, (unsigned)B), dim3(256), 0, st>>>(
-                  a, ws_o, ws_ml, pl.nsplit, ninv, ginv);
+        tree_merge_kernel<T, DD><<<dim3((unsigned)((rows + 256 / DD - 1) / (256 / DD)), (unsigned)Hkv, (unsigned)B), dim3(256), 0, st>>>(
+            a, ws_o, ws_ml, pl.nsplit, ninv, ginv, pl.lstride);
     };
-    auto by_q = [&](auto kd, auto dd) {
-      if (pl.nq == 1) go(kd, dd, std::integral_constant<int, 1>{});
-      else go(kd, dd, std::integral_constant<int, 2>{});
+    auto by_kind = [&](auto kd) {
+      if (D == 64) by_d(kd, std::integral_constant<int, 64>{});
+      else by_d(kd, std::integral_constant<int, 128>{});
     };
-    auto by_d = [&](auto kd) {
-      if (D == 64) by_q(kd, std::integral_constant<int, 64>{});
-      else by_q(kd, std::integral_constant<int, 128>{});
-    };
-    if (code == 0) by_d(std::integral_constant<int, 0>{});
-    else if (code == TPP_CODE_E4M3) by_d(std::integral_constant<int, TPP_CODE_E4M3>{});
-    else by_d(std::integral_constant<int, TPP_CODE_INT8>{});
+    if (code == 0) by_kind(std::integral_constant<int, 0>{});
+    else if (code == TPP_CODE_E4M3) by_kind(std::integral_constant<int, TPP_CODE_E4M3>{});
+    else by_kind(std::integral_constant<int, TPP_CODE_INT8>{});
     return check_launch(name);
   });
 }
