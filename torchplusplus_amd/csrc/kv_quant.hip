@@ -51,48 +51,60 @@ template <int CODE> __device__ __forceinline__ int row_exponent(unsigned u) {
   return max(e, 1);
 }
 
-// D / 8 lanes a row, 8 elements (16 bytes in, 8 out) a lane.
-template <typename T, int CODE, int D>
+// D / 8 lanes a row, 8 elements (16 bytes in, 8 out) a lane, U rows a thread: their
+// loads before the first use. Rows run over a head's tokens, so that a block writes
+// one run of codes.
+template <typename T, int CODE, int D, int U>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs p) {
   typedef typename VecT<T>::v8 V8;
-  constexpr int LPR = D / 8;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  constexpr int LPR = D / 8, RPP = 256 / LPR; // rows of a pass
   const int c = threadIdx.x % LPR, w = blockIdx.y;
-  if (row >= p.rows) return;
-  const int64_t bs = row / p.H;
-  const int h = (int)(row - bs * p.H);
-  const int64_t b = bs / p.S, s = bs - b * p.S;
-  const int64_t pos = (p.positions ? (int64_t)p.positions[b] : p.start) + s;
-  if (pos < 0 || pos >= p.Lmax || (p.counts && s >= p.counts[b])) return; // whole rows of lanes
-  const T *src = (const T *)p.x[w] + b * p.xs[w][0] + s * p.xs[w][1] + h * p.xs[w][2] + c * 8;
-  const V8 t = ld_nt(reinterpret_cast<const V8 *>(src));
-  float x[8];
-  unsigned u = 0;
+  const int64_t row0 = (int64_t)blockIdx.x * (RPP * U) + threadIdx.x / LPR;
+  V8 t[U];
+  bool put[U];
+  int64_t pos[U], bb[U];
+  int hh[U];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = to_f32(t[j]);
-    u = max(u, __float_as_uint(x[j]) & 0x7fffffffu);
+  for (int i = 0; i < U; ++i) {
+    const int64_t row = row0 + i * RPP < p.rows ? row0 + i * RPP : p.rows - 1;
+    const int64_t bh = row / p.S, s = row - bh * p.S, b = bh / p.H;
+    const int h = (int)(bh - b * p.H);
+    t[i] = ld_nt(reinterpret_cast<const V8 *>((const T *)p.x[w] + b * p.xs[w][0] + s * p.xs[w][1] + h * p.xs[w][2] + c * 8));
+    pos[i] = (p.positions ? (int64_t)p.positions[b] : p.start) + s;
+    put[i] = row0 + i * RPP < p.rows && pos[i] >= 0 && pos[i] < p.Lmax && !(p.counts && s >= p.counts[b]);
+    bb[i] = b, hh[i] = h;
   }
-  const int e = row_exponent<CODE>(group_umax<LPR>(u));
-  // times 2^(127 - e): exact, or below half the least code
-  const float inv = e == 255 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23);
-  u32x2 out = {0u, 0u};
-  if (e != 255) {
-    if constexpr (CODE == TPP_CODE_E4M3) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        int v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * inv, x[4 * j + 1] * inv, 0, false);
-        out[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * inv, x[4 * j + 3] * inv, v, true);
-      }
-    } else {
+  for (int i = 0; i < U; ++i) {
+    float x[8];
+    unsigned u = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        out[j / 4] |= ((unsigned)(int)__builtin_rintf(x[j] * inv) & 0xffu) << (8 * (j % 4));
+    for (int j = 0; j < 8; ++j) {
+      x[j] = to_f32(t[i][j]);
+      u = max(u, __float_as_uint(x[j]) & 0x7fffffffu);
     }
+    const int e = row_exponent<CODE>(group_umax<LPR>(u));
+    // times 2^(127 - e): exact, or below half the least code
+    const float inv = e == 255 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23);
+    u32x2 out = {0u, 0u};
+    if (e != 255) {
+      if constexpr (CODE == TPP_CODE_E4M3) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          int v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * inv, x[4 * j + 1] * inv, 0, false);
+          out[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * inv, x[4 * j + 3] * inv, v, true);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          out[j / 4] |= ((unsigned)(int)__builtin_rintf(x[j] * inv) & 0xffu) << (8 * (j % 4));
+      }
+    }
+    if (!put[i]) continue; // (whole rows of lanes)
+    uint8_t *dst = (uint8_t *)p.codes[w] + bb[i] * p.cs[0] + hh[i] * p.cs[1] + pos[i] * D + c * 8;
+    *reinterpret_cast<u32x2 *>(dst) = out;
+    if (c == 0) p.exps[w][bb[i] * p.es[0] + hh[i] * p.es[1] + pos[i]] = (uint8_t)e;
   }
-  uint8_t *dst = (uint8_t *)p.codes[w] + b * p.cs[0] + h * p.cs[1] + pos * D + c * 8;
-  *reinterpret_cast<u32x2 *>(dst) = out;
-  if (c == 0) p.exps[w][b * p.es[0] + h * p.es[1] + pos] = (uint8_t)e;
 }
 
 struct KvReadArgs {
@@ -105,40 +117,45 @@ struct KvReadArgs {
   int H;
 };
 
-template <typename T, int CODE, int D>
+template <typename T, int CODE, int D, int U>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs p) {
   constexpr int LPR = D / 8;
   const int w = blockIdx.y;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= p.chunks) return;
-  const int64_t row = id / LPR;
-  const int c = (int)(id % LPR);
-  const int64_t bh = row / p.len, pos = row - bh * p.len;
-  const int64_t b = bh / p.H, h = bh - b * p.H;
-  const uint8_t *src = (const uint8_t *)p.codes[w] + b * p.cs[0] + h * p.cs[1] + pos * D + c * 8;
-  const u32x2 t = *reinterpret_cast<const u32x2 *>(src);
-  const int e = p.exps[w][b * p.es[0] + h * p.es[1] + pos];
-  // 2^(e - 127); e = 255 is a NaN (bits of a NaN: exponent field 255, mantissa not 0)
-  const float sc = __uint_as_float(e == 255 ? 0x7fc00000u : (unsigned)e << 23);
-  float v[8];
-  if constexpr (CODE == TPP_CODE_E4M3) {
+  const int64_t id0 = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+  u32x2 t[U];
+  int e[U];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)t[j], false);
-      const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)t[j], true);
-      v[4 * j] = lo[0], v[4 * j + 1] = lo[1], v[4 * j + 2] = hi[0], v[4 * j + 3] = hi[1];
+  for (int i = 0; i < U; ++i) {
+    const int64_t id = id0 + i * 256 < p.chunks ? id0 + i * 256 : p.chunks - 1;
+    const int64_t row = id / LPR, bh = row / p.len, pos = row - bh * p.len, b = bh / p.H, h = bh - b * p.H;
+    t[i] = ld_nt(reinterpret_cast<const u32x2 *>((const uint8_t *)p.codes[w] + b * p.cs[0] + h * p.cs[1] + pos * D +
+                                                 (id % LPR) * 8));
+    e[i] = p.exps[w][b * p.es[0] + h * p.es[1] + pos];
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    // 2^(e - 127); e = 255 is a NaN (bits of a NaN: exponent field 255, mantissa not 0)
+    const float sc = __uint_as_float(e[i] == 255 ? 0x7fc00000u : (unsigned)e[i] << 23);
+    float v[8];
+    if constexpr (CODE == TPP_CODE_E4M3) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)t[i][j], false);
+        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)t[i][j], true);
+        v[4 * j] = lo[0], v[4 * j + 1] = lo[1], v[4 * j + 2] = hi[0], v[4 * j + 3] = hi[1];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)(t[i][j / 4] >> (8 * (j % 4)));
     }
-  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)(t[j / 4] >> (8 * (j % 4)));
+    for (int j = 0; j < 8; ++j) {
+      v[j] *= sc;
+      // a code rounded up from the largest fp16 may stand for 65536
+      if constexpr (__is_same(T, f16)) v[j] = v[j] != v[j] ? v[j] : fminf(fmaxf(v[j], -65504.f), 65504.f);
+    }
+    if (id0 + i * 256 < p.chunks) store8((T *)p.out[w] + (id0 + i * 256) * 8, v);
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    v[j] *= sc;
-    // a code rounded up from the largest fp16 may stand for 65536
-    if constexpr (__is_same(T, f16)) v[j] = v[j] != v[j] ? v[j] : fminf(fmaxf(v[j], -65504.f), 65504.f);
-  }
-  store8((T *)p.out[w] + id * 8, v);
 }
 
 static int check_codes(const char *name, const void *kc, const void *vc, const void *ke,
@@ -188,13 +205,16 @@ extern "C" int tpp_kv_quant_append(const void *k, const void *v, const int64_t *
   for (int i = 0; i < 2; ++i) a.cs[i] = code_strides[i], a.es[i] = exp_strides[i];
   a.positions = positions, a.counts = counts, a.start = start, a.S = S, a.H = (int)H, a.Lmax = (int)Lmax;
   a.rows = B * S * H;
-  const int64_t per = 256 / (D / 8), blocks = (a.rows + per - 1) / per;
+  // four rows a thread where that still fills the card (2048 threads a CU)
+  const bool four = a.rows * (D / 8) * 2 >= 4LL * 2048 * 256;
+  const int64_t per = 256 / (D / 8) * (four ? 4 : 1), blocks = (a.rows + per - 1) / per;
   if (blocks > 0x7fffffffLL) return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
   hipStream_t st = as_stream(stream);
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto cd, auto dd) {
-      kv_append_kernel<T, decltype(cd)::value, decltype(dd)::value>
-          <<<dim3((unsigned)blocks, 2), dim3(256), 0, st>>>(a);
+      const dim3 grid((unsigned)blocks, 2);
+      if (four) kv_append_kernel<T, decltype(cd)::value, decltype(dd)::value, 4><<<grid, dim3(256), 0, st>>>(a);
+      else kv_append_kernel<T, decltype(cd)::value, decltype(dd)::value, 1><<<grid, dim3(256), 0, st>>>(a);
     };
     auto by_d = [&](auto cd) {
       if (D == 64) go(cd, std::integral_constant<int, 64>{});
@@ -225,13 +245,16 @@ extern "C" int tpp_kv_quant_read(const void *k_codes, const void *v_codes, const
   for (int i = 0; i < 2; ++i) a.cs[i] = code_strides[i], a.es[i] = exp_strides[i];
   a.out[0] = k_out, a.out[1] = v_out, a.len = len, a.H = (int)H;
   a.chunks = B * H * len * (D / 8);
-  const int64_t blocks = (a.chunks + 255) / 256;
+  // four chunks of 8 a thread where that still fills the card
+  const bool four = a.chunks * 2 >= 4LL * 2048 * 256;
+  const int64_t per = four ? 1024 : 256, blocks = (a.chunks + per - 1) / per;
   if (blocks > 0x7fffffffLL) return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
   hipStream_t st = as_stream(stream);
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto cd, auto dd) {
-      kv_read_kernel<T, decltype(cd)::value, decltype(dd)::value>
-          <<<dim3((unsigned)blocks, 2), dim3(256), 0, st>>>(a);
+      const dim3 grid((unsigned)blocks, 2);
+      if (four) kv_read_kernel<T, decltype(cd)::value, decltype(dd)::value, 4><<<grid, dim3(256), 0, st>>>(a);
+      else kv_read_kernel<T, decltype(cd)::value, decltype(dd)::value, 1><<<grid, dim3(256), 0, st>>>(a);
     };
     auto by_d = [&](auto cd) {
       if (D == 64) go(cd, std::integral_constant<int, 64>{});

@@ -34,7 +34,7 @@ struct RopeAtArgs {
   int64_t units; // B * S * hgroups * upt
 };
 
-template <typename T, int PW, bool IL>
+template <typename T, int PW, bool IL, int U>
 __global__ __launch_bounds__(256) void rope_at_kernel(RopeAtArgs p) {
   typedef uint16_t W __attribute__((ext_vector_type(PW))); // PW elements
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -63,35 +63,46 @@ __global__ __launch_bounds__(256) void rope_at_kernel(RopeAtArgs p) {
     }
   }
   const int H = p.Hq + p.Hk, h0 = hg * p.hpt, h1 = min(h0 + p.hpt, H);
-  for (int h = h0; h < h1; ++h) {
-    const bool isq = h < p.Hq;
-    const int hh = isq ? h : h - p.Hq;
-    const int64_t *is = isq ? p.qs : p.ks, *os = isq ? p.qos : p.kos;
-    const T *src = (const T *)(isq ? p.q : p.k) + b * is[0] + s * is[1] + hh * is[2];
-    T *dst = (T *)(isq ? p.qo : p.ko) + b * os[0] + s * os[1] + hh * os[2];
-    W x = *reinterpret_cast<const W *>(src + lo), y = *reinterpret_cast<const W *>(src + hi);
-    if (turn) {
-      float v[2 * PW];
+  for (int h = h0; h < h1; h += U) { // U heads' loads before the first use
+    const T *src[U];
+    T *dst[U];
+    W x[U], y[U];
 #pragma unroll
-      for (int j = 0; j < PW; ++j) {
-        v[j] = to_f32(__builtin_bit_cast(T, (uint16_t)x[j]));
-        v[PW + j] = to_f32(__builtin_bit_cast(T, (uint16_t)y[j]));
-      }
-#pragma unroll
-      for (int j = 0; j < PW; ++j) {
-        const int ia = IL ? 2 * j : j, ib = IL ? 2 * j + 1 : PW + j;
-        const float a = v[ia], bb = v[ib];
-        v[ia] = a * c[j] - bb * sn[j];
-        v[ib] = bb * c[j] + a * sn[j];
-      }
-#pragma unroll
-      for (int j = 0; j < PW; ++j) {
-        x[j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[j]));
-        y[j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[PW + j]));
-      }
+    for (int i = 0; i < U; ++i) {
+      const int hc = min(h + i, h1 - 1); // (past the last: the last again, not stored)
+      const bool isq = hc < p.Hq;
+      const int hh = isq ? hc : hc - p.Hq;
+      const int64_t *is = isq ? p.qs : p.ks, *os = isq ? p.qos : p.kos;
+      src[i] = (const T *)(isq ? p.q : p.k) + b * is[0] + s * is[1] + hh * is[2];
+      dst[i] = (T *)(isq ? p.qo : p.ko) + b * os[0] + s * os[1] + hh * os[2];
+      x[i] = ld_nt(reinterpret_cast<const W *>(src[i] + lo)), y[i] = ld_nt(reinterpret_cast<const W *>(src[i] + hi));
     }
-    *reinterpret_cast<W *>(dst + lo) = x;
-    *reinterpret_cast<W *>(dst + hi) = y;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (i && h + i >= h1) break;
+      if (turn) {
+        float v[2 * PW];
+#pragma unroll
+        for (int j = 0; j < PW; ++j) {
+          v[j] = to_f32(__builtin_bit_cast(T, (uint16_t)x[i][j]));
+          v[PW + j] = to_f32(__builtin_bit_cast(T, (uint16_t)y[i][j]));
+        }
+#pragma unroll
+        for (int j = 0; j < PW; ++j) {
+          const int ia = IL ? 2 * j : j, ib = IL ? 2 * j + 1 : PW + j;
+          const float a = v[ia], bb = v[ib];
+          v[ia] = a * c[j] - bb * sn[j];
+          v[ib] = bb * c[j] + a * sn[j];
+        }
+#pragma unroll
+        for (int j = 0; j < PW; ++j) {
+          x[i][j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[j]));
+          y[i][j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[PW + j]));
+        }
+      }
+      *reinterpret_cast<W *>(dst[i] + lo) = x[i];
+      *reinterpret_cast<W *>(dst[i] + hi) = y[i];
+    }
   }
 }
 
@@ -136,7 +147,8 @@ extern "C" int tpp_rope_at(const void *q, const void *k, void *q_out, void *k_ou
   a.S = (int)S, a.Hq = (int)Hq, a.Hk = (int)Hk, a.D = (int)D, a.R = (int)R;
   a.upt = (int)(D / (2 * pw));
   const int H = (int)(Hq + Hk);
-  a.hpt = 1;
+  // threads of four heads where they still fill the card (2048 a CU), else of one
+  a.hpt = B * S * ((H + 3) / 4) * a.upt >= 2048 * 256 ? 4 : 1;
   a.hgroups = (H + a.hpt - 1) / a.hpt;
   a.units = B * S * a.hgroups * a.upt;
   const int64_t blocks = (a.units + 255) / 256;
@@ -145,8 +157,15 @@ extern "C" int tpp_rope_at(const void *q, const void *k, void *q_out, void *k_ou
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto w) {
       constexpr int PW = decltype(w)::value;
-      if (interleaved) rope_at_kernel<T, PW, true><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(a);
-      else rope_at_kernel<T, PW, false><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(a);
+      const dim3 grid((unsigned)blocks), block(256);
+      if (a.hpt == 4) {
+        if (interleaved) rope_at_kernel<T, PW, true, 4><<<grid, block, 0, st>>>(a);
+        else rope_at_kernel<T, PW, false, 4><<<grid, block, 0, st>>>(a);
+      } else if (interleaved) {
+        rope_at_kernel<T, PW, true, 1><<<grid, block, 0, st>>>(a);
+      } else {
+        rope_at_kernel<T, PW, false, 1><<<grid, block, 0, st>>>(a);
+      }
     };
     if (pw == 8) go(std::integral_constant<int, 8>{});
     else if (pw == 4) go(std::integral_constant<int, 4>{});

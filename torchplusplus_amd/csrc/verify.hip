@@ -22,12 +22,13 @@
 // 150000 tokens at one draw in a few hundred, so the token would depend on the
 // order of the sum.
 //
-// Two launches. The first cuts the row that the walk ends at into chunks of
-// 4096 masses and sums each (every block repeats the walk: a gather of one
-// mass per drafted token, all at once, then a walk in registers; cheaper than
-// a launch of its own). The second finds the chunk and the index. What bounds
-// it: the latency of both launches and the dependent gathers; the rows are
-// B V 4 bytes (with q twice that).
+// Two launches. The first cuts the row that the walk ends at into chunks of 4096
+// masses and sums each; the second finds the chunk and the index. Every wave of the
+// first repeats the walk (one gather of a mass per drafted token, all at once, then
+// a walk in registers): cheaper than a launch of its own, or a barrier. Every wave
+// of the second scans the chunks' sums. What bounds it: the latency of two launches
+// and of four dependent trips to memory in each; the rows are B V 4 bytes (with q
+// twice that).
 #include "tpp_common.hpp"
 
 namespace tpp {
@@ -67,14 +68,14 @@ __device__ __forceinline__ double readlane_f64(double v, int lane) {
 
 // The walk, by one whole wave (lane i = drafted token i).
 template <typename P>
-__device__ VerState ver_walk(const VerArgs &a, int64_t b, bool write) {
+__device__ __forceinline__ VerState ver_walk(const VerArgs &a, int64_t b, bool write, int &tok) {
   const int lane = lane_id(), T = a.T;
   const bool in = lane < T;
   const int64_t t64 = in ? a.tok[b * T + lane] : -1;
   int par = in ? (a.parents ? a.parents[b * T + lane] : lane - 1) : -3;
   if (par < -1 || par >= lane) par = -3; // padding: no node's child
   const bool valid = in && par != -3 && t64 >= 0 && t64 < a.V;
-  const int tok = valid ? (int)t64 : -1;
+  tok = valid ? (int)t64 : -1;
   const float u = in ? a.u[b * (T + 1) + lane] : 0.f;
   double pm = 0.0, qm = 0.0;
   if (valid) {
@@ -92,24 +93,24 @@ __device__ VerState ver_walk(const VerArgs &a, int64_t b, bool write) {
     st.children = 0;
     if (write && in) a.path[b * T + lane] = lane < n ? lane : -1;
   } else {
-    // mass of earlier siblings; a token that one of them has counts as none
-    double below = 0.0;
-    bool dup = !valid;
-    for (int j = 0; j < T; ++j) {
-      const int pj = __builtin_amdgcn_readlane(par, j), tj = __builtin_amdgcn_readlane(tok, j);
-      const double mj = readlane_f64(dup ? 0.0 : pm, j);
-      if (j < lane && pj == par) {
-        below += mj;
-        dup |= tj == tok;
-      }
-    }
+    // down from the context: the node's children in order, `below` the mass of
+    // those passed; a token that an earlier sibling has counts as none
     int cur = -1, mine = -1;
     while (n < T) {
+      const unsigned long long kids = __ballot(valid && par == cur);
       const double ud = (double)readlane_f32(u, n);
-      const unsigned long long hit = __ballot(!dup && par == cur && below <= ud && ud < below + pm);
-      if (!hit) break;
-      cur = __builtin_ctzll(hit);
-      if (lane == n) mine = cur;
+      double below = 0.0;
+      int hit = -1;
+      for (unsigned long long c = kids; c && hit < 0; c &= c - 1) {
+        const int j = __builtin_ctzll(c);
+        if (__ballot(tok == __builtin_amdgcn_readlane(tok, j)) & kids & ((1ull << j) - 1)) continue;
+        const double up = below + readlane_f64(pm, j);
+        if (below <= ud && ud < up) hit = j;
+        below = up;
+      }
+      if (hit < 0) break;
+      if (lane == n) mine = hit;
+      cur = hit;
       ++n;
     }
     st.row = cur + 1;
@@ -124,24 +125,63 @@ __device__ VerState ver_walk(const VerArgs &a, int64_t b, bool write) {
   return st;
 }
 
-// Bits of a chunk's masses that are children of the node (one per token).
-__device__ __forceinline__ void mark_children(const VerArgs &a, int64_t b, const VerState &st,
-                                              int64_t base, unsigned *ex) {
-  for (int i = threadIdx.x; i < kVerChunk / 32; i += blockDim.x) ex[i] = 0;
-  __syncthreads();
-  if (threadIdx.x < a.T && ((st.children >> threadIdx.x) & 1)) {
-    const int64_t t = a.tok[b * a.T + threadIdx.x] - base;
-    if (t >= 0 && t < kVerChunk) atomicOr(&ex[t / 32], 1u << (t % 32));
-  }
-  __syncthreads();
-}
+constexpr int kVerEach = kVerChunk / 256; // masses of a thread
 
-// weights of index base + i (i in the chunk): of the draw, and of the row
-template <typename P>
-__device__ __forceinline__ void weights(const P *p, const P *q, int i, const unsigned *ex, double &w,
-                                        double &full) {
-  full = mass(to_f32(p[i]));
-  w = q ? fmax(full - mass(to_f32(q[i])), 0.0) : ((ex[i / 32] >> (i % 32)) & 1) ? 0.0 : full;
+// A thread's masses of a chunk of n: i-th at place(i). Unconditional loads from
+// clamped places, all before the first use; VEC: 16 bytes at a time.
+template <bool RUNS> __device__ __forceinline__ int ver_place(int i, int per) {
+  // RUNS: a thread's masses are neighbours; else 256 threads' runs of `per` are
+  return RUNS ? threadIdx.x * kVerEach + i : (i / per * 256 + threadIdx.x) * per + i % per;
+}
+template <typename P, bool RUNS, bool VEC>
+__device__ __forceinline__ void ver_load(const P *row, int n, float (&x)[kVerEach]) {
+  constexpr int PER = VEC ? 16 / sizeof(P) : 1;
+  typedef P V __attribute__((ext_vector_type(PER)));
+#pragma unroll
+  for (int i = 0; i < kVerEach; i += PER) {
+    const int at = ver_place<RUNS>(i, PER);
+    if constexpr (PER == 1) {
+      x[i] = to_f32(row[min(at, n - 1)]);
+    } else { // n is a multiple of PER
+      const V v = *reinterpret_cast<const V *>(row + min(at, n - PER));
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[i + e] = to_f32(v[e]);
+    }
+    if (at >= n)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[i + e] = 0.f;
+  }
+}
+// Weights of the draw w and masses of the row f of a thread's part of a chunk.
+template <typename P, bool RUNS, bool VEC>
+__device__ __forceinline__ void ver_weights(const VerArgs &a, int64_t b, const VerState &st, int tok, int64_t base,
+                                            double (&w)[kVerEach], double (&f)[kVerEach]) {
+  const int n = (int)min((int64_t)kVerChunk, a.V - base);
+  float x[kVerEach], y[kVerEach];
+  ver_load<P, RUNS, VEC>((const P *)a.p + b * a.p_sb + (int64_t)st.row * a.p_st + base, n, x);
+  if (st.rejected) ver_load<P, RUNS, VEC>((const P *)a.q + b * a.q_sb + (int64_t)st.row * a.q_st + base, n, y);
+#pragma unroll
+  for (int i = 0; i < kVerEach; ++i) {
+    f[i] = mass(x[i]);
+    w[i] = st.rejected ? fmax(f[i] - mass(y[i]), 0.0) : f[i];
+  }
+  for (unsigned long long c = st.children; c; c &= c - 1) {
+    const int64_t at = (int64_t)__builtin_amdgcn_readlane(tok, __builtin_ctzll(c)) - base;
+    if (at < 0 || at >= kVerChunk) continue;
+#pragma unroll
+    for (int i = 0; i < kVerEach; ++i)
+      if (ver_place<RUNS>(i, VEC ? 16 / sizeof(P) : 1) == at) w[i] = 0.0;
+  }
+}
+__device__ __forceinline__ double tree_sum(const double (&v)[kVerEach]) {
+  double t[kVerEach / 2];
+#pragma unroll
+  for (int i = 0; i < kVerEach / 2; ++i) t[i] = v[2 * i] + v[2 * i + 1];
+#pragma unroll
+  for (int m = kVerEach / 4; m > 0; m /= 2)
+#pragma unroll
+    for (int i = 0; i < m; ++i) t[i] = t[2 * i] + t[2 * i + 1];
+  return t[0];
 }
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
@@ -150,31 +190,15 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   return v;
 }
 
-template <typename P> __global__ __launch_bounds__(256) void ver_sum_kernel(VerArgs a) {
-  __shared__ unsigned ex[kVerChunk / 32];
+template <typename P, bool VEC> __global__ __launch_bounds__(256) void ver_sum_kernel(VerArgs a) {
   __shared__ double red[4][2];
-  __shared__ VerState s_st;
   const int64_t b = blockIdx.y;
-  if (wave_id() == 0) {
-    const VerState st = ver_walk<P>(a, b, blockIdx.x == 0);
-    if (threadIdx.x == 0) s_st = st;
-  }
-  __syncthreads();
-  const VerState st = s_st;
-  const int64_t base = (int64_t)blockIdx.x * kVerChunk;
-  const int n = (int)min((int64_t)kVerChunk, a.V - base);
-  mark_children(a, b, st, base, ex);
-  const P *p = (const P *)a.p + b * a.p_sb + (int64_t)st.row * a.p_st + base;
-  const P *q = st.rejected ? (const P *)a.q + b * a.q_sb + (int64_t)st.row * a.q_st + base : nullptr;
-  double w = 0.0, f = 0.0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < n; i += 256) {
-    double wi, fi;
-    weights(p, q, i, ex, wi, fi);
-    w += wi, f += fi;
-  }
-  w = wave_sum_f64(w), f = wave_sum_f64(f);
-  if (lane_id() == 0) red[wave_id()][0] = w, red[wave_id()][1] = f;
+  int tok;
+  const VerState st = ver_walk<P>(a, b, blockIdx.x == 0 && threadIdx.x < kWave, tok);
+  double w[kVerEach], f[kVerEach];
+  ver_weights<P, false, VEC>(a, b, st, tok, (int64_t)blockIdx.x * kVerChunk, w, f);
+  const double ws = wave_sum_f64(tree_sum(w)), fs = wave_sum_f64(tree_sum(f));
+  if (lane_id() == 0) red[wave_id()][0] = ws, red[wave_id()][1] = fs;
   __syncthreads();
   if (threadIdx.x < 2)
     a.part[(b * a.chunks + blockIdx.x) * 2 + threadIdx.x] =
@@ -192,86 +216,79 @@ __device__ __forceinline__ double wave_scan_f64(double v) {
   return v;
 }
 
-template <typename P> __global__ __launch_bounds__(1024) void ver_pick_kernel(VerArgs a) {
-  __shared__ unsigned ex[kVerChunk / 32];
-  __shared__ double s_wave[16], s_before, s_thr;
-  __shared__ int s_chunk, s_which, s_found, s_last;
+template <typename P, bool VEC> __global__ __launch_bounds__(256) void ver_pick_kernel(VerArgs a) {
+  __shared__ double s_wave[4];
+  __shared__ int s_found[4], s_last[4];
   const int64_t b = blockIdx.x;
+  const int lane = lane_id();
   const VerState st = a.state[b];
+  const int tok = lane < a.T ? (int)a.tok[b * a.T + lane] : -1;
+  const double u = fmax((double)a.u[b * (a.T + 1) + a.T], 0.0);
   const double *part = a.part + b * a.chunks * 2;
-  if (wave_id() == 0) {
-    const int lane = lane_id();
+  // 64 chunks at a time: the running sums of the draw's weights (which 0), or,
+  // where those have none, of the whole row (1), to the end, then to the chunk
+  int chunk = -1, which = 0;
+  double before = 0.0, thr = 0.0;
+  for (; which < 2 && chunk < 0; ++which) {
     double total = 0.0;
-    int which = 0;
-    for (; which < 2; ++which) { // the draw's weights, else the whole row
-      total = 0.0;
-      for (int c = 0; c < a.chunks; c += kWave) {
-        const double v = wave_scan_f64(c + lane < a.chunks ? part[(c + lane) * 2 + which] : 0.0);
-        total += __shfl(v, kWave - 1, kWave);
+    for (int c = 0; c < a.chunks; c += kWave)
+      total += __shfl(wave_scan_f64(c + lane < a.chunks ? part[(c + lane) * 2 + which] : 0.0), kWave - 1, kWave);
+    if (!(total > 0.0)) continue;
+    thr = u * total;
+    double carry = 0.0;
+    for (int c = 0; c < a.chunks; c += kWave) {
+      const double own = c + lane < a.chunks ? part[(c + lane) * 2 + which] : 0.0;
+      const double v = wave_scan_f64(own);
+      const unsigned long long hit = __ballot(carry + v > thr && own > 0.0), pos = __ballot(own > 0.0);
+      if (hit || pos) { // else, so far, the last chunk with mass
+        const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(pos);
+        chunk = c + l, before = carry + (__shfl(v, l, kWave) - __shfl(own, l, kWave));
       }
-      if (total > 0.0) break;
+      if (hit) break;
+      carry += __shfl(v, kWave - 1, kWave);
     }
-    const float u = a.u[b * (a.T + 1) + a.T];
-    const double thr = fmax((double)u, 0.0) * total;
-    int chunk = -1;
-    double before = 0.0;
-    if (which < 2) {
-      double carry = 0.0;
-      int lastpos = -1; // the last chunk with mass
-      double lastbefore = 0.0;
-      for (int c = 0; c < a.chunks && chunk < 0; c += kWave) {
-        const double own = c + lane < a.chunks ? part[(c + lane) * 2 + which] : 0.0;
-        const double v = wave_scan_f64(own);
-        const unsigned long long hit = __ballot(carry + v > thr && own > 0.0), pos = __ballot(own > 0.0);
-        const int l = hit ? __builtin_ctzll(hit) : pos ? 63 - __builtin_clzll(pos) : 0;
-        const double bf = carry + __shfl(v, l, kWave) - __shfl(own, l, kWave);
-        if (hit) chunk = c + l, before = bf;
-        else if (pos) lastpos = c + l, lastbefore = bf;
-        carry += __shfl(v, kWave - 1, kWave);
-      }
-      if (chunk < 0) chunk = lastpos, before = lastbefore;
-    }
-    if (lane == 0) s_chunk = chunk, s_which = which, s_before = before, s_thr = thr, s_found = 0x7fffffff, s_last = -1;
+    if (chunk >= 0) break;
   }
-  __syncthreads();
-  const int chunk = s_chunk, which = s_which;
-  if (chunk < 0) {
+  if (chunk < 0) { // (every wave)
     if (threadIdx.x == 0) a.next[b] = -1;
     return;
   }
+  chunk = __builtin_amdgcn_readfirstlane(chunk);
   const int64_t base = (int64_t)chunk * kVerChunk;
-  const int n = (int)min((int64_t)kVerChunk, a.V - base);
-  mark_children(a, b, st, base, ex);
-  const P *p = (const P *)a.p + b * a.p_sb + (int64_t)st.row * a.p_st + base;
-  const P *q = st.rejected ? (const P *)a.q + b * a.q_sb + (int64_t)st.row * a.q_st + base : nullptr;
-  double w[4], sum = 0.0;
+  double w[kVerEach], f[kVerEach];
+  ver_weights<P, true, VEC>(a, b, st, tok, base, w, f);
+  double sum = 0.0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = threadIdx.x * 4 + j;
-    double x = 0.0, f = 0.0;
-    if (i < n) weights(p, q, i, ex, x, f);
-    w[j] = which ? f : x;
-    sum += w[j];
+  for (int i = 0; i < kVerEach; ++i) {
+    w[i] = which ? f[i] : w[i];
+    sum += w[i];
   }
   const double incl = wave_scan_f64(sum);
-  if (lane_id() == kWave - 1) s_wave[wave_id()] = incl;
+  if (lane == kWave - 1) s_wave[wave_id()] = incl;
   __syncthreads();
-  double run = s_before;
+  double run = before;
   for (int i = 0; i < wave_id(); ++i) run += s_wave[i];
   run += incl - sum;
   int found = 0x7fffffff, last = -1;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    run += w[j];
-    if (w[j] > 0.0) {
-      last = threadIdx.x * 4 + j;
-      if (run > s_thr) found = min(found, last);
+  for (int i = 0; i < kVerEach; ++i) {
+    run += w[i];
+    if (w[i] > 0.0) {
+      last = threadIdx.x * kVerEach + i;
+      if (run > thr) found = min(found, last);
     }
   }
-  if (found != 0x7fffffff) atomicMin(&s_found, found);
-  if (last >= 0) atomicMax(&s_last, last);
+  // the first that passes, or the last with mass, of the wave, then of the block
+  const unsigned long long hit = __ballot(found != 0x7fffffff), pos = __ballot(last >= 0);
+  const int wf = hit ? __shfl(found, __builtin_ctzll(hit), kWave) : 0x7fffffff;
+  const int wl = pos ? __shfl(last, 63 - __builtin_clzll(pos), kWave) : -1;
+  if (lane == 0) s_found[wave_id()] = wf, s_last[wave_id()] = wl;
   __syncthreads();
-  if (threadIdx.x == 0) a.next[b] = base + (s_found != 0x7fffffff ? s_found : s_last);
+  if (threadIdx.x == 0) {
+    const int ff = min(min(s_found[0], s_found[1]), min(s_found[2], s_found[3]));
+    const int ll = max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3]));
+    a.next[b] = base + (ff != 0x7fffffff ? ff : ll);
+  }
 }
 
 static int64_t ver_chunks(int64_t V) { return (V + kVerChunk - 1) / kVerChunk; }
@@ -315,10 +332,21 @@ extern "C" int tpp_verify_draft(const int64_t *draft_tokens, const int32_t *pare
   a.part = (double *)workspace;
   a.state = (VerState *)(a.part + (size_t)B * a.chunks * 2);
   hipStream_t st = as_stream(stream);
+  // 16 bytes at a time where every row begins at such an address and ends whole
+  const int es = dtype == TPP_F32 ? 4 : 2;
+  uint64_t low = (uint64_t)(uintptr_t)target_probs | (uint64_t)(a.p_sb * es) | (uint64_t)(a.p_st * es) | (uint64_t)(V * es);
+  if (draft_probs) low |= (uint64_t)(uintptr_t)draft_probs | (uint64_t)(a.q_sb * es) | (uint64_t)(a.q_st * es);
+  const bool vec = !(low & 15);
   auto go = [&](auto zero) {
     typedef decltype(zero) P;
-    ver_sum_kernel<P><<<dim3((unsigned)a.chunks, (unsigned)B), dim3(256), 0, st>>>(a);
-    ver_pick_kernel<P><<<dim3((unsigned)B), dim3(1024), 0, st>>>(a);
+    const dim3 grid((unsigned)a.chunks, (unsigned)B);
+    if (vec) {
+      ver_sum_kernel<P, true><<<grid, dim3(256), 0, st>>>(a);
+      ver_pick_kernel<P, true><<<dim3((unsigned)B), dim3(256), 0, st>>>(a);
+    } else {
+      ver_sum_kernel<P, false><<<grid, dim3(256), 0, st>>>(a);
+      ver_pick_kernel<P, false><<<dim3((unsigned)B), dim3(256), 0, st>>>(a);
+    }
   };
   if (dtype == TPP_F32) go(0.f);
   else if (dtype == TPP_F16) go(f16(0));
