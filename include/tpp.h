@@ -534,8 +534,8 @@ int tpp_tree_attn(const void *q, const void *k, const void *v, void *o,
                   float softmax_scale, int code, int dtype, void *workspace,
                   size_t ws_bytes, void *stream);
 
-/* Workspace bytes of tpp_tree_attn (16-byte aligned, no initialisation; 0:
- * none). */
+/* Workspace bytes of tpp_tree_attn (128-byte aligned, no initialisation; 0: none).
+ * It belongs to one call until that has run. */
 size_t tpp_tree_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
                                     int64_t D, int64_t Lmax, int code);
 

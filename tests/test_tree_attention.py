@@ -224,6 +224,32 @@ def test_captured_two_graphs_and_two_streams(dev, code):
 
 
 @pytest.mark.gpu
+def test_many_calls_on_two_streams(dev):
+    """Calls whose splits one launch merges, on two streams at once and often
+    enough for the arrival words (2^18, 256 pairs a call) to come round."""
+    from torchplusplus_amd.attention import tree_attention
+    b, hkv, d, room = 32, 8, 64, 1024
+    q, cache, kw, _ = make(b, 1, 8, hkv, d, room, torch.bfloat16, torch.int8, 3, dev)
+    lens = torch.randint(1, room - 1, (b,), generator=torch.Generator().manual_seed(1)).int()
+    a, c = lens.to(dev), lens.flip(0).contiguous().to(dev)
+    want = [tree_attention(q, *cache, x, None, **kw) for x in (a, c)]
+    check(q, cache, kw, [osp.values(t.cpu(), e.cpu()) for t, e in zip(cache, (kw["k_exps"], kw["v_exps"]))], lens,
+          None, torch.bfloat16, "mixed lengths", got=want[0])
+    torch.cuda.synchronize()
+    streams, bad = [torch.cuda.Stream() for _ in "ac"], []
+    for s, x, w in zip(streams, (a, c), want):
+        with torch.cuda.stream(s):
+            bad.append(torch.zeros((), dtype=torch.int32, device=dev))
+    torch.cuda.synchronize()
+    for _ in range(700):
+        for i, (s, x, w) in enumerate(zip(streams, (a, c), want)):
+            with torch.cuda.stream(s):
+                bad[i] += (tree_attention(q, *cache, x, None, **kw) != w).any()
+    torch.cuda.synchronize()
+    assert [int(n) for n in bad] == [0, 0]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("code", [None, torch.int8])
 def test_offsets_past_32_bits(dev, code):
     """A cache whose last sequence begins past 2^32 bytes."""

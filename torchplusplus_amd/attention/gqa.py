@@ -7,6 +7,8 @@ Same constructor and forward signature. Per call the layer runs:
   3. flash attention with native GQA (no repeat_interleave / .contiguous()
      copies), or split-KV decode attention when a single token is appended
   4. the output projection.
+With a QuantKVCache step 2 rotates in place and appends codes, and step 3 reads
+them (_attend_codes).
 The fused projection weight is built from Wq/Wk/Wv on first use and rebuilt
 whenever one of them changes (load_state_dict, in-place edits), as the
 reference reads its projection weights on every call (gqa.py:82-84).
@@ -19,9 +21,12 @@ import torch
 import torch.nn as nn
 
 from torchplusplus_amd._native import ext as _ext
+from torchplusplus_amd.attention._common import norm_rope_qk
+from torchplusplus_amd.attention.flash import flash_attn_func
+from torchplusplus_amd.attention.tree import TREE_MAX_TOKENS, tree_attention
 from torchplusplus_amd.dlops.derived import DerivedWeight, attach
 from torchplusplus_amd.dlops.linear import linear
-from torchplusplus_amd.llmops.kvcache import KVCache
+from torchplusplus_amd.llmops.kvcache import KVCache, QuantKVCache
 
 _C = _ext()
 
@@ -129,6 +134,8 @@ class GroupedQueryAttention(nn.Module):
                cache_pos: Optional[int] = None) -> torch.Tensor:
         """Steps 2-3: rope/cache the projected qkv and attend; returns the
         attention output [B, S, Hq*D] (before the output projection)."""
+        if isinstance(kv_cache, QuantKVCache):
+            return self._attend_codes(qkv, cos, sin, kv_cache, cache_pos)
         norms = self._norms()
         shape = (self.num_heads, self.n_kv_heads, self.head_dim)
         if kv_cache is None:
@@ -141,6 +148,26 @@ class GroupedQueryAttention(nn.Module):
         o = _C.gqa_attend(qkv, *norms, cos, sin, kv_cache.k_cache, kv_cache.v_cache, start, *shape)
         kv_cache.cache_len = max(kv_cache.cache_len, start + seq_len)
         return o
+
+    def _attend_codes(self, qkv, cos, sin, cache: QuantKVCache, cache_pos: Optional[int]):
+        """attend() on a cache of 8-bit codes: norm and rotation in one launch,
+        K/V appended as codes, then attention over the codes in place (up to 64
+        new tokens, a chain behind the cached ones), or over the decoded prefix."""
+        bs, seq_len = qkv.shape[0], qkv.shape[1]
+        start = cache.cache_len if cache_pos is None else int(cache_pos)
+        cache.ensure(bs, start + seq_len)
+        q, k, v = (t.unflatten(-1, (-1, self.head_dim)) for t in qkv.split(
+            [self.num_heads * self.head_dim] + [self.n_kv_heads * self.head_dim] * 2, -1))
+        end = start + seq_len
+        q, k = norm_rope_qk(q, k, self.q_norm, self.k_norm, cos[start:end], sin[start:end])
+        cache.append(k, v, start)
+        if seq_len <= TREE_MAX_TOKENS:
+            kc, vc, ke, ve = cache.rows(bs)
+            o = tree_attention(q, kc, vc, _positions(bs, start, qkv.device), k_exps=ke, v_exps=ve)
+        else:
+            k, v = cache.read(end, bs)
+            o = flash_attn_func(q, k.transpose(1, 2), v.transpose(1, 2), causal=True)
+        return o.reshape(bs, seq_len, self.d_out)
 
     def forward(self, x, cos, sin, kv_cache: Optional[KVCache] = None,
                 cache_pos: Optional[int] = None):

@@ -11,6 +11,8 @@ from torchplusplus_amd._native import ext as _ext
 
 _C = _ext()
 
+TREE_MAX_TOKENS = 64  # drafted tokens a sequence: a bit each in the kernels' masks
+
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                    seqlens: torch.Tensor, parents: Optional[torch.Tensor] = None,

@@ -11,6 +11,8 @@
 // with exponent 255 is NaN.
 #include "tpp_common.hpp"
 
+#include <atomic>
+
 namespace tpp {
 
 constexpr int kTreeMaxT = 64;
@@ -589,12 +591,158 @@ template <typename P> __device__ __forceinline__ unsigned lds_addr(P *x) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)x;
 }
 
+// Merging a row's splits, in one order wherever it is done: four parts, part g the
+// splits g, g + 4, .. (four at a time), then the parts.
+constexpr int kMergeParts = 4, kMergeAhead = 4;
+template <int NP> struct TreeMerge { // parts g0, g0 + step, .. of a row, chunk c of four values
+  float m[NP], l[NP];
+  f32x4 o[NP];
+  float ma[NP][kMergeAhead], la[NP][kMergeAhead];
+  f32x4 oa[NP][kMergeAhead];
+  // the splits s0 .. s0 + 15, those past `last` read it (and are not used); HERE:
+  // maxima and weights past the L1
+  template <int D, bool HERE>
+  __device__ __forceinline__ void load(const float *ws_o, const float *ws_ml, int64_t slot, int c, int s0, int g0,
+                                       int step, int last) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+#pragma unroll
+      for (int j = 0; j < kMergeAhead; ++j) {
+        const int64_t at = slot + min(s0 + j * kMergeParts + g0 + n * step, last);
+        if constexpr (HERE) {
+          ma[n][j] = __hip_atomic_load(&ws_ml[at * 2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          la[n][j] = __hip_atomic_load(&ws_ml[at * 2 + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        } else {
+          ma[n][j] = ws_ml[at * 2], la[n][j] = ws_ml[at * 2 + 1];
+        }
+        oa[n][j] = *reinterpret_cast<const f32x4 *>(ws_o + at * D + c * 4);
+      }
+  }
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) m[n] = -INFINITY, l[n] = 0.f, o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void add(int s0, int g0, int step, int live) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      float mn = m[n];
+#pragma unroll
+      for (int j = 0; j < kMergeAhead; ++j)
+        if (s0 + j * kMergeParts + g0 + n * step < live) mn = fmaxf(mn, ma[n][j]);
+      const float mu = mn == -INFINITY ? 0.f : mn, a = __builtin_amdgcn_exp2f(m[n] - mu);
+      l[n] *= a;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] *= a;
+#pragma unroll
+      for (int j = 0; j < kMergeAhead; ++j) {
+        if (s0 + j * kMergeParts + g0 + n * step >= live) break; // (such a slot may hold anything)
+        const float cf = __builtin_amdgcn_exp2f(ma[n][j] - mu);
+        l[n] += la[n][j] * cf;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] += oa[n][j][e] * cf;
+      }
+      m[n] = mn;
+    }
+  }
+};
+// The parts of a row, from LDS (pitch f32x4 values of o, two of m and l): chunk c of
+// the output.
+template <typename T>
+__device__ __forceinline__ typename VecT<T>::v4 tree_merge_parts(const f32x4 *o, int pitch, const float *ml) {
+  float mx = -INFINITY, ls = 0.f;
+#pragma unroll
+  for (int g = 0; g < kMergeParts; ++g) mx = fmaxf(mx, ml[g * 2]);
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  f32x4 os = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < kMergeParts; ++g) {
+    const float cf = __builtin_amdgcn_exp2f(ml[g * 2] - mu);
+    ls += ml[g * 2 + 1] * cf;
+    const f32x4 x = o[g * pitch];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) os[e] += x[e] * cf;
+  }
+  typename VecT<T>::v4 ov;
+  const float inv = ls != 0.f ? 1.f / ls : 0.f; // (NaN stays NaN)
+#pragma unroll
+  for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
+  return ov;
+}
+
+// The splits of up to 16 rows, by the pair's last block to finish (its blocks run on
+// one XCD, so that its L2 holds what they wrote): one launch instead of two, 7.8 ->
+// 6.0 us where a sequence needs one split only.
+// A block counts itself in on a word that the call has for itself while it runs:
+// the host deals them out in turn from a ring, and the last block leaves its word at
+// zero. A word comes up again a thousand calls later (2^18 words, 256 pairs), long
+// after this one's kernel. A captured call, which would have the same words in every
+// replay, takes the second launch. (A word of the call's own workspace, set by
+// compare-and-swap for want of a zero, cost 1.5 us a block: 15 -> 61 us at 32
+// splits.) Partial sums are whole 128-byte lines of one writer, and a block reads
+// others' only here, so that its L1 has no stale copy; maxima and weights, which share
+// lines, are read past the L1.
+constexpr unsigned kTreeWords = 1u << 18;
+static __device__ unsigned g_tree_arrived[kTreeWords]; // zero when loaded
+
+template <typename T, int D>
+__device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlock &k, int rows, int nsplit,
+                                                const float *__restrict__ ws_o, const float *__restrict__ ws_ml,
+                                                unsigned g_inv, unsigned *__restrict__ arrived, char *lds) {
+  constexpr int C4 = D / 4, NG = 256 / C4;
+  __shared__ int s_last;
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wave's sums are in the L2
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned old = __hip_atomic_fetch_add(arrived + k.pair, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = (int)old == k.live - 1;
+    if (s_last) __hip_atomic_store(arrived + k.pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!s_last) return;
+  // NG groups of lanes over the rows, up to four (one a part) a row
+  const int grp = threadIdx.x / C4, c = threadIdx.x % C4;
+  f32x4 *const s_o = reinterpret_cast<f32x4 *>(lds);                           // [row][part][chunk]
+  float *const s_ml = reinterpret_cast<float *>(lds + NG * kMergeParts * C4 * 16); // [row][part][2]
+  auto run = [&](auto npc) {
+    constexpr int NP = decltype(npc)::value, STEP = kMergeParts / NP, RPB = NG / STEP;
+    for (int base = 0; base < rows; base += RPB) {
+      const int q = grp / STEP, g0 = grp % STEP, r = min(base + q, rows - 1);
+      const int64_t slot = ((int64_t)k.pair * rows + r) * nsplit;
+      TreeMerge<NP> mg;
+      mg.begin();
+      for (int s0 = 0; s0 < k.live; s0 += kMergeParts * kMergeAhead) {
+        mg.template load<D, true>(ws_o, ws_ml, slot, c, s0, g0, STEP, k.live - 1);
+        mg.add(s0, g0, STEP, k.live);
+      }
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        const int at = q * kMergeParts + g0 + n * STEP;
+        s_o[at * C4 + c] = mg.o[n];
+        if (c == 0) s_ml[at * 2] = mg.m[n], s_ml[at * 2 + 1] = mg.l[n];
+      }
+      __syncthreads();
+      if (g0 == 0 && base + q < rows) {
+        const int t = div_inv((unsigned)r, g_inv), g = r - t * p.G;
+        T *op = (T *)p.o + (int64_t)k.b * p.o_s[0] + (int64_t)t * p.o_s[1] + (int64_t)(k.hk * p.G + g) * p.o_s[2];
+        *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) =
+            tree_merge_parts<T>(s_o + q * kMergeParts * C4 + c, C4, s_ml + q * kMergeParts * 2);
+      }
+      __syncthreads();
+    }
+  };
+  if (rows * kMergeParts <= NG) run(std::integral_constant<int, 1>{});
+  else if (rows * 2 <= NG) run(std::integral_constant<int, 2>{});
+  else run(std::integral_constant<int, 4>{});
+}
+
 // Up to 32 rows a block: the four waves share the rows and split the keys.
 template <typename T, int KIND, int D, int NC>
 __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs p, float *__restrict__ ws_o,
                                                            float *__restrict__ ws_ml, int nsplit,
                                                            unsigned nsplit_inv, unsigned hkv_inv,
-                                                           unsigned g_inv, int by_xcd) {
+                                                           unsigned g_inv, int by_xcd,
+                                                           unsigned *__restrict__ arrived) {
   typedef TreeTile<KIND, D> TT;
   typedef TreeWave<T, KIND, D, NC> W;
   constexpr int KT = TT::KT, NW = 4, STRIDE = NW * KT, NDMA = TT::TILEB / 1024, C4 = D / 4, ROWS = 16 * NC;
@@ -696,6 +844,8 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs p, float *__
       if (c == 0) ws_ml[slot * 2] = mx, ws_ml[slot * 2 + 1] = ls;
     }
   }
+  if constexpr (NC == 1)
+    if (arrived && k.live > 1) tree_merge_here<T, D>(p, k, rows, nsplit, ws_o, ws_ml, g_inv, arrived, smem);
 }
 
 // More rows: the four waves share the tiles of the split's keys, each with rows
@@ -797,87 +947,42 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(TreeArgs p, float *__
   else run(std::integral_constant<int, 1>{});
 }
 
-// The splits of every row, which are runs of batches of 2^lstride keys. Four groups
-// of D / 4 lanes share a row's splits, each 16 splits' loads at once and before the
-// sequence's length has come (slots that no split wrote are read and not used): a
-// chain of length, maxima and sums would be three trips to memory, twice the
-// launch's time.
+// The splits of every row, which are runs of batches of 2^lstride keys: a part a
+// group of D / 4 lanes, the first splits' loads before the sequence's length has come
+// (slots that no split wrote are read and not used): a chain of length, maxima and
+// sums would be three trips to memory, twice the launch's time.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, const float *__restrict__ ws_o,
                                                          const float *__restrict__ ws_ml, int nsplit,
                                                          unsigned nsplit_inv, unsigned g_inv, int lstride) {
-  constexpr int C4 = D / 4, SG = 4, U = 4, RPB = 256 / (C4 * SG);
-  __shared__ f32x4 s_o[RPB][SG][C4];
-  __shared__ float s_m[RPB][SG], s_l[RPB][SG];
-  const int rb = threadIdx.x / (C4 * SG), sg = threadIdx.x / C4 % SG, c = threadIdx.x % C4;
-  const int rows = p.T * p.G, r = min(blockIdx.x * RPB + rb, rows - 1);
+  constexpr int C4 = D / 4, RPB = 256 / (C4 * kMergeParts);
+  __shared__ f32x4 s_o[RPB * kMergeParts * C4];
+  __shared__ float s_ml[RPB * kMergeParts * 2];
+  const int grp = threadIdx.x / C4, q = grp / kMergeParts, g0 = grp % kMergeParts, c = threadIdx.x % C4;
+  const int rows = p.T * p.G, r = min((int)blockIdx.x * RPB + q, rows - 1);
   const int hk = blockIdx.y, b = blockIdx.z;
   const int64_t slot = (((int64_t)b * p.Hkv + hk) * rows + r) * nsplit;
   const int len = p.seqlens[b];
-  f32x4 pr[U];
-  float m[U], l[U];
-  auto load = [&](int s0) {
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int64_t at = slot + min(s0 + j * SG + sg, nsplit - 1);
-      m[j] = ws_ml[at * 2], l[j] = ws_ml[at * 2 + 1];
-      pr[j] = *reinterpret_cast<const f32x4 *>(ws_o + at * D + c * 4);
-    }
-  };
-  load(0);
+  TreeMerge<1> mg;
+  mg.begin();
+  mg.template load<D, false>(ws_o, ws_ml, slot, c, 0, g0, 1, nsplit - 1);
   const int L = min(max(len, 0), p.Lmax), end = min(L + p.T, p.Lmax);
   const int nbatch = (int)(((unsigned)end + (1u << lstride) - 1) >> lstride);
   const int per = div_inv((unsigned)(nbatch + nsplit - 1), nsplit_inv);
   const int live = (int)((unsigned)(nbatch + per - 1) / (unsigned)per);
   if (live == 1) return; // written by the tile kernel
-  float mx = -INFINITY, ls = 0.f;
-  f32x4 os = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < live; s0 += U * SG) {
-    if (s0) load(s0);
-    float mn = mx;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      if (s0 + j * SG + sg >= live) m[j] = -INFINITY;
-      mn = fmaxf(mn, m[j]);
-    }
-    const float mu = mn == -INFINITY ? 0.f : mn, a = __builtin_amdgcn_exp2f(mx - mu);
-    ls *= a;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) os[e] *= a;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      if (s0 + j * SG + sg >= live) break; // (what such a slot holds may be anything)
-      const float cf = __builtin_amdgcn_exp2f(m[j] - mu);
-      ls += l[j] * cf;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) os[e] += pr[j][e] * cf;
-    }
-    mx = mn;
+  for (int s0 = 0; s0 < live; s0 += kMergeParts * kMergeAhead) {
+    if (s0) mg.template load<D, false>(ws_o, ws_ml, slot, c, s0, g0, 1, nsplit - 1);
+    mg.add(s0, g0, 1, live);
   }
-  s_o[rb][sg][c] = os;
-  if (c == 0) s_m[rb][sg] = mx, s_l[rb][sg] = ls;
+  s_o[grp * C4 + c] = mg.o[0];
+  if (c == 0) s_ml[grp * 2] = mg.m[0], s_ml[grp * 2 + 1] = mg.l[0];
   __syncthreads();
-  if (sg || blockIdx.x * RPB + rb >= rows) return;
-  float mt = mx;
-#pragma unroll
-  for (int g = 1; g < SG; ++g) mt = fmaxf(mt, s_m[rb][g]);
-  const float mu = mt == -INFINITY ? 0.f : mt;
-  ls = 0.f;
-  os = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int g = 0; g < SG; ++g) {
-    const float cf = __builtin_amdgcn_exp2f(s_m[rb][g] - mu);
-    ls += s_l[rb][g] * cf;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) os[e] += s_o[rb][g][c][e] * cf;
-  }
+  if (g0 || (int)blockIdx.x * RPB + q >= rows) return;
   const int t = div_inv((unsigned)r, g_inv), g = r - t * p.G;
   T *op = (T *)p.o + (int64_t)b * p.o_s[0] + (int64_t)t * p.o_s[1] + (int64_t)(hk * p.G + g) * p.o_s[2];
-  typename VecT<T>::v4 ov;
-  const float inv = ls != 0.f ? 1.f / ls : 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
-  *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
+  *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) =
+      tree_merge_parts<T>(s_o + q * kMergeParts * C4 + c, C4, s_ml + q * kMergeParts * 2);
 }
 
 // How a call is cut: groups of 16 query rows a block (nc: of a wave that shares
@@ -901,6 +1006,26 @@ static TreePlan tree_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
   if (ns > most) ns = most;
   pl.nsplit = (int)(ns > 256 ? 256 : ns < 1 ? 1 : ns);
   return pl;
+}
+
+// The words of the current device for the pairs of a call (none: nullptr).
+static unsigned *tree_words(int64_t pairs) {
+  static std::atomic<unsigned *> at[64];
+  static std::atomic<uint64_t> next[64];
+  int dev = -1;
+  if (pairs > (int64_t)kTreeWords || hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return nullptr;
+  unsigned *base = at[dev].load(std::memory_order_acquire);
+  if (!base) {
+    if (hipGetSymbolAddress((void **)&base, HIP_SYMBOL(g_tree_arrived)) != hipSuccess) {
+      (void)hipGetLastError();
+      return nullptr;
+    }
+    at[dev].store(base, std::memory_order_release);
+  }
+  uint64_t was = next[dev].load(std::memory_order_relaxed), first;
+  do first = was + (uint64_t)pairs <= kTreeWords ? was : 0; // over the end: from the start
+  while (!next[dev].compare_exchange_weak(was, first + (uint64_t)pairs, std::memory_order_relaxed));
+  return base + first;
 }
 
 } // namespace tpp
@@ -971,11 +1096,18 @@ extern "C" int tpp_tree_attn(const void *q, const void *k, const void *v, void *
   const int64_t rows = T * a.G, pairs = B * Hkv;
   float *ws_o = (float *)workspace, *ws_ml = nullptr;
   if (pl.nsplit > 1) {
-    if (!workspace || !aligned16(workspace) || ws_bytes < tpp_tree_attn_workspace_size(B, T, Hq, Hkv, D, Lmax, code))
+    if (!workspace || ((uintptr_t)workspace & 127) || ws_bytes < tpp_tree_attn_workspace_size(B, T, Hq, Hkv, D, Lmax, code))
       return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
     ws_ml = ws_o + (size_t)(pairs * rows) * pl.nsplit * D;
   }
   const bool by_xcd = pairs % 8 == 0;
+  // the merge by a pair's last block
+  unsigned *arrived = nullptr;
+  if (pl.nsplit > 1 && pl.nc == 1 && by_xcd && xcd_grouping_holds(st, true)) {
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &cs) != hipSuccess) (void)hipGetLastError();
+    else if (cs == hipStreamCaptureStatusNone) arrived = tree_words(pairs);
+  }
   const dim3 grid(by_xcd ? 8 * pl.qtiles : pl.qtiles, pl.nsplit, (unsigned)(by_xcd ? pairs / 8 : pairs));
   const unsigned ninv = inv_of(pl.nsplit), hinv = inv_of((int)Hkv), ginv = inv_of(a.G);
   return TPP_DISPATCH_HALF(dtype, [&] {
@@ -984,10 +1116,10 @@ extern "C" int tpp_tree_attn(const void *q, const void *k, const void *v, void *
       if (pl.nc == 0)
         tree_rows_kernel<T, KIND, DD><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, pl.groups);
       else if (pl.nc == 1)
-        tree_tile_kernel<T, KIND, DD, 1><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd);
+        tree_tile_kernel<T, KIND, DD, 1><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, arrived);
       else
-        tree_tile_kernel<T, KIND, DD, 2><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd);
-      if (pl.nsplit > 1)
+        tree_tile_kernel<T, KIND, DD, 2><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, nullptr);
+      if (pl.nsplit > 1 && !arrived)
         tree_merge_kernel<T, DD><<<dim3((unsigned)((rows + 256 / DD - 1) / (256 / DD)), (unsigned)Hkv, (unsigned)B), dim3(256), 0, st>>>(
             a, ws_o, ws_ml, pl.nsplit, ninv, ginv, pl.lstride);
     };

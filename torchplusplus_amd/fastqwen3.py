@@ -37,7 +37,7 @@ from torchplusplus_amd.dlops.linear import (GEMV_MAX_ROWS, LinearSILU, interleav
                                              linear)
 from torchplusplus_amd.dlops.normalization import RmsNormFused
 from torchplusplus_amd.dlops.rope import compute_rope_params
-from torchplusplus_amd.llmops.kvcache import KVCache
+from torchplusplus_amd.llmops.kvcache import KVCache, QuantKVCache
 from torchplusplus_amd.llmops.llm import LLMInference
 
 _C = _ext()
@@ -196,7 +196,7 @@ class FastQwen3(LLMInference):
             at, n1, n2 = blk.attn, blk.rms_norm1, blk.rms_norm2
             kv = kv_caches[i] if kv_caches is not None else None
             qkv = _C.gemv_fused(resid, at.fused_qkv_weight(), n1.weight, n1.eps)
-            if kv is not None and resid.shape[1] == 1:
+            if kv is not None and resid.shape[1] == 1 and not isinstance(kv, QuantKVCache):
                 at.attend_oproj(qkv, self.cos, self.sin, kv, cache_position, resid)
             else:
                 o = at.attend(qkv, self.cos, self.sin, kv, cache_position)
@@ -211,12 +211,19 @@ class FastQwen3(LLMInference):
         """Greedy generation: prefill, then one captured decode graph per token."""
         bsz, seq_len = input_ids.shape
         self.setup_kv_cache(seq_len + max_new_token, bsz)
+        _check_values(self.kv_cache_array)
         self.reset_kv_cache()
         logits = self.forward_impl(input_ids, self.kv_cache_array, 0, last_only=True)
         first = _C.argmax_rows(logits[:, -1, :].contiguous())
         dec = GreedyDecoder(self, bsz)
         toks = dec.run(first, seq_len, max_new_token - 1, use_graph=use_graph)
         return torch.cat([input_ids, first.view(bsz, 1), toks], dim=1)
+
+
+def _check_values(caches) -> None:
+    if any(isinstance(c, QuantKVCache) for c in caches):
+        raise ValueError("the captured decode step keeps 16-bit caches: clear_kv_cache() first, or use "
+                         "generate(), which decodes over caches of 8-bit codes")
 
 
 class GreedyDecoder:
@@ -239,6 +246,7 @@ class GreedyDecoder:
         self.graph = None
         self.caches = model.kv_cache_array
         assert self.caches is not None, "setup_kv_cache() first"
+        _check_values(self.caches)
 
     def step(self):
         m, B, resid = self.m, self.B, self.resid

@@ -150,8 +150,8 @@ class QuantKVCache:
     torch.float8_e4m3fn (3 bits after the first of each element) or torch.int8
     (7 bits after the first of the row's largest element).
 
-    append() writes tokens, tree_attention() of the attention package and
-    attend() here read the codes in place, read() decodes a prefix, update() is
+    append() writes tokens, attention.tree_attention reads the codes in place
+    (GroupedQueryAttention does both), read() decodes a prefix, update() is
     KVCache.update: append, then the decoded prefix."""
 
     def __init__(self, max_seq_len: int, n_kv_heads: int, head_dim: int,
@@ -196,7 +196,8 @@ class QuantKVCache:
             self.v_exps = torch.full(shape[:3], 127, dtype=torch.uint8, **kw)
             self.cache_len = 0
 
-    def _rows(self, bsz: int):
+    def rows(self, bsz: int):
+        """(k_codes, v_codes, k_exps, v_exps) of the first `bsz` sequences."""
         return self.k_codes[:bsz], self.v_codes[:bsz], self.k_exps[:bsz], self.v_exps[:bsz]
 
     def append(self, k: torch.Tensor, v: torch.Tensor, positions: Union[int, torch.Tensor],
@@ -211,7 +212,7 @@ class QuantKVCache:
             if positions < 0:
                 raise ValueError(f"position {positions} is below 0")
             self.ensure(bsz, int(positions) + seq_len)
-        kv_quant_append(k, v, *self._rows(bsz), positions, counts)
+        kv_quant_append(k, v, *self.rows(bsz), positions, counts)
         if not isinstance(positions, torch.Tensor):
             self.cache_len = max(self.cache_len, int(positions) + seq_len)
 
@@ -220,7 +221,7 @@ class QuantKVCache:
         """The first `length` (default cache_len) positions of the first
         `batch_size` sequences as values [B, n_kv_heads, length, D]."""
         bsz = self.batch_size if batch_size is None else batch_size
-        return kv_quant_read(*self._rows(bsz), self.cache_len if length is None else length, self.dtype)
+        return kv_quant_read(*self.rows(bsz), self.cache_len if length is None else length, self.dtype)
 
     def update(self, k: torch.Tensor, v: torch.Tensor, index: Optional[int] = None
                ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -235,7 +236,7 @@ class QuantKVCache:
 
     def keep(self, start: torch.Tensor, path: torch.Tensor) -> None:
         """KVCache.keep on codes and exponents."""
-        for rows in self._rows(path.shape[0]):
+        for rows in self.rows(path.shape[0]):
             _keep(rows, start, path)
 
     def reset(self) -> None:

@@ -17,7 +17,8 @@ from typing import Callable, List, Optional
 import torch
 import torch.nn as nn
 
-from torchplusplus_amd.llmops.kvcache import KVCache
+from torchplusplus_amd.llmops.kvcache import KVCache, QuantKVCache
+from torchplusplus_amd.llmops.speculative import verify_draft
 
 
 class LLMInference(nn.Module, ABC):
@@ -45,19 +46,23 @@ class LLMInference(nn.Module, ABC):
     def _device(self):
         return next(self.parameters()).device
 
-    def setup_kv_cache(self, max_seq_len: int, batch_size: Optional[int] = None):
+    def setup_kv_cache(self, max_seq_len: int, batch_size: Optional[int] = None,
+                       code_dtype: Optional[torch.dtype] = None):
         """One KVCache per layer (llm.py:52-71). Reuses existing caches when
-        they are large enough, so repeated generate() calls do not reallocate."""
-        if self.kv_cache_array is not None and all(
+        they are large enough, so repeated generate() calls do not reallocate.
+        code_dtype (torch.float8_e4m3fn or torch.int8): caches of 8-bit codes;
+        None keeps the kind that the model has, 16-bit values at first and after
+        clear_kv_cache()."""
+        have = self.kv_cache_array[0] if self.kv_cache_array else None
+        kind = code_dtype or getattr(have, "code_dtype", None)
+        if have is not None and kind == getattr(have, "code_dtype", None) and all(
                 c.max_seq_len >= max_seq_len for c in self.kv_cache_array) and (
                 batch_size is None or all(c.batch_size >= batch_size for c in self.kv_cache_array)):
             return
-        dev = self._device()
-        self.kv_cache_array = [
-            KVCache(max_seq_len, self.get_kv_heads(), self.get_head_dim(), self.get_dtype(), dev,
-                    batch_size)
-            for _ in range(self.get_num_layers())
-        ]
+        args = (max_seq_len, self.get_kv_heads(), self.get_head_dim(), self.get_dtype(), self._device(),
+                batch_size)
+        self.kv_cache_array = [QuantKVCache(*args, code_dtype=kind) if kind else KVCache(*args)
+                               for _ in range(self.get_num_layers())]
 
     def reset_kv_cache(self):
         if self.kv_cache_array:
@@ -97,6 +102,16 @@ class LLMInference(nn.Module, ABC):
         values, idx = torch.topk(logits, top_k)
         filtered = torch.full_like(logits, filter_value).scatter_(-1, idx, values)
         return torch.multinomial(torch.softmax(filtered, dim=-1), num_samples=1)
+
+    def sample_draft(self, draft_tokens, logits, temp: float = 1.0, uniforms=None, draft_probs=None,
+                     parents=None):
+        """Verify drafted tokens [B, T] against the target's logits [B, T + 1, V]
+        at a temperature; uniforms default to torch.rand. Returns (accepted,
+        path, next_token), see llmops.speculative.verify_draft."""
+        probs = torch.softmax(logits.float() / temp, -1)
+        if uniforms is None:
+            uniforms = torch.rand(probs.shape[:2], device=probs.device)
+        return verify_draft(draft_tokens, probs, uniforms, draft_probs, parents)
 
     def sample_greedy(self, logits):
         return torch.argmax(logits, dim=-1, keepdim=True)
