@@ -998,15 +998,15 @@ at::Tensor or_none(const c10::optional<at::Tensor> &t) {
   return t.has_value() && t->defined() ? *t : at::Tensor();
 }
 
-std::vector<at::Tensor> rope_at(at::Tensor q, c10::optional<at::Tensor> k_opt, at::Tensor positions,
-                                at::Tensor inv_freq, bool interleaved, double attention_factor,
-                                bool inplace) {
+std::tuple<at::Tensor, at::Tensor> rope_at(const at::Tensor &q, const c10::optional<at::Tensor> &k_opt,
+                                           at::Tensor positions, const at::Tensor &inv_freq,
+                                           bool interleaved, double attention_factor, bool inplace) {
   const at::Tensor k = or_none(k_opt);
   TORCH_CHECK(q.is_cuda(), "q must be on CUDA");
   check_same_device(q, {&k, &positions, &inv_freq});
   TORCH_CHECK(q.dim() == 4, "q must be 4D [batch, seq_len, heads, head_dim]");
   const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
-  for (const at::Tensor *t : std::initializer_list<const at::Tensor *>{&q, &k}) {
+  for (const at::Tensor *t : {&q, &k}) {
     if (!t->defined()) continue;
     TORCH_CHECK(is_half_or_bf16(*t) && t->scalar_type() == q.scalar_type(),
                 "q and k must be float16 or bfloat16, of one dtype");
@@ -1032,13 +1032,12 @@ std::vector<at::Tensor> rope_at(at::Tensor q, c10::optional<at::Tensor> k_opt, a
   at::Tensor qo = inplace ? q : torch::empty(q.sizes(), q.options()), ko;
   if (k.defined()) ko = inplace ? k : torch::empty(k.sizes(), k.options());
   if (q.numel() == 0) return {qo, ko};
-  auto str = [](const at::Tensor &t) { return std::vector<int64_t>{t.stride(0), t.stride(1), t.stride(2)}; };
-  const auto qs = str(q), qos = str(qo);
-  std::vector<int64_t> ks, kos;
-  if (k.defined()) ks = str(k), kos = str(ko);
+  const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)}, qos[3] = {qo.stride(0), qo.stride(1), qo.stride(2)};
+  int64_t ks[3] = {0, 0, 0}, kos[3] = {0, 0, 0};
+  if (k.defined())
+    for (int i = 0; i < 3; ++i) ks[i] = k.stride(i), kos[i] = ko.stride(i);
   check_rc(tpp_rope_at(q.data_ptr(), k.defined() ? k.data_ptr() : nullptr, qo.data_ptr(),
-                       k.defined() ? ko.data_ptr() : nullptr, qs.data(), ks.data(), qos.data(),
-                       kos.data(), positions.data_ptr(), positions.dim() == 2 ? positions.stride(0) : 0,
+                       k.defined() ? ko.data_ptr() : nullptr, qs, ks, qos, kos, positions.data_ptr(), positions.dim() == 2 ? positions.stride(0) : 0,
                        positions.scalar_type() == at::kLong, inv_freq.data_ptr<double>(),
                        (float)attention_factor, B, S, q.size(2), k.defined() ? k.size(2) : 0, D, R,
                        interleaved, dtype_code(q), cur_stream(q)),
@@ -1055,12 +1054,12 @@ int code_of(const at::Tensor &codes) {
 // codes [B, H, L, D] and exponents [B, H, L] of K and V, of one layout
 int check_codes(const at::Tensor &kc, const at::Tensor &vc, const at::Tensor &ke, const at::Tensor &ve,
                 int64_t B) {
+  const int code = code_of(kc);
+  TORCH_CHECK_TYPE(code > 0 && code_of(vc) > 0, "cache codes must be float8_e4m3fn or int8");
+  TORCH_CHECK_TYPE(ke.scalar_type() == at::kByte && ve.scalar_type() == at::kByte, "cache exponents must be uint8");
+  TORCH_CHECK(vc.scalar_type() == kc.scalar_type(), "K and V codes must have one dtype");
   TORCH_CHECK(kc.is_cuda(), "cache codes must be on CUDA");
   check_same_device(kc, {&vc, &ke, &ve});
-  const int code = code_of(kc);
-  TORCH_CHECK(code > 0 && vc.scalar_type() == kc.scalar_type(),
-              "cache codes must be float8_e4m3fn or int8, of one dtype");
-  TORCH_CHECK(ke.scalar_type() == at::kByte && ve.scalar_type() == at::kByte, "cache exponents must be uint8");
   TORCH_CHECK(kc.dim() == 4 && vc.sizes() == kc.sizes() && vc.strides() == kc.strides(),
               "cache codes must be [B, Hkv, L, D], K and V of one layout");
   TORCH_CHECK(ke.dim() == 3 && ve.sizes() == ke.sizes() && ve.strides() == ke.strides() &&
@@ -1079,14 +1078,14 @@ const int32_t *int32_b(const at::Tensor &t, int64_t B, const char *what) {
   return t.data_ptr<int32_t>();
 }
 
-void kv_quant_append(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor vc, at::Tensor ke,
-                     at::Tensor ve, c10::optional<at::Tensor> positions, int64_t start,
-                     c10::optional<at::Tensor> counts) {
+void kv_quant_append(const at::Tensor &k, const at::Tensor &v, const at::Tensor &kc, const at::Tensor &vc,
+                     const at::Tensor &ke, const at::Tensor &ve, const c10::optional<at::Tensor> &positions,
+                     int64_t start, const c10::optional<at::Tensor> &counts) {
+  const int code = check_codes(kc, vc, ke, ve, k.dim() > 0 ? k.size(0) : -1);
   check_bshd(k, "k");
   check_bshd(v, "v");
   TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "k and v differ");
   const int64_t B = k.size(0), S = k.size(1), H = k.size(2), D = k.size(3);
-  const int code = check_codes(kc, vc, ke, ve, B);
   TORCH_CHECK(kc.size(1) == H && kc.size(3) == D, "cache shape mismatch");
   const at::Tensor pos = or_none(positions), cnt = or_none(counts);
   check_same_device(k, {&v, &kc, &pos, &cnt});
@@ -1101,28 +1100,28 @@ void kv_quant_append(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor vc, a
            "kv_quant_append");
 }
 
-std::vector<at::Tensor> kv_quant_read(at::Tensor kc, at::Tensor vc, at::Tensor ke, at::Tensor ve,
-                                      int64_t length, bool bf16) {
-  TORCH_CHECK(kc.dim() == 4, "cache codes must be [B, Hkv, L, D]");
+std::tuple<at::Tensor, at::Tensor> kv_quant_read(const at::Tensor &kc, const at::Tensor &vc, const at::Tensor &ke,
+                                                 const at::Tensor &ve, int64_t length, at::ScalarType dtype) {
+  TORCH_CHECK_TYPE(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be float16 or bfloat16, got ", dtype);
+  const int code = check_codes(kc, vc, ke, ve, kc.dim() > 0 ? kc.size(0) : -1);
   const int64_t B = kc.size(0), H = kc.size(1), D = kc.size(3);
-  const int code = check_codes(kc, vc, ke, ve, B);
   TORCH_CHECK(length >= 0 && length <= kc.size(2), "length ", length, " of a cache of ", kc.size(2));
   c10::DeviceGuard g(kc.device());
-  const auto opt = kc.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+  const auto opt = kc.options().dtype(dtype);
   auto k = torch::empty({B, H, length, D}, opt), v = torch::empty({B, H, length, D}, opt);
   if (k.numel() == 0) return {k, v};
   const int64_t cs[2] = {kc.stride(0), kc.stride(1)}, es[2] = {ke.stride(0), ke.stride(1)};
   check_rc(tpp_kv_quant_read(kc.data_ptr(), vc.data_ptr(), ke.data_ptr(), ve.data_ptr(), cs, es,
                              k.data_ptr(), v.data_ptr(), B, H, length, D, kc.size(2), code,
-                             bf16 ? TPP_BF16 : TPP_F16, cur_stream(kc)),
+                             dtype_code(k), cur_stream(kc)),
            "kv_quant_read");
   return {k, v};
 }
 
-at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor seqlens,
-                          c10::optional<at::Tensor> parents_opt, c10::optional<at::Tensor> k_exps,
-                          c10::optional<at::Tensor> v_exps, double softmax_scale,
-                          c10::optional<at::Tensor> out) {
+at::Tensor tree_attention(const at::Tensor &q, const at::Tensor &kc, const at::Tensor &vc,
+                          const at::Tensor &seqlens, const c10::optional<at::Tensor> &parents_opt,
+                          const c10::optional<at::Tensor> &k_exps, const c10::optional<at::Tensor> &v_exps,
+                          double softmax_scale, const c10::optional<at::Tensor> &out) {
   check_bshd(q, "q");
   const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3);
   const at::Tensor parents = or_none(parents_opt), ke = or_none(k_exps), ve = or_none(v_exps);
@@ -1175,9 +1174,9 @@ at::Tensor tree_attention(at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor
   return o;
 }
 
-std::vector<at::Tensor> verify_draft(at::Tensor tokens, at::Tensor target, at::Tensor uniforms,
-                                     c10::optional<at::Tensor> draft_opt,
-                                     c10::optional<at::Tensor> parents_opt) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+verify_draft(at::Tensor tokens, const at::Tensor &target, at::Tensor uniforms,
+             const c10::optional<at::Tensor> &draft_opt, const c10::optional<at::Tensor> &parents_opt) {
   TORCH_CHECK(target.is_cuda() && target.dim() == 3, "target_probs must be a CUDA tensor [B, T + 1, V]");
   const at::Tensor draft = or_none(draft_opt), parents = or_none(parents_opt);
   check_same_device(target, {&tokens, &uniforms, &draft, &parents});
@@ -1233,7 +1232,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("positions"), py::arg("start") = 0, py::arg("counts") = py::none());
   m.def("kv_quant_read", &kv_quant_read, "decode the first rows of a cache of 8-bit codes",
         py::arg("k_codes"), py::arg("v_codes"), py::arg("k_exps"), py::arg("v_exps"), py::arg("length"),
-        py::arg("bf16"));
+        py::arg("dtype"));
   m.def("tree_attention", &tree_attention, "attention of drafted tokens over a KV cache", py::arg("q"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("seqlens"), py::arg("parents") = py::none(),
         py::arg("k_exps") = py::none(), py::arg("v_exps") = py::none(), py::arg("softmax_scale") = 0.0,

@@ -66,9 +66,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs p) {
   int hh[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const int64_t row = row0 + i * RPP < p.rows ? row0 + i * RPP : p.rows - 1;
-    const int64_t bh = row / p.S, s = row - bh * p.S, b = bh / p.H;
-    const int h = (int)(bh - b * p.H);
+    const unsigned row = (unsigned)(row0 + i * RPP < p.rows ? row0 + i * RPP : p.rows - 1); // (rows < 2^32)
+    const unsigned bh = row / (unsigned)p.S;
+    const int64_t s = row - bh * (unsigned)p.S, b = bh / (unsigned)p.H;
+    const int h = (int)(bh - (unsigned)b * (unsigned)p.H);
     t[i] = ld_nt(reinterpret_cast<const V8 *>((const T *)p.x[w] + b * p.xs[w][0] + s * p.xs[w][1] + h * p.xs[w][2] + c * 8));
     pos[i] = (p.positions ? (int64_t)p.positions[b] : p.start) + s;
     put[i] = row0 + i * RPP < p.rows && pos[i] >= 0 && pos[i] < p.Lmax && !(p.counts && s >= p.counts[b]);
@@ -127,7 +128,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs p) {
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int64_t id = id0 + i * 256 < p.chunks ? id0 + i * 256 : p.chunks - 1;
-    const int64_t row = id / LPR, bh = row / p.len, pos = row - bh * p.len, b = bh / p.H, h = bh - b * p.H;
+    const unsigned row = (unsigned)(id / LPR), bh = row / (unsigned)p.len, b0 = bh / (unsigned)p.H; // (rows < 2^32)
+    const int64_t pos = row - bh * (unsigned)p.len, b = b0, h = bh - b0 * (unsigned)p.H;
     t[i] = ld_nt(reinterpret_cast<const u32x2 *>((const uint8_t *)p.codes[w] + b * p.cs[0] + h * p.cs[1] + pos * D +
                                                  (id % LPR) * 8));
     e[i] = p.exps[w][b * p.es[0] + h * p.es[1] + pos];
@@ -208,7 +210,7 @@ extern "C" int tpp_kv_quant_append(const void *k, const void *v, const int64_t *
   // four rows a thread where that still fills the card (2048 threads a CU)
   const bool four = a.rows * (D / 8) * 2 >= 4LL * 2048 * 256;
   const int64_t per = 256 / (D / 8) * (four ? 4 : 1), blocks = (a.rows + per - 1) / per;
-  if (blocks > 0x7fffffffLL) return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
+  if (S > 0x7fffffffLL || blocks > 0x7fffffffLL || a.rows > 0xffffffffLL) return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
   hipStream_t st = as_stream(stream);
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto cd, auto dd) {
@@ -248,7 +250,7 @@ extern "C" int tpp_kv_quant_read(const void *k_codes, const void *v_codes, const
   // four chunks of 8 a thread where that still fills the card
   const bool four = a.chunks * 2 >= 4LL * 2048 * 256;
   const int64_t per = four ? 1024 : 256, blocks = (a.chunks + per - 1) / per;
-  if (blocks > 0x7fffffffLL) return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
+  if (blocks > 0x7fffffffLL || a.chunks / (D / 8) > 0xffffffffLL) return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
   hipStream_t st = as_stream(stream);
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto cd, auto dd) {

@@ -16,8 +16,8 @@
 // turns and were within 1.3e-7 of sin and cos over that range.
 //
 // Bound by HBM: each element is read once and written once. A thread owns PW
-// pairs of one token (16-byte accesses at PW = 8) and walks `hpt` heads with
-// their angles.
+// pairs of one token (16-byte accesses at PW = 8) in one head, or in four where there
+// is work enough: their loads are in flight while the angles are worked out.
 #include "tpp_common.hpp"
 
 namespace tpp {
@@ -30,21 +30,19 @@ struct RopeAtArgs {
   int64_t pos_sb;
   const double *inv_freq;
   float factor;
-  int S, Hq, Hk, D, R, hpt, upt, hgroups, pos64;
-  int64_t units; // B * S * hgroups * upt
+  int S, Hq, Hk, D, R, pos64;
+  unsigned upt, hgroups, units; // units = B * S * hgroups * upt
 };
 
 template <typename T, int PW, bool IL, int U>
 __global__ __launch_bounds__(256) void rope_at_kernel(RopeAtArgs p) {
   typedef uint16_t W __attribute__((ext_vector_type(PW))); // PW elements
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const unsigned id = blockIdx.x * 256u + threadIdx.x; // (units < 2^32)
   if (id >= p.units) return;
   // unit (fastest), head group, token
-  const int u = (int)(id % p.upt);
-  const int64_t r = id / p.upt;
-  const int hg = (int)(r % p.hgroups);
-  const int64_t tok = r / p.hgroups;
-  const int64_t b = tok / p.S, s = tok - b * p.S;
+  const unsigned r = id / p.upt, tok = r / p.hgroups;
+  const int u = (int)(id - r * p.upt), hg = (int)(r - tok * p.hgroups);
+  const int64_t b = tok / (unsigned)p.S, s = tok - (unsigned)b * (unsigned)p.S;
   const int64_t at = b * p.pos_sb + s;
   const int64_t pos = p.pos64 ? ((const int64_t *)p.pos)[at] : ((const int32_t *)p.pos)[at];
   // the unit's two runs of PW elements: of pairs, or past R copied
@@ -52,6 +50,20 @@ __global__ __launch_bounds__(256) void rope_at_kernel(RopeAtArgs p) {
   const int lo = IL || u * 2 * PW >= p.R ? u * 2 * PW : u * PW;
   const int hi = IL || u * 2 * PW >= p.R ? lo + PW : lo + p.R / 2;
   if (!turn && p.q == p.qo && p.k == p.ko) return; // in place: nothing to copy
+  const int H = p.Hq + p.Hk, h0 = hg * U, h1 = min(h0 + U, H);
+  // U heads' loads before anything is worked out
+  T *dst[U];
+  W x[U], y[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int hc = min(h0 + i, h1 - 1); // (past the last: the last again, not stored)
+    const bool isq = hc < p.Hq;
+    const int hh = isq ? hc : hc - p.Hq;
+    const int64_t *is = isq ? p.qs : p.ks, *os = isq ? p.qos : p.kos;
+    const T *src = (const T *)(isq ? p.q : p.k) + b * is[0] + s * is[1] + hh * is[2];
+    dst[i] = (T *)(isq ? p.qo : p.ko) + b * os[0] + s * os[1] + hh * os[2];
+    x[i] = ld_nt(reinterpret_cast<const W *>(src + lo)), y[i] = ld_nt(reinterpret_cast<const W *>(src + hi));
+  }
   float c[PW], sn[PW];
   if (turn) {
 #pragma unroll
@@ -62,47 +74,31 @@ __global__ __launch_bounds__(256) void rope_at_kernel(RopeAtArgs p) {
       sn[j] = __builtin_amdgcn_sinf(f) * p.factor;
     }
   }
-  const int H = p.Hq + p.Hk, h0 = hg * p.hpt, h1 = min(h0 + p.hpt, H);
-  for (int h = h0; h < h1; h += U) { // U heads' loads before the first use
-    const T *src[U];
-    T *dst[U];
-    W x[U], y[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int hc = min(h + i, h1 - 1); // (past the last: the last again, not stored)
-      const bool isq = hc < p.Hq;
-      const int hh = isq ? hc : hc - p.Hq;
-      const int64_t *is = isq ? p.qs : p.ks, *os = isq ? p.qos : p.kos;
-      src[i] = (const T *)(isq ? p.q : p.k) + b * is[0] + s * is[1] + hh * is[2];
-      dst[i] = (T *)(isq ? p.qo : p.ko) + b * os[0] + s * os[1] + hh * os[2];
-      x[i] = ld_nt(reinterpret_cast<const W *>(src[i] + lo)), y[i] = ld_nt(reinterpret_cast<const W *>(src[i] + hi));
-    }
+  for (int i = 0; i < U; ++i) {
+    if (i && h0 + i >= h1) break;
+    if (turn) {
+      float v[2 * PW];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (i && h + i >= h1) break;
-      if (turn) {
-        float v[2 * PW];
-#pragma unroll
-        for (int j = 0; j < PW; ++j) {
-          v[j] = to_f32(__builtin_bit_cast(T, (uint16_t)x[i][j]));
-          v[PW + j] = to_f32(__builtin_bit_cast(T, (uint16_t)y[i][j]));
-        }
-#pragma unroll
-        for (int j = 0; j < PW; ++j) {
-          const int ia = IL ? 2 * j : j, ib = IL ? 2 * j + 1 : PW + j;
-          const float a = v[ia], bb = v[ib];
-          v[ia] = a * c[j] - bb * sn[j];
-          v[ib] = bb * c[j] + a * sn[j];
-        }
-#pragma unroll
-        for (int j = 0; j < PW; ++j) {
-          x[i][j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[j]));
-          y[i][j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[PW + j]));
-        }
+      for (int j = 0; j < PW; ++j) {
+        v[j] = to_f32(__builtin_bit_cast(T, (uint16_t)x[i][j]));
+        v[PW + j] = to_f32(__builtin_bit_cast(T, (uint16_t)y[i][j]));
       }
-      *reinterpret_cast<W *>(dst[i] + lo) = x[i];
-      *reinterpret_cast<W *>(dst[i] + hi) = y[i];
+#pragma unroll
+      for (int j = 0; j < PW; ++j) {
+        const int ia = IL ? 2 * j : j, ib = IL ? 2 * j + 1 : PW + j;
+        const float a = v[ia], bb = v[ib];
+        v[ia] = a * c[j] - bb * sn[j];
+        v[ib] = bb * c[j] + a * sn[j];
+      }
+#pragma unroll
+      for (int j = 0; j < PW; ++j) {
+        x[i][j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[j]));
+        y[i][j] = __builtin_bit_cast(uint16_t, from_f32<T>(v[PW + j]));
+      }
     }
+    *reinterpret_cast<W *>(dst[i] + lo) = x[i];
+    *reinterpret_cast<W *>(dst[i] + hi) = y[i];
   }
 }
 
@@ -145,20 +141,21 @@ extern "C" int tpp_rope_at(const void *q, const void *k, void *q_out, void *k_ou
   a.pos = positions, a.pos_sb = pos_stride, a.pos64 = pos_is_64 ? 1 : 0;
   a.inv_freq = inv_freq, a.factor = factor;
   a.S = (int)S, a.Hq = (int)Hq, a.Hk = (int)Hk, a.D = (int)D, a.R = (int)R;
-  a.upt = (int)(D / (2 * pw));
-  const int H = (int)(Hq + Hk);
+  a.upt = (unsigned)(D / (2 * pw));
+  const int64_t H = Hq + Hk;
   // threads of four heads where they still fill the card (2048 a CU), else of one
-  a.hpt = B * S * ((H + 3) / 4) * a.upt >= 2048 * 256 ? 4 : 1;
-  a.hgroups = (H + a.hpt - 1) / a.hpt;
-  a.units = B * S * a.hgroups * a.upt;
-  const int64_t blocks = (a.units + 255) / 256;
-  if (blocks > 0x7fffffffLL) return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
+  const bool four = B * S * ((H + 3) / 4) * a.upt >= 2048 * 256;
+  a.hgroups = (unsigned)(four ? (H + 3) / 4 : H);
+  if (B > (int64_t)(0xffffff00u / ((uint64_t)S * a.hgroups * a.upt)))
+    return set_error(TPP_E_UNSUPPORTED, "%s: too many rows", name);
+  a.units = (unsigned)(B * S * a.hgroups * a.upt);
+  const unsigned blocks = (a.units + 255) / 256;
   hipStream_t st = as_stream(stream);
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto w) {
       constexpr int PW = decltype(w)::value;
-      const dim3 grid((unsigned)blocks), block(256);
-      if (a.hpt == 4) {
+      const dim3 grid(blocks), block(256);
+      if (four) {
         if (interleaved) rope_at_kernel<T, PW, true, 4><<<grid, block, 0, st>>>(a);
         else rope_at_kernel<T, PW, false, 4><<<grid, block, 0, st>>>(a);
       } else if (interleaved) {

@@ -102,11 +102,11 @@ def rope_apply_at(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.T
     (j, j + R/2) or, interleaved, (2j, 2j + 1); the rest, and tokens at negative
     positions (padding), are copied. inv_freq as from rope_frequencies. q and k
     may be views of a fused projection (any strides, contiguous last dim)."""
-    return tuple(_C.rope_at(q, k, positions, inv_freq, interleaved, attention_factor, False))
+    return _C.rope_at(q, k, positions, inv_freq, interleaved, attention_factor, False)
 
 
 def rope_apply_at_(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                    inv_freq: torch.Tensor, interleaved: bool = False,
                    attention_factor: float = 1.0):
     """rope_apply_at in place; returns (q, k)."""
-    return tuple(_C.rope_at(q, k, positions, inv_freq, interleaved, attention_factor, True))
+    return _C.rope_at(q, k, positions, inv_freq, interleaved, attention_factor, True)

@@ -44,16 +44,7 @@ def _keep(rows: torch.Tensor, start: torch.Tensor, path: torch.Tensor) -> None:
     raw[seq, :, to] = raw[seq, :, src]
 
 
-def _check_codes(k_codes, v_codes, k_exps, v_exps) -> None:
-    for c, e in ((k_codes, k_exps), (v_codes, v_exps)):
-        if c.dtype not in QUANT_CODES:
-            raise TypeError(f"cache codes must be float8_e4m3fn or int8, got {c.dtype}")
-        if e.dtype != torch.uint8:
-            raise TypeError(f"cache exponents must be uint8, got {e.dtype}")
-
-
-# element types of a cache of 8-bit codes -> the kernels' code numbers
-QUANT_CODES = {torch.float8_e4m3fn: 1, torch.int8: 2}
+QUANT_CODES = (torch.float8_e4m3fn, torch.int8)  # element types of a cache of 8-bit codes
 
 
 def kv_quant_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
@@ -66,10 +57,10 @@ def kv_quant_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_c
     Token s of sequence b goes to positions[b] + s (an int: the same for all);
     tokens outside the cache, or past counts[b], are not written. A row with an
     infinity or NaN is kept as NaN. D in {64, 128, 256}."""
-    _check_codes(k_codes, v_codes, k_exps, v_exps)
-    at = positions if isinstance(positions, torch.Tensor) else None
-    _C.kv_quant_append(k, v, k_codes, v_codes, k_exps, v_exps, at, 0 if at is not None else int(positions),
-                       counts)
+    if isinstance(positions, torch.Tensor):
+        _C.kv_quant_append(k, v, k_codes, v_codes, k_exps, v_exps, positions, 0, counts)
+    else:
+        _C.kv_quant_append(k, v, k_codes, v_codes, k_exps, v_exps, None, positions, counts)
 
 
 def kv_quant_read(k_codes: torch.Tensor, v_codes: torch.Tensor, k_exps: torch.Tensor,
@@ -78,13 +69,7 @@ def kv_quant_read(k_codes: torch.Tensor, v_codes: torch.Tensor, k_exps: torch.Te
     """The first `length` rows of such caches as values: two new tensors
     [B, Hkv, length, D] of `dtype` (exact in bfloat16; one rounding, limited to
     +-65504, in float16)."""
-    _check_codes(k_codes, v_codes, k_exps, v_exps)
-    return tuple(_C.kv_quant_read(k_codes, v_codes, k_exps, v_exps, int(length), dtype == torch.bfloat16
-                                  if dtype in (torch.float16, torch.bfloat16) else _bad_type(dtype)))
-
-
-def _bad_type(dtype):
-    raise TypeError(f"dtype must be float16 or bfloat16, got {dtype}")
+    return _C.kv_quant_read(k_codes, v_codes, k_exps, v_exps, length, dtype)
 
 
 class KVCache:
@@ -160,7 +145,7 @@ class QuantKVCache:
         if code_dtype not in QUANT_CODES:
             raise TypeError(f"code_dtype must be float8_e4m3fn or int8, got {code_dtype}")
         if dtype not in (torch.float16, torch.bfloat16):
-            _bad_type(dtype)
+            raise TypeError(f"dtype must be float16 or bfloat16, got {dtype}")
         if head_dim not in (64, 128, 256):
             raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
         self.max_seq_len = max_seq_len

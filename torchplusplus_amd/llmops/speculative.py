@@ -31,4 +31,4 @@ def verify_draft(draft_tokens: torch.Tensor, target_probs: torch.Tensor, uniform
 
     Returns accepted [B] int32, path [B, T] int32 (the accepted tokens' indices,
     then -1) and next_token [B] int64 (-1 where the target's row has no mass)."""
-    return tuple(_C.verify_draft(draft_tokens, target_probs, uniforms, draft_probs, parents))
+    return _C.verify_draft(draft_tokens, target_probs, uniforms, draft_probs, parents)
