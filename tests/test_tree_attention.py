@@ -297,6 +297,6 @@ def test_refusals(dev):
                      ((torch.zeros(2, 1, 4, 512, dtype=torch.float16, device=dev),
                        torch.zeros(2, 2, 8, 512, dtype=torch.float16, device=dev),
                        torch.zeros(2, 2, 8, 512, dtype=torch.float16, device=dev), n), {})):
-        with pytest.raises(RuntimeError):
+        with pytest.raises((RuntimeError, TypeError)):
             tree_attention(*args, **kw)
     assert tree_attention(q[:0], c[:0], c[:0], n[:0]).shape == (0, 3, 4, 64)

@@ -98,6 +98,35 @@ int device_cu_count() {
   return n;
 }
 
+// ---- arrival words -----------------------------------------------------------
+constexpr unsigned kArrivalWords = 1u << 18;
+static __device__ unsigned g_arrival[kArrivalWords]; // zero when the library is loaded
+
+unsigned *arrival_words(hipStream_t st, int64_t n) {
+  static std::atomic<unsigned *> at[64];
+  static std::atomic<uint64_t> next[64];
+  int dev = -1;
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (n < 1 || n > (int64_t)kArrivalWords / 64) return nullptr;
+  if (hipStreamIsCapturing(st, &cs) != hipSuccess || hipGetDevice(&dev) != hipSuccess) {
+    (void)hipGetLastError();
+    return nullptr;
+  }
+  if (cs != hipStreamCaptureStatusNone || dev < 0 || dev >= 64) return nullptr;
+  unsigned *base = at[dev].load(std::memory_order_acquire);
+  if (!base) {
+    if (hipGetSymbolAddress((void **)&base, HIP_SYMBOL(g_arrival)) != hipSuccess) {
+      (void)hipGetLastError();
+      return nullptr;
+    }
+    at[dev].store(base, std::memory_order_release);
+  }
+  uint64_t was = next[dev].load(std::memory_order_relaxed), first;
+  do first = was + (uint64_t)n <= kArrivalWords ? was : 0; // over the end: from the start
+  while (!next[dev].compare_exchange_weak(was, first + (uint64_t)n, std::memory_order_relaxed));
+  return base + first;
+}
+
 } // namespace tpp
 
 extern "C" int tpp_prepare_device(void *stream, int *xcd_local, int *cu_count) {

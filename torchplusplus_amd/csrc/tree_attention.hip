@@ -11,8 +11,6 @@
 // with exponent 255 is NaN.
 #include "tpp_common.hpp"
 
-#include <atomic>
-
 namespace tpp {
 
 constexpr int kTreeMaxT = 64;
@@ -591,6 +589,27 @@ template <typename P> __device__ __forceinline__ unsigned lds_addr(P *x) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)x;
 }
 
+// Four floats to and from memory past the caches, for another block of the launch
+// that may run on another XCD.
+__device__ __forceinline__ void store_through(float *p, const f32x4 &x) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x2 w = {__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1])};
+    __hip_atomic_store((unsigned long long *)p + i, __builtin_bit_cast(unsigned long long, w), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
+__device__ __forceinline__ f32x4 load_through(const float *p) {
+  f32x4 x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x2 w = __builtin_bit_cast(
+        u32x2, __hip_atomic_load((const unsigned long long *)p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    x[2 * i] = __uint_as_float(w[0]), x[2 * i + 1] = __uint_as_float(w[1]);
+  }
+  return x;
+}
+
 // Merging a row's splits, in one order wherever it is done: four parts, part g the
 // splits g, g + 4, .. (four at a time), then the parts.
 constexpr int kMergeParts = 4, kMergeAhead = 4;
@@ -615,7 +634,8 @@ template <int NP> struct TreeMerge { // parts g0, g0 + step, .. of a row, chunk 
         } else {
           ma[n][j] = ws_ml[at * 2], la[n][j] = ws_ml[at * 2 + 1];
         }
-        oa[n][j] = *reinterpret_cast<const f32x4 *>(ws_o + at * D + c * 4);
+        if constexpr (HERE) oa[n][j] = load_through(ws_o + at * D + c * 4);
+        else oa[n][j] = *reinterpret_cast<const f32x4 *>(ws_o + at * D + c * 4);
       }
   }
   __device__ __forceinline__ void begin() {
@@ -669,21 +689,11 @@ __device__ __forceinline__ typename VecT<T>::v4 tree_merge_parts(const f32x4 *o,
   return ov;
 }
 
-// The splits of up to 16 rows, by the pair's last block to finish (its blocks run on
-// one XCD, so that its L2 holds what they wrote): one launch instead of two, 7.8 ->
-// 6.0 us where a sequence needs one split only.
-// A block counts itself in on a word that the call has for itself while it runs:
-// the host deals them out in turn from a ring, and the last block leaves its word at
-// zero. A word comes up again a thousand calls later (2^18 words, 256 pairs), long
-// after this one's kernel. A captured call, which would have the same words in every
-// replay, takes the second launch. (A word of the call's own workspace, set by
-// compare-and-swap for want of a zero, cost 1.5 us a block: 15 -> 61 us at 32
-// splits.) Partial sums are whole 128-byte lines of one writer, and a block reads
-// others' only here, so that its L1 has no stale copy; maxima and weights, which share
-// lines, are read past the L1.
-constexpr unsigned kTreeWords = 1u << 18;
-static __device__ unsigned g_tree_arrived[kTreeWords]; // zero when loaded
-
+// The splits of up to 16 rows, by the pair's last block to finish: one launch instead
+// of two, 7.8 -> 5.5 us where the sequences are so short that they need no merge. The
+// block counts itself in on an arrival word; what it has summed went past the caches
+// before, and comes so, since the blocks may run on any XCD. Captured calls take the
+// second launch.
 template <typename T, int D>
 __device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlock &k, int rows, int nsplit,
                                                 const float *__restrict__ ws_o, const float *__restrict__ ws_ml,
@@ -840,8 +850,16 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs p, float *__
       *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
     } else {
       const int64_t slot = ((int64_t)k.pair * rows + r) * nsplit + k.split;
-      *reinterpret_cast<f32x4 *>(ws_o + slot * D + c * 4) = os;
-      if (c == 0) ws_ml[slot * 2] = mx, ws_ml[slot * 2 + 1] = ls;
+      if (NC == 1 && arrived) {
+        store_through(ws_o + slot * D + c * 4, os);
+        if (c == 0) {
+          __hip_atomic_store(&ws_ml[slot * 2], mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __hip_atomic_store(&ws_ml[slot * 2 + 1], ls, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      } else {
+        *reinterpret_cast<f32x4 *>(ws_o + slot * D + c * 4) = os;
+        if (c == 0) ws_ml[slot * 2] = mx, ws_ml[slot * 2 + 1] = ls;
+      }
     }
   }
   if constexpr (NC == 1)
@@ -1008,26 +1026,6 @@ static TreePlan tree_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
   return pl;
 }
 
-// The words of the current device for the pairs of a call (none: nullptr).
-static unsigned *tree_words(int64_t pairs) {
-  static std::atomic<unsigned *> at[64];
-  static std::atomic<uint64_t> next[64];
-  int dev = -1;
-  if (pairs > (int64_t)kTreeWords || hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return nullptr;
-  unsigned *base = at[dev].load(std::memory_order_acquire);
-  if (!base) {
-    if (hipGetSymbolAddress((void **)&base, HIP_SYMBOL(g_tree_arrived)) != hipSuccess) {
-      (void)hipGetLastError();
-      return nullptr;
-    }
-    at[dev].store(base, std::memory_order_release);
-  }
-  uint64_t was = next[dev].load(std::memory_order_relaxed), first;
-  do first = was + (uint64_t)pairs <= kTreeWords ? was : 0; // over the end: from the start
-  while (!next[dev].compare_exchange_weak(was, first + (uint64_t)pairs, std::memory_order_relaxed));
-  return base + first;
-}
-
 } // namespace tpp
 
 using namespace tpp;
@@ -1102,12 +1100,7 @@ extern "C" int tpp_tree_attn(const void *q, const void *k, const void *v, void *
   }
   const bool by_xcd = pairs % 8 == 0;
   // the merge by a pair's last block
-  unsigned *arrived = nullptr;
-  if (pl.nsplit > 1 && pl.nc == 1 && by_xcd && xcd_grouping_holds(st, true)) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(st, &cs) != hipSuccess) (void)hipGetLastError();
-    else if (cs == hipStreamCaptureStatusNone) arrived = tree_words(pairs);
-  }
+  unsigned *arrived = pl.nsplit > 1 && pl.nc == 1 ? arrival_words(st, pairs) : nullptr;
   const dim3 grid(by_xcd ? 8 * pl.qtiles : pl.qtiles, pl.nsplit, (unsigned)(by_xcd ? pairs / 8 : pairs));
   const unsigned ninv = inv_of(pl.nsplit), hinv = inv_of((int)Hkv), ginv = inv_of(a.G);
   return TPP_DISPATCH_HALF(dtype, [&] {
