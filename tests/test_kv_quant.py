@@ -209,7 +209,7 @@ def test_refusals(dev):
     for bad in ((k, k.bfloat16(), *c, pos), (k, k[:, :2], *c, pos), (k[:1], k[:1], *c, pos),
                 (k, k, *c, pos.long()), (k, k, *c, pos[:1]), (k, k, c[0], c[1][:, :, :8], *c[2:], pos),
                 (k, k, c[0], c[1].view(torch.float8_e4m3fn), *c[2:], pos), (k, k, *c[:2], c[2][:, :, 1:], c[3], pos),
-                (odd, odd, *c, pos), (k.float(), k.float(), *c, pos), (k, k, *c, pos.cpu())):
+                (odd, odd, *c, pos), (k, k, c[0], c[0], *c[2:], pos), (k, k, *c[:2], c[2], c[2], pos), (k.float(), k.float(), *c, pos), (k, k, *c, pos.cpu())):
         with pytest.raises(RuntimeError):
             kv_quant_append(*bad)
     with pytest.raises(RuntimeError):

@@ -157,4 +157,6 @@ def test_rope_at_refusals(dev):
             rope_apply_at(*bad)
     with pytest.raises(RuntimeError, match="overlap"):
         rope_apply_at_(q[:, :1].expand(2, 3, 2, 64), None, p, f)
+    with pytest.raises(RuntimeError, match="one tensor"):
+        rope_apply_at_(q, q, p, f)
     assert rope_apply_at(q[:, :0], None, p[:, :0], f)[0].shape == (2, 0, 2, 64)

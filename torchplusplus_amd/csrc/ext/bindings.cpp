@@ -1028,6 +1028,8 @@ std::tuple<at::Tensor, at::Tensor> rope_at(const at::Tensor &q, const c10::optio
               "inv_freq must be a contiguous float64 vector of rotary_dim / 2 frequencies");
   const int64_t R = 2 * inv_freq.size(0);
   TORCH_CHECK(R >= 2 && R <= D && D % 2 == 0, "rotary_dim ", R, " does not fit head_dim ", D);
+  TORCH_CHECK(!inplace || !k.defined() || k.numel() == 0 || k.data_ptr() != q.data_ptr(),
+              "in place: q and k are one tensor");
   c10::DeviceGuard g(q.device());
   at::Tensor qo = inplace ? q : torch::empty(q.sizes(), q.options()), ko;
   if (k.defined()) ko = inplace ? k : torch::empty(k.sizes(), k.options());
@@ -1087,6 +1089,8 @@ void kv_quant_append(const at::Tensor &k, const at::Tensor &v, const at::Tensor 
   TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "k and v differ");
   const int64_t B = k.size(0), S = k.size(1), H = k.size(2), D = k.size(3);
   TORCH_CHECK(kc.size(1) == H && kc.size(3) == D, "cache shape mismatch");
+  TORCH_CHECK(kc.numel() == 0 || (kc.data_ptr() != vc.data_ptr() && ke.data_ptr() != ve.data_ptr()),
+              "K and V must have caches of their own");
   const at::Tensor pos = or_none(positions), cnt = or_none(counts);
   check_same_device(k, {&v, &kc, &pos, &cnt});
   c10::DeviceGuard g(k.device());
