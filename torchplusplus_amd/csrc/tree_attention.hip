@@ -134,9 +134,13 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
 // largest count): one would be off by 2^-9, more than the output's rounding in
 // fp16. The sum of weights is kept in fp32.
 // ---------------------------------------------------------------------------
-template <int KIND, int D> struct TreeTile {
-  static constexpr int ROWB = D * (KIND ? 1 : 2);  // bytes of a row
-  static constexpr int KT = ROWB == 256 ? 32 : 64; // keys of a tile
+// Keys of a tile: 8 KB of K, 32 or 64. The kernel of up to 16 rows takes 32 of coded
+// caches too, three blocks a CU instead of two (32 sequences of 2098 e4m3 keys, 16 / 8
+// heads, 28.9 -> 26.7 us; one of 700 int8 keys 8.8 -> 7.6 us).
+constexpr int tree_keys(int kind, int d) { return d * (kind ? 1 : 2) == 256 ? 32 : 64; }
+template <int KIND, int D, int KEYS = tree_keys(KIND, D)> struct TreeTile {
+  static constexpr int ROWB = D * (KIND ? 1 : 2); // bytes of a row
+  static constexpr int KT = KEYS;                 // keys of a tile
   static constexpr int UPR = ROWB / 16, TILEB = KT * ROWB;
   // 16-byte unit u of row r is stored at u ^ ksw(r) in a K tile: 16 lanes that
   // read one unit of 16 rows hit all 64 banks
@@ -215,11 +219,11 @@ __device__ __forceinline__ float quarter_max(float v) {
 }
 
 // One wave's part: NC groups of 16 query rows and what they have summed up.
-template <typename T, int KIND, int D, int NC> struct TreeWave {
+template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> struct TreeWave {
   typedef typename VecT<T>::v8 V8;
   typedef std::conditional_t<KIND == 0, T, bf16> PT; // type of P and V operands
   typedef typename VecT<PT>::v8 P8;
-  typedef TreeTile<KIND, D> TT;
+  typedef TreeTile<KIND, D, KEYS> TT;
   static constexpr int KT = TT::KT, ROWB = TT::ROWB, UPR = TT::UPR, EB = KIND ? 1 : 2, EX = KIND ? 1 : 0;
   static constexpr int NST = KT / 16, NX = ROWB / 64, NCS = KT / 32, NT = D / 16;
   static constexpr float kUp = KIND == 0 && !__is_same(T, bf16) ? 15.f : 0.f; // P times 2^15
@@ -334,7 +338,7 @@ template <typename T, int KIND, int D, int NC> struct TreeWave {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       if constexpr (KIND != 0)
-        static_for<16>([&](auto rr) {
+        static_for<4 * NST>([&](auto rr) {
           constexpr int r = decltype(rr)::value;
           s[i][r / 4][r % 4] *= exp_of<r % 4>(ex[0][r / 4]);
         });
@@ -384,7 +388,7 @@ template <typename T, int KIND, int D, int NC> struct TreeWave {
           for (int r = 0; r < 4; ++r) o[i][tt][r] *= alpha;
       }
       if constexpr (KIND != 0) {
-        static_for<16>([&](auto rr) {
+        static_for<4 * NST>([&](auto rr) {
           constexpr int r = decltype(rr)::value;
           s[i][r / 4][r % 4] *= exp_of<r % 4>(ex[1][r / 4]);
         });
@@ -543,8 +547,8 @@ __device__ __forceinline__ TreeBlock tree_block(const TreeArgs &p, unsigned hkv_
 // offsets of this lane's units from the tile's first row: a tile whose keys all
 // exist is one uniform address and these. Else keys past the last read its row
 // (masked).
-template <int KIND, int D, int N, int POL> struct TreeDma {
-  typedef TreeTile<KIND, D> TT;
+template <int KIND, int D, int N, int POL, int KEYS = tree_keys(KIND, D)> struct TreeDma {
+  typedef TreeTile<KIND, D, KEYS> TT;
   static constexpr int EB = KIND ? 1 : 2, KPI = 64 / TT::UPR;
   unsigned off[N];
   int j0;
@@ -689,6 +693,10 @@ __device__ __forceinline__ typename VecT<T>::v4 tree_merge_parts(const f32x4 *o,
   return ov;
 }
 
+// LDS bytes of the merge by a block: four parts of 256 / (D / 4) rows, with their
+// maxima and weights.
+template <int D> constexpr int tree_merge_lds = kMergeParts * (256 * 16 + 256 / (D / 4) * 8);
+
 // The splits of up to 16 rows, by the pair's last block to finish: one launch instead
 // of two, 7.8 -> 5.5 us where the sequences are so short that they need no merge. The
 // block counts itself in on an arrival word; what it has summed went past the caches
@@ -748,16 +756,18 @@ __device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlo
 
 // Up to 32 rows a block: the four waves share the rows and split the keys.
 template <typename T, int KIND, int D, int NC>
-__global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs p, float *__restrict__ ws_o,
+__global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel(TreeArgs p, float *__restrict__ ws_o,
                                                            float *__restrict__ ws_ml, int nsplit,
                                                            unsigned nsplit_inv, unsigned hkv_inv,
                                                            unsigned g_inv, int by_xcd,
                                                            unsigned *__restrict__ arrived) {
-  typedef TreeTile<KIND, D> TT;
-  typedef TreeWave<T, KIND, D, NC> W;
+  constexpr int KEYS = KIND && NC == 1 ? 32 : tree_keys(KIND, D);
+  typedef TreeTile<KIND, D, KEYS> TT;
+  typedef TreeWave<T, KIND, D, NC, KEYS> W;
   constexpr int KT = TT::KT, NW = 4, STRIDE = NW * KT, NDMA = TT::TILEB / 1024, C4 = D / 4, ROWS = 16 * NC;
-  static_assert(2 * TT::TILEB >= ROWS * D * 4 && (KIND == 0 || KT == 64), "a wave's rows fit its tiles");
-  __shared__ __attribute__((aligned(16))) char smem[NW * 2 * TT::TILEB];
+  static_assert(2 * TT::TILEB >= ROWS * D * 4, "a wave's rows fit its tiles");
+  constexpr int kRing = NW * 2 * TT::TILEB, kMerge = NC == 1 ? tree_merge_lds<D> : 0;
+  __shared__ __attribute__((aligned(16))) char smem[kRing > kMerge ? kRing : kMerge];
   __shared__ __attribute__((aligned(16))) unsigned s_e[NW][64];
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
 
@@ -782,7 +792,7 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs p, float *__
   const char *vs = (const char *)p.v + ((int64_t)k.b * p.v_s[0] + (int64_t)k.hk * p.v_s[1]) * W::EB;
   const int64_t eb = (int64_t)k.b * p.e_s[0] + (int64_t)k.hk * p.e_s[1];
   char *const ring = smem + w * (2 * TT::TILEB);
-  TreeDma<KIND, D, NDMA, kCpolNT> dk, dv;
+  TreeDma<KIND, D, NDMA, kCpolNT, KEYS> dk, dv;
   dk.begin(true, 0, p.k_s[2]);
   dv.begin(false, 0, p.v_s[2]);
   auto issue_k = [&](int base) {
@@ -1016,11 +1026,14 @@ static TreePlan tree_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
   pl.nc = groups > 2 ? 0 : (int)groups;
   pl.qtiles = groups > 2 ? (int)((groups + 7) / 8) : 1;
   pl.groups = (int)((groups + pl.qtiles - 1) / pl.qtiles);
-  const int lkt = D * (code ? 1 : 2) == 256 ? 5 : 6;
+  const int lkt = D * (code ? 1 : 2) == 256 || (code && pl.nc == 1) ? 5 : 6;
   pl.lstride = pl.nc ? lkt + 2 : lkt;
   const int64_t most = (Lmax + (4 << lkt) - 1) >> (lkt + 2), blocks = B * Hkv * pl.qtiles;
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  int64_t ns = 2 * (int64_t)cus / blocks; // two blocks a CU are resident
+  // Two blocks a CU, as many as are resident at once: with 3, 4 and 8 a CU 8 trees of 16
+  // over 1500-2288 keys took 25.5, 31.1 and 32.6 us for 21.4, 32 tokens over 2098 keys
+  // 31.4, 32.2 and 39.3 for 28.9, and mixed lengths gained nothing.
+  int64_t ns = 2 * (int64_t)cus / blocks;
   if (ns > most) ns = most;
   pl.nsplit = (int)(ns > 256 ? 256 : ns < 1 ? 1 : ns);
   return pl;
