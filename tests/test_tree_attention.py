@@ -225,8 +225,7 @@ def test_captured_two_graphs_and_two_streams(dev, code):
 
 @pytest.mark.gpu
 def test_many_calls_on_two_streams(dev):
-    """Calls whose splits one launch merges, on two streams at once and often
-    enough for the arrival words (2^18, 256 pairs a call) to come round."""
+    """Calls whose splits one launch merges, many times on two streams at once."""
     from torchplusplus_amd.attention import tree_attention
     b, hkv, d, room = 32, 8, 64, 1024
     q, cache, kw, _ = make(b, 1, 8, hkv, d, room, torch.bfloat16, torch.int8, 3, dev)
@@ -300,3 +299,26 @@ def test_refusals(dev):
         with pytest.raises((RuntimeError, TypeError)):
             tree_attention(*args, **kw)
     assert tree_attention(q[:0], c[:0], c[:0], n[:0]).shape == (0, 3, 4, 64)
+
+
+@pytest.mark.gpu
+def test_stream_that_lags(dev):
+    """A call that waits behind other work on its stream while another stream makes
+    thousands: their blocks count themselves in on words of their own."""
+    from torchplusplus_amd.attention import tree_attention
+    q, cache, kw, _ = make(32, 1, 8, 8, 64, 1024, torch.bfloat16, torch.int8, 4, dev)
+    lens = torch.randint(300, 1023, (32,), generator=torch.Generator().manual_seed(2)).int().to(dev)
+    want = tree_attention(q, *cache, lens, None, **kw)
+    busy = torch.randn(4096, 4096, device=dev)
+    slow, fast, got = torch.cuda.Stream(), torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(slow):
+        for _ in range(20):
+            busy @ busy
+            got.append(tree_attention(q, *cache, lens, None, **kw))
+    with torch.cuda.stream(fast):
+        wrong = torch.zeros((), dtype=torch.int32, device=dev)
+        for _ in range(1500):
+            wrong += (tree_attention(q, *cache, lens, None, **kw) != want).any()
+    torch.cuda.synchronize()
+    assert int(wrong) == 0 and all(torch.equal(x, want) for x in got)

@@ -99,15 +99,15 @@ int device_cu_count() {
 }
 
 // ---- arrival words -----------------------------------------------------------
-constexpr unsigned kArrivalWords = 1u << 18;
-static __device__ unsigned g_arrival[kArrivalWords]; // zero when the library is loaded
+constexpr int kArrivalStreams = 512, kArrivalWords = 512;
+static __device__ unsigned g_arrival[kArrivalStreams * kArrivalWords]; // zero when the library is loaded
 
 unsigned *arrival_words(hipStream_t st, int64_t n) {
   static std::atomic<unsigned *> at[64];
-  static std::atomic<uint64_t> next[64];
+  static std::atomic<uintptr_t> owner[64][kArrivalStreams]; // handle + 1
   int dev = -1;
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  if (n < 1 || n > (int64_t)kArrivalWords / 64) return nullptr;
+  if (n < 1 || n > kArrivalWords || st == hipStreamPerThread) return nullptr;
   if (hipStreamIsCapturing(st, &cs) != hipSuccess || hipGetDevice(&dev) != hipSuccess) {
     (void)hipGetLastError();
     return nullptr;
@@ -121,10 +121,14 @@ unsigned *arrival_words(hipStream_t st, int64_t n) {
     }
     at[dev].store(base, std::memory_order_release);
   }
-  uint64_t was = next[dev].load(std::memory_order_relaxed), first;
-  do first = was + (uint64_t)n <= kArrivalWords ? was : 0; // over the end: from the start
-  while (!next[dev].compare_exchange_weak(was, first + (uint64_t)n, std::memory_order_relaxed));
-  return base + first;
+  const uintptr_t me = (uintptr_t)st + 1;
+  for (int i = 0; i < kArrivalStreams; ++i) {
+    const int slot = (int)((((uintptr_t)st >> 6) + (uintptr_t)i) % kArrivalStreams);
+    uintptr_t have = owner[dev][slot].load(std::memory_order_relaxed);
+    if (have == 0 && owner[dev][slot].compare_exchange_strong(have, me, std::memory_order_relaxed)) have = me;
+    if (have == me) return base + slot * kArrivalWords;
+  }
+  return nullptr;
 }
 
 } // namespace tpp

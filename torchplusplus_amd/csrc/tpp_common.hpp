@@ -225,12 +225,12 @@ int check_launch(const char *what);
 bool xcd_grouping_holds(hipStream_t st, bool may_probe);
 // Compute units of the current device (0 if unknown).
 int device_cu_count();
-// `n` words of the current device for a launch on `st` whose blocks count themselves
-// in (one word a group of blocks; the last block leaves its word at zero again):
-// dealt out in turn from a ring of zeros, so that launches in flight at the same time
-// have words of their own. A word comes up again after 2^18 others, long after the
-// launch that had it. nullptr while the stream is being captured (every replay would
-// have the same words) or where the ring is too small.
+// `n` (at most 512) words of the current device for a launch on `st` whose blocks
+// count themselves in (one word a group of blocks; the last block leaves its word at
+// zero again). They are the stream's own, whose launches run one after another, so
+// that none in flight at the same time share them. nullptr while the stream is being
+// captured (replays may run beside it), for the per-thread stream (one handle for
+// many) and past 512 streams.
 unsigned *arrival_words(hipStream_t st, int64_t n);
 __host__ __device__ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }

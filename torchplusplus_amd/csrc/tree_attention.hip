@@ -117,9 +117,8 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
 // each wave streams its own tiles of KT keys (8 KB of K) by LDS-DMA into a
 // private slot: no barrier in the loop, the next K tile is requested once this
 // one's fragments are in registers, the next V tile after this one's. Waves are
-// merged through LDS, splits by tree_merge_kernel (a second launch: arrival
-// counters would have to be shared by calls, which two replayed graphs may not
-// do).
+// merged through LDS, splits by the pair's last block (tree_merge_here) or by
+// tree_merge_kernel, a second launch.
 //
 // Key order: S^T gives lane quarter u the keys 16 st + 4 u + i (i = 0 .. 3) of
 // tile st. The product with V takes them as its K index 8 u + j of step c: j < 4
@@ -701,7 +700,7 @@ template <int D> constexpr int tree_merge_lds = kMergeParts * (256 * 16 + 256 / 
 // of two, 7.8 -> 5.5 us where the sequences are so short that they need no merge. The
 // block counts itself in on an arrival word; what it has summed went past the caches
 // before, and comes so, since the blocks may run on any XCD. Captured calls take the
-// second launch.
+// second launch, as do more rows: 32 of 8 sequences took 32.0 us so for 21.4.
 template <typename T, int D>
 __device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlock &k, int rows, int nsplit,
                                                 const float *__restrict__ ws_o, const float *__restrict__ ws_ml,
