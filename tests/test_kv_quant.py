@@ -216,3 +216,13 @@ def test_refusals(dev):
         kv_quant_read(*c, 17)
     with pytest.raises(RuntimeError):
         kv_quant_read(*c, -1)
+
+
+@pytest.mark.gpu
+def test_append_refuses_rows_that_sequences_share(dev):
+    c = _cache(1, 2, 16, 64, torch.int8, dev)
+    k = torch.zeros(2, 3, 2, 64, dtype=torch.float16, device=dev)
+    shared = [x.expand(2, *x.shape[1:]) for x in c]
+    with pytest.raises(RuntimeError, match="of their own"):
+        kv_quant_append(k, k, *shared, 0)
+    assert kv_quant_read(*shared, 5)[0].shape == (2, 2, 5, 64)  # reading a shared prompt is fine

@@ -322,3 +322,16 @@ def test_stream_that_lags(dev):
             wrong += (tree_attention(q, *cache, lens, None, **kw) != want).any()
     torch.cuda.synchronize()
     assert int(wrong) == 0 and all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.gpu
+def test_refuses_an_out_that_is_not_its_own(dev):
+    from torchplusplus_amd.attention import tree_attention
+    q = torch.zeros(2, 3, 4, 64, dtype=torch.float16, device=dev)
+    c = torch.zeros(2, 4, 3, 64, dtype=torch.float16, device=dev)
+    n = torch.zeros(2, dtype=torch.int32, device=dev)
+    for out in (q, c.view(2, 3, 4, 64), q[:1].expand(2, 3, 4, 64), torch.zeros_like(q)[:, :1].expand(2, 3, 4, 64)):
+        with pytest.raises(RuntimeError, match="of its own"):
+            tree_attention(q, c, c.clone(), n, out=out)
+    both = torch.zeros(4, 3, 4, 64, dtype=torch.float16, device=dev)  # one buffer, two halves
+    assert tree_attention(both[:2], c, c, n, out=both[2:]).data_ptr() == both[2:].data_ptr()
