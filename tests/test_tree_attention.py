@@ -335,3 +335,30 @@ def test_refuses_an_out_that_is_not_its_own(dev):
             tree_attention(q, c, c.clone(), n, out=out)
     both = torch.zeros(4, 3, 4, 64, dtype=torch.float16, device=dev)  # one buffer, two halves
     assert tree_attention(both[:2], c, c, n, out=both[2:]).data_ptr() == both[2:].data_ptr()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("t,step", [(1, 0.05), (1, 0.4), (24, 0.05), (24, 0.4), (6, -0.05)])
+def test_scores_that_rise_or_fall_along_the_keys(dev, dtype, code, t, step):
+    """Scores that pass the running reference maximum by less and by more than its
+    step of 2^8 from tile to tile, within a wave's tiles and between splits."""
+    from torchplusplus_amd.llmops.kvcache import kv_quant_append
+    b, hq, hkv, d, room, n = 2, 8, 4, 128, 1024, 900
+    g = torch.Generator().manual_seed(t)
+    q = torch.full((b, t, hq, d), 1.0)
+    at = torch.arange(room, dtype=torch.float64).view(1, room, 1, 1)
+    k = (at * step / d ** 0.5 + torch.randn(b, room, hkv, d, generator=g) * 0.02).to(dtype)
+    v = torch.randn(b, room, hkv, d, generator=g).to(dtype)
+    q, k, v = q.to(dtype).to(dev), k.to(dev), v.to(dev)
+    if code is None:
+        cache, kw = [x.transpose(1, 2).contiguous() for x in (k, v)], {}
+        vals = [x.cpu() for x in cache]
+    else:
+        cache = [torch.zeros(b, hkv, room, d, dtype=torch.uint8, device=dev).view(code) for _ in "kv"]
+        exps = [torch.full((b, hkv, room), 127, dtype=torch.uint8, device=dev) for _ in "kv"]
+        kv_quant_append(k, v, *cache, *exps, 0)
+        kw = dict(k_exps=exps[0], v_exps=exps[1])
+        vals = [osp.values(c.cpu(), e.cpu()) for c, e in zip(cache, exps)]
+    check(q, cache, kw, vals, torch.tensor([n, 37], dtype=torch.int32), None, dtype, (code, t, step))
