@@ -362,3 +362,18 @@ def test_scores_that_rise_or_fall_along_the_keys(dev, dtype, code, t, step):
         kw = dict(k_exps=exps[0], v_exps=exps[1])
         vals = [osp.values(c.cpu(), e.cpu()) for c, e in zip(cache, exps)]
     check(q, cache, kw, vals, torch.tensor([n, 37], dtype=torch.int32), None, dtype, (code, t, step))
+
+
+@pytest.mark.gpu
+def test_thousands_of_heads_of_one_kv_head(dev):
+    """64 x 20000 query rows of one KV head: row / G by a multiplication in 32 bits
+    would be off by one (row * G passes 2^32)."""
+    from torchplusplus_amd.attention import tree_attention
+    t, hq, d, room = 64, 20000, 64, 128
+    q, cache, kw, vals = make(1, t, 16, 1, d, room, torch.float16, None, 6, dev)
+    lens, parents = torch.tensor([5], dtype=torch.int32), tree(1, t, 2)
+    many = torch.zeros(1, t, hq, d, dtype=torch.float16, device=dev)
+    many[:, :, :8], many[:, :, -8:] = q[:, :, :8], q[:, :, 8:]
+    got = tree_attention(many, *cache, lens.to(dev), parents.to(dev), **kw)
+    got = torch.cat((got[:, :, :8], got[:, :, -8:]), 2)
+    check(q, cache, kw, vals, lens, parents, torch.float16, "first and last heads", got=got)

@@ -1098,6 +1098,8 @@ extern "C" int tpp_tree_attn(const void *q, const void *k, const void *v, void *
     low_o |= (uint64_t)(a.o_s[i] * 2);
   }
   bool tiles = (D == 64 || D == 128) && !(low & 15) && !(low_o & 7) && B * Hkv <= 65535;
+  // (div_inv of a row by G is exact below this)
+  tiles = tiles && (uint64_t)(T * a.G) * (uint64_t)a.G < 1ull << 32;
   // (a tile's rows by 32-bit byte offsets)
   for (int64_t r : {a.k_s[2], a.v_s[2]}) tiles = tiles && r >= 0 && r < (1 << 23);
   if (code)
