@@ -83,6 +83,28 @@ constexpr int kPrefillQG = 1;
 // overlaps the other's MFMAs
 constexpr int kPrefillWaves = 8;
 
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32x32(typename VecT<T>::v8 a, typename VecT<T>::v8 b,
+                                            f32x16 c) {
+  if constexpr (__is_same(T, bf16))
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// V tiles are stored row-major like K ([key][16-byte unit]) and read as
+// MFMA operands with ds_read_b64_tr_b16, whose 16-lane groups return lane
+// 4a+b the b-th 16-bit element of the words lanes a, a+4, a+8, a+12 point at:
+// pointing lane a'+4c' at V[k0 + c'][d0 + 4a'] gives lane l of the group
+// V[k0 + 0..3][d0 + l]. Unit u of key row r is stored at u ^ vswz(r): the
+// 32 lanes one read cycle serves (4 keys x 32 columns) then hit distinct
+// banks (D = 128: 256-byte rows, XOR 4*(r%4); D = 64: 128-byte rows, two
+// per bank row, XOR 4*((r/2)%2)).
+template <int D> __device__ __forceinline__ int vswz(int r) {
+  if constexpr (D == 128) return 4 * (r & 3);
+  else return 4 * ((r >> 1) & 1);
+}
+
 // Tiles [t_begin, t_end) of `kt` keys that queries q0 .. q_last see (causal
 // and window bounds are aligned bottom-right: query i sits at key i + Sk - Sq).
 struct KeyBand {

@@ -327,29 +327,7 @@ template <int N, typename F> __device__ __forceinline__ void static_for(F &&f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-// ---- attention tiles and splits (attention.hip, tree_attention.hip) ----------
-template <typename T>
-__device__ __forceinline__ f32x16 mfma32x32(typename VecT<T>::v8 a, typename VecT<T>::v8 b,
-                                            f32x16 c) {
-  if constexpr (__is_same(T, bf16))
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// V tiles are stored row-major like K ([key][16-byte unit]) and read as
-// MFMA operands with ds_read_b64_tr_b16, whose 16-lane groups return lane
-// 4a+b the b-th 16-bit element of the words lanes a, a+4, a+8, a+12 point at:
-// pointing lane a'+4c' at V[k0 + c'][d0 + 4a'] gives lane l of the group
-// V[k0 + 0..3][d0 + l]. Unit u of key row r is stored at u ^ vswz(r): the
-// 32 lanes one read cycle serves (4 keys x 32 columns) then hit distinct
-// banks (D = 128: 256-byte rows, XOR 4*(r%4); D = 64: 128-byte rows, two
-// per bank row, XOR 4*((r/2)%2)).
-template <int D> __device__ __forceinline__ int vswz(int r) {
-  if constexpr (D == 128) return 4 * (r & 3);
-  else return 4 * ((r >> 1) & 1);
-}
-
+// ---- attention splits (attention.hip, tree_attention.hip) ---------------------
 // x / n as a multiply by inv = 2^32 / n rounded up (0 for n = 1), exact for
 // x * n < 2^32. A decode attention block's first loads wait for its split and sequence:
 // two integer divisions there (~60 dependent instructions) cost 0.2 us.
