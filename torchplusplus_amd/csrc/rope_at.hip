@@ -17,7 +17,9 @@
 //
 // Bound by HBM: each element is read once and written once. A thread owns PW
 // pairs of one token (16-byte accesses at PW = 8) in one head, or in four where there
-// is work enough: their loads are in flight while the angles are worked out.
+// is work enough: their loads are in flight while the angles are worked out (4 x 4096
+// tokens, 16 + 8 heads of 128, half of each turned: 45.0 -> 41.6 us, 4.84 TB/s, 95% of
+// a copy's rate). Non-temporal stores were 19% slower.
 #include "tpp_common.hpp"
 
 namespace tpp {

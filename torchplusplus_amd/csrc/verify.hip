@@ -28,7 +28,8 @@
 // a walk in registers): cheaper than a launch of its own, or a barrier. Every wave
 // of the second scans the chunks' sums. What bounds it: the latency of two launches
 // and of four dependent trips to memory in each; the rows are B V 4 bytes (with q
-// twice that).
+// twice that). 8 chains of 5 over 150000 tokens 10.5 us, 16 trees of 31 11.6; in one
+// launch, the last block of a sequence to finish picking, 11.9 for the chains.
 #include "tpp_common.hpp"
 
 namespace tpp {
