@@ -130,14 +130,19 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
 // Codes stay codes up to the registers: a tile of codes has half the bytes and
 // twice the keys. K fragments become T (exact: e4m3 and int8 values fit both
 // types), V fragments bfloat16; the exponents are applied to the scores and to
-// the probabilities. P is the sum of two values of V's type (16 bits of it in
-// bfloat16, 22 in fp16, there times 2^15 so that weights down to 2^-39 of the
-// largest count): one would be off by 2^-9, more than the output's rounding in
-// fp16. The sum of weights is kept in fp32.
+// the probabilities. P keeps its fp32 bits: it is the sum of three values of V's
+// type, whose products are summed in fp32. In bfloat16 those are 8 bits each, all of
+// P down to 2^-110. In fp16 they are 11 bits each at 2^15, 2^26 and 2^37 times P (1 at
+// most), each folded into the next at its scale: 22 bits of a weight down to 2^-40
+// of the largest, 11 to 2^-51, and what is cut is below 2^-61, so that V up to 65504
+// over 2^20 keys loses less than half of fp16's least step. (Two parts at one scale
+// lost every weight below 2^-39, and in bfloat16 the last 8 bits.)
 // ---------------------------------------------------------------------------
-// Keys of a tile: 8 KB of K, 32 or 64. The kernel of up to 16 rows takes 32 of coded
-// caches too, three blocks a CU instead of two (32 sequences of 2098 e4m3 keys, 16 / 8
-// heads, 28.9 -> 26.7 us; one of 700 int8 keys 8.8 -> 7.6 us).
+// Keys of a tile: 8 KB of K, 32 or 64. The kernel of up to 32 rows takes 32 of coded
+// caches too: of 16 rows three blocks a CU instead of two (32 sequences of 2098 e4m3
+// keys, 16 / 8 heads, 28.9 -> 26.7 us; one of 700 int8 keys 8.8 -> 7.6 us), of 32 rows
+// the three parts of P for half the keys, which stay in registers (8 trees of 16 over
+// 1500-2288 e4m3 keys, 37.5 -> 20.0 us).
 constexpr int tree_keys(int kind, int d) { return d * (kind ? 1 : 2) == 256 ? 32 : 64; }
 template <int KIND, int D, int KEYS = tree_keys(KIND, D)> struct TreeTile {
   static constexpr int ROWB = D * (KIND ? 1 : 2); // bytes of a row
@@ -187,27 +192,33 @@ template <int I> __device__ __forceinline__ float exp_of(unsigned w) {
   return __uint_as_float(((w >> (8 * I)) & 0xffu) << 23);
 }
 
-// Eight probabilities, a's then b's, as the sum of two values of type PT each,
-// both cut and not rounded, so that lo is what hi leaves.
+// Eight probabilities, a's then b's, as the sum of three values of type PT each, all
+// cut and not rounded: a part is what the ones ahead leave, in fp16 times 2^11 more than
+// the one ahead of it (kPartUp), so that it does not fall among the subnormals.
+constexpr float kPartUp = 2048.f;
 template <typename PT>
-__device__ __forceinline__ void two_parts(const f32x4 &a, const f32x4 &b, typename VecT<PT>::v8 &hi,
-                                          typename VecT<PT>::v8 &lo) {
-  u32x4 h, l;
+__device__ __forceinline__ void three_parts(const f32x4 &a, const f32x4 &b, typename VecT<PT>::v8 (&r)[3]) {
+  u32x4 w[3];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float x = j < 2 ? a[2 * j] : b[2 * j - 4], y = j < 2 ? a[2 * j + 1] : b[2 * j - 3];
-    if constexpr (__is_same(PT, bf16)) { // a bfloat16 is the upper half of a float
-      h[j] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
-      const float rx = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-      const float ry = y - __uint_as_float(__float_as_uint(y) & 0xffff0000u);
-      l[j] = __builtin_amdgcn_perm(__float_as_uint(ry), __float_as_uint(rx), 0x07060302u);
-    } else {
-      const auto t = __builtin_amdgcn_cvt_pkrtz(x, y);
-      h[j] = __builtin_bit_cast(unsigned, t);
-      l[j] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(x - (float)t[0], y - (float)t[1]));
+    float x = j < 2 ? a[2 * j] : b[2 * j - 4], y = j < 2 ? a[2 * j + 1] : b[2 * j - 3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      if constexpr (__is_same(PT, bf16)) { // a bfloat16 is the upper half of a float
+        w[i][j] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        if (i < 2) {
+          x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+          y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+        }
+      } else {
+        const auto t = __builtin_amdgcn_cvt_pkrtz(x, y);
+        w[i][j] = __builtin_bit_cast(unsigned, t);
+        if (i < 2) x = (x - (float)t[0]) * kPartUp, y = (y - (float)t[1]) * kPartUp;
+      }
     }
   }
-  hi = __builtin_bit_cast(typename VecT<PT>::v8, h), lo = __builtin_bit_cast(typename VecT<PT>::v8, l);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) r[i] = __builtin_bit_cast(typename VecT<PT>::v8, w[i]);
 }
 
 // the largest over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -230,7 +241,8 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
   // The reference maximum moves when a tile's passes it by 2^8 (76.2 -> 74.6 us), for
   // that rescales every sum; not in fp16, whose P has no such room.
   static constexpr float kLazy = KIND == 0 && !__is_same(T, bf16) ? 0.f : 8.f;
-  static constexpr float kUp = KIND == 0 && !__is_same(T, bf16) ? 15.f : 0.f; // P times 2^15
+  static constexpr bool kApart = !__is_same(PT, bf16);  // parts of P have scales of their own
+  static constexpr float kUp = kApart ? 15.f : 0.f;     // P times 2^15
 
   V8 qf[NC][D / 32];
   unsigned long long see[NC];
@@ -343,7 +355,7 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
     });
 
     __builtin_amdgcn_s_setprio(0);
-    P8 hi[NC][NCS], lo[NC][NCS];
+    P8 pt[NC][NCS][3];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       if constexpr (KIND != 0)
@@ -413,18 +425,30 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
         }
       }
 #pragma unroll
-      for (int c = 0; c < NCS; ++c) two_parts<PT>(s[i][2 * c], s[i][2 * c + 1], hi[i][c], lo[i][c]);
+      for (int c = 0; c < NCS; ++c) three_parts<PT>(s[i][2 * c], s[i][2 * c + 1], pt[i][c]);
     }
 
     wait_v();
     __builtin_amdgcn_s_setprio(1);
-    constexpr int R = KIND ? 4 : 8, NG = NCS * NT / 4; // four d tiles of a step at a time
+    // DT d tiles of a step at a time
+    constexpr int DT = KIND == 0 && NC == 2 ? 2 : 4, R = KIND ? DT : 2 * DT, NG = NCS * NT / DT;
+    // fp16 parts have scales of their own: t to the scale of the part ahead, plus y
+    auto fold = [](auto &t, auto y) {
+#pragma unroll
+      for (int j = 0; j < (NC == 1 ? 4 : 2); ++j)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const f32x4 a = y(j, i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[j][i][e] = fmaf(t[j][i][e], 1.f / kPartUp, a[e]);
+        }
+    };
     typedef std::conditional_t<KIND == 0, s16x4, u32x2> VR;
     VR vr[2][R];
     auto vfrag = [&](auto gg) {
-      constexpr int g = decltype(gg)::value, c = g / (NT / 4), t0 = 4 * (g % (NT / 4));
+      constexpr int g = decltype(gg)::value, c = g / (NT / DT), t0 = DT * (g % (NT / DT));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < DT; ++j) {
         if constexpr (KIND == 0) {
           vr[g % 2][2 * j] = lds_read_tr16<c * 32 * ROWB>(vo[t0 + j] + off);
           vr[g % 2][2 * j + 1] = lds_read_tr16<c * 32 * ROWB + 16 * ROWB>(vo[t0 + j] + off);
@@ -435,7 +459,7 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
     };
     vfrag(std::integral_constant<int, 0>{});
     static_for<NG>([&](auto gg) {
-      constexpr int g = decltype(gg)::value, c = g / (NT / 4), t0 = 4 * (g % (NT / 4));
+      constexpr int g = decltype(gg)::value, c = g / (NT / DT), t0 = DT * (g % (NT / DT));
       if constexpr (g + 1 < NG) vfrag(std::integral_constant<int, g + 1>{});
       lds_wait_tied<(g + 1 < NG ? R : 0)>(vr[g % 2]);
       if constexpr (g + 1 == NG) {
@@ -443,10 +467,12 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
         after_v();
       }
       __builtin_amdgcn_sched_barrier(0);
+      // the parts of P, the least first
       constexpr int JG = NC == 1 ? 4 : 2;
 #pragma unroll
-      for (int j0 = 0; j0 < 4; j0 += JG) {
+      for (int j0 = 0; j0 < DT; j0 += JG) {
         P8 f[JG];
+        f32x4 t[JG][NC];
 #pragma unroll
         for (int j = 0; j < JG; ++j) {
           if constexpr (KIND == 0) {
@@ -457,12 +483,19 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
             f[j] = codes8<PT, KIND>(vr[g % 2][j0 + j][0], vr[g % 2][j0 + j][1]);
           }
 #pragma unroll
-          for (int i = 0; i < NC; ++i) o[i][t0 + j0 + j] = mfma16x16<PT>(f[j], lo[i][c], o[i][t0 + j0 + j]);
+          for (int i = 0; i < NC; ++i)
+            t[j][i] = mfma16x16<PT>(f[j], pt[i][c][2], kApart ? f32x4{0.f, 0.f, 0.f, 0.f} : o[i][t0 + j0 + j]);
         }
+        if constexpr (kApart) fold(t, [](int, int) { return f32x4{0.f, 0.f, 0.f, 0.f}; });
 #pragma unroll
         for (int j = 0; j < JG; ++j)
 #pragma unroll
-          for (int i = 0; i < NC; ++i) o[i][t0 + j0 + j] = mfma16x16<PT>(f[j], hi[i][c], o[i][t0 + j0 + j]);
+          for (int i = 0; i < NC; ++i) t[j][i] = mfma16x16<PT>(f[j], pt[i][c][1], t[j][i]);
+        if constexpr (kApart) fold(t, [&](int j, int i) { return o[i][t0 + j0 + j]; });
+#pragma unroll
+        for (int j = 0; j < JG; ++j)
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i][t0 + j0 + j] = mfma16x16<PT>(f[j], pt[i][c][0], t[j][i]);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -772,12 +805,13 @@ __global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel
                                                            unsigned nsplit_inv, unsigned hkv_inv,
                                                            unsigned g_inv, int by_xcd,
                                                            unsigned *__restrict__ arrived) {
-  constexpr int KEYS = KIND && NC == 1 ? 32 : tree_keys(KIND, D);
+  constexpr int KEYS = KIND ? 32 : tree_keys(KIND, D);
   typedef TreeTile<KIND, D, KEYS> TT;
   typedef TreeWave<T, KIND, D, NC, KEYS> W;
   constexpr int KT = TT::KT, NW = 4, STRIDE = NW * KT, NDMA = TT::TILEB / 1024, C4 = D / 4, ROWS = 16 * NC;
-  static_assert(2 * TT::TILEB >= ROWS * D * 4, "a wave's rows fit its tiles");
-  constexpr int kRing = NW * 2 * TT::TILEB, kMerge = NC == 1 ? tree_merge_lds<D> : 0;
+  // a wave's tiles, later its rows
+  constexpr int SLOT = 2 * TT::TILEB > ROWS * D * 4 ? 2 * TT::TILEB : ROWS * D * 4;
+  constexpr int kRing = NW * SLOT, kMerge = NC == 1 ? tree_merge_lds<D> : 0;
   __shared__ __attribute__((aligned(16))) char smem[kRing > kMerge ? kRing : kMerge];
   __shared__ __attribute__((aligned(16))) unsigned s_e[NW][64];
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
@@ -802,7 +836,7 @@ __global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel
   const char *ks = (const char *)p.k + ((int64_t)k.b * p.k_s[0] + (int64_t)k.hk * p.k_s[1]) * W::EB;
   const char *vs = (const char *)p.v + ((int64_t)k.b * p.v_s[0] + (int64_t)k.hk * p.v_s[1]) * W::EB;
   const int64_t eb = (int64_t)k.b * p.e_s[0] + (int64_t)k.hk * p.e_s[1];
-  char *const ring = smem + w * (2 * TT::TILEB);
+  char *const ring = smem + w * SLOT;
   TreeDma<KIND, D, NDMA, kCpolNT, KEYS> dk, dv;
   dk.begin(true, 0, p.k_s[2]);
   dv.begin(false, 0, p.v_s[2]);
@@ -858,7 +892,7 @@ __global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel
     for (int ww = 0; ww < NW; ++ww) {
       const float cf = __builtin_amdgcn_exp2f(s_m[ww][q] - mu);
       ls += s_l[ww][q] * cf;
-      const f32x4 pr = reinterpret_cast<const f32x4 *>(smem + ww * (2 * TT::TILEB))[q * C4 + (c ^ (q & (C4 - 1)))];
+      const f32x4 pr = reinterpret_cast<const f32x4 *>(smem + ww * SLOT)[q * C4 + (c ^ (q & (C4 - 1)))];
 #pragma unroll
       for (int e = 0; e < 4; ++e) os[e] += pr[e] * cf;
     }
@@ -1039,7 +1073,7 @@ static TreePlan tree_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
   pl.nc = groups > 2 ? 0 : (int)groups;
   pl.qtiles = groups > 2 ? (int)((groups + 7) / 8) : 1;
   pl.groups = (int)((groups + pl.qtiles - 1) / pl.qtiles);
-  const int lkt = D * (code ? 1 : 2) == 256 || (code && pl.nc == 1) ? 5 : 6;
+  const int lkt = D * (code ? 1 : 2) == 256 || (code && pl.nc) ? 5 : 6;
   pl.lstride = pl.nc ? lkt + 2 : lkt;
   const int64_t most = (Lmax + (4 << lkt) - 1) >> (lkt + 2), blocks = B * Hkv * pl.qtiles;
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
