@@ -520,7 +520,7 @@ int tpp_decode_force_sync_error(void *workspace, int kernel, void *stream);
  * earlier token, or -1: the context; any other value is padding and sees
  * nothing, nor do its children; NULL: a chain). Lengths are limited to [0,
  * Lmax]; a token whose own key would lie past Lmax sees nothing. Rows that see
- * nothing are 0. code 0:
+ * nothing are 0, rows whose scores are all -inf NaN. code 0:
  * caches of `dtype`; a tpp_code: 8-bit codes with k_exps / v_exps [B, Hkv, Lmax]
  * as written by tpp_kv_quant_append. softmax_scale <= 0 means 1/sqrt(D). D <=
  * 256. Next to flash_attn_func with Sq = 1 over the cache prefix

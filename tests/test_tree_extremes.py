@@ -1,0 +1,43 @@
+"""tree_attention where scores or values are infinite or near the type's end: every
+kernel (the sizes of test_tree_precision.py) answers as the formula does. Queries are
+one-hot and the scale is 1, so that a score is one element of a key, exactly."""
+import math
+
+import pytest
+import torch
+
+from tests.test_tree_precision import SHAPES, make
+
+INF = math.inf
+
+
+def attend(dev, shape, scores, values, dtype, code, n, par):
+    from torchplusplus_amd.attention import tree_attention
+    q, cache, kw = make(shape, scores, values, dtype, code, dev)
+    lens = torch.full((shape[0],), n, dtype=torch.int32)
+    return tree_attention(q, *cache, lens.to(dev), par.to(dev), softmax_scale=1.0, **kw).float().cpu()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("n", [20, 704])
+def test_scores_of_minus_infinity(dev, dtype, shape, n):
+    """All visible scores -inf: NaN, as the softmax of such a row is. One finite score
+    among them: its value. A token that sees nothing: 0."""
+    b, t = shape[:2]
+    scores, values = [-INF] * (n + 64), [3.0] * (n + 64)
+    par = torch.full((b, t), -1, dtype=torch.int32)
+    finite = t - 1 if t > 1 else None  # the last token's own key
+    if finite is not None:
+        scores[n + finite], values[n + finite] = 1.0, 7.0
+    if t > 2:
+        par[:, 1] = -2
+    o = attend(dev, shape, scores, values, dtype, None, n, par)
+    for i in range(t):
+        if t > 2 and i == 1:
+            assert bool((o[:, i] == 0).all())
+        elif i == finite:
+            assert bool((o[:, i] == 7.0).all())
+        else:
+            assert bool(torch.isnan(o[:, i]).all()), f"token {i}: {o[0, i, 0, :4]}"

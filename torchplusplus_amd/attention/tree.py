@@ -25,7 +25,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     the context, itself and its ancestors by `parents` (int32 [B, T]: an earlier
     token, or -1 for the context; any other value is padding and sees nothing,
     nor do its children; None: a chain). Rows that see nothing are 0, as are
-    those of tokens past the cache's end.
+    those of tokens past the cache's end; a row whose scores are all -inf is NaN.
 
     Caches of q's dtype, or of float8_e4m3fn / int8 codes with the exponent
     bytes k_exps, v_exps of a QuantKVCache. T = 1 is a decode step over either.

@@ -6,7 +6,8 @@
 // query heads share a KV head). `parents` gives each drafted token's parent:
 // an earlier token, or -1 for the context's last; any other value marks
 // padding, which sees nothing, as do its children. One token per sequence is
-// decode over the cache. A row that sees nothing is 0.
+// decode over the cache. A row that sees nothing is 0; one that sees scores of -inf
+// alone is NaN, as its softmax is.
 // A code's value is code * 2^(exponent byte - 127), see kv_quant.hip; a row
 // with exponent 255 is NaN.
 #include "tpp_common.hpp"
@@ -502,15 +503,16 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
     __builtin_amdgcn_s_setprio(0);
   }
 
-  // l, m (times the scale) over the four lanes of a row; rows that see nothing
-  // have none. True where a sum is not finite.
+  // l over the four lanes of a row. A row that sees nothing gets a weight of 1 on
+  // nothing: 0 after the merges, where a row of scores of -inf, with no weight, is 0 / 0.
+  // True where a sum is not finite.
   __device__ __forceinline__ bool end(const TreeArgs &p) {
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       l[i] += __shfl_xor(l[i], 16, kWave);
       l[i] += __shfl_xor(l[i], 32, kWave);
-      if (!see[i]) l[i] = 0.f, m[i] = -INFINITY;
+      if (!see[i]) l[i] = 1.f, m[i] = 0.f;
 #pragma unroll
       for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
@@ -731,7 +733,7 @@ __device__ __forceinline__ typename VecT<T>::v4 tree_merge_parts(const f32x4 *o,
     for (int e = 0; e < 4; ++e) os[e] += x[e] * cf;
   }
   typename VecT<T>::v4 ov;
-  const float inv = ls != 0.f ? 1.f / ls : 0.f; // (NaN stays NaN)
+  const float inv = 1.f / ls;
 #pragma unroll
   for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
   return ov;
@@ -899,7 +901,7 @@ __global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel
     if (k.live == 1) {
       T *op = W::row_of((T *)p.o, p.o_s, p, k.b, k.hk, r, div_inv((unsigned)r, g_inv));
       typename VecT<T>::v4 ov;
-      const float inv = ls != 0.f ? 1.f / ls : 0.f; // (NaN stays NaN)
+      const float inv = 1.f / ls;
 #pragma unroll
       for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
       *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
@@ -985,7 +987,7 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(TreeArgs p, float *__
       const int r = row0[i] + q;
       if (k.live == 1) {
         T *op = W::row_of((T *)p.o, p.o_s, p, k.b, k.hk, r, div_inv((unsigned)r, g_inv)) + d;
-        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const float inv = 1.f / l;
         if constexpr (M == 4) {
           typename VecT<T>::v4 ov;
 #pragma unroll
