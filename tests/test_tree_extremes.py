@@ -41,3 +41,23 @@ def test_scores_of_minus_infinity(dev, dtype, shape, n):
             assert bool((o[:, i] == 7.0).all())
         else:
             assert bool(torch.isnan(o[:, i]).all()), f"token {i}: {o[0, i, 0, :4]}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("n,at", [(20, 5), (704, 3), (704, 600)])
+def test_infinite_values_in_the_context(dev, dtype, shape, n, at):
+    """A value of infinity that all tokens see, of any weight above 0: infinity of its
+    sign; two of opposite signs: NaN."""
+    b, t = shape[:2]
+    g = torch.Generator().manual_seed(at)
+    par = torch.full((b, t), -1, dtype=torch.int32)
+    scores = (torch.randint(-32, 33, (n + 64,), generator=g).float() / 16).tolist()
+    scores[1] = 3.0
+    for where in (at, 1):  # some weight, and the largest
+        values = torch.randint(-3, 4, (n + 64,), generator=g).float().tolist()
+        values[where] = -INF
+        assert bool((attend(dev, shape, scores, values, dtype, None, n, par) == -INF).all())
+        values[where + 7] = INF
+        assert bool(torch.isnan(attend(dev, shape, scores, values, dtype, None, n, par)).all())

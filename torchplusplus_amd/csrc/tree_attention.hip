@@ -528,10 +528,11 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
   }
 
   // A row behind the context that is not finite, times a weight of 0, is a NaN in
-  // the products of those that do not see it. A wave that had such a tile and has
-  // a sum that is not finite sums again, key by key over what each row sees: its
-  // n tiles from key `first`, `stride` apart, up to k_end. put(i, q, d, x): the
-  // sum of element d of row q of group i.
+  // the products of those that do not see it; so is an infinity among 16-bit values
+  // times a part of P that is 0. A wave that had such a tile and has a sum that is not
+  // finite sums again, key by key over what each row sees: its n tiles from key
+  // `first`, `stride` apart, up to k_end. put(i, q, d, x): the sum of element d of row
+  // q of group i.
   template <typename PUT>
   __device__ __forceinline__ void again(const TreeArgs &p, int b, int hk, const char *ks, const char *vs, int64_t eb,
                                         int first, int stride, int n, int k_end, int L, unsigned g_inv,
@@ -875,7 +876,7 @@ __global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel
     for (int tt = 0; tt < W::NT; ++tt) part[r * C4 + ((tt * 4 + u4) ^ (r & (C4 - 1)))] = wv.o[i][tt];
     if (u4 == 0) s_m[w][r] = wv.top(p, i), s_l[w][r] = wv.l[i];
   }
-  if (n > 0 && first + (n - 1) * STRIDE + KT > k.L && __any(odd))
+  if (n > 0 && (KIND == 0 || first + (n - 1) * STRIDE + KT > k.L) && __any(odd))
     wv.again(p, k.b, k.hk, ks, vs, eb, first, STRIDE, n, k_end, k.L, g_inv, row0, rows, [&](int i, int q, int d, float x) {
       const int r = i * 16 + q;
       reinterpret_cast<float *>(part + r * C4 + ((d / 4) ^ (r & (C4 - 1))))[d % 4] = x;
@@ -1000,7 +1001,7 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(TreeArgs p, float *__
         *reinterpret_cast<decltype(x) *>(ws_o + (((int64_t)k.pair * rows + r) * nsplit + k.split) * D + d) = x;
       }
     };
-    const bool redo = first + n * KT > k.L && __any(odd);
+    const bool redo = (KIND == 0 || first + n * KT > k.L) && __any(odd);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int q = lane & 15, u4 = lane >> 4;
