@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from tests.test_tree_attention import CODES
 from tests.test_tree_precision import SHAPES, make
 
 INF = math.inf
@@ -61,3 +62,26 @@ def test_infinite_values_in_the_context(dev, dtype, shape, n, at):
         assert bool((attend(dev, shape, scores, values, dtype, None, n, par) == -INF).all())
         values[where + 7] = INF
         assert bool(torch.isnan(attend(dev, shape, scores, values, dtype, None, n, par)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("t,hq,d", [(1, 1, 128), (4, 2, 64), (16, 2, 128), (33, 1, 64), (12, 4, 128), (1, 1, 96)])
+def test_values_near_the_end_of_bfloat16(dev, code, t, hq, d):
+    """One value of 2^126 among keys whose scores rise by less than 8 log(2) along a
+    wave's tiles (512 pairs: one block has all of a pair's keys): weights above 1 would
+    leave fp32's range. Tolerance: the output's rounding, the weights' error, (2 ln 2 *
+    7.3 + 2) 2^-24, and the roundings of their sum, 10 tiles and 32 a tile: 2^-18."""
+    from torchplusplus_amd.attention import tree_attention
+    b, hkv, n = 64, 8, 300
+    scores = [0.0] * 160 + [5.0] * (n - 96)
+    values = [0.0] * (n + 64)
+    values[n - 10] = 2.0 ** 126
+    q, cache, kw = make((1, t, hq, 1, d), scores, values, torch.bfloat16, code, dev)
+    spread = lambda x: x.view(torch.uint8).expand(b, hkv, *x.view(torch.uint8).shape[2:]).contiguous().view(x.dtype)  # noqa: E731
+    q = q.repeat(b, 1, hkv, 1)
+    cache, kw = [spread(x) for x in cache], {k: spread(x) for k, x in kw.items()}
+    par, lens = torch.full((b, t), -1, dtype=torch.int32), torch.full((b,), n, dtype=torch.int32)
+    o = tree_attention(q, *cache, lens.to(dev), par.to(dev), softmax_scale=1.0, **kw).double().cpu()
+    want = 2.0 ** 126 * math.exp(5.0) / (160 + (n - 159) * math.exp(5.0))
+    assert bool(((o - want).abs() <= (2.0 ** -9 + 2.0 ** -18) * want).all()), (float(o.min()), float(o.max()), want)

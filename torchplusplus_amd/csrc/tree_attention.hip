@@ -133,11 +133,12 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
 // types), V fragments bfloat16; the exponents are applied to the scores and to
 // the probabilities. P keeps its fp32 bits: it is the sum of three values of V's
 // type, whose products are summed in fp32. In bfloat16 those are 8 bits each, all of
-// P down to 2^-110. In fp16 they are 11 bits each at 2^15, 2^26 and 2^37 times P (1 at
-// most), each folded into the next at its scale: 22 bits of a weight down to 2^-40
-// of the largest, 11 to 2^-51, and what is cut is below 2^-61, so that V up to 65504
-// over 2^20 keys loses less than half of fp16's least step. (Two parts at one scale
-// lost every weight below 2^-39, and in bfloat16 the last 8 bits.)
+// P down to 2^-100 of the largest (2^-118 is the least that counts). In fp16 they are
+// 11 bits each at 2^15, 2^26 and 2^37 times P (1 at most), each folded into the next
+// at its scale: 22 bits of a weight down to 2^-40 of the largest, 11 to 2^-51, and what
+// is cut is below 2^-61, so that V up to 65504 over 2^20 keys loses less than half of
+// fp16's least step. (Two parts at one scale lost every weight below 2^-39, and in
+// bfloat16 the last 8 bits.)
 // ---------------------------------------------------------------------------
 // Keys of a tile: 8 KB of K, 32 or 64. The kernel of up to 32 rows takes 32 of coded
 // caches too: of 16 rows three blocks a CU instead of two (32 sequences of 2098 e4m3
@@ -239,11 +240,13 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
   typedef TreeTile<KIND, D, KEYS> TT;
   static constexpr int KT = TT::KT, ROWB = TT::ROWB, UPR = TT::UPR, EB = KIND ? 1 : 2, EX = KIND ? 1 : 0;
   static constexpr int NST = KT / 16, NX = ROWB / 64, NCS = KT / 32, NT = D / 16;
-  // The reference maximum moves when a tile's passes it by 2^8 (76.2 -> 74.6 us), for
-  // that rescales every sum; not in fp16, whose P has no such room.
-  static constexpr float kLazy = KIND == 0 && !__is_same(T, bf16) ? 0.f : 8.f;
   static constexpr bool kApart = !__is_same(PT, bf16);  // parts of P have scales of their own
-  static constexpr float kUp = kApart ? 15.f : 0.f;     // P times 2^15
+  // The reference maximum moves when a tile's passes it by 2^8, for that rescales every
+  // sum (2 trees of 33 over 26000 keys 89.1 -> 86.9 us);
+  // P is times 2^-8, so 1 at most all the same: above 1 it took finite values from 2^120
+  // on to infinity. Not in fp16, whose parts have no such room: there P is times 2^15.
+  static constexpr float kLazy = kApart ? 0.f : 8.f;
+  static constexpr float kUp = kApart ? 15.f : -kLazy;
 
   V8 qf[NC][D / 32];
   unsigned long long see[NC];
