@@ -510,7 +510,7 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
   // nothing: 0 after the merges, where a row of scores of -inf, with no weight, is 0 / 0.
   // True where a sum is not finite.
   __device__ __forceinline__ bool end(const TreeArgs &p) {
-    bool odd = false;
+    f32x4 zero = {0.f, 0.f, 0.f, 0.f}; // or NaN (64 comparisons took 0.8 us here)
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       l[i] += __shfl_xor(l[i], 16, kWave);
@@ -521,10 +521,11 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (!see[i]) o[i][tt][e] = 0.f;
-          odd |= !(fabsf(o[i][tt][e]) < INFINITY);
+          zero[e] = fmaf(o[i][tt][e], 0.f, zero[e]);
         }
     }
-    return odd;
+    const float z = (zero[0] + zero[1]) + (zero[2] + zero[3]);
+    return z != z;
   }
   __device__ __forceinline__ float top(const TreeArgs &p, int i) const {
     return m[i] == -INFINITY ? -INFINITY : m[i] * p.scale_log2;
