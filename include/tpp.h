@@ -192,11 +192,12 @@ int tpp_rope_at(const void *q, const void *k, void *q_out, void *k_out,
  * contiguous, rows 16-byte aligned) into a cache of codes [B, H, Lmax, D]
  * ({batch, head} strides, rows contiguous) and exponent bytes [B, H, Lmax]
  * ({batch, head} strides): a row is its codes times 2^(byte - 127), the least
- * power of two that holds it, each code the nearest (ties to even). Token s of
- * sequence b goes to positions[b] + s (positions NULL: start + s) where that is
- * in [0, Lmax) and s < counts[b] (counts NULL: all); other rows keep what they
- * hold. A row with an infinity or NaN is stored as NaN (byte 255). code a
- * tpp_code, D in {64, 128, 256}. Next to KVCache.update
+ * power of two that holds it, each code the nearest (ties to even); a value past
+ * the largest below 2^128 that codes hold (240 * 2^120 in e4m3, 127 * 2^121 in
+ * int8) counts as that. Token s of sequence b goes to positions[b] + s (positions
+ * NULL: start + s) where that is in [0, Lmax) and s < counts[b] (counts NULL:
+ * all); other rows keep what they hold. A row with an infinity or NaN is stored as
+ * NaN (byte 255). code a tpp_code, D in {64, 128, 256}. Next to KVCache.update
  * (torchpp/llmops/kvcache.py:50-108), which keeps 16-bit values. */
 int tpp_kv_quant_append(const void *k, const void *v, const int64_t *k_strides,
                         const int64_t *v_strides, void *k_codes, void *v_codes,

@@ -7,6 +7,8 @@ import math
 import torch
 
 CODE_MAX = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+# the largest value below 2^128 that a row of codes holds
+VALUE_MAX = {torch.float8_e4m3fn: 240 * 2.0 ** 120, torch.int8: 127 * 2.0 ** 121}
 
 
 def rope_at(x, positions, inv_freq, interleaved=False, factor=1.0):
@@ -40,6 +42,7 @@ def quantise(x, code_dtype):
         if not bool(torch.isfinite(r).all()):
             exps[i] = 255
             continue
+        r = r.clamp(-VALUE_MAX[code_dtype], VALUE_MAX[code_dtype])
         amax, e = float(r.abs().max()), -126
         while amax > most * 2.0 ** e:
             e += 1

@@ -7,7 +7,9 @@
 // rounded half to even. With powers of two the division is exact, so a code
 // is the one correct rounding of its element (relative error at most 2^-4 in
 // e4m3, absolute at most 2^(E - 128) in int8) and decoding is exact in
-// bfloat16. A scale of max / M exactly would use int8's range better by up to
+// bfloat16. A bfloat16 past the largest value below 2^128 that a row of codes holds
+// (240 * 2^120 in e4m3, 127 * 2^121 in int8) is stored as that: the nearest code, 256 or
+// 64 times more, would read back as infinity. A scale of max / M exactly would use int8's range better by up to
 // one bit (half a bit on average), at four bytes a row and two more roundings.
 // A row with an infinity or a NaN gets E = 255 and codes 0 and reads back as
 // NaN throughout.
@@ -43,9 +45,13 @@ template <int LPR> __device__ __forceinline__ unsigned group_umax(unsigned v) {
   return v;
 }
 
+// The largest value below 2^128 that a row of codes holds.
+template <int CODE> constexpr float kCodedMax = CODE == TPP_CODE_E4M3 ? 0x1.ep127f : 0x1.fcp127f;
+
 // The exponent byte for a row whose largest magnitude has the float bits `u`.
 template <int CODE> __device__ __forceinline__ int row_exponent(unsigned u) {
   if (u >= 0x7f800000u) return 255; // an infinity or a NaN
+  u = min(u, __builtin_bit_cast(unsigned, kCodedMax<CODE>));
   // M = 1.75 * 2^8 or 1.984375 * 2^6: one more where the mantissa is past M's
   const int e = CODE == TPP_CODE_E4M3 ? (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u)
                                       : (int)(u >> 23) - 6 + ((u & 0x7fffffu) > 0x7e0000u);
@@ -85,7 +91,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs p) {
       x[j] = to_f32(t[i][j]);
       u = max(u, __float_as_uint(x[j]) & 0x7fffffffu);
     }
-    const int e = row_exponent<CODE>(group_umax<LPR>(u));
+    u = group_umax<LPR>(u);
+    const int e = row_exponent<CODE>(u);
+    if (__is_same(T, bf16) && u > __builtin_bit_cast(unsigned, kCodedMax<CODE>)) // (hardly ever)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_fmed3f(x[j], -kCodedMax<CODE>, kCodedMax<CODE>);
     // times 2^(127 - e): exact, or below half the least code
     const float inv = e == 255 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23);
     u32x2 out = {0u, 0u};

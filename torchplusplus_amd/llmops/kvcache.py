@@ -53,7 +53,8 @@ def kv_quant_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_c
     """Write k, v [B, S, Hkv, D] (fp16 or bf16, any strides that keep rows
     16-byte aligned) into caches of codes [B, Hkv, L, D] (float8_e4m3fn or int8)
     and exponent bytes [B, Hkv, L] (uint8): a row is codes * 2^(byte - 127), the
-    least power of two that holds it, codes rounded to nearest (ties to even).
+    least power of two that holds it, codes rounded to nearest (ties to even); a
+    value past the largest below 2^128 that codes hold counts as that.
     Token s of sequence b goes to positions[b] + s (an int: the same for all);
     tokens outside the cache, or past counts[b], are not written. A row with an
     infinity or NaN is kept as NaN. D in {64, 128, 256}."""
