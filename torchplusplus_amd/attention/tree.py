@@ -29,6 +29,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     Caches of q's dtype, or of float8_e4m3fn / int8 codes with the exponent
     bytes k_exps, v_exps of a QuantKVCache. T = 1 is a decode step over either.
-    Returns o [B, T, Hq, D]."""
+    softmax_scale is above 0, by default 1/sqrt(D). Returns o [B, T, Hq, D]."""
+    if softmax_scale is not None and not 2.0 ** -126 <= softmax_scale < 2.0 ** 126:  # fp32's normal range
+        raise ValueError(f"softmax_scale must be above 0 and finite, got {softmax_scale}")
     return _C.tree_attention(q, k_cache, v_cache, seqlens, parents, k_exps, v_exps,
-                             float(softmax_scale) if softmax_scale else 0.0, out)
+                             0.0 if softmax_scale is None else float(softmax_scale), out)
