@@ -106,9 +106,16 @@ class LLMInference(nn.Module, ABC):
     def sample_draft(self, draft_tokens, logits, temp: float = 1.0, uniforms=None, draft_probs=None,
                      parents=None):
         """Verify drafted tokens [B, T] against the target's logits [B, T + 1, V]
-        at a temperature; uniforms default to torch.rand. Returns (accepted,
-        path, next_token), see llmops.speculative.verify_draft."""
-        probs = torch.softmax(logits.float() / temp, -1)
+        at a temperature (0: the largest logit's token, as sample_greedy takes
+        it); uniforms default to torch.rand. Returns (accepted, path, next_token),
+        see llmops.speculative.verify_draft. The whole distribution counts: no
+        top_p or top_k."""
+        if not temp >= 0:
+            raise ValueError(f"temp must be 0 or above, got {temp}")
+        if temp == 0:
+            probs = torch.zeros_like(logits, dtype=torch.float32).scatter_(-1, self.sample_greedy(logits), 1.0)
+        else:
+            probs = torch.softmax(logits.float() / temp, -1)
         if uniforms is None:
             uniforms = torch.rand(probs.shape[:2], device=probs.device)
         return verify_draft(draft_tokens, probs, uniforms, draft_probs, parents)
