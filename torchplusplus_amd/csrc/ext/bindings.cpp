@@ -12,11 +12,11 @@
 // run on the current HIP stream of the input's device.
 #include <torch/extension.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <limits>
 #include <string>
 #include <vector>
@@ -1006,6 +1006,77 @@ at::Tensor or_none(const c10::optional<at::Tensor> &t) {
   return t.has_value() && t->defined() ? *t : at::Tensor();
 }
 
+// A tensor's memory: runs of `run` bytes at base + the sum of index * stride (bytes)
+// over its outer dims. `tail` dims at the end are contiguous and make one run.
+struct Runs {
+  const char *base;
+  int64_t run, span; // of a run; from the first byte to the end of the last run
+  int dims = 0;
+  int64_t n[4], s[4];
+  explicit Runs(const at::Tensor &t, int tail = 1) : base((const char *)t.data_ptr()), run(t.element_size()) {
+    for (int i = 0; i < tail; ++i) run *= t.size(t.dim() - 1 - i);
+    span = run;
+    for (int i = 0; i < t.dim() - tail; ++i) {
+      if (t.size(i) == 0) run = 0;
+      if (t.size(i) <= 1) continue;
+      n[dims] = t.size(i), s[dims] = t.stride(i) * t.element_size();
+      span += (n[dims] - 1) * s[dims];
+      ++dims;
+    }
+    if (run == 0) span = 0;
+  }
+};
+
+// Whether two runs meet that `off` and, for each dim k, d_k strides s_k lie apart, lo_k
+// <= d_k <= hi_k (strides falling; `own`: not all d_k are 0): -after < off + sum < ahead.
+// Only the d_k that the dims behind can still make up for are tried: one or two of a
+// layout whose strides nest. True past `tries`.
+struct RunsApart {
+  int dims = 0;
+  int64_t s[8], lo[8], hi[8], ahead, after;
+  int tries = 10000;
+  void dim(int64_t stride, int64_t l, int64_t h) {
+    for (int i = 0; i < dims; ++i)
+      if (s[i] == stride) {
+        lo[i] += l, hi[i] += h;
+        return;
+      }
+    int at = dims++;
+    for (; at > 0 && s[at - 1] < stride; --at) s[at] = s[at - 1], lo[at] = lo[at - 1], hi[at] = hi[at - 1];
+    s[at] = stride, lo[at] = l, hi[at] = h;
+  }
+  bool meet(int64_t off, int k, bool own) {
+    if (--tries < 0) return true;
+    if (k == dims) return !own && -after < off && off < ahead;
+    if (s[k] == 0) return lo[k] < hi[k] ? meet(off, k + 1, false) : meet(off, k + 1, own);
+    int64_t least = 0, most = 0; // of the dims behind
+    for (int i = k + 1; i < dims; ++i) least += lo[i] * s[i], most += hi[i] * s[i];
+    auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t from = std::max(lo[k], -floor_div(off + most + after - 1, s[k]));
+    const int64_t to = std::min(hi[k], floor_div(ahead - 1 - off - least, s[k]));
+    for (int64_t d = from; d <= to; ++d)
+      if (meet(off + d * s[k], k + 1, own && d == 0)) return true;
+    return false;
+  }
+};
+bool runs_meet(const Runs &a, const Runs &b) {
+  if (a.run == 0 || b.run == 0 || a.base >= b.base + b.span || b.base >= a.base + a.span) return false;
+  RunsApart x;
+  for (int i = 0; i < a.dims; ++i) x.dim(a.s[i], 1 - a.n[i], 0);
+  for (int i = 0; i < b.dims; ++i) x.dim(b.s[i], 0, b.n[i] - 1);
+  x.ahead = a.run, x.after = b.run;
+  return x.meet(b.base - a.base, 0, false);
+}
+// whether two elements of one tensor share memory
+bool runs_meet(const Runs &a) {
+  if (a.run == 0) return false;
+  RunsApart x;
+  for (int i = 0; i < a.dims; ++i) x.dim(a.s[i], 1 - a.n[i], a.n[i] - 1);
+  if (x.dims < a.dims) return true; // two dims of one stride
+  x.ahead = x.after = a.run;
+  return x.meet(0, 0, true);
+}
+
 std::tuple<at::Tensor, at::Tensor> rope_at(const at::Tensor &q, const c10::optional<at::Tensor> &k_opt,
                                            at::Tensor positions, const at::Tensor &inv_freq,
                                            bool interleaved, double attention_factor, bool inplace) {
@@ -1022,9 +1093,7 @@ std::tuple<at::Tensor, at::Tensor> rope_at(const at::Tensor &q, const c10::optio
                 "q and k must be [B, S, H, D] with the same B, S and D");
     TORCH_CHECK(t->numel() == 0 || t->stride(3) == 1, "q and k must have a contiguous last dimension");
     TORCH_CHECK(t->size(2) > 0, "q and k must have at least one head");
-    if (inplace)
-      for (int i = 0; i < 3; ++i)
-        TORCH_CHECK(t->size(i) <= 1 || t->stride(i) >= D, "in place: rows of q or k overlap");
+    if (inplace) TORCH_CHECK(!runs_meet(Runs(*t)), "in place: rows of q or k overlap");
   }
   TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
               "positions must be int32 or int64");
@@ -1038,6 +1107,7 @@ std::tuple<at::Tensor, at::Tensor> rope_at(const at::Tensor &q, const c10::optio
   TORCH_CHECK(R >= 2 && R <= D && D % 2 == 0, "rotary_dim ", R, " does not fit head_dim ", D);
   TORCH_CHECK(!inplace || !k.defined() || k.numel() == 0 || k.data_ptr() != q.data_ptr(),
               "in place: q and k are one tensor");
+  TORCH_CHECK(!inplace || !k.defined() || !runs_meet(Runs(q), Runs(k)), "in place: q and k overlap");
   c10::DeviceGuard g(q.device());
   at::Tensor qo = inplace ? q : new_on(q, q.sizes(), q.scalar_type()), ko;
   if (k.defined()) ko = inplace ? k : new_on(q, k.sizes(), q.scalar_type());
@@ -1097,12 +1167,15 @@ void kv_quant_append(const at::Tensor &k, const at::Tensor &v, const at::Tensor 
   TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "k and v differ");
   const int64_t B = k.size(0), S = k.size(1), H = k.size(2), D = k.size(3);
   TORCH_CHECK(kc.size(1) == H && kc.size(3) == D, "cache shape mismatch");
-  TORCH_CHECK(kc.numel() == 0 || (kc.data_ptr() != vc.data_ptr() && ke.data_ptr() != ve.data_ptr()),
-              "K and V must have caches of their own");
-  TORCH_CHECK(at::has_internal_overlap(kc) != at::MemOverlap::Yes && at::has_internal_overlap(ke) != at::MemOverlap::Yes,
-              "sequences must have rows of their own");
   const at::Tensor pos = or_none(positions), cnt = or_none(counts);
   check_same_device(k, {&v, &kc, &pos, &cnt});
+  const Runs cache[4] = {Runs(kc, 2), Runs(vc, 2), Runs(ke), Runs(ve)}, in[2] = {Runs(k), Runs(v)};
+  for (int i = 0; i < 4; i += 2) // (K and V have one layout)
+    TORCH_CHECK(!runs_meet(cache[i]), "sequences must have rows of their own");
+  for (int i = 0; i < 4; ++i) {
+    for (int j = i + 1; j < 4; ++j) TORCH_CHECK(!runs_meet(cache[i], cache[j]), "K and V must have caches of their own");
+    TORCH_CHECK(!runs_meet(in[0], cache[i]) && !runs_meet(in[1], cache[i]), "k and v must not lie in the cache");
+  }
   c10::DeviceGuard g(k.device());
   const int64_t ks[3] = {k.stride(0), k.stride(1), k.stride(2)}, vs[3] = {v.stride(0), v.stride(1), v.stride(2)};
   const int64_t cs[2] = {kc.stride(0), kc.stride(1)}, es[2] = {ke.stride(0), ke.stride(1)};
@@ -1129,17 +1202,6 @@ std::tuple<at::Tensor, at::Tensor> kv_quant_read(const at::Tensor &kc, const at:
                              dtype_code(k), cur_stream(kc)),
            "kv_quant_read");
   return {k, v};
-}
-
-// whether the bytes from the first to the last element of two tensors meet
-bool ranges_meet(const at::Tensor &a, const at::Tensor &b) {
-  auto end = [](const at::Tensor &t) {
-    int64_t n = 1;
-    for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
-    return (const char *)t.data_ptr() + n * t.element_size();
-  };
-  if (!a.numel() || !b.numel()) return false;
-  return (const char *)a.data_ptr() < end(b) && (const char *)b.data_ptr() < end(a);
 }
 
 at::Tensor tree_attention(const at::Tensor &q, const at::Tensor &kc, const at::Tensor &vc,
@@ -1181,9 +1243,11 @@ at::Tensor tree_attention(const at::Tensor &q, const at::Tensor &kc, const at::T
     TORCH_CHECK(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device() &&
                     (o.numel() == 0 || o.stride(3) == 1),
                 "out must match q");
-    TORCH_CHECK(at::has_internal_overlap(o) != at::MemOverlap::Yes && !ranges_meet(o, q) && !ranges_meet(o, kc) &&
-                    !ranges_meet(o, vc),
-                "out must have memory of its own");
+    const Runs mem(o);
+    bool own = !runs_meet(mem);
+    for (const at::Tensor *t : {&q, &kc, &vc, &ke, &ve, &seqlens, &parents})
+      own = own && !(t->defined() && runs_meet(mem, Runs(*t)));
+    TORCH_CHECK(own, "out must have memory of its own");
   } else {
     o = new_on(q, q.sizes(), q.scalar_type());
   }
