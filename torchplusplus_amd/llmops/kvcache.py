@@ -30,6 +30,9 @@ def _keep(rows: torch.Tensor, start: torch.Tensor, path: torch.Tensor) -> None:
     each path[b, i] >= 0; other rows keep what they hold. Gathered whole before
     anything is written, each row written once (entries of -1, and those past
     the cache's end, write a row of their own back to itself)."""
+    if path.dim() != 2 or path.shape[0] != rows.shape[0] or start.shape != path.shape[:1]:
+        raise ValueError(f"start {tuple(start.shape)} and path {tuple(path.shape)} must be [B] and [B, n], "
+                         f"for at most the cache's sequences")
     n, length = path.shape[1], rows.shape[2]
     if n > length:
         raise ValueError(f"a path of {n} tokens in a cache of {length} positions")
@@ -118,7 +121,8 @@ class KVCache:
     def keep(self, start: torch.Tensor, path: torch.Tensor) -> None:
         """After a verification: the rows of the accepted drafted tokens, at
         start[b] + path[b, i] (entries of -1 are none), move to start[b] + i.
-        start [B], path [B, n]; cache_len is the caller's to advance."""
+        start [B] (where the first drafted token's row is), path [B, n]; cache_len
+        is the caller's to advance."""
         for rows in (self.k_cache, self.v_cache):
             _keep(rows[: path.shape[0]], start, path)
 
