@@ -15,8 +15,9 @@
 // NaN throughout.
 //
 // Bound by HBM: append reads 2 bytes and writes 1 an element, read the other
-// way round. 8 x 2048 tokens, 8 heads of 128, into e4m3: 24.4 us (4.1 TB/s, 26.1 with
-// one row a thread); 8 x 2304 positions back: 19.5 us (5.8 TB/s).
+// way round. 8 x 2048 tokens, 8 heads of 128, into e4m3: 24.5 us (4.1 TB/s, 26.1 with
+// one row a thread); 8 x 2304 positions back: 19.5 us (5.8 TB/s, part of the codes from
+// the caches, where a call before left them).
 #include "tpp_common.hpp"
 
 namespace tpp {

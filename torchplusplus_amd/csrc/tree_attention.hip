@@ -65,7 +65,8 @@ __device__ __forceinline__ float exp_scale(const uint8_t *e, int64_t i) {
 }
 
 // Any head size up to 256, any alignment: one wave per (sequence, token,
-// head), keys one at a time with a wave reduction.
+// head), keys one at a time with a wave reduction, so bound by latency, 1 us a key (one
+// token over 4096 int8 keys of 256, 16 / 4 heads: 4.3 ms; 16-bit 8.3).
 template <typename T, int KIND>
 __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
   const int lane = lane_id(), t = blockIdx.x % p.T, h = blockIdx.x / p.T, b = blockIdx.y;
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
 // one's fragments are in registers, the next V tile after this one's. Waves are
 // merged through LDS, splits by the pair's last block (tree_merge_here) or by
 // tree_merge_kernel, a second launch. Bound by HBM up to 32 rows (32 sequences of 4096
-// e4m3 keys, 16 / 8 heads of 128, one token: 45.5 us, 5.9 TB/s; of bfloat16 83 us, 6.4
+// e4m3 keys, 16 / 8 heads of 128, one token: 48.8 us, 5.5 TB/s; of bfloat16 84.2 us, 6.4
 // TB/s), by the products and the softmax past that (tree_rows_kernel).
 //
 // Key order: S^T gives lane quarter u the keys 16 st + 4 u + i (i = 0 .. 3) of
@@ -138,7 +139,8 @@ __global__ __launch_bounds__(64) void tree_generic_kernel(TreeArgs p, int D) {
 // at its scale: 22 bits of a weight down to 2^-40 of the largest, 11 to 2^-51, and what
 // is cut is below 2^-61, so that V up to 65504 over 2^20 keys loses less than half of
 // fp16's least step. (Two parts at one scale lost every weight below 2^-39, and in
-// bfloat16 the last 8 bits.)
+// bfloat16 the last 8 bits.) Over codes, whose powers of two P is multiplied by, all
+// of its bits count where the product is above 2^-102.
 // ---------------------------------------------------------------------------
 // Keys of a tile: 8 KB of K, 32 or 64. The kernel of up to 32 rows takes 32 of coded
 // caches too: of 16 rows three blocks a CU instead of two (32 sequences of 2098 e4m3
@@ -933,7 +935,7 @@ __global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel
 // tile, after which the slot of the tile before last is asked for anew. With
 // waves that stream their own tiles, 264 rows over 32700 e4m3 keys moved 9 times
 // the cache through the L1s and took 122 us where the DMA alone took 44. Bound by the
-// sum of matrix and VALU work, of which two waves a SIMD hide half: 71-80 us for 2 x 264
+// sum of matrix and VALU work, of which two waves a SIMD hide half: 70-104 us for 2 x 264
 // rows over 20000-32700 e4m3 keys and 4 KV heads.
 template <typename T, int KIND, int D>
 __global__ __launch_bounds__(256, 2) void tree_rows_kernel(TreeArgs p, float *__restrict__ ws_o,

@@ -26,10 +26,12 @@
 // masses and sums each; the second finds the chunk and the index. Every wave of the
 // first repeats the walk (one gather of a mass per drafted token, all at once, then
 // a walk in registers): cheaper than a launch of its own, or a barrier. Every wave
-// of the second scans the chunks' sums. What bounds it: the latency of two launches
-// and of four dependent trips to memory in each; the rows are B V 4 bytes (with q
-// twice that). 8 chains of 5 over 150000 tokens 10.5 us, 16 trees of 31 11.6; in one
-// launch, the last block of a sequence to finish picking, 11.9 for the chains.
+// of the second scans the chunks' sums. What bounds it: the latency of two launches,
+// of three dependent trips to memory in the first (tokens, their masses, the row) and
+// two in the second (the chunks' sums, the chunk), and there of three scans of fp64
+// sums over a wave, one after the other; the rows are B V 4 bytes (with q twice that).
+// 8 chains of 5 over 150000 tokens 10.5 us, 16 trees of 31 11.7; in one launch, the last
+// block of a sequence to finish picking, 11.9 for the chains.
 #include "tpp_common.hpp"
 
 namespace tpp {

@@ -140,6 +140,9 @@ class QuantKVCache:
     torch.float8_e4m3fn (3 bits after the first of each element) or torch.int8
     (7 bits after the first of the row's largest element).
 
+    head_dim 64 or 128; 256 too, but no attention kernel is fast there (one for any size
+    reads a key at a time, over codes as over 16-bit values).
+
     append() writes tokens, attention.tree_attention reads the codes in place
     (GroupedQueryAttention does both), read() decodes a prefix, update() is
     KVCache.update: append, then the decoded prefix."""
