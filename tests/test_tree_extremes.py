@@ -65,6 +65,26 @@ def test_infinite_values_in_the_context(dev, dtype, shape, n, at):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_nan_scores_and_values(dev, dtype, shape):
+    """A NaN among the scores of the context: NaN for all; in a drafted token's key or
+    value: for those that see it alone."""
+    from torchplusplus_amd.attention import tree_attention
+    b, t = shape[:2]
+    n = 300
+    par = torch.full((b, t), -1, dtype=torch.int32)
+    for where in (70, n):
+        for which in (0, 1):
+            q, cache, _ = make(shape, [0.5] * (n + 64), [2.0] * (n + 64), dtype, None, dev)
+            cache[which][:, :, where, 0 if which == 0 else slice(None)] = math.nan
+            lens = torch.full((b,), n, dtype=torch.int32, device=dev)
+            o = tree_attention(q, *cache, lens, par.to(dev), softmax_scale=1.0).float().cpu()
+            assert bool(torch.isnan(o[:, 0]).all())
+            assert bool(torch.isnan(o[:, 1:]).all()) if where < n else bool((o[:, 1:] == 2.0).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("t,hq,d", [(1, 1, 128), (4, 2, 64), (16, 2, 128), (33, 1, 64), (12, 4, 128), (1, 1, 96)])
 def test_values_near_the_end_of_bfloat16(dev, code, t, hq, d):

@@ -244,9 +244,9 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
   static constexpr int NST = KT / 16, NX = ROWB / 64, NCS = KT / 32, NT = D / 16;
   static constexpr bool kApart = !__is_same(PT, bf16);  // parts of P have scales of their own
   // The reference maximum moves when a tile's passes it by 2^8, for that rescales every
-  // sum (2 trees of 33 over 26000 keys 89.1 -> 86.9 us);
-  // P is times 2^-8, so 1 at most all the same: above 1 it took finite values from 2^120
-  // on to infinity. Not in fp16, whose parts have no such room: there P is times 2^15.
+  // sum (2 trees of 33 over 26000 keys 89.1 -> 86.9 us). P is times 2^-8, so 1 at most
+  // all the same: above 1 it took finite values from 2^120 on to infinity. Not in fp16,
+  // whose parts have no such room: there P is times 2^15.
   static constexpr float kLazy = kApart ? 0.f : 8.f;
   static constexpr float kUp = kApart ? 15.f : -kLazy;
 
@@ -537,8 +537,8 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
   // the products of those that do not see it; so is an infinity among 16-bit values
   // times a part of P that is 0. A wave that had such a tile and has a sum that is not
   // finite sums again, key by key over what each row sees: its n tiles from key
-  // `first`, `stride` apart, up to k_end. put(i, q, d, x): the sum of element d of row
-  // q of group i.
+  // `first`, `stride` apart, up to k_end (a row with a NaN among its scores is NaN
+  // without). put(i, q, d, x): the sum of element d of row q of group i.
   template <typename PUT>
   __device__ __forceinline__ void again(const TreeArgs &p, int b, int hk, const char *ks, const char *vs, int64_t eb,
                                         int first, int stride, int n, int k_end, int L, unsigned g_inv,
@@ -550,11 +550,12 @@ template <typename T, int KIND, int D, int NC, int KEYS = tree_keys(KIND, D)> st
         const unsigned long long sq = ((unsigned long long)(unsigned)__shfl((int)(see[i] >> 32), q, kWave) << 32) |
                                       (unsigned)__shfl((int)see[i], q, kWave);
         const float mq = __shfl(m[i], q, kWave), mc = mq == -INFINITY ? 0.f : mq * p.scale_log2;
+        const float lq = __shfl(l[i], q, kWave);
         const T *qp = row_of((const T *)p.q, p.q_s, p, b, hk, row0[i] + q, div_inv((unsigned)(row0[i] + q), g_inv));
         float acc[D / 64];
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) acc[c] = 0.f;
-        for (int it = 0; it < n && sq; ++it)
+        for (int c = 0; c < D / 64; ++c) acc[c] = lq == lq ? 0.f : lq;
+        for (int it = 0; it < n && sq && lq == lq; ++it)
           for (int j = first + it * stride; j < min(first + it * stride + KT, k_end); ++j) {
             if (j >= L && !((sq >> (j - L)) & 1)) continue;
             const char *kr = ks + (int64_t)j * p.k_s[2] * EB, *vr = vs + (int64_t)j * p.v_s[2] * EB;
