@@ -186,6 +186,74 @@ int tpp_rope_at(const void *q, const void *k, void *q_out, void *k_out,
                 int64_t Hq, int64_t Hk, int64_t D, int64_t R, int interleaved,
                 int dtype, void *stream);
 
+/* ---- a batch of sequences of different lengths over a paged cache ------------- */
+
+/* Flash attention forward of sequences packed one behind the other: q, o [Nq, Hq,
+ * D] and k, v [Nk, Hkv, D] ({token, head} strides, last dim contiguous). Sequence
+ * b has the query rows cu_q[b] .. cu_q[b + 1] - 1 and the key rows cu_k[b] ..
+ * cu_k[b + 1] - 1 (int32 [B + 1] on the device, ascending; cut to the tensors; cu_k
+ * NULL: cu_q, Nk = Nq). Scale, causal and window as in tpp_attn_prefill, in each
+ * sequence. Rows that see nothing are 0, rows whose scores are all -inf NaN. Rows
+ * of no sequence become 0 if `fill`, else stay as they were. D <= 256. Workspace
+ * (16-byte aligned, no initialisation, this call's own) of
+ * tpp_attn_packed_workspace_size bytes (0: none). Next to flash_attn_func
+ * (torchpp/attention/gqa.py:128), whose sequences have one length. */
+int tpp_attn_packed(const void *q, const void *k, const void *v, void *o,
+                    const int64_t *q_strides, const int64_t *k_strides,
+                    const int64_t *v_strides, const int64_t *o_strides,
+                    const int32_t *cu_q, const int32_t *cu_k, int64_t B, int64_t Nq,
+                    int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,
+                    float softmax_scale, int causal, int window_left,
+                    int window_right, int fill, int dtype, void *workspace,
+                    size_t ws_bytes, void *stream);
+size_t tpp_attn_packed_workspace_size(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq,
+                                      int64_t Hkv, int64_t D);
+
+/* Attention of one new token a sequence over a cache held in pages: q, o [B, Hq, D]
+ * ({sequence, head} strides), k_pages, v_pages [pages, Hkv, page_size, D] ({page,
+ * head, row} strides), last dim contiguous. Key j < seqlens[b] (int32 [B] on the
+ * device, limited to the table's positions) is row j % page_size of page
+ * block_tables[b * table_stride + j / page_size] (int32, table_pages entries a
+ * sequence); the positions of an entry outside [0, pages) are not seen. window_left
+ * >= 0 keeps keys >= seqlens[b] - 1 - window_left. Rows that see nothing are 0, rows
+ * whose scores are all -inf NaN. page_size a power of two, 16 to 1024; D <= 256.
+ * softmax_scale <= 0 means 1/sqrt(D). Next to flash_attn_func with Sq = 1 over the
+ * cache prefix (torchpp/attention/gqa.py:117-128). */
+int tpp_attn_paged(const void *q, const void *k_pages, const void *v_pages, void *o,
+                   const int64_t *q_strides, const int64_t *k_strides,
+                   const int64_t *v_strides, const int64_t *o_strides,
+                   const int32_t *block_tables, int64_t table_stride,
+                   int64_t table_pages, const int32_t *seqlens, int64_t B,
+                   int64_t Hq, int64_t Hkv, int64_t D, int64_t pages,
+                   int64_t page_size, float softmax_scale, int window_left,
+                   int dtype, void *workspace, size_t ws_bytes, void *stream);
+
+/* Workspace bytes of tpp_attn_paged (128-byte aligned, no initialisation; 0: none)
+ * for tables of Lmax = table_pages * page_size positions. It belongs to one call until
+ * that has run. */
+size_t tpp_attn_paged_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                     int64_t Lmax);
+
+/* The step from a packed batch's fused projection to its attention: qkv [N, (Hq + 2
+ * Hkv) * D] (token stride qkv_stride, not changed), per-head RMSNorm of q and k
+ * (q_norm_w, k_norm_w [D], NULL = none), RoPE by row positions[t] of cos/sin [ctx,
+ * D], one rounding; q_out [N, Hq, D] and k_out [N, Hkv, D] (NULL: not wanted)
+ * contiguous; keys and values of token t into row slots[t] % page_size of page
+ * slots[t] / page_size (int64, distinct) of k_pages, v_pages ({page, head, row}
+ * strides, last dim contiguous). Slots outside [0, pages * page_size) are not
+ * written; a token at a position outside [0, ctx) is padding: its q and k are 0 and
+ * no slot is written. D in {64, 128, 256}, page_size as in tpp_attn_paged, 16-byte
+ * aligned pointers and strides. Next to q_norm, k_norm, rope_apply and
+ * KVCache.update (torchpp/attention/gqa.py:86-118). */
+int tpp_qkv_rope_paged(const void *qkv, int64_t qkv_stride, void *q_out, void *k_out,
+                       void *k_pages, void *v_pages, const int64_t *k_strides,
+                       const int64_t *v_strides, const void *q_norm_w,
+                       const void *k_norm_w, const void *cos, const void *sin,
+                       int64_t ctx, const int32_t *positions, const int64_t *slots,
+                       int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages,
+                       int64_t page_size, float eps, int dtype, int cs_dtype,
+                       void *stream);
+
 /* ---- 8-bit KV cache -------------------------------------------------------- */
 
 /* Writes k and v [B, S, H, D] ({batch, token, head} strides, last dim
@@ -550,6 +618,21 @@ int tpp_argmax_rows(const void *x, int64_t *out, int64_t B, int64_t N,
 
 /* Workspace bytes of tpp_verify_draft (8-byte aligned, no initialisation). */
 size_t tpp_verify_draft_workspace_size(int64_t B, int64_t V);
+
+/* Log probabilities of rows of logits [N, V] of `dtype` (fp32, fp16 or bf16; rows
+ * row_stride apart, last dim contiguous): logprobs[n] of tokens[n] (0 for a token
+ * outside [0, V): padding), entropy[n] in nats, and, for top > 0, the `top` (at most 32
+ * and V) largest logits' log probabilities and tokens [N, top] in falling order, the
+ * lowest index first among equal ones. fp32 sums relative to the row's maximum; logits
+ * of -inf have no share. A row with a NaN or +inf, or of -inf alone, gives NaN (top
+ * tokens -1 with a NaN or +inf). Workspace (16-byte aligned, no initialisation, this
+ * call's own) of tpp_token_logprobs_workspace_size bytes (0: none). Next to the
+ * samplers of torchpp/llmops/llm.py:114-186, which need the probabilities alone. */
+int tpp_token_logprobs(const void *logits, int64_t row_stride, const int64_t *tokens,
+                       float *logprobs, float *entropy, float *top_logprobs,
+                       int64_t *top_tokens, int64_t N, int64_t V, int64_t top,
+                       int dtype, void *workspace, size_t ws_bytes, void *stream);
+size_t tpp_token_logprobs_workspace_size(int64_t N, int64_t V, int64_t top, int dtype);
 
 /* Verification of T drafted tokens (1 to 64) per sequence against the target's
  * probabilities. target_probs [B, T + 1, V] and draft_probs [B, T, V] of

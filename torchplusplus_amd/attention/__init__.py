@@ -8,3 +8,4 @@ from torchplusplus_amd.attention.mha import MultiHeadAttention  # noqa: F401
 from torchplusplus_amd.attention.mqa import MultiQueryAttention  # noqa: F401
 from torchplusplus_amd.attention.swa import SlidingWindowAttention  # noqa: F401
 from torchplusplus_amd.attention.tree import tree_attention  # noqa: F401
+from torchplusplus_amd.attention.packed import packed_attention, paged_attention  # noqa: F401

@@ -1311,6 +1311,173 @@ verify_draft(at::Tensor tokens, const at::Tensor &target, at::Tensor uniforms,
   return {accepted, path, next};
 }
 
+// out as given, or new. Given: like `like`, of memory of its own.
+at::Tensor out_like(const at::Tensor &like, const c10::optional<at::Tensor> &out,
+                    std::initializer_list<const at::Tensor *> in) {
+  if (!out.has_value() || !out->defined()) return new_on(like, like.sizes(), like.scalar_type());
+  const at::Tensor &o = *out;
+  TORCH_CHECK(o.sizes() == like.sizes() && o.scalar_type() == like.scalar_type() && o.device() == like.device() &&
+                  (o.numel() == 0 || o.stride(-1) == 1),
+              "out must match q");
+  const Runs mem(o);
+  bool own = !runs_meet(mem);
+  for (const at::Tensor *t : in) own = own && !(t->defined() && runs_meet(mem, Runs(*t)));
+  TORCH_CHECK(own, "out must have memory of its own");
+  return o;
+}
+
+int window_int(int64_t w) { // below 0: unbounded
+  return (int)std::max<int64_t>(-1, std::min<int64_t>(w, std::numeric_limits<int>::max()));
+}
+
+at::Tensor packed_attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &cu_q,
+                            const c10::optional<at::Tensor> &cu_k_opt, double softmax_scale, bool causal,
+                            int64_t window_left, int64_t window_right, const c10::optional<at::Tensor> &out) {
+  const at::Tensor cu_k = or_none(cu_k_opt);
+  TORCH_CHECK(q.is_cuda() && is_half_or_bf16(q), "q must be a CUDA half/bfloat16 tensor");
+  check_same_device(q, {&k, &v, &cu_q, &cu_k});
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes(), "q must be [Nq, Hq, D], k and v [Nk, Hkv, D]");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
+  const int64_t Nq = q.size(0), Hq = q.size(1), D = q.size(2), Nk = k.size(0), Hkv = k.size(1);
+  TORCH_CHECK(k.size(2) == D && D > 0, "head_dim mismatch");
+  TORCH_CHECK(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "number of query heads must be divisible by KV heads");
+  for (const at::Tensor *t : {&q, &k, &v})
+    TORCH_CHECK(t->numel() == 0 || t->stride(2) == 1, "q, k and v must have a contiguous last dim");
+  TORCH_CHECK(cu_q.scalar_type() == at::kInt && cu_q.dim() == 1 && cu_q.is_contiguous() && cu_q.size(0) > 0,
+              "cu_seqlens must be a contiguous int32 vector [B + 1]");
+  const int64_t B = cu_q.size(0) - 1;
+  TORCH_CHECK(!cu_k.defined() || (cu_k.scalar_type() == at::kInt && cu_k.dim() == 1 && cu_k.is_contiguous() &&
+                                  cu_k.size(0) == B + 1),
+              "cu_seqlens_k must be a contiguous int32 vector [B + 1]");
+  TORCH_CHECK(cu_k.defined() || Nk == Nq, "k and v of other lengths than q need cu_seqlens_k");
+  c10::DeviceGuard g(q.device());
+  const bool fill = !(out.has_value() && out->defined());
+  at::Tensor o = out_like(q, out, {&q, &k, &v, &cu_q, &cu_k});
+  if (q.numel() == 0) return o;
+  const size_t wsb = tpp_attn_packed_workspace_size(B, Nq, Nk, Hq, Hkv, D);
+  at::Tensor ws; // this call's own, from the caching allocator
+  if (wsb) ws = new_on(q, {(int64_t)wsb}, at::kByte);
+  const int64_t qs[2] = {q.stride(0), q.stride(1)}, ks[2] = {k.stride(0), k.stride(1)},
+                vs[2] = {v.stride(0), v.stride(1)}, os[2] = {o.stride(0), o.stride(1)};
+  check_rc(tpp_attn_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), qs, ks, vs, os,
+                           cu_q.data_ptr<int32_t>(), cu_k.defined() ? cu_k.data_ptr<int32_t>() : nullptr, B, Nq, Nk,
+                           Hq, Hkv, D, (float)softmax_scale, causal, window_int(window_left), window_int(window_right),
+                           fill, dtype_code(q), wsb ? ws.data_ptr() : nullptr, wsb, cur_stream(q)),
+           "packed_attention");
+  return o;
+}
+
+void check_pages(const at::Tensor &like, const at::Tensor &kp, const at::Tensor &vp) {
+  TORCH_CHECK(kp.dim() == 4 && vp.sizes() == kp.sizes(), "k_pages and v_pages must be [pages, Hkv, page_size, D]");
+  TORCH_CHECK(kp.scalar_type() == like.scalar_type() && vp.scalar_type() == like.scalar_type(),
+              "the pages must have q's dtype");
+  TORCH_CHECK(kp.numel() == 0 || (kp.stride(3) == 1 && vp.stride(3) == 1), "the pages must have a contiguous last dim");
+}
+
+at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &kp, const at::Tensor &vp, const at::Tensor &tables,
+                           const at::Tensor &seqlens, double softmax_scale, int64_t window_left,
+                           const c10::optional<at::Tensor> &out) {
+  TORCH_CHECK(q.is_cuda() && is_half_or_bf16(q), "q must be a CUDA half/bfloat16 tensor");
+  check_same_device(q, {&kp, &vp, &tables, &seqlens});
+  TORCH_CHECK(q.dim() == 3 && (q.numel() == 0 || q.stride(2) == 1), "q must be [B, Hq, D] with a contiguous last dim");
+  check_pages(q, kp, vp);
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = kp.size(1);
+  TORCH_CHECK(kp.size(3) == D && D > 0, "head_dim mismatch");
+  TORCH_CHECK(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "number of query heads must be divisible by KV heads");
+  TORCH_CHECK(tables.scalar_type() == at::kInt && tables.dim() == 2 && tables.size(0) == B &&
+                  (tables.numel() == 0 || tables.stride(1) == 1),
+              "block_tables must be int32 [B, pages of a sequence] with a contiguous last dim");
+  const int32_t *sl = int32_b(seqlens, B, "seqlens");
+  c10::DeviceGuard g(q.device());
+  at::Tensor o = out_like(q, out, {&q, &kp, &vp, &tables, &seqlens});
+  if (q.numel() == 0) return o;
+  const size_t wsb = tpp_attn_paged_workspace_size(B, Hq, Hkv, D, tables.size(1) * kp.size(2));
+  at::Tensor ws; // this call's own, from the caching allocator
+  if (wsb) ws = new_on(q, {(int64_t)wsb}, at::kByte);
+  const int64_t qs[2] = {q.stride(0), q.stride(1)}, os[2] = {o.stride(0), o.stride(1)};
+  const int64_t ks[3] = {kp.stride(0), kp.stride(1), kp.stride(2)}, vs[3] = {vp.stride(0), vp.stride(1), vp.stride(2)};
+  check_rc(tpp_attn_paged(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), o.data_ptr(), qs, ks, vs, os,
+                          tables.data_ptr<int32_t>(), B > 1 ? tables.stride(0) : 0, tables.size(1), sl, B, Hq, Hkv, D,
+                          kp.size(0), kp.size(2), (float)softmax_scale, window_int(window_left), dtype_code(q),
+                          wsb ? ws.data_ptr() : nullptr, wsb, cur_stream(q)),
+           "paged_attention");
+  return o;
+}
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>>
+qkv_rope_paged(const at::Tensor &qkv, const at::Tensor &positions, const at::Tensor &slots, const at::Tensor &kp,
+               const at::Tensor &vp, const at::Tensor &cos, const at::Tensor &sin,
+               const c10::optional<at::Tensor> &q_norm_w, const c10::optional<at::Tensor> &k_norm_w, double eps,
+               bool with_k) {
+  TORCH_CHECK(qkv.is_cuda() && is_half_or_bf16(qkv), "qkv must be a CUDA half/bfloat16 tensor");
+  check_same_device(qkv, {&positions, &slots, &kp, &vp, &cos, &sin});
+  for (const auto *w : {&q_norm_w, &k_norm_w})
+    if (w->has_value() && (*w)->defined()) check_same_device(qkv, {&**w});
+  TORCH_CHECK(qkv.dim() == 2 && (qkv.numel() == 0 || qkv.stride(1) == 1),
+              "qkv must be [tokens, (Hq + 2 Hkv) * D] with a contiguous last dim");
+  check_pages(qkv, kp, vp);
+  const int64_t N = qkv.size(0), Hkv = kp.size(1), D = kp.size(3);
+  TORCH_CHECK(D > 0 && Hkv > 0 && qkv.size(1) % D == 0, "qkv size mismatch");
+  const int64_t Hq = qkv.size(1) / D - 2 * Hkv;
+  TORCH_CHECK(Hq > 0 && Hq % Hkv == 0, "qkv size does not give a valid head count");
+  TORCH_CHECK(positions.scalar_type() == at::kInt && positions.dim() == 1 && positions.size(0) == N &&
+                  positions.is_contiguous(),
+              "positions must be a contiguous int32 vector, one a token");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == N && slots.is_contiguous(),
+              "slots must be a contiguous int64 vector, one a token");
+  TORCH_CHECK(cos.is_contiguous() && sin.is_contiguous() && cos.dim() == 2 && cos.size(1) == D && cos.size(0) > 0 &&
+                  sin.sizes() == cos.sizes() && sin.scalar_type() == cos.scalar_type() && dtype_code(cos) >= 0,
+              "cos/sin must be contiguous [ctx, D] tables");
+  const void *qw = norm_ptr(q_norm_w, qkv, D), *kw = norm_ptr(k_norm_w, qkv, D);
+  const Runs km(kp), vm(vp);
+  bool own = !runs_meet(km) && !runs_meet(vm) && !runs_meet(km, vm);
+  for (const at::Tensor *t : {&qkv, &positions, &slots, &cos, &sin})
+    own = own && !runs_meet(km, Runs(*t)) && !runs_meet(vm, Runs(*t));
+  for (const auto *w : {&q_norm_w, &k_norm_w})
+    if (w->has_value() && (*w)->defined()) own = own && !runs_meet(km, Runs(**w)) && !runs_meet(vm, Runs(**w));
+  TORCH_CHECK(own, "the pages must have memory of their own");
+  c10::DeviceGuard g(qkv.device());
+  at::Tensor q = new_on(qkv, {N, Hq, D}, qkv.scalar_type());
+  c10::optional<at::Tensor> k;
+  if (with_k) k = new_on(qkv, {N, Hkv, D}, qkv.scalar_type());
+  if (N == 0) return {q, k};
+  const int64_t ks[3] = {kp.stride(0), kp.stride(1), kp.stride(2)}, vs[3] = {vp.stride(0), vp.stride(1), vp.stride(2)};
+  check_rc(tpp_qkv_rope_paged(qkv.data_ptr(), N > 1 ? qkv.stride(0) : qkv.size(1), q.data_ptr(),
+                              with_k ? k->data_ptr() : nullptr, kp.data_ptr(), vp.data_ptr(), ks, vs, qw, kw,
+                              cos.data_ptr(), sin.data_ptr(), cos.size(0), positions.data_ptr<int32_t>(),
+                              slots.data_ptr<int64_t>(), N, Hq, Hkv, D, kp.size(0), kp.size(2), (float)eps,
+                              dtype_code(qkv), dtype_code(cos), cur_stream(qkv)),
+           "qkv_rope_paged");
+  return {q, k};
+}
+
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+token_logprobs(const at::Tensor &logits, at::Tensor tokens, int64_t top_k) {
+  TORCH_CHECK(logits.is_cuda() && dtype_code(logits) >= 0, "logits must be a CUDA float32, float16 or bfloat16 tensor");
+  check_same_device(logits, {&tokens});
+  TORCH_CHECK(logits.dim() == 2 && tokens.dim() == 1 && tokens.size(0) == logits.size(0),
+              "logits must be [N, V], tokens [N]");
+  TORCH_CHECK(tokens.scalar_type() == at::kLong, "tokens must be int64");
+  const int64_t N = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V > 0 && (N == 0 || logits.stride(1) == 1 || V == 1), "logits must have a contiguous last dim");
+  TORCH_CHECK(top_k >= 0 && top_k <= 32 && top_k <= V, "top_k must be 0 to 32 and at most the vocabulary, got ", top_k);
+  c10::DeviceGuard g(logits.device());
+  tokens = tokens.contiguous();
+  at::Tensor lp = new_on(logits, {N}, at::kFloat), ent = new_on(logits, {N}, at::kFloat);
+  c10::optional<at::Tensor> tl, tt;
+  if (top_k) tl = new_on(logits, {N, top_k}, at::kFloat), tt = new_on(logits, {N, top_k}, at::kLong);
+  if (N == 0) return {lp, ent, tl, tt};
+  const size_t wsb = tpp_token_logprobs_workspace_size(N, V, top_k, dtype_code(logits));
+  at::Tensor ws; // this call's own, from the caching allocator
+  if (wsb) ws = new_on(logits, {(int64_t)wsb}, at::kByte);
+  check_rc(tpp_token_logprobs(logits.data_ptr(), N > 1 ? logits.stride(0) : V, tokens.data_ptr<int64_t>(),
+                              lp.data_ptr<float>(), ent.data_ptr<float>(), top_k ? tl->data_ptr<float>() : nullptr,
+                              top_k ? tt->data_ptr<int64_t>() : nullptr, N, V, top_k, dtype_code(logits),
+                              wsb ? ws.data_ptr() : nullptr, wsb, cur_stream(logits)),
+           "token_logprobs");
+  return {lp, ent, tl, tt};
+}
+
 } // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1330,6 +1497,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("verify_draft", &verify_draft, "which drafted tokens stay, and the next token",
         py::arg("draft_tokens"), py::arg("target_probs"), py::arg("uniforms"),
         py::arg("draft_probs") = py::none(), py::arg("parents") = py::none());
+  m.def("packed_attention", &packed_attention, "attention of packed sequences of different lengths", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("cu_seqlens_k") = py::none(),
+        py::arg("softmax_scale") = 0.0, py::arg("causal") = true, py::arg("window_left") = -1,
+        py::arg("window_right") = -1, py::arg("out") = py::none());
+  m.def("paged_attention", &paged_attention, "attention of one new token a sequence over pages", py::arg("q"),
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("block_tables"), py::arg("seqlens"),
+        py::arg("softmax_scale") = 0.0, py::arg("window_left") = -1, py::arg("out") = py::none());
+  m.def("qkv_rope_paged", &qkv_rope_paged, "QK norm, rotation at positions, keys and values into pages",
+        py::arg("qkv"), py::arg("positions"), py::arg("slots"), py::arg("k_pages"), py::arg("v_pages"), py::arg("cos"),
+        py::arg("sin"), py::arg("q_norm_w") = py::none(), py::arg("k_norm_w") = py::none(), py::arg("eps") = 1e-6,
+        py::arg("with_k") = true);
+  m.def("token_logprobs", &token_logprobs, "log probabilities of tokens, entropy and the largest logits",
+        py::arg("logits"), py::arg("tokens"), py::arg("top_k") = 0);
   m.def("attn_decode_oproj", &attn_decode_oproj,
         "decode attention (fused QK-norm + RoPE + KV append) then the output projection and the "
         "residual add, in place on residual; returns the attention output",
