@@ -84,6 +84,30 @@ def test_entries_that_are_no_page(dev, d):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128, 48])
+def test_holes_behind_a_window(dev, d):
+    """A row whose window shows holes alone is 0, whatever stands ahead of it; scores of
+    -inf beside holes are NaN."""
+    from torchplusplus_amd.attention import paged_attention
+    lens = [200, 1000, 65, 1000]
+    q, kp, vp, table = make(lens, 4, 2, d, 16, torch.float16, 11, dev)
+    table[0, 11:], table[1, 60:], table[2, 4] = -1, -1, -1
+    table[3, :30] = -1
+    q[3] = q[3].abs() + 0.1
+    for i in range(30, 63):
+        kp[int(table[3, i])] = -math.inf
+    for left in (0, 7, 20, 23):
+        got = paged_attention(q, kp, vp, table, i32(lens, dev), window_left=left)
+        o = oracle.paged_attention(q, kp, vp, table.cpu(), lens, left=left)[0]
+        assert (got[:2] == 0).all() and torch.isnan(got[3]).all()
+        assert (got[2].double().cpu() - o[2]).abs().max() < 0.01
+    got = paged_attention(q, kp, vp, table, i32(lens, dev))
+    assert torch.isnan(got[3]).all() and torch.isfinite(got[:3]).all()
+    table[3, 30:] = -1
+    assert (paged_attention(q, kp, vp, table, i32(lens, dev))[3] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 48])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_rows_that_are_not_seen_may_hold_anything(dev, d, dtype):
     from torchplusplus_amd.attention import paged_attention

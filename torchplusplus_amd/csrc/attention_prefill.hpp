@@ -190,7 +190,6 @@ __global__ __launch_bounds__(64 * NW) void attn_prefill_kernel(A p, int hpb) {
   int npair = p.B * nhg;
   if constexpr (PACKED) { // one list of query tiles for every head
     nqt = __builtin_amdgcn_readfirstlane(p.plan[0]), npair = nhg;
-    asm volatile("" : "+s"(nqt)); // (as in setup)
   }
   const int nitems = npair * nqt;
   int off = Sk - Sq;
@@ -236,9 +235,6 @@ __global__ __launch_bounds__(64 * NW) void attn_prefill_kernel(A p, int hpb) {
       int x[5];
 #pragma unroll
       for (int i = 0; i < 5; ++i) x[i] = __builtin_amdgcn_readfirstlane(it[i]);
-      // here, not where they are used: a scalar load in flight among the counted waits for
-      // LDS reads would be taken for one of them
-      asm volatile("" : "+s"(x[0]), "+s"(x[1]), "+s"(x[2]), "+s"(x[3]), "+s"(x[4]));
       seq_q = x[0], q0 = x[1], Sq = x[2], seq_k = x[3], Sk = x[4], off = Sk - Sq;
     }
     q_last = (q0 + qt_len < Sq ? q0 + qt_len : Sq) - 1;

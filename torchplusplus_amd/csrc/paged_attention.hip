@@ -4,29 +4,29 @@
 // j >= seqlens[b] - 1 - left). The positions of an entry that is no page (outside [0,
 // pages)) are not seen. A row that sees nothing is 0, one whose scores are all -inf NaN.
 #include "attn_row.hpp"
+#include "tree_wave.hpp"
 
 namespace tpp {
 
-struct PagedArgs {
-  const void *q, *k, *v;
-  void *o;
-  int64_t q_s[2], o_s[2];   // {sequence, head}
-  int64_t k_s[3], v_s[3];   // {page, head, row}
-  const int32_t *table, *seqlens;
+// TreeArgs with one token a sequence, {page, head, row} strides in k_s and v_s, and T = 1.
+struct PagedArgs : TreeArgs {
+  static constexpr bool kPaged = true;
+  const int32_t *table;
   int64_t t_sb;
-  int B, Hq, Hkv, G, pages, lpage, Lmax; // pages of 2^lpage rows; Lmax: the table's positions
-  float scale_log2;
-  int left;
+  int pages, lpage, left, lkt; // pages of 2^lpage rows; tiles of 2^lkt keys
+  // of len positions: the first that is seen, the first tile's first, and the keys from there
+  __device__ __forceinline__ int lowest(int len) const { return left >= 0 ? max(len - 1 - left, 0) : 0; }
+  __device__ __forceinline__ int begin(int len) const { return lowest(len) >> lkt << lkt; }
+  __device__ __forceinline__ int keys(int len) const { return max(len - begin(len), 1); } // (none: one split, of zeros)
 };
 
 // Any head size up to 256, any alignment: one wave per (sequence, head).
 template <typename T> __global__ __launch_bounds__(64) void paged_generic_kernel(PagedArgs p, int D) {
   const int lane = lane_id(), h = blockIdx.x, b = blockIdx.y, hk = h / p.G;
-  const int L = min(max(p.seqlens[b], 0), p.Lmax);
-  const int lo = p.left >= 0 ? max(L - 1 - p.left, 0) : 0;
+  const int L = min(max(p.seqlens[b], 0), p.Lmax), lo = p.lowest(L);
   const int32_t *table = p.table + b * p.t_sb;
   AttnRow r;
-  attn_row<T>(r, (const T *)p.q + b * p.q_s[0] + h * p.q_s[1], D, lo, L, p.scale_log2,
+  attn_row<T>(r, (const T *)p.q + b * p.q_s[0] + h * p.q_s[2], D, lo, L, p.scale_log2,
               [&](int j, const T *&k, const T *&v) {
                 const int pg = __builtin_amdgcn_readfirstlane(table[j >> p.lpage]);
                 if (pg < 0 || pg >= p.pages) return false;
@@ -35,17 +35,250 @@ template <typename T> __global__ __launch_bounds__(64) void paged_generic_kernel
                 v = (const T *)p.v + pg * p.v_s[0] + hk * p.v_s[1] + row * p.v_s[2];
                 return true;
               });
-  T *op = (T *)p.o + b * p.o_s[0] + h * p.o_s[1];
+  T *op = (T *)p.o + b * p.o_s[0] + h * p.o_s[2];
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (c * 64 + lane < D) op[c * 64 + lane] = from_f32<T>(r.out(c));
+}
+
+// ---------------------------------------------------------------------------
+// Head sizes 64 and 128, 16-byte rows: TreeWave's products and softmax (tree_wave.hpp), the
+// G query rows of a KV head in one group of 16 or two, a block's four waves over one split of
+// the sequence's keys, each streaming its own tiles of 32 (D = 128) or 64 keys by LDS-DMA.
+//
+// A page holds whole groups of 16 keys and a DMA instruction brings 4 or 8 keys, so one page
+// an instruction: its address is that page's, uniform, plus lane offsets fixed for the launch.
+// The table's entries of a tile's groups are in the wave's first lanes; they come by LDS-DMA
+// a tile ahead, between that tile's K and V (a load into registers was waited for at once, and
+// K with it, where its value is carried around the loop).
+// ---------------------------------------------------------------------------
+// What tile keys kb .. are shown of: pages that exist, positions from the window's first on.
+struct PagedShown {
+  unsigned groups; // bit g: keys 16 g .. of the tile have a page
+  int rel;         // the window's first key in the tile
+  bool any;
+  __device__ __forceinline__ unsigned word(int c) const {
+    const unsigned two = groups >> (2 * c) & 3u, r = (unsigned)(rel - 32 * c);
+    return ((two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u)) &
+           (rel - 32 * c <= 0 ? ~0u : r >= 32u ? 0u : ~0u << r);
+  }
+};
+
+template <typename T, int D, int NC>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs p, float *__restrict__ ws_o,
+                                                            float *__restrict__ ws_ml, int nsplit,
+                                                            unsigned nsplit_inv, unsigned hkv_inv, unsigned g_inv,
+                                                            int by_xcd, unsigned *__restrict__ arrived) {
+  typedef TreeTile<0, D> TT;
+  typedef TreeWave<T, 0, D, NC> W;
+  constexpr int KT = TT::KT, NW = 4, STRIDE = NW * KT, NDMA = TT::TILEB / 1024, C4 = D / 4, ROWS = 16 * NC;
+  constexpr int KPI = 64 / TT::UPR, NG = KT / 16; // keys of a DMA instruction, groups of 16 keys
+  constexpr int SLOT = 2 * TT::TILEB > ROWS * D * 4 ? 2 * TT::TILEB : ROWS * D * 4;
+  constexpr int kRing = NW * SLOT, kMerge = NC == 1 ? tree_merge_lds<D> : 0;
+  __shared__ __attribute__((aligned(16))) char smem[kRing > kMerge ? kRing : kMerge];
+  __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
+  __shared__ unsigned s_entry[NW][64];
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int u4 = lane >> 4, l16 = lane & 15;
+  TreeBlock k = tree_block(p, hkv_inv, by_xcd);
+  const int rows = p.G;
+  W wv;
+  int row0[NC], row[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) row0[i] = k.qt * ROWS + i * 16, row[i] = min(row0[i] + l16, rows - 1);
+  wv.ask(p, k.b, k.hk, g_inv, row);
+  const int len = min(max(__builtin_amdgcn_readfirstlane(p.seqlens[k.b]), 0), p.Lmax);
+  const int lowest = p.lowest(len), begin = p.begin(len);
+  const int nbatch = (int)((unsigned)(p.keys(len) + STRIDE - 1) / (unsigned)STRIDE);
+  const int per = div_inv((unsigned)(nbatch + nsplit - 1), nsplit_inv);
+  k.live = (int)((unsigned)(nbatch + per - 1) / (unsigned)per);
+  if (k.split >= k.live) return;
+  const int c0 = begin + k.split * per * STRIDE; // (below 2^31, as two tiles on: the host's check)
+  const int k_end = (int)min((int64_t)c0 + (int64_t)per * STRIDE, (int64_t)len);
+  const int first = c0 + w * KT;
+  const int n = first < k_end ? (k_end - first + STRIDE - 1) / STRIDE : 0; // this wave's tiles
+
+  const char *ks = (const char *)p.k + (int64_t)k.hk * p.k_s[1] * 2, *vs = (const char *)p.v + (int64_t)k.hk * p.v_s[1] * 2;
+  const int32_t *const table = p.table + (int64_t)k.b * p.t_sb;
+  char *const ring = smem + w * SLOT;
+  unsigned koff[NDMA], voff[NDMA];
+#pragma unroll
+  for (int j = 0; j < NDMA; ++j) {
+    const int kr = lane / TT::UPR, key = j * KPI + kr, u = lane % TT::UPR;
+    koff[j] = (unsigned)(kr * (int)p.k_s[2] * 2 + ((u ^ TT::ksw(key)) << 4));
+    voff[j] = (unsigned)(kr * (int)p.v_s[2] * 2 + ((u ^ TT::vsw(key)) << 4));
+  }
+  // the page of group lane % NG of the tile at kb (past the last key: the last key's)
+  auto entry = [&](int kb) { return table + (min((kb >> 4) + (lane & (NG - 1)), (len - 1) >> 4) >> (p.lpage - 4)); };
+  const int pmask = (1 << p.lpage) - 1;
+  auto issue = [&](const char *head, const int64_t (&st)[3], const unsigned (&off)[NDMA], int kb, int page, char *dst,
+                   auto swizzle) {
+    auto dma = [&](int j, auto place) {
+      const char *src = head + (int64_t)__builtin_amdgcn_readlane(page, j * KPI / 16) * st[0] * 2 + place(kb + j * KPI);
+      __builtin_amdgcn_global_load_lds((const void *)src, (__attribute__((address_space(3))) void *)(dst + j * 1024), 16,
+                                       0, kCpolNT);
+    };
+    if (kb + KT <= len) {
+#pragma unroll
+      for (int j = 0; j < NDMA; ++j) dma(j, [&](int key) { return (int64_t)(key & pmask) * st[2] * 2 + off[j]; });
+    } else { // keys past the last read its row (masked)
+      const int kr = lane / TT::UPR, u = lane % TT::UPR;
+#pragma unroll
+      for (int j = 0; j < NDMA; ++j)
+        dma(j, [&](int key) {
+          return (int64_t)(min(key + kr, len - 1) & pmask) * st[2] * 2 + ((u ^ swizzle(j * KPI + kr)) << 4);
+        });
+    }
+  };
+  // entries that are no page read page 0 (and are hidden)
+  auto real = [&](int page) { return page >= 0 && page < p.pages; };
+  auto shown = [&](int page) { return (unsigned)__ballot(real(page)) & ((1u << NG) - 1u); };
+  auto issue_k = [&](int kb, int page) {
+    issue(ks, p.k_s, koff, kb, real(page) ? page : 0, ring, [](int r) { return TT::ksw(r); });
+  };
+  auto issue_v = [&](int kb, int page) {
+    issue(vs, p.v_s, voff, kb, real(page) ? page : 0, ring + TT::TILEB, [](int r) { return TT::vsw(r); });
+  };
+  auto issue_entry = [&](int kb) {
+    __builtin_amdgcn_global_load_lds((const void *)entry(kb), (__attribute__((address_space(3))) void *)s_entry[w], 4, 0, 0);
+  };
+  int page = 0; // of this tile's groups
+  unsigned groups = 0;
+  bool saw = false;
+  if (n > 0) page = *entry(first);
+  // (waits for the query rows, which have come when the entries have: no tile's loads ahead)
+  wv.begin(len > 0 ? 1ull : 0ull, lds_addr(ring), lds_addr(ring) + TT::TILEB, 0);
+  if (n > 0) {
+    issue_k(first, page);
+    issue_entry(first + STRIDE); // (past the last tile: the last entry)
+    issue_v(first, page);
+    groups = shown(page);
+  }
+  const unsigned entry_at = lds_addr(s_entry[w]) + 4 * lane;
+  for (int it = 0; it < n; ++it) {
+    const int kb = first + it * STRIDE;
+    const bool more = it + 1 < n;
+    PagedShown mask;
+    mask.groups = groups, mask.rel = lowest - kb;
+    mask.any = groups != (1u << NG) - 1u || kb < lowest;
+    saw = saw || groups >> (max(lowest - kb, 0) >> 4); // (a group of keys ahead of the window is none)
+    vm_wait<NDMA>(); // this tile's K and the next one's entries landed, its V may be in flight
+    float next = lds_read_b32<0>(entry_at);
+    wv.step(p, kb, len - 1, 0, 0,
+            [&] { // (the entries came ahead of the K fragments, which were waited for)
+              asm volatile("" : "+v"(next));
+              if (!more) return;
+              page = __float_as_int(next), groups = shown(page);
+              issue_k(kb + STRIDE, page);
+              issue_entry(kb + 2 * STRIDE);
+            },
+            [&] { // the next K, and the entries behind it, may be in flight
+              if (more) vm_wait<NDMA + 1>();
+              else vm_wait<0>();
+            },
+            [&] { if (more) issue_v(kb + STRIDE, page); }, mask);
+  }
+
+  // The wave's rows, then the block's: chunk c (4 values) of row r at c ^ r. A wave that sees
+  // no key has a weight of 1 on nothing below every score, one that sees scores of -inf alone
+  // none, above that: a row of all holes is 0, one of -inf (and holes) 0 / 0.
+  f32x4 *const part = reinterpret_cast<f32x4 *>(ring);
+  const bool odd = wv.end(p) && saw;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int r = i * 16 + l16;
+#pragma unroll
+    for (int tt = 0; tt < W::NT; ++tt)
+      part[r * C4 + ((tt * 4 + u4) ^ (r & (C4 - 1)))] = saw ? wv.o[i][tt] : f32x4{0.f, 0.f, 0.f, 0.f};
+    if (u4 == 0) {
+      s_m[w][r] = !saw ? -3.4e38f : wv.m[i] == -INFINITY ? -3e38f : wv.top(p, i);
+      s_l[w][r] = saw ? wv.l[i] : 1.f;
+    }
+  }
+  if (n > 0 && __any(odd))
+    wv.again(p, k.b, k.hk,
+             [&](int j, const char *&kr, const char *&vr) {
+               const int pg = table[j >> p.lpage];
+               if (pg < 0 || pg >= p.pages || j < lowest) return false;
+               kr = ks + ((int64_t)pg * p.k_s[0] + (int64_t)(j & pmask) * p.k_s[2]) * 2;
+               vr = vs + ((int64_t)pg * p.v_s[0] + (int64_t)(j & pmask) * p.v_s[2]) * 2;
+               return true;
+             },
+             0, first, STRIDE, n, k_end, len - 1, g_inv, row0, rows, [&](int i, int q, int d, float x) {
+               const int r = i * 16 + q;
+               reinterpret_cast<float *>(part + r * C4 + ((d / 4) ^ (r & (C4 - 1))))[d % 4] = x;
+             });
+  __syncthreads();
+  for (int idx = tid; idx < ROWS * C4; idx += 64 * NW) {
+    const int q = idx / C4, c = idx % C4, r = row0[0] + q;
+    if (r >= rows) break;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int ww = 0; ww < NW; ++ww) mx = fmaxf(mx, s_m[ww][q]);
+    float ls = 0.f;
+    f32x4 os = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ww = 0; ww < NW; ++ww) {
+      const float cf = __builtin_amdgcn_exp2f(s_m[ww][q] - mx);
+      ls += s_l[ww][q] * cf;
+      const f32x4 pr = reinterpret_cast<const f32x4 *>(smem + ww * SLOT)[q * C4 + (c ^ (q & (C4 - 1)))];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) os[e] += pr[e] * cf;
+    }
+    if (k.live == 1) {
+      T *op = W::row_of((T *)p.o, p.o_s, p, k.b, k.hk, r, 0);
+      typename VecT<T>::v4 ov;
+      const float inv = 1.f / ls;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
+      *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
+    } else {
+      const int64_t slot = ((int64_t)k.pair * rows + r) * nsplit + k.split;
+      if (NC == 1 && arrived) {
+        store_through(ws_o + slot * D + c * 4, os);
+        if (c == 0) {
+          __hip_atomic_store(&ws_ml[slot * 2], mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __hip_atomic_store(&ws_ml[slot * 2 + 1], ls, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      } else {
+        *reinterpret_cast<f32x4 *>(ws_o + slot * D + c * 4) = os;
+        if (c == 0) ws_ml[slot * 2] = mx, ws_ml[slot * 2 + 1] = ls;
+      }
+    }
+  }
+  if constexpr (NC == 1)
+    if (arrived && k.live > 1) tree_merge_here<T, D>(p, k, rows, nsplit, ws_o, ws_ml, g_inv, arrived, smem);
+}
+
+// How a call is cut: groups of 16 query rows a block, blocks a pair, splits of the keys.
+struct PagedPlan {
+  int nc, qtiles, nsplit;
+};
+static PagedPlan paged_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Lmax) {
+  PagedPlan pl = {0, 0, 0};
+  if (D != 64 && D != 128) return pl;
+  const int64_t G = Hq / Hkv, kt = D == 128 ? 32 : 64;
+  pl.nc = G > 16 ? 2 : 1;
+  pl.qtiles = (int)((G + 16 * pl.nc - 1) / (16 * pl.nc));
+  // two blocks a CU, as many as are resident at once (tree_plan)
+  const int64_t most = (Lmax + 4 * kt - 1) / (4 * kt);
+  const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  int64_t ns = 2 * (int64_t)cus / (B * Hkv * pl.qtiles);
+  if (ns > most) ns = most;
+  pl.nsplit = (int)(ns > 256 ? 256 : ns < 1 ? 1 : ns);
+  return pl;
 }
 
 } // namespace tpp
 
 using namespace tpp;
 
-extern "C" size_t tpp_attn_paged_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Lmax) { return 0; }
+extern "C" size_t tpp_attn_paged_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Lmax) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Lmax <= 0) return 0;
+  const PagedPlan pl = paged_plan(B, Hq, Hkv, D, Lmax);
+  return pl.nsplit > 1 ? (size_t)(B * Hq) * pl.nsplit * (D + 2) * sizeof(float) : 0;
+}
 
 extern "C" int tpp_attn_paged(const void *q, const void *k_pages, const void *v_pages, void *o,
                               const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
@@ -64,24 +297,63 @@ extern "C" int tpp_attn_paged(const void *q, const void *k_pages, const void *v_
   if ((1 << lpage) != page_size)
     return set_error(TPP_E_UNSUPPORTED, "%s: pages of %lld rows; powers of two from 16 to 1024 are handled", name,
                      (long long)page_size);
-  if (D > 256 || B > 65535 || Hq > 65535 || pages > 0x7fffffffLL || table_pages > (0x7fffffffLL >> lpage) - 1)
+  if (D > 256 || B > 65535 || Hq > 65535 || pages > 0x7fffffffLL || table_pages > (0x7fff0000LL >> lpage))
     return set_error(TPP_E_UNSUPPORTED, "%s: head_dim above 256, or too many sequences, heads or pages", name);
   if (B == 0) return TPP_OK;
   if (!q || !o || !seqlens || (pages > 0 && (!k_pages || !v_pages)) || (table_pages > 0 && !block_tables))
     return set_error(TPP_E_INVALID, "%s: null pointer", name);
   PagedArgs a = {};
   a.q = q, a.k = k_pages, a.v = v_pages, a.o = o;
-  for (int i = 0; i < 2; ++i) a.q_s[i] = q_strides[i], a.o_s[i] = o_strides[i];
+  a.q_s[0] = q_strides[0], a.q_s[2] = q_strides[1], a.o_s[0] = o_strides[0], a.o_s[2] = o_strides[1];
   for (int i = 0; i < 3; ++i) a.k_s[i] = k_strides[i], a.v_s[i] = v_strides[i];
   a.table = block_tables, a.t_sb = table_stride, a.seqlens = seqlens;
-  a.B = (int)B, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
-  a.pages = (int)pages, a.lpage = lpage, a.Lmax = (int)(table_pages << lpage);
+  a.B = (int)B, a.T = 1, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
+  a.pages = (int)pages, a.lpage = lpage, a.Lmax = (int)(table_pages << lpage), a.lkt = D == 128 ? 5 : 6;
   const float sc = softmax_scale > 0.f ? softmax_scale : 1.f / sqrtf((float)D);
   a.scale_log2 = sc * 1.4426950408889634f;
   a.left = window_left < 0 ? -1 : window_left;
   hipStream_t st = as_stream(stream);
+  // the matrix-core kernel: whole 16-byte rows, a DMA instruction's by 32-bit byte offsets
+  uint64_t low = (uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)k_pages | (uint64_t)(uintptr_t)v_pages;
+  uint64_t low_o = (uint64_t)(uintptr_t)o;
+  for (int i = 0; i < 3; ++i) {
+    low |= (uint64_t)(a.q_s[i] * 2) | (uint64_t)(a.k_s[i] * 2) | (uint64_t)(a.v_s[i] * 2);
+    low_o |= (uint64_t)(a.o_s[i] * 2);
+  }
+  bool tiles = (D == 64 || D == 128) && !(low & 15) && !(low_o & 7) && pages > 0 && table_pages > 0 &&
+               B * Hkv <= 65535 && (uint64_t)a.G * (uint64_t)a.G < 1ull << 32;
+  for (int64_t r : {a.k_s[2], a.v_s[2]}) tiles = tiles && r >= 0 && r < (1 << 23);
+  if (!tiles)
+    return TPP_DISPATCH_HALF(dtype, [&] {
+      paged_generic_kernel<T><<<dim3((unsigned)Hq, (unsigned)B), dim3(64), 0, st>>>(a, (int)D);
+      return check_launch(name);
+    });
+  const PagedPlan pl = paged_plan(B, Hq, Hkv, D, a.Lmax);
+  const int64_t pairs = B * Hkv;
+  float *ws_o = (float *)workspace, *ws_ml = nullptr;
+  if (pl.nsplit > 1) {
+    if (!workspace || ((uintptr_t)workspace & 127) || ws_bytes < tpp_attn_paged_workspace_size(B, Hq, Hkv, D, a.Lmax))
+      return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
+    ws_ml = ws_o + (size_t)(pairs * a.G) * pl.nsplit * D;
+  }
+  const bool by_xcd = pairs % 8 == 0;
+  // the merge by a pair's last block (one a pair)
+  unsigned *arrived = pl.nsplit > 1 && pl.nc == 1 ? arrival_words(st, pairs) : nullptr;
+  const dim3 grid(by_xcd ? 8 * pl.qtiles : pl.qtiles, pl.nsplit, (unsigned)(by_xcd ? pairs / 8 : pairs));
+  const unsigned ninv = inv_of(pl.nsplit), hinv = inv_of((int)Hkv), ginv = inv_of(a.G);
   return TPP_DISPATCH_HALF(dtype, [&] {
-    paged_generic_kernel<T><<<dim3((unsigned)Hq, (unsigned)B), dim3(64), 0, st>>>(a, (int)D);
+    auto go = [&](auto dd) {
+      constexpr int DD = decltype(dd)::value;
+      if (pl.nc == 1)
+        paged_tile_kernel<T, DD, 1><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, arrived);
+      else
+        paged_tile_kernel<T, DD, 2><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, nullptr);
+      if (pl.nsplit > 1 && !arrived)
+        tree_merge_kernel<T, DD><<<dim3((unsigned)((a.G + 256 / DD - 1) / (256 / DD)), (unsigned)Hkv, (unsigned)B), dim3(256), 0, st>>>(
+            a, ws_o, ws_ml, pl.nsplit, ninv, ginv, a.lkt + 2);
+    };
+    if (D == 128) go(std::integral_constant<int, 128>{});
+    else go(std::integral_constant<int, 64>{});
     return check_launch(name);
   });
 }
