@@ -9,7 +9,8 @@
 //
 // One pass over the row: a thread keeps its running maximum with the two sums, and the
 // place where it met that maximum first. The rows are 2 or 4 V bytes and everything else is
-// small, so HBM bounds the pass.
+// small, so HBM bounds the pass. Rows that do not fill the card are cut into chunks, a block
+// each, whose sums and largest logits a second launch joins.
 //
 // The largest: of 64 groups of threads the `top`-th largest maximum bounds the `top`-th
 // largest logit from below, so only threads whose maximum reaches it have any of them: those
@@ -32,6 +33,8 @@ struct LpArgs {
   int64_t *top_id;
   int64_t x_s, V;
   int top;
+  f32x4 *sums; // of chunks: maximum, the two sums
+  u64 *keys;   // and their largest logits
 };
 
 // Larger floats as larger words (-0 as 0); the place breaks ties, lower first.
@@ -90,106 +93,73 @@ __device__ __forceinline__ LpSums lp_wave(LpSums a) {
   return a;
 }
 
-template <typename P> __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LpArgs p) {
-  __shared__ LpSums s_sum[4];
+// The sums of a block's threads.
+__device__ __forceinline__ LpSums lp_block(const LpSums &a) {
+  __shared__ float s_sum[4][3];
+  const LpSums ws = lp_wave(a);
+  if (lane_id() == 0) s_sum[wave_id()][0] = ws.m, s_sum[wave_id()][1] = ws.s, s_sum[wave_id()][2] = ws.t;
+  __syncthreads();
+  LpSums all = {s_sum[0][0], s_sum[0][1], s_sum[0][2]};
+#pragma unroll
+  for (int i = 1; i < 4; ++i) all.add(LpSums{s_sum[i][0], s_sum[i][1], s_sum[i][2]});
+  return all;
+}
+
+// The `top` largest of a block's elements, put(rank, key) once for each rank (all of them
+// where there are fewer). `mine`: a bound of this thread's keys that one of them reaches;
+// thread_keys(t, lane, bound, f): f(key) by the lanes of a wave for thread t's keys that reach
+// the bound.
+template <typename TK, typename PUT> __device__ __forceinline__ void lp_select(u64 mine, int top, TK thread_keys, PUT put) {
   __shared__ u64 s_max[kLpThreads], s_cand[kLpRoom], s_bound, s_best[4];
   __shared__ int s_active[kLpThreads], s_n[2];
   const int tid = threadIdx.x, lane = lane_id(), w = wave_id();
-  const int64_t r = blockIdx.x, n = p.V;
-  const P *row = (const P *)p.x + r * p.x_s;
-  const int iters = (int)((n + kLpStep - 1) / kLpStep);
-
-  LpSums a = {-INFINITY, 0.f, 0.f};
-  int first = 0; // iteration in which this thread met its maximum
-  for (int i = 0; i < iters; ++i) {
-    float x[kLpRun];
-    lp_load(row, (int64_t)i * kLpStep + tid * kLpRun, n, x);
-    float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (mx > a.m) a.shift(mx), first = i;
-    const float mu = a.m == -INFINITY ? 0.f : a.m;
-#pragma unroll
-    for (int e = 0; e < kLpRun; ++e) {
-      const float d = x[e] - mu, f = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
-      a.s += f;
-      a.t = fmaf(f, fmaxf(d, -1e30f), a.t); // (0 times -inf is none)
-    }
-  }
-  const LpSums ws = lp_wave(a);
-  if (lane == 0) s_sum[w] = ws;
-  const u64 mine = lp_key(a.m, (unsigned)(first * kLpThreads + tid)); // place: the run of eight
   s_max[tid] = mine;
   if (tid < 2) s_n[tid] = 0;
+  if (tid == 0) s_bound = 0;
   __syncthreads();
-  LpSums all = s_sum[0];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) all.add(s_sum[i]);
-  const bool nan = all.s != all.s; // a NaN, or +inf less +inf
-  const float log_z = all.m == -INFINITY ? NAN : logf(all.s);
-  if (tid == 0) {
-    const int64_t t = p.tok[r];
-    p.lp[r] = t < 0 || t >= n ? 0.f : to_f32(row[t]) - all.m - log_z;
-    p.ent[r] = log_z - all.t / all.s;
-  }
-  if (p.top == 0) return;
-  if (nan) { // (the whole block)
-    if (tid < p.top) p.top_lp[r * p.top + tid] = NAN, p.top_id[r * p.top + tid] = -1;
-    return;
-  }
-
-  // the bound: the top-th largest of 64 groups' maxima (four threads a group)
-  if (w == 0) {
+  if (w == 0) { // the top-th largest of 64 groups' (four threads a group)
     u64 g = s_max[lane];
 #pragma unroll
     for (int i = 1; i < 4; ++i) g = max(g, s_max[i * kWave + lane]);
     int rank = 0;
-    for (int l = 0; l < kWave; ++l) rank += __shfl(g, l, kWave) > g;
-    if (rank == p.top - 1) s_bound = g;
+#pragma unroll
+    for (int l = 0; l < kWave; ++l) {
+      const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(g >> 32), l);
+      const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)g, l);
+      rank += (((u64)hi << 32) | lo) > g;
+    }
+    if (rank == top - 1) s_bound = g;
   }
   __syncthreads();
   const u64 bound = s_bound;
   if (mine >= bound) s_active[atomicAdd(&s_n[0], 1)] = tid;
   __syncthreads();
   const int active = s_n[0];
-  // an element as a key with its run's place: reaches the bound or not
-  auto each = [&](auto f) {
-    for (int k = w; k < active; k += 4)
-      for (int i = lane; i < iters; i += kWave) {
-        const unsigned run = (unsigned)(i * kLpThreads + s_active[k]);
-        if ((int64_t)run * kLpRun >= n) continue;
-        float x[kLpRun];
-        lp_load(row, (int64_t)run * kLpRun, n, x);
-#pragma unroll
-        for (int e = 0; e < kLpRun; ++e)
-          if ((int64_t)run * kLpRun + e < n && lp_key(x[e], run) >= bound) f(lp_key(x[e], run * kLpRun + e));
-      }
-  };
-  each([&](u64 key) {
-    const int at = atomicAdd(&s_n[1], 1);
-    if (at < kLpRoom) s_cand[at] = key;
-  });
+  for (int k = w; k < active; k += 4)
+    thread_keys(s_active[k], lane, bound, [&](u64 key) {
+      const int at = atomicAdd(&s_n[1], 1);
+      if (at < kLpRoom) s_cand[at] = key;
+    });
   __syncthreads();
   const int found = s_n[1];
-  auto put = [&](int rank, u64 key) {
-    p.top_lp[r * p.top + rank] = lp_value((unsigned)(key >> 32)) - all.m - log_z;
-    p.top_id[r * p.top + rank] = (int64_t)(0xffffffffu - (unsigned)key);
-  };
   if (found <= kLpRoom) {
     for (int c = tid; c < found; c += kLpThreads) {
       const u64 key = s_cand[c];
       int rank = 0;
       for (int k = 0; k < found; ++k) rank += s_cand[k] > key;
-      if (rank < p.top) put(rank, key);
+      if (rank < top) put(rank, key);
     }
     return;
   }
   // more than the list holds (most of a few threads' elements among the largest): one
   // after the other
   u64 last = ~0ull;
-  for (int k = 0; k < p.top; ++k) {
+  for (int k = 0; k < top; ++k) {
     u64 best = 0;
-    each([&](u64 key) {
-      if (key < last) best = max(best, key);
-    });
+    for (int c = w; c < active; c += 4)
+      thread_keys(s_active[c], lane, bound, [&](u64 key) {
+        if (key < last) best = max(best, key);
+      });
 #pragma unroll
     for (int sh = 1; sh < kWave; sh <<= 1) best = max(best, (u64)__shfl_xor(best, sh, kWave));
     __syncthreads();
@@ -200,11 +170,148 @@ template <typename P> __global__ __launch_bounds__(kLpThreads) void logprob_kern
   }
 }
 
+// What the row's results are made of, by the block that has all of it.
+struct LpRow {
+  float m, log_z;
+  bool nan; // a NaN, or +inf less +inf
+};
+template <typename P> __device__ __forceinline__ LpRow lp_finish(const LpArgs &p, int64_t r, const LpSums &all) {
+  const P *row = (const P *)p.x + r * p.x_s;
+  const LpRow o = {all.m, all.m == -INFINITY ? NAN : logf(all.s), all.s != all.s};
+  if (threadIdx.x == 0) {
+    const int64_t t = p.tok[r];
+    p.lp[r] = t < 0 || t >= p.V ? 0.f : to_f32(row[t]) - all.m - o.log_z;
+    p.ent[r] = o.log_z - all.t / all.s;
+  }
+  if (o.nan && (int)threadIdx.x < p.top) p.top_lp[r * p.top + threadIdx.x] = NAN, p.top_id[r * p.top + threadIdx.x] = -1;
+  return o;
+}
+__device__ __forceinline__ void lp_put(const LpArgs &p, int64_t r, const LpRow &o, int rank, u64 key) {
+  p.top_lp[r * p.top + rank] = lp_value((unsigned)(key >> 32)) - o.m - o.log_z;
+  p.top_id[r * p.top + rank] = (int64_t)(0xffffffffu - (unsigned)key);
+}
+
+// A row (WHOLE), or chunk blockIdx.y of one: `steps` iterations of the block.
+template <typename P, bool WHOLE> __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LpArgs p, int steps) {
+  constexpr int U = 4; // iterations whose loads are in flight
+  typedef typename LpVec<P>::type V;
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x, base = WHOLE ? 0 : (int64_t)blockIdx.y * steps * kLpStep;
+  const P *row = (const P *)p.x + r * p.x_s;
+  const int64_t n = WHOLE ? p.V : min(p.V, base + (int64_t)steps * kLpStep);
+  const int iters = (int)((n - base + kLpStep - 1) / kLpStep), full = (int)((n - base) / kLpStep);
+
+  LpSums a = {-INFINITY, 0.f, 0.f};
+  int first = 0; // iteration in which this thread met its maximum
+  auto add = [&](const float (&x)[kLpRun], int i) {
+    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (mx > a.m) a.shift(mx), first = i;
+    const float mu = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+    for (int e = 0; e < kLpRun; ++e) {
+      const float d = x[e] - mu, f = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+      a.s += f;
+      a.t = fmaf(f, fmaxf(d, -1e30f), a.t); // (0 times -inf is none)
+    }
+  };
+  const P *mine_at = row + base + tid * kLpRun;
+  int i = 0;
+  if (full >= U) {
+    V v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = __builtin_nontemporal_load((const V *)(mine_at + (int64_t)u * kLpStep));
+    for (; i + U <= full; i += U)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[kLpRun];
+#pragma unroll
+        for (int e = 0; e < kLpRun; ++e) x[e] = to_f32(v[u][e]);
+        // (past the last whole round: an iteration that is there, not used)
+        const int next = i + u + U < full / U * U ? i + u + U : i + u;
+        v[u] = __builtin_nontemporal_load((const V *)(mine_at + (int64_t)next * kLpStep));
+        add(x, i + u);
+      }
+  }
+  for (; i < iters; ++i) {
+    float x[kLpRun];
+    lp_load(row, base + (int64_t)i * kLpStep + tid * kLpRun, n, x);
+    add(x, i);
+  }
+
+  const unsigned run0 = (unsigned)(base / kLpRun); // a place is a run of eight, counted over the row
+  const u64 mine = lp_key(a.m, run0 + (unsigned)(first * kLpThreads + tid));
+  const LpSums all = lp_block(a);
+  auto keys = [&](int t, int lane, u64 bound, auto f) {
+    for (int j = lane; j < iters; j += kWave) {
+      const unsigned run = run0 + (unsigned)(j * kLpThreads + t);
+      if ((int64_t)run * kLpRun >= n) continue;
+      float x[kLpRun];
+      lp_load(row, (int64_t)run * kLpRun, n, x);
+#pragma unroll
+      for (int e = 0; e < kLpRun; ++e)
+        if ((int64_t)run * kLpRun + e < n && lp_key(x[e], run) >= bound) f(lp_key(x[e], run * kLpRun + e));
+    }
+  };
+  if constexpr (WHOLE) {
+    const LpRow o = lp_finish<P>(p, r, all);
+    if (p.top && !o.nan) lp_select(mine, p.top, keys, [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
+  } else {
+    const int64_t slot = r * gridDim.y + blockIdx.y;
+    if (tid == 0) p.sums[slot] = f32x4{all.m, all.s, all.t, 0.f};
+    if (p.top == 0) return;
+    u64 *out = p.keys + slot * p.top;
+    if (all.s != all.s) return; // (the row is NaN, no key is read)
+    if (n - base < p.top && tid < p.top) out[tid] = 0; // below every key; those that are there replace it
+    __syncthreads();
+    lp_select(mine, p.top, keys, [&](int rank, u64 key) { out[rank] = key; });
+  }
+}
+
+// The chunks of a row.
+template <typename P> __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(LpArgs p, int chunks) {
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x;
+  LpSums a = {-INFINITY, 0.f, 0.f};
+  for (int c = tid; c < chunks; c += kLpThreads) {
+    const f32x4 x = p.sums[r * chunks + c];
+    a.add(LpSums{x[0], x[1], x[2]});
+  }
+  const u64 *in = p.keys + r * chunks * p.top;
+  const int n = chunks * p.top;
+  u64 mine = 0;
+  for (int c = tid; c < n; c += kLpThreads) mine = max(mine, in[c]);
+  const LpRow o = lp_finish<P>(p, r, lp_block(a));
+  if (p.top && !o.nan)
+    lp_select(mine, p.top,
+              [&](int t, int lane, u64 bound, auto f) {
+                for (int c = t + lane * kLpThreads; c < n; c += kWave * kLpThreads)
+                  if (in[c] >= bound) f(in[c]);
+              },
+              [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
+}
+
+// Chunks of a row (1: none), of `steps` iterations: four blocks a CU.
+struct LpPlan {
+  int chunks, steps;
+};
+static LpPlan lp_plan(int64_t N, int64_t V) {
+  const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  const int64_t iters = (V + kLpStep - 1) / kLpStep;
+  int64_t c = (4 * cus + N - 1) / N;
+  if (c > iters) c = iters;
+  const int64_t steps = (iters + c - 1) / c;
+  return {(int)((iters + steps - 1) / steps), (int)steps};
+}
+
 } // namespace tpp
 
 using namespace tpp;
 
-extern "C" size_t tpp_token_logprobs_workspace_size(int64_t N, int64_t V, int64_t top, int dtype) { return 0; }
+extern "C" size_t tpp_token_logprobs_workspace_size(int64_t N, int64_t V, int64_t top, int dtype) {
+  if (N <= 0 || V <= 0 || top < 0) return 0;
+  const LpPlan pl = lp_plan(N, V);
+  return pl.chunks > 1 ? (size_t)N * pl.chunks * (sizeof(f32x4) + (size_t)top * sizeof(u64)) : 0;
+}
 
 extern "C" int tpp_token_logprobs(const void *logits, int64_t row_stride, const int64_t *tokens, float *logprobs,
                                   float *entropy, float *top_logprobs, int64_t *top_tokens, int64_t N, int64_t V,
@@ -223,10 +330,21 @@ extern "C" int tpp_token_logprobs(const void *logits, int64_t row_stride, const 
   LpArgs a = {};
   a.x = logits, a.tok = tokens, a.lp = logprobs, a.ent = entropy, a.top_lp = top_logprobs, a.top_id = top_tokens;
   a.x_s = row_stride, a.V = V, a.top = (int)top;
+  const LpPlan pl = lp_plan(N, V);
+  if (pl.chunks > 1) {
+    if (!workspace || !aligned16(workspace) || ws_bytes < tpp_token_logprobs_workspace_size(N, V, top, dtype))
+      return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
+    a.sums = (f32x4 *)workspace, a.keys = (u64 *)(a.sums + N * pl.chunks);
+  }
   hipStream_t st = as_stream(stream);
   auto go = [&](auto zero) {
     typedef decltype(zero) P;
-    logprob_kernel<P><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a);
+    if (pl.chunks == 1) {
+      logprob_kernel<P, true><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a, pl.steps);
+    } else {
+      logprob_kernel<P, false><<<dim3((unsigned)N, pl.chunks), dim3(kLpThreads), 0, st>>>(a, pl.steps);
+      logprob_join_kernel<P><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a, pl.chunks);
+    }
     return check_launch(name);
   };
   return dtype == TPP_F32 ? go(0.f) : dtype == TPP_F16 ? go(f16(0)) : go(bf16(0));
