@@ -10,7 +10,9 @@
 // One pass over the row: a thread keeps its running maximum with the two sums, and the
 // place where it met that maximum first. The rows are 2 or 4 V bytes and everything else is
 // small, so HBM bounds the pass. Rows that do not fill the card are cut into chunks, a block
-// each, whose sums and largest logits a second launch joins.
+// each, whose sums and largest logits the row's last block to finish joins: it is found by an
+// arrival word, and the chunks' results go past the caches, since the blocks may run on any
+// XCD. Captured calls, and those of more rows than there are words, join in a second launch.
 //
 // The largest: of 64 groups of threads the `top`-th largest maximum bounds the `top`-th
 // largest logit from below, so only threads whose maximum reaches it have any of them: those
@@ -33,8 +35,8 @@ struct LpArgs {
   int64_t *top_id;
   int64_t x_s, V;
   int top;
-  f32x4 *sums; // of chunks: maximum, the two sums
-  u64 *keys;   // and their largest logits
+  u64 *sums, *keys; // of chunks: maximum and the two sums, two words; their largest logits
+  unsigned *arrived; // a word a row, or null
 };
 
 // Larger floats as larger words (-0 as 0); the place breaks ties, lower first.
@@ -83,20 +85,14 @@ struct LpSums { // of elements met so far: maximum, sum of e^(x - m), sum of e^(
   }
 };
 
-__device__ __forceinline__ LpSums lp_wave(LpSums a) {
-#pragma unroll
-  for (int sh = 1; sh < kWave; sh <<= 1) {
-    LpSums o;
-    o.m = __shfl_xor(a.m, sh, kWave), o.s = __shfl_xor(a.s, sh, kWave), o.t = __shfl_xor(a.t, sh, kWave);
-    a.add(o);
-  }
-  return a;
-}
-
 // The sums of a block's threads.
 __device__ __forceinline__ LpSums lp_block(const LpSums &a) {
   __shared__ float s_sum[4][3];
-  const LpSums ws = lp_wave(a);
+  float mx = row16_max(a.m);
+  mx = fmaxf(fmaxf(readlane_f32(mx, 0), readlane_f32(mx, 16)), fmaxf(readlane_f32(mx, 32), readlane_f32(mx, 48)));
+  LpSums ws = a;
+  ws.shift(mx);
+  ws.s = wave_sum(ws.s), ws.t = wave_sum(ws.t);
   if (lane_id() == 0) s_sum[wave_id()][0] = ws.m, s_sum[wave_id()][1] = ws.s, s_sum[wave_id()][2] = ws.t;
   __syncthreads();
   LpSums all = {s_sum[0][0], s_sum[0][1], s_sum[0][2]};
@@ -107,39 +103,50 @@ __device__ __forceinline__ LpSums lp_block(const LpSums &a) {
 
 // The `top` largest of a block's elements, put(rank, key) once for each rank (all of them
 // where there are fewer). `mine`: a bound of this thread's keys that one of them reaches;
-// thread_keys(t, lane, bound, f): f(key) by the lanes of a wave for thread t's keys that reach
-// the bound.
-template <typename TK, typename PUT> __device__ __forceinline__ void lp_select(u64 mine, int top, TK thread_keys, PUT put) {
+// keys(t, j, bound, f), j < items: f(key) for those of thread t's j-th item that reach the
+// bound.
+template <typename TK, typename PUT>
+__device__ __forceinline__ void lp_select(u64 mine, int top, int items, TK keys, PUT put) {
   __shared__ u64 s_max[kLpThreads], s_cand[kLpRoom], s_bound, s_best[4];
-  __shared__ int s_active[kLpThreads], s_n[2];
+  __shared__ int s_active[kLpThreads], s_n[2], s_rank[kWave];
   const int tid = threadIdx.x, lane = lane_id(), w = wave_id();
   s_max[tid] = mine;
   if (tid < 2) s_n[tid] = 0;
   if (tid == 0) s_bound = 0;
+  if (w == 0) s_rank[lane] = 0;
   __syncthreads();
-  if (w == 0) { // the top-th largest of 64 groups' (four threads a group)
-    u64 g = s_max[lane];
+  // the top-th largest of 64 groups' (four threads a group); a wave counts a quarter of what is larger
+  u64 g = s_max[lane];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) g = max(g, s_max[i * kWave + lane]);
-    int rank = 0;
+  for (int i = 1; i < 4; ++i) g = max(g, s_max[i * kWave + lane]);
+  int larger = 0;
 #pragma unroll
-    for (int l = 0; l < kWave; ++l) {
-      const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(g >> 32), l);
-      const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)g, l);
-      rank += (((u64)hi << 32) | lo) > g;
-    }
-    if (rank == top - 1) s_bound = g;
+  for (int l = 0; l < kWave / 4; ++l) {
+    const int from = (w * (kWave / 4) + l);
+    const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(g >> 32), from);
+    const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)g, from);
+    larger += (((u64)hi << 32) | lo) > g;
   }
+  atomicAdd(&s_rank[lane], larger);
+  __syncthreads();
+  if (w == 0 && s_rank[lane] == top - 1) s_bound = g;
   __syncthreads();
   const u64 bound = s_bound;
   if (mine >= bound) s_active[atomicAdd(&s_n[0], 1)] = tid;
   __syncthreads();
-  const int active = s_n[0];
-  for (int k = w; k < active; k += 4)
-    thread_keys(s_active[k], lane, bound, [&](u64 key) {
-      const int at = atomicAdd(&s_n[1], 1);
-      if (at < kLpRoom) s_cand[at] = key;
-    });
+  // the active threads' items over the block (a wave a thread would wait for memory once for
+  // each of them)
+  const unsigned all = (unsigned)(s_n[0] * items);
+  auto each = [&](auto f) {
+    for (unsigned i = tid; i < all; i += kLpThreads) {
+      const unsigned k = i / (unsigned)items;
+      keys(s_active[k], (int)(i - k * (unsigned)items), bound, f);
+    }
+  };
+  each([&](u64 key) {
+    const int at = atomicAdd(&s_n[1], 1);
+    if (at < kLpRoom) s_cand[at] = key;
+  });
   __syncthreads();
   const int found = s_n[1];
   if (found <= kLpRoom) {
@@ -156,10 +163,9 @@ template <typename TK, typename PUT> __device__ __forceinline__ void lp_select(u
   u64 last = ~0ull;
   for (int k = 0; k < top; ++k) {
     u64 best = 0;
-    for (int c = w; c < active; c += 4)
-      thread_keys(s_active[c], lane, bound, [&](u64 key) {
-        if (key < last) best = max(best, key);
-      });
+    each([&](u64 key) {
+      if (key < last) best = max(best, key);
+    });
 #pragma unroll
     for (int sh = 1; sh < kWave; sh <<= 1) best = max(best, (u64)__shfl_xor(best, sh, kWave));
     __syncthreads();
@@ -175,12 +181,24 @@ struct LpRow {
   float m, log_z;
   bool nan; // a NaN, or +inf less +inf
 };
-template <typename P> __device__ __forceinline__ LpRow lp_finish(const LpArgs &p, int64_t r, const LpSums &all) {
-  const P *row = (const P *)p.x + r * p.x_s;
-  const LpRow o = {all.m, all.m == -INFINITY ? NAN : logf(all.s), all.s != all.s};
+// The row's token's logit, by thread 0: asked for ahead of everything else.
+struct LpToken {
+  float x;
+  bool real;
+};
+template <typename P> __device__ __forceinline__ LpToken lp_token(const LpArgs &p, int64_t r) {
+  LpToken k = {0.f, false};
   if (threadIdx.x == 0) {
     const int64_t t = p.tok[r];
-    p.lp[r] = t < 0 || t >= p.V ? 0.f : to_f32(row[t]) - all.m - o.log_z;
+    k.real = t >= 0 && t < p.V;
+    if (k.real) k.x = to_f32(((const P *)p.x)[r * p.x_s + t]);
+  }
+  return k;
+}
+__device__ __forceinline__ LpRow lp_finish(const LpArgs &p, int64_t r, const LpSums &all, const LpToken &k) {
+  const LpRow o = {all.m, all.m == -INFINITY ? NAN : logf(all.s), all.s != all.s};
+  if (threadIdx.x == 0) {
+    p.lp[r] = k.real ? k.x - all.m - o.log_z : 0.f;
     p.ent[r] = o.log_z - all.t / all.s;
   }
   if (o.nan && (int)threadIdx.x < p.top) p.top_lp[r * p.top + threadIdx.x] = NAN, p.top_id[r * p.top + threadIdx.x] = -1;
@@ -189,6 +207,44 @@ template <typename P> __device__ __forceinline__ LpRow lp_finish(const LpArgs &p
 __device__ __forceinline__ void lp_put(const LpArgs &p, int64_t r, const LpRow &o, int rank, u64 key) {
   p.top_lp[r * p.top + rank] = lp_value((unsigned)(key >> 32)) - o.m - o.log_z;
   p.top_id[r * p.top + rank] = (int64_t)(0xffffffffu - (unsigned)key);
+}
+
+// To and from another block of the launch.
+__device__ __forceinline__ void lp_store(u64 *p, u64 x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ u64 lp_fetch(const u64 *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The chunks of a row, by one block.
+__device__ __forceinline__ void lp_join(const LpArgs &p, int64_t r, int chunks, const LpToken &k) {
+  constexpr int kKeep = 4; // keys a thread keeps (past them, memory is asked again)
+  const int tid = threadIdx.x;
+  const u64 *sums = p.sums + r * chunks * 2, *in = p.keys + r * chunks * p.top;
+  const int n = chunks * p.top;
+  LpSums a = {-INFINITY, 0.f, 0.f};
+  __shared__ u64 s_key[kKeep * kLpThreads];
+  u64 key[kKeep], mine = 0;
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) key[j] = j * kLpThreads + tid < n ? lp_fetch(in + j * kLpThreads + tid) : 0;
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) s_key[j * kLpThreads + tid] = key[j], mine = max(mine, key[j]);
+  for (int c = kKeep * kLpThreads + tid; c < n; c += kLpThreads) mine = max(mine, lp_fetch(in + c));
+  for (int c = tid; c < chunks; c += kLpThreads) {
+    const u32x2 x = __builtin_bit_cast(u32x2, lp_fetch(sums + c * 2)), y = __builtin_bit_cast(u32x2, lp_fetch(sums + c * 2 + 1));
+    a.add(LpSums{__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(y[0])});
+  }
+  const LpRow o = lp_finish(p, r, lp_block(a), k);
+  if (p.top && !o.nan)
+    lp_select(mine, p.top, (n + kLpThreads - 1) / kLpThreads,
+              [&](int t, int j, u64 bound, auto f) {
+                const int c = j * kLpThreads + t;
+                if (c >= n) return;
+                const u64 x = c < kKeep * kLpThreads ? s_key[c] : lp_fetch(in + c);
+                if (x >= bound) f(x);
+              },
+              [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
 }
 
 // A row (WHOLE), or chunk blockIdx.y of one: `steps` iterations of the block.
@@ -201,6 +257,7 @@ template <typename P, bool WHOLE> __global__ __launch_bounds__(kLpThreads) void 
   const int64_t n = WHOLE ? p.V : min(p.V, base + (int64_t)steps * kLpStep);
   const int iters = (int)((n - base + kLpStep - 1) / kLpStep), full = (int)((n - base) / kLpStep);
 
+  const LpToken token = lp_token<P>(p, r);
   LpSums a = {-INFINITY, 0.f, 0.f};
   int first = 0; // iteration in which this thread met its maximum
   auto add = [&](const float (&x)[kLpRun], int i) {
@@ -241,63 +298,59 @@ template <typename P, bool WHOLE> __global__ __launch_bounds__(kLpThreads) void 
   const unsigned run0 = (unsigned)(base / kLpRun); // a place is a run of eight, counted over the row
   const u64 mine = lp_key(a.m, run0 + (unsigned)(first * kLpThreads + tid));
   const LpSums all = lp_block(a);
-  auto keys = [&](int t, int lane, u64 bound, auto f) {
-    for (int j = lane; j < iters; j += kWave) {
-      const unsigned run = run0 + (unsigned)(j * kLpThreads + t);
-      if ((int64_t)run * kLpRun >= n) continue;
-      float x[kLpRun];
-      lp_load(row, (int64_t)run * kLpRun, n, x);
+  auto keys = [&](int t, int j, u64 bound, auto f) {
+    const unsigned run = run0 + (unsigned)(j * kLpThreads + t);
+    if ((int64_t)run * kLpRun >= n) return;
+    float x[kLpRun];
+    lp_load(row, (int64_t)run * kLpRun, n, x);
 #pragma unroll
-      for (int e = 0; e < kLpRun; ++e)
-        if ((int64_t)run * kLpRun + e < n && lp_key(x[e], run) >= bound) f(lp_key(x[e], run * kLpRun + e));
-    }
+    for (int e = 0; e < kLpRun; ++e)
+      if ((int64_t)run * kLpRun + e < n && lp_key(x[e], run) >= bound) f(lp_key(x[e], run * kLpRun + e));
   };
   if constexpr (WHOLE) {
-    const LpRow o = lp_finish<P>(p, r, all);
-    if (p.top && !o.nan) lp_select(mine, p.top, keys, [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
+    const LpRow o = lp_finish(p, r, all, token);
+    if (p.top && !o.nan) lp_select(mine, p.top, iters, keys, [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
   } else {
-    const int64_t slot = r * gridDim.y + blockIdx.y;
-    if (tid == 0) p.sums[slot] = f32x4{all.m, all.s, all.t, 0.f};
-    if (p.top == 0) return;
-    u64 *out = p.keys + slot * p.top;
-    if (all.s != all.s) return; // (the row is NaN, no key is read)
-    if (n - base < p.top && tid < p.top) out[tid] = 0; // below every key; those that are there replace it
+    const int chunks = gridDim.y;
+    const int64_t slot = r * chunks + blockIdx.y;
+    if (tid == 0) {
+      lp_store(p.sums + slot * 2, __builtin_bit_cast(u64, u32x2{__float_as_uint(all.m), __float_as_uint(all.s)}));
+      lp_store(p.sums + slot * 2 + 1, (u64)__float_as_uint(all.t));
+    }
+    if (p.top && all.s == all.s) { // (else the row is NaN, no key is used)
+      u64 *out = p.keys + slot * p.top;
+      if (n - base < p.top && tid >= n - base && tid < p.top) lp_store(out + tid, 0); // fewer elements: below every key
+      lp_select(mine, p.top, iters, keys, [&](int rank, u64 key) { lp_store(out + rank, key); });
+    }
+    if (!p.arrived) return;
+    __shared__ int s_last;
+    asm volatile("" ::: "memory");
+    vm_wait<0>(); // this wave's results are in memory
     __syncthreads();
-    lp_select(mine, p.top, keys, [&](int rank, u64 key) { out[rank] = key; });
+    if (tid == 0) {
+      const unsigned old = __hip_atomic_fetch_add(p.arrived + r, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = (int)old == chunks - 1;
+      if (s_last) __hip_atomic_store(p.arrived + r, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (s_last) lp_join(p, r, chunks, token);
   }
 }
 
-// The chunks of a row.
 template <typename P> __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(LpArgs p, int chunks) {
-  const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x;
-  LpSums a = {-INFINITY, 0.f, 0.f};
-  for (int c = tid; c < chunks; c += kLpThreads) {
-    const f32x4 x = p.sums[r * chunks + c];
-    a.add(LpSums{x[0], x[1], x[2]});
-  }
-  const u64 *in = p.keys + r * chunks * p.top;
-  const int n = chunks * p.top;
-  u64 mine = 0;
-  for (int c = tid; c < n; c += kLpThreads) mine = max(mine, in[c]);
-  const LpRow o = lp_finish<P>(p, r, lp_block(a));
-  if (p.top && !o.nan)
-    lp_select(mine, p.top,
-              [&](int t, int lane, u64 bound, auto f) {
-                for (int c = t + lane * kLpThreads; c < n; c += kWave * kLpThreads)
-                  if (in[c] >= bound) f(in[c]);
-              },
-              [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
+  lp_join(p, blockIdx.x, chunks, lp_token<P>(p, blockIdx.x));
 }
 
-// Chunks of a row (1: none), of `steps` iterations: four blocks a CU.
+// Chunks of a row (1: none), of `steps` iterations: one block a CU. (8 bf16 rows of 151936,
+// five alternatives, one to eight blocks a CU: 10.3, 10.8, 12.2 us; 77 fp32 rows of 50257, 20
+// alternatives: 14.4, 15.2, 15.7: what is selected a chunk costs more than the chunk's loads.)
 struct LpPlan {
   int chunks, steps;
 };
 static LpPlan lp_plan(int64_t N, int64_t V) {
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
   const int64_t iters = (V + kLpStep - 1) / kLpStep;
-  int64_t c = (4 * cus + N - 1) / N;
+  int64_t c = (cus + N - 1) / N;
   if (c > iters) c = iters;
   const int64_t steps = (iters + c - 1) / c;
   return {(int)((iters + steps - 1) / steps), (int)steps};
@@ -310,7 +363,7 @@ using namespace tpp;
 extern "C" size_t tpp_token_logprobs_workspace_size(int64_t N, int64_t V, int64_t top, int dtype) {
   if (N <= 0 || V <= 0 || top < 0) return 0;
   const LpPlan pl = lp_plan(N, V);
-  return pl.chunks > 1 ? (size_t)N * pl.chunks * (sizeof(f32x4) + (size_t)top * sizeof(u64)) : 0;
+  return pl.chunks > 1 ? (size_t)N * pl.chunks * (2 + (size_t)top) * sizeof(u64) : 0;
 }
 
 extern "C" int tpp_token_logprobs(const void *logits, int64_t row_stride, const int64_t *tokens, float *logprobs,
@@ -334,16 +387,17 @@ extern "C" int tpp_token_logprobs(const void *logits, int64_t row_stride, const 
   if (pl.chunks > 1) {
     if (!workspace || !aligned16(workspace) || ws_bytes < tpp_token_logprobs_workspace_size(N, V, top, dtype))
       return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
-    a.sums = (f32x4 *)workspace, a.keys = (u64 *)(a.sums + N * pl.chunks);
+    a.sums = (u64 *)workspace, a.keys = a.sums + N * pl.chunks * 2;
   }
   hipStream_t st = as_stream(stream);
+  if (pl.chunks > 1) a.arrived = arrival_words(st, N);
   auto go = [&](auto zero) {
     typedef decltype(zero) P;
     if (pl.chunks == 1) {
       logprob_kernel<P, true><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a, pl.steps);
     } else {
       logprob_kernel<P, false><<<dim3((unsigned)N, pl.chunks), dim3(kLpThreads), 0, st>>>(a, pl.steps);
-      logprob_join_kernel<P><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a, pl.chunks);
+      if (!a.arrived) logprob_join_kernel<P><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a, pl.chunks);
     }
     return check_launch(name);
   };
