@@ -196,7 +196,7 @@ int tpp_rope_at(const void *q, const void *k, void *q_out, void *k_out,
  * sequence. Rows that see nothing are 0, rows whose scores are all -inf NaN. Rows
  * of no sequence become 0 if `fill`, else stay as they were. D <= 256. Workspace
  * (16-byte aligned, no initialisation, this call's own) of
- * tpp_attn_packed_workspace_size bytes (0: none). Next to flash_attn_func
+ * tpp_attn_packed_workspace_size bytes (0: none; `self`: cu_k is NULL). Next to flash_attn_func
  * (torchpp/attention/gqa.py:128), whose sequences have one length. */
 int tpp_attn_packed(const void *q, const void *k, const void *v, void *o,
                     const int64_t *q_strides, const int64_t *k_strides,
@@ -207,7 +207,8 @@ int tpp_attn_packed(const void *q, const void *k, const void *v, void *o,
                     int window_right, int fill, int dtype, void *workspace,
                     size_t ws_bytes, void *stream);
 size_t tpp_attn_packed_workspace_size(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq,
-                                      int64_t Hkv, int64_t D);
+                                      int64_t Hkv, int64_t D, int causal,
+                                      int window_left, int window_right, int self);
 
 /* Attention of one new token a sequence over a cache held in pages: q, o [B, Hq, D]
  * ({sequence, head} strides), k_pages, v_pages [pages, Hkv, page_size, D] ({page,

@@ -1,6 +1,6 @@
 // Prefill attention on the matrix cores: the kernels of attention.hip, for a batch of one
-// length, and of packed_attention.hip, for sequences of different lengths packed one behind
-// the other. attention.hip's head explains the layouts.
+// length, of which packed_attention.hip takes attn_prefill_kernel for sequences of different
+// lengths packed one behind the other. attention.hip's head explains the layouts.
 #pragma once
 #include "attn_row.hpp"
 
@@ -63,31 +63,30 @@ __device__ __forceinline__ KeyRange packed_keys(const PackedArgs &p, int i, int 
 // be infinite; fp16's weights want the room above them, not to lose those below 2^-24.
 template <typename T, bool PACKED> constexpr float kWeightUp = !PACKED ? 0.f : __is_same(T, bf16) ? -20.f : 7.f;
 
-// A packed row again, by one wave from its definition, and past the other kernels' 0: an
-// infinity or NaN among the values that a row does not see, times its weight of 0, is a NaN
-// in the sums of a tile.
+// Row qrow of q and o again, by one wave from its definition over rows klo .. khi - 1 of k and
+// v: an infinity or NaN among the values that a row does not see, times its weight of 0, is a
+// NaN in the sums of a tile.
 template <typename T, int D>
-__device__ __forceinline__ void packed_row_again(const PackedArgs &p, const PackedSeq &s, int i, int hq, int hk) {
+__device__ __forceinline__ void packed_row_again(const PackedArgs &p, int qrow, int klo, int khi, int hq, int hk) {
   AttnRow r;
-  const KeyRange kr = packed_keys(p, i, s.Sq, s.Sk);
-  attn_row<T>(r, (const T *)p.q + (int64_t)(s.q0 + i) * p.q_ss + hq * p.q_sh, D, kr.lo, kr.hi, p.scale_log2,
+  attn_row<T>(r, (const T *)p.q + (int64_t)qrow * p.q_ss + hq * p.q_sh, D, klo, khi, p.scale_log2,
               [&](int j, const T *&k, const T *&v) {
-                k = (const T *)p.k + (int64_t)(s.k0 + j) * p.k_ss + hk * p.k_sh;
-                v = (const T *)p.v + (int64_t)(s.k0 + j) * p.v_ss + hk * p.v_sh;
+                k = (const T *)p.k + (int64_t)j * p.k_ss + hk * p.k_sh;
+                v = (const T *)p.v + (int64_t)j * p.v_ss + hk * p.v_sh;
                 return true;
               });
-  T *op = (T *)p.o + (int64_t)(s.q0 + i) * p.o_ss + hq * p.o_sh;
+  T *op = (T *)p.o + (int64_t)qrow * p.o_ss + hq * p.o_sh;
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) op[c * 64 + lane_id()] = from_f32<T>(r.out(c));
 }
-// Whether a value that is not finite stands among keys [a, b) (one wave).
+// Whether a value that is not finite stands in rows [a, b) of v (one wave).
 template <typename T, int D>
-__device__ __forceinline__ bool packed_odd_values(const PackedArgs &p, const PackedSeq &s, int hk, int a, int b) {
+__device__ __forceinline__ bool packed_odd_values(const PackedArgs &p, int hk, int a, int b) {
   bool odd = false;
   for (int j = a; j < b; ++j)
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
-      const float x = to_f32(((const T *)p.v)[(int64_t)(s.k0 + j) * p.v_ss + hk * p.v_sh + c * 64 + lane_id()]);
+      const float x = to_f32(((const T *)p.v)[(int64_t)j * p.v_ss + hk * p.v_sh + c * 64 + lane_id()]);
       odd = odd || !(fabsf(x) < INFINITY);
     }
   return __any(odd);
@@ -684,11 +683,15 @@ __global__ __launch_bounds__(64 * NW) void attn_prefill_kernel(A p, int hpb) {
         if (bad) {
           const int qa = oqw + g * 32, qe = min(qa + 31, oSq - 1);
           const KeyRange ka = packed_keys(p, qa, oseq.Sq, oseq.Sk), ke = packed_keys(p, qe, oseq.Sq, oseq.Sk);
-          if (packed_odd_values<T, D>(p, oseq, ohk, o_tb * kKvTile, min(ke.lo, oseq.Sk)) ||
-              packed_odd_values<T, D>(p, oseq, ohk, max(ka.hi, 0), min(o_te * kKvTile, oseq.Sk))) {
+          const int k0 = oseq.k0;
+          if (packed_odd_values<T, D>(p, ohk, k0 + o_tb * kKvTile, k0 + min(ke.lo, oseq.Sk)) ||
+              packed_odd_values<T, D>(p, ohk, k0 + max(ka.hi, 0), k0 + min(o_te * kKvTile, oseq.Sk))) {
             vm_wait<0>(); // the rows above are written before
-            for (; bad; bad &= bad - 1)
-              packed_row_again<T, D>(p, oseq, qa + __builtin_ctzll(bad), ohq, ohk);
+            for (; bad; bad &= bad - 1) {
+              const int i = qa + __builtin_ctzll(bad);
+              const KeyRange kr = packed_keys(p, i, oseq.Sq, oseq.Sk);
+              packed_row_again<T, D>(p, oseq.q0 + i, k0 + kr.lo, k0 + kr.hi, ohq, ohk);
+            }
           }
         }
       }
@@ -719,37 +722,10 @@ __global__ __launch_bounds__(64 * NW) void attn_prefill_kernel(A p, int hpb) {
 template <int D> constexpr int kSplitTile = D == 128 ? 32 : 64; // keys per tile (8 KB of K)
 constexpr int kSplitGroups = 4;
 
-// The sequence and the tile in it of query tile `t`, counted over the batch in tiles of QL
-// queries; -1 past the last. By every wave: 64 sequences at a time.
-__device__ __forceinline__ int packed_tile(const PackedArgs &p, int t, int QL, PackedSeq &out) {
-  const int lane = lane_id(), count = packed_count(p);
-  for (int c = 0, before = 0; c < count; c += kWave) {
-    PackedSeq s = {0, 0, 0, 0};
-    if (c + lane < count) s = packed_seq(p, c + lane);
-    const int n = (s.Sq + QL - 1) / QL;
-    int sum = n; // tiles up to this lane's sequence
-#pragma unroll
-    for (int sh = 1; sh < kWave; sh <<= 1) {
-      const int o = __shfl_up(sum, sh, kWave);
-      if (lane >= sh) sum += o;
-    }
-    const unsigned long long hit = __ballot(before + sum > t);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      out.q0 = __builtin_amdgcn_readlane(s.q0, l), out.Sq = __builtin_amdgcn_readlane(s.Sq, l);
-      out.k0 = __builtin_amdgcn_readlane(s.k0, l), out.Sk = __builtin_amdgcn_readlane(s.Sk, l);
-      return t - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
-    }
-    before += __builtin_amdgcn_readlane(sum, kWave - 1);
-  }
-  return -1;
-}
-
-template <typename T, int D, typename A>
-__global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, int ct, int nsmax,
+template <typename T, int D>
+__global__ __launch_bounds__(512) void attn_prefill_split_kernel(AttnArgs p, int hpb, int ct, int nsmax,
                                                                  float *__restrict__ ws_o,
                                                                  float *__restrict__ ws_ml) {
-  constexpr bool PACKED = A::kPacked;
   typedef typename VecT<T>::v8 V8;
   constexpr int KT = kSplitTile<D>, NB = KT / 32; // 32-key blocks per tile
   constexpr int CPR = D / 8, NT = D / 32, NG = kSplitGroups;
@@ -763,8 +739,7 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = w >> 1, wu = w & 1, h = lane >> 5, ql = lane & 31;
   const int G = p.Hq / p.Hkv, QL = hpb == 2 ? 32 : 64;
-  int Sq = p.Sq, Sk = p.Sk; // packed: of the block's sequence
-  const int nqt = PACKED ? ct : (Sq + QL - 1) / QL, nhg = p.Hq / hpb, npair = PACKED ? nhg : p.B * nhg, ipp = nqt * nsmax;
+  const int nqt = (p.Sq + QL - 1) / QL, nhg = p.Hq / hpb, npair = p.B * nhg, ipp = nqt * nsmax;
   // all items of a (batch, head group) pair on one XCD (XCD = blockIdx % 8)
   // when the pairs split evenly: their K / V rows stay in its L2
   int pair, r;
@@ -776,21 +751,14 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
     pair = blockIdx.x / ipp;
     r = blockIdx.x % ipp;
   }
-  int qt = nqt - 1 - r / nsmax; // late (causal: heavy) query tiles first
-  const int split = r % nsmax;
+  const int qt = nqt - 1 - r / nsmax, split = r % nsmax; // late (causal: heavy) query tiles first
   const int b = pair / nhg, hg = pair % nhg;
   const int hq = hg * hpb + (hpb == 2 ? wu : 0), hk = (hg * hpb) / G;
-  PackedSeq seq = {0, 0, 0, 0};
-  if constexpr (PACKED) {
-    qt = packed_tile(p, qt, QL, seq);
-    if (qt < 0) return;
-    Sq = seq.Sq, Sk = seq.Sk;
-  }
-  const int q0 = qt * QL, q_last = (q0 + QL < Sq ? q0 + QL : Sq) - 1;
+  const int q0 = qt * QL, q_last = (q0 + QL < p.Sq ? q0 + QL : p.Sq) - 1;
   const int qw = q0 + (hpb == 2 ? 0 : wu * 32);
-  const int off = Sk - Sq;
-  const KeyBand kb = key_band(q0, q_last, Sq, Sk, p.left, p.right, KT);
-  const KeyBand chunk = key_chunk(kb, split, ct, nsmax); // (packed: one chunk)
+  const int off = p.Sk - p.Sq;
+  const KeyBand kb = key_band(q0, q_last, p.Sq, p.Sk, p.left, p.right, KT);
+  const KeyBand chunk = key_chunk(kb, split, ct, nsmax);
   const int t0 = chunk.t_begin, t1 = chunk.t_end;
   if (t0 >= t1 && (split > 0 || nsmax > 1)) return; // (no key at all and one chunk: rows of zeros)
   const int niter = t0 < t1 ? (t1 - t0 + NG - 1) / NG : 0;
@@ -800,14 +768,13 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
   const int64_t ss = kwave ? p.k_ss : p.v_ss;
   const char *src = kwave ? (const char *)((const T *)p.k + (int64_t)b * p.k_sb + (int64_t)hk * p.k_sh)
                           : (const char *)((const T *)p.v + (int64_t)b * p.v_sb + (int64_t)hk * p.v_sh);
-  if constexpr (PACKED) src += (int64_t)seq.k0 * ss * (int64_t)sizeof(T);
   const int dkey = lane / CPR, dslot = lane % CPR;
   V8 *const gring = smem + g * (4 * TU); // [slot][K | V][TU]
   auto issue = [&](int i) {
     const int t = t0 + i * NG + g;
     if (t >= t1) return; // wave-uniform
     const char *tb = src + (int64_t)t * KT * ss * (int64_t)sizeof(T);
-    const int kmax = Sk - 1 - t * KT; // keys past Sk read the last one (masked)
+    const int kmax = p.Sk - 1 - t * KT; // keys past Sk read the last one (masked)
     V8 *dst = gring + (i & 1) * (2 * TU) + (kwave ? 0 : TU);
 #pragma unroll
     for (int j = 0; j < NDMA; ++j) {
@@ -823,7 +790,7 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
   // q rows, past Sq the last one (never stored); one round trip with the
   // first tiles, waited for here so that no wait for them sits in the loop
   const T *qp = (const T *)p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh +
-                (int64_t)(seq.q0 + min(qw + ql, Sq - 1)) * p.q_ss;
+                (int64_t)min(qw + ql, p.Sq - 1) * p.q_ss;
   V8 qf[D / 16];
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const V8 *>(qp + ks * 16 + h * 8);
@@ -885,9 +852,9 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
     // more than 2^8, masking on band edges
     const int k0 = t * KT;
     if ((p.right >= 0 && k0 + KT - 1 > q0 + off + p.right) ||
-        (p.left >= 0 && k0 < q_last + off - p.left) || k0 + KT > Sk) {
+        (p.left >= 0 && k0 < q_last + off - p.left) || k0 + KT > p.Sk) {
       const int qpos = qw + ql + off;
-      int hi = Sk - 1;
+      int hi = p.Sk - 1;
       if (p.right >= 0) hi = min(hi, qpos + p.right);
       const int lo = p.left >= 0 ? max(qpos - p.left, 0) : 0;
       const int jb = k0 + h * 4;
@@ -921,7 +888,7 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
     for (int st = 0; st < NB; ++st)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[st][i], c2, PACKED ? kWeightUp<T, PACKED> - mc : -mc));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[st][i], c2, -mc));
         s[st][i] = e;
         ps[i & 3] += e;
       }
@@ -990,14 +957,11 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
     }
   const float l = l_run + __shfl_xor(l_run, 32, kWave);
   if (h == 0) s_m[w][ql] = m_run, s_l[w][ql] = l;
-  __shared__ unsigned s_bad[2];
-  if constexpr (PACKED)
-    if (tid < 2) s_bad[tid] = 0;
   __syncthreads();
   for (int idx = tid; idx < 64 * CPR; idx += 512) {
     const int row = idx / CPR, c = idx % CPR, u = row >> 5, rl = row & 31; // u: wave of the groups
     const int qi = q0 + (hpb == 2 ? 0 : u * 32) + rl, hr = hg * hpb + (hpb == 2 ? u : 0);
-    if (qi >= Sq) continue;
+    if (qi >= p.Sq) continue;
     float mg[NG], mx = -INFINITY;
 #pragma unroll
     for (int gg = 0; gg < NG; ++gg) mg[gg] = s_m[gg * 2 + u][rl], mx = fmaxf(mx, mg[gg]);
@@ -1015,40 +979,18 @@ __global__ __launch_bounds__(512) void attn_prefill_split_kernel(A p, int hpb, i
       for (int e = 0; e < 4; ++e) v[e] += a * x[e], v[e + 4] += a * y[e];
     }
     if (nsmax == 1) {
-      float inv = ls > 0.f ? 1.f / ls : 0.f;
-      if constexpr (PACKED) { // as attn_prefill_kernel
-        const KeyRange kr = packed_keys(p, qi, Sq, Sk);
-        inv = kr.lo < kr.hi ? 1.f / ls : 0.f;
-        float z = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z = fmaf(v[e], 0.f, z);
-        if (z != z && ls == ls) atomicOr(&s_bad[u], 1u << rl);
-      }
+      const float inv = ls > 0.f ? 1.f / ls : 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= inv;
-      store8((T *)p.o + (int64_t)b * p.o_sb + (int64_t)(seq.q0 + qi) * p.o_ss + (int64_t)hr * p.o_sh + c * 8, v);
+      store8((T *)p.o + (int64_t)b * p.o_sb + (int64_t)qi * p.o_ss + (int64_t)hr * p.o_sh + c * 8, v);
     } else {
-      const int64_t sl = (((int64_t)b * p.Hq + hr) * Sq + qi) * nsmax + split;
+      const int64_t sl = (((int64_t)b * p.Hq + hr) * p.Sq + qi) * nsmax + split;
       f32x4 x, y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = v[e], y[e] = v[e + 4];
       *reinterpret_cast<f32x4 *>(ws_o + sl * D + c * 8) = x;
       *reinterpret_cast<f32x4 *>(ws_o + sl * D + c * 8 + 4) = y;
       if (c == 0) ws_ml[sl * 2] = mx, ws_ml[sl * 2 + 1] = ls;
-    }
-  }
-  if constexpr (PACKED) { // (packed_row_again)
-    __syncthreads();      // every row above is written, and what is odd known
-    for (int u = 0; u < 2; ++u) {
-      const int qa = q0 + (hpb == 2 ? 0 : u * 32), qe = min(qa + 31, Sq - 1);
-      unsigned bad = s_bad[u];
-      if (!bad) continue;
-      const KeyRange ka = packed_keys(p, qa, Sq, Sk), ke = packed_keys(p, qe, Sq, Sk);
-      if (!packed_odd_values<T, D>(p, seq, hk, t0 * KT, min(ke.lo, Sk)) &&
-          !packed_odd_values<T, D>(p, seq, hk, max(ka.hi, 0), min(t1 * KT, Sk)))
-        continue;
-      for (int n = 0; bad; bad &= bad - 1, ++n)
-        if (n % 8 == w) packed_row_again<T, D>(p, seq, qa + __builtin_ctz(bad), hg * hpb + (hpb == 2 ? u : 0), hk);
     }
   }
 }

@@ -1354,7 +1354,8 @@ at::Tensor packed_attention(const at::Tensor &q, const at::Tensor &k, const at::
   const bool fill = !(out.has_value() && out->defined());
   at::Tensor o = out_like(q, out, {&q, &k, &v, &cu_q, &cu_k});
   if (q.numel() == 0) return o;
-  const size_t wsb = tpp_attn_packed_workspace_size(B, Nq, Nk, Hq, Hkv, D);
+  const size_t wsb = tpp_attn_packed_workspace_size(B, Nq, Nk, Hq, Hkv, D, causal, window_int(window_left),
+                                                   window_int(window_right), !cu_k.defined());
   at::Tensor ws; // this call's own, from the caching allocator
   if (wsb) ws = new_on(q, {(int64_t)wsb}, at::kByte);
   const int64_t qs[2] = {q.stride(0), q.stride(1)}, ks[2] = {k.stride(0), k.stride(1)},

@@ -9,9 +9,8 @@
 // attention_prefill.hpp with each query tile's sequence in place of the batch index. Grids are
 // sized by what is known on the host, the number of tokens and of sequences: N tokens in B
 // sequences have at most N / tile + B query tiles.
-//  * few tiles: attn_prefill_split_kernel, tiles of 32 queries of two heads whose keys the
-//    block's four pairs of waves share out. Each block finds its sequence by a scan of the
-//    lengths, so it is one launch.
+//  * short or few sequences: packed_wave_kernel, tiles of 32 queries of one head, each wave on
+//    its own. A block finds its sequence by a scan of the lengths, so it is one launch.
 //  * else attn_prefill_kernel, one block a CU, 128 queries of two heads (or 64 of four, 256 of
 //    one) a tile. Its static dealing of tiles to blocks wants them from the heaviest to the
 //    lightest: packed_plan_kernel sorts them first.
@@ -50,6 +49,367 @@ template <typename T> __global__ __launch_bounds__(64) void packed_generic_kerne
     if (c * 64 + lane < D) op[c * 64 + lane] = from_f32<T>(r.out(c));
 }
 
+// The sequence and the tile in it of query tile `t`, counted over the batch in tiles of QL
+// queries; -1 past the last. By every wave, 256 sequences' lengths in flight at once.
+__device__ __forceinline__ int packed_tile(const PackedArgs &p, int t, int QL, PackedSeq &out) {
+  constexpr int U = 4;
+  const int lane = lane_id(), count = packed_count(p);
+  for (int c0 = 0, before = 0; c0 < count; c0 += U * kWave) {
+    PackedSeq s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = {0, 0, 0, 0};
+      if (c0 + u * kWave + lane < count) s[u] = packed_seq(p, c0 + u * kWave + lane);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int n = (s[u].Sq + QL - 1) / QL;
+      const int sum = wave_scan(n); // tiles up to this lane's sequence
+      const unsigned long long hit = __ballot(before + sum > t);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        out.q0 = __builtin_amdgcn_readlane(s[u].q0, l), out.Sq = __builtin_amdgcn_readlane(s[u].Sq, l);
+        out.k0 = __builtin_amdgcn_readlane(s[u].k0, l), out.Sk = __builtin_amdgcn_readlane(s[u].Sk, l);
+        return t - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
+      }
+      before += __builtin_amdgcn_readlane(sum, kWave - 1);
+      if (c0 + (u + 1) * kWave >= count) return -1;
+    }
+  }
+  return -1;
+}
+
+// A query row of a lane: its sequence, its index there and whether it is to be written.
+struct PackedRow {
+  PackedSeq seq;
+  int i;
+  bool real;
+};
+// Self-attention: tile `t` is rows 32 t .. 32 t + 31 of the batch, whatever sequences they are
+// of, so that short ones share a tile. The first sequence that ends past the tile's first row
+// is found by a search in 64 parts, each lane's own from there on, 64 sequences at a time.
+__device__ __forceinline__ PackedRow packed_row_self(const PackedArgs &p, int t) {
+  const int lane = lane_id(), first = t * 32, r = min(first + (lane & 31), p.Nq - 1);
+  int lo = 0, hi = p.B; // the sequence is in [lo, hi), or there is none
+  while (hi - lo > kWave) {
+    const int step = (hi - lo + kWave - 1) / kWave, at = min(lo + (lane + 1) * step, hi) - 1;
+    const unsigned long long past = __ballot(p.cu_q[at + 1] > first);
+    const int l = past ? __builtin_ctzll(past) : kWave - 1;
+    const int next = lo + l * step;
+    hi = min(next + step, hi), lo = min(next, hi);
+  }
+  PackedRow o = {{r, 0, 0, 0}, 0, first + (lane & 31) < p.Nq && p.fill != 0}; // of no sequence
+  bool found = false;
+  for (; lo < p.B; lo += kWave) {
+    const int end = lo + lane < p.B ? p.cu_q[lo + lane + 1] : 0x7fffffff, begin = p.cu_q[lo];
+    const int last = __builtin_amdgcn_readlane(end, kWave - 1);
+    int n = 0; // ends at or ahead of the row: of 64 in order
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1)
+      if (__shfl(end, n + s - 1, kWave) <= r) n += s;
+    const int mine = __shfl(end, n, kWave), ahead = __shfl(end, max(n - 1, 0), kWave);
+    if (!found && (n < kWave - 1 || last > r)) {
+      found = true;
+      // (packed_seq's rows, without another trip to memory)
+      const int q0 = min(max(n ? ahead : begin, 0), p.Nq), q1 = min(mine, p.Nq);
+      if (lo + n < p.B && r >= q0 && r < q1) o = {{q0, q1 - q0, q0, q1 - q0}, r - q0, first + (lane & 31) < p.Nq};
+    }
+    if (__all(found)) break;
+  }
+  return o;
+}
+
+// ---------------------------------------------------------------------------
+// Short or few sequences: a wave has 32 queries of one head and streams its own KT-key tiles of
+// K and V by LDS-DMA into a slot of its own, the next K tile asked for once this one's
+// fragments are in registers, the next V tile after this one's. No wave waits for another.
+// SH = 1: the four waves of a block are four heads of the same queries. SH = 4: they share one
+// head's keys, every fourth tile each, and are merged through LDS. (Eight waves a row were
+// slower everywhere: the rate at which a CU's LDS-DMA brings tiles, ~80 bytes a ns, bounds
+// both.) The keys that rows see rise with the rows, so the first and last row that see any
+// give the wave's range; keys of a tile that a row does not see, other sequences' among them,
+// are masked.
+// ---------------------------------------------------------------------------
+template <typename T, int D, int SH, bool SELF>
+__global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int nh) {
+  constexpr bool SPLIT = SH > 1;
+  typedef typename VecT<T>::v8 V8;
+  typedef typename VecT<T>::v4 V4;
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  constexpr int KT = kSplitTile<D>, NB = KT / 32, CPR = D / 8, NT = D / 32, TU = KT * CPR, KPI = 64 / CPR;
+  constexpr int NW = 4, NDMA = KT / KPI, KS = D / 16, LDO = D + 4, RBY = D * 2, ORPI = 64 / CPR;
+  constexpr float kUp = kWeightUp<T, true>;
+  constexpr int kRing = NW * 2 * TU * 16, kMerge = SPLIT ? NW * 32 * LDO * 4 : 0;
+  __shared__ __attribute__((aligned(16))) char smem[kRing > kMerge ? kRing : kMerge];
+  __shared__ float s_m[NW][32], s_l[NW][32];
+  __shared__ unsigned s_bad;
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, ql = lane & 31;
+  const int e = blockIdx.x / nh, hb = blockIdx.x - e * nh;
+  const int hq = SPLIT ? hb : hb * 4 + w;
+  if (hq >= p.Hq) return;
+  PackedRow row;
+  if constexpr (SELF) {
+    row = packed_row_self(p, e);
+  } else {
+    PackedSeq seq = {0, 0, 0, 0};
+    const int qt = packed_tile(p, e, 32, seq);
+    if (qt < 0) return; // (every wave)
+    row = {seq, min(qt * 32 + ql, seq.Sq - 1), qt * 32 + ql < seq.Sq};
+  }
+  const int hk = hq / (p.Hq / p.Hkv), qrow = row.seq.q0 + row.i;
+  const KeyRange kr = packed_keys(p, row.i, row.seq.Sq, row.seq.Sk);
+  const int klo = row.seq.k0 + kr.lo, khi = row.seq.k0 + kr.hi; // rows of k and v that the row sees
+  const bool sees = row.real && kr.lo < kr.hi;
+  const unsigned seeing = (unsigned)__ballot(sees);
+  const int ra = seeing ? __builtin_ctz(seeing) : 0, rb = seeing ? 31 - __builtin_clz(seeing) : 0;
+  const int kmin = __builtin_amdgcn_readlane(klo, ra), kmax = seeing ? __builtin_amdgcn_readlane(khi, rb) : kmin;
+  // keys [all_lo, all_hi) are seen by every row that sees any
+  const int all_lo = __builtin_amdgcn_readlane(klo, rb), all_hi = __builtin_amdgcn_readlane(khi, ra);
+  const int k0 = kmin + (SPLIT ? w * KT : 0);
+
+  const char *kp = (const char *)((const T *)p.k + (int64_t)hk * p.k_sh);
+  const char *vp = (const char *)((const T *)p.v + (int64_t)hk * p.v_sh);
+  char *const ring = smem + w * (2 * TU * 16);
+  const int dkey = lane / CPR, dslot = lane % CPR;
+  // (keys past the last that is seen read it, masked)
+  auto issue = [&](const char *head, int64_t ss, int kb, char *dst, auto swizzle) {
+    const char *tb = head + (int64_t)kb * ss * 2;
+    const int most = kmax - 1 - kb;
+#pragma unroll
+    for (int j = 0; j < NDMA; ++j) {
+      const int key = j * KPI + dkey;
+      __builtin_amdgcn_global_load_lds((const void *)(tb + (unsigned)(min(key, most) * (int)ss * 2 + ((dslot ^ swizzle(key)) << 4))),
+                                       (__attribute__((address_space(3))) void *)(dst + j * 1024), 16, 0, 0);
+    }
+  };
+  auto issue_k = [&](int kb) { issue(kp, p.k_ss, kb, ring, [](int r) { return r & (CPR - 1); }); };
+  auto issue_v = [&](int kb) { issue(vp, p.v_ss, kb, ring + TU * 16, [](int r) { return vswz<D>(r); }); };
+
+  const T *qp = (const T *)p.q + (int64_t)qrow * p.q_ss + (int64_t)hq * p.q_sh;
+  V8 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const V8 *>(qp + ks * 16 + h * 8);
+  if (k0 < kmax) {
+    issue_k(k0);
+    issue_v(k0);
+  }
+  f32x16 o[NT];
+#pragma unroll
+  for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[tt][i] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+  const float c2 = p.scale_log2;
+  const unsigned kbase = lds_offset(ring);
+  unsigned ko[KS], vo[NT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) ko[ks] = kbase + (unsigned)((ql * CPR + ((ks * 2 + h) ^ (ql & (CPR - 1)))) * 16);
+  // V operand addresses within a tile (attn_prefill_kernel explains the layout)
+  const int grp = lane >> 4, a4 = lane & 3, c4 = (lane >> 2) & 3, kl = 4 * (grp >> 1) + c4;
+#pragma unroll
+  for (int tt = 0; tt < NT; ++tt) {
+    const int d0 = tt * 32 + 16 * (grp & 1) + 4 * a4;
+    vo[tt] = kbase + TU * 16 + kl * D * 2 + (((d0 >> 3) ^ vswz<D>(kl)) << 4) + ((d0 & 7) << 1);
+  }
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks])); // here, not in the loop
+
+  for (int kb = k0; kb < kmax; kb += SH * KT) {
+    const bool more = kb + SH * KT < kmax;
+    vm_wait<NDMA>(); // this tile's K landed, its V may be in flight
+    // S^T = K Q^T: eight fragments, read i is K step i (two blocks of 32 keys: step i / 2)
+    V8 kr[4][2];
+    static_for<8>([&](auto ii) {
+      constexpr int i = decltype(ii)::value;
+      kr[i / 2][i % 2] = lds_read_b128<(NB == 2 ? i % 2 : 0) * 32 * D * 2, V8>(ko[NB == 2 ? i / 2 : i]);
+    });
+    f32x16 s[NB];
+#pragma unroll
+    for (int st = 0; st < NB; ++st)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[st][i] = 0.f;
+    static_for<4>([&](auto ii) {
+      constexpr int i = decltype(ii)::value;
+      lds_wait_tied<(3 - i) * 2>(kr[i]);
+      if constexpr (i == 3) { // every K fragment is in registers
+        asm volatile("" ::: "memory");
+        if (more) issue_k(kb + SH * KT);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[j % NB] = mfma32x32<T>(kr[i][j], qf[NB == 2 ? i : 2 * i + j], s[j % NB]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    // online softmax, as attn_prefill_kernel
+    if (kb < all_lo || kb + KT > all_hi) {
+      const int jb = kb + h * 4;
+      const int ca = max(klo - jb, 0), cb = min(khi - 1 - jb, KT - 1);
+      const unsigned ninf = __float_as_uint(-INFINITY);
+#pragma unroll
+      for (int st = 0; st < NB; ++st) {
+        const int l0 = max(ca - 32 * st, 0), h0 = min(cb - 32 * st, 31);
+        const unsigned keep = l0 <= h0 ? ((2u << h0) - 1u) & ~((1u << l0) - 1u) : 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const unsigned bm = (unsigned)__builtin_amdgcn_sbfe((int)keep, (i >> 2) * 8 + (i & 3), 1);
+          s[st][i] = __uint_as_float((__float_as_uint(s[st][i]) & bm) | (ninf & ~bm));
+        }
+      }
+    }
+    float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+#pragma unroll
+    for (int st = 0; st < NB; ++st)
+#pragma unroll
+      for (int i = st == 0 ? 4 : 0; i < 16; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[st][i]);
+    float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+    mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    const bool move = (mt - m_run) * c2 > 8.f;
+    const float m_new = move ? mt : m_run;
+    const float mc = m_new == -INFINITY ? 0.f : m_new * c2;
+    const float alpha = move ? __builtin_amdgcn_exp2f(m_run * c2 - mc) : 1.f;
+    float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int st = 0; st < NB; ++st)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[st][i], c2, kUp - mc));
+        s[st][i] = x;
+        ps[i & 3] += x;
+      }
+    l_run = l_run * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
+    m_run = m_new;
+    if (__any(move)) {
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[tt][i] *= alpha;
+    }
+    V8 pb[2 * NB]; // the one rounding of the weights, to the type of V (l has them unrounded)
+#pragma unroll
+    for (int c = 0; c < 2 * NB; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pb[c][j] = from_f32<T>(s[c >> 1][(c & 1) * 8 + j]);
+    // O^T += V^T P^T
+    if (more) vm_wait<NDMA>(); // the next K may be in flight
+    else vm_wait<0>();
+    constexpr int R = 2 * NT, NC = 2 * NB;
+    s16x4 vr[NC][R];
+    static_for<NC>([&](auto cc) {
+      constexpr int c = decltype(cc)::value;
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt) {
+        vr[c][2 * tt] = lds_read_tr16<c * 32 * D>(vo[tt]);
+        vr[c][2 * tt + 1] = lds_read_tr16<c * 32 * D + 16 * D>(vo[tt]);
+      }
+    });
+    static_for<NC>([&](auto cc) {
+      constexpr int c = decltype(cc)::value;
+      lds_wait_tied<(NC - 1 - c) * R>(vr[c]);
+      if constexpr (c == NC - 1) { // every V fragment is in registers
+        asm volatile("" ::: "memory");
+        if (more) issue_v(kb + SH * KT);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt) {
+        const s16x8 r12 = __builtin_shufflevector(vr[c][2 * tt], vr[c][2 * tt + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        o[tt] = mfma32x32<T>(__builtin_bit_cast(V8, r12), pb[c], o[tt]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+
+  const float l = l_run + __shfl_xor(l_run, 32, kWave);
+  // values that are not finite and not seen (packed_row_again): the rows in `bad`, by `waves`
+  auto again = [&](unsigned bad, int w0, int waves) {
+    if (!packed_odd_values<T, D>(p, hk, kmin, all_lo) && !packed_odd_values<T, D>(p, hk, all_hi, kmax)) return;
+    for (int n = 0; bad; bad &= bad - 1, ++n) {
+      if (n % waves != w0) continue;
+      const int l = __builtin_ctz(bad);
+      packed_row_again<T, D>(p, __builtin_amdgcn_readlane(qrow, l), __builtin_amdgcn_readlane(klo, l),
+                             __builtin_amdgcn_readlane(khi, l), hq, hk);
+    }
+  };
+  if constexpr (!SPLIT) {
+    // the rows through LDS, so that a store instruction writes whole rows
+    const float inv = 1.f / l; // (rows whose scores are all -inf are NaN)
+    float z = 0.f;
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {
+        V4 pk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          z = fmaf(o[tt][rg * 4 + i], 0.f, z);
+          pk[i] = from_f32<T>(sees ? o[tt][rg * 4 + i] * inv : 0.f);
+        }
+        *reinterpret_cast<V4 *>(ring + ql * RBY + ((tt * 4 + rg) ^ (ql % CPR)) * 16 + h * 8) = pk;
+      }
+    T *const op = (T *)p.o + (int64_t)hq * p.o_sh;
+    const unsigned reals = (unsigned)__ballot(row.real);
+#pragma unroll
+    for (int r = 0; r < 32 / ORPI; ++r) {
+      const int n = r * ORPI + lane / CPR, c = lane % CPR;
+      const V8 x = *reinterpret_cast<const V8 *>(ring + n * RBY + ((c ^ (n % CPR)) * 16));
+      const int at = __shfl(qrow, n, kWave);
+      if (reals >> n & 1) *reinterpret_cast<V8 *>(op + (int64_t)at * p.o_ss + c * 8) = x;
+    }
+    unsigned long long bad = __ballot(z != z && l == l && sees);
+    if (bad) {
+      vm_wait<0>(); // the rows above are written before
+      again((unsigned)(bad | (bad >> 32)), 0, 1);
+    }
+  } else {
+    if (tid == 0) s_bad = 0;
+    __syncthreads(); // every wave is done with its slot
+    float *const mo = reinterpret_cast<float *>(smem) + (w * 32 + ql) * LDO;
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = o[tt][rg * 4 + i];
+        *reinterpret_cast<f32x4 *>(mo + tt * 32 + rg * 8 + h * 4) = x;
+      }
+    if (h == 0) s_m[w][ql] = m_run, s_l[w][ql] = l;
+    __syncthreads();
+    const unsigned reals = (unsigned)__ballot(row.real);
+    for (int idx = tid; idx < 32 * CPR; idx += 64 * NW) { // (whole waves)
+      const int n = idx / CPR, c = idx % CPR, at = __shfl(qrow, n, kWave);
+      if (!(reals >> n & 1)) continue;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < NW; ++g) mx = fmaxf(mx, s_m[g][n]);
+      const float ms = mx == -INFINITY ? 0.f : mx;
+      float ls = 0.f, v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NW; ++g) {
+        const float a = __builtin_amdgcn_exp2f((s_m[g][n] - ms) * c2);
+        ls += a * s_l[g][n];
+        const float *x = reinterpret_cast<const float *>(smem) + (g * 32 + n) * LDO + c * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += a * x[i];
+      }
+      const bool any = seeing >> n & 1;
+      const float inv = 1.f / ls;
+      float z = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z = fmaf(v[i], 0.f, z), v[i] = any ? v[i] * inv : 0.f;
+      if (z != z && ls == ls && any) atomicOr(&s_bad, 1u << n);
+      store8((T *)p.o + (int64_t)at * p.o_ss + (int64_t)hq * p.o_sh + c * 8, v);
+    }
+    __syncthreads(); // every row above is written, and what is odd known
+    if (s_bad) again(s_bad, w, NW);
+  }
+}
+
 // The query tiles of every sequence, those with the most key tiles first: a counting sort by
 // one block. A wave loads 64 sequences at once and takes its share of them; a lane a tile.
 constexpr int kPlanBins = 1024;
@@ -79,12 +439,7 @@ __global__ __launch_bounds__(1024) void packed_plan_kernel(PackedArgs p, int QL,
   each([&](const PackedSeq &, int, int bin) { atomicAdd(&s_at[bin], 1); });
   __syncthreads();
   const int n = s_at[tid];
-  int sum = n;
-#pragma unroll
-  for (int sh = 1; sh < kWave; sh <<= 1) {
-    const int o = __shfl_up(sum, sh, kWave);
-    if (lane >= sh) sum += o;
-  }
+  int sum = wave_scan(n);
   if (lane == kWave - 1) s_sum[w] = sum;
   __syncthreads();
   for (int i = 0; i < w; ++i) sum += s_sum[i];
@@ -99,26 +454,48 @@ __global__ __launch_bounds__(1024) void packed_plan_kernel(PackedArgs p, int QL,
   });
 }
 
-// How a call is cut: query heads of a tile, queries a tile, the most tiles there can be, and
-// whether tiles are of the kernel that splits keys in the block.
+// How a call is cut: the kernel (share: packed_wave_kernel's waves a row, 0: attn_prefill_kernel),
+// query heads and queries of a tile, the most tiles there can be.
 struct PackedPlan {
-  bool tiles, split;
-  int hpb, QL;
+  bool tiles;
+  int share, hpb, QL;
   int64_t most;
 };
-static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Hq, int64_t Hkv, int64_t D) {
+// Estimated times in us, of sequences of the batch's mean lengths (no other is known here),
+// from measurements of 1 to 256 sequences of 17 to 8000 tokens (bf16, 16 / 8 heads of 128, the
+// middle line for heads of 64):
+//  * packed_wave_kernel: 2.5, 4.5 for each 2048 waves, and the longest row's tiles, 0.8 each,
+//    or all waves' tiles at 1.1 ns (16 KB each from the L2s); with its keys shared by four
+//    waves 4, 4.2 for each 512 blocks, and the row's share of tiles or 0.93 ns.
+//  * attn_prefill_kernel: 7 with its plan, and 4.5 and 2.0 (1.2) a tile of 64 keys for all tiles
+//    over the CUs, or the longest tile alone, 4.5 and 1.6 (1.2).
+// E.g. one sequence of 230 6.7 (17.8 on the other kernel), of 1000 17 (38), 64 of 3 to 200 15 (34),
+// 16 of 200 16 (21); and back, 16 of 1000 139 (107), eight of 501 to 4001 278 (219).
+static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int left, int right,
+                              bool self) {
   PackedPlan pl = {};
   if (D != 64 && D != 128) return pl;
   pl.tiles = true;
+  const double cus = device_cu_count() > 0 ? device_cu_count() : 256, kt = D == 128 ? 32 : 64;
+  auto most = [&](int64_t QL) { return self && QL == 32 ? (Nq + 31) / 32 : Nq / QL + (B + 2 < Nq ? B + 2 : Nq); };
+  const double n = B > 0 ? B : 1, lq = Nq / n, lk = Nk / n;
+  // keys that the last query sees, and that one does on the average
+  double longest = lk, mean = right >= 0 && lq <= lk ? lk - lq / 2 : lk;
+  if (left >= 0 && right >= 0 && left + right + 33.0 < longest) longest = left + right + 33.0;
+  if (mean > longest) mean = longest;
+  const double items = (double)most(32) * Hq, work = items * (mean / kt + 0.5), chain = longest / kt + 1;
+  auto larger = [](double a, double b) { return a > b ? a : b; };
+  const double alone = 2.5 + 4.5 * larger(1, items / (8 * cus)) + larger(0.8 * chain, 1.1e-3 * work);
+  double best = alone;
+  pl.share = 1;
+  const double shared = 4 + 4.2 * larger(1, items / (2 * cus)) + larger(0.8 * chain / 4 + 1, 0.93e-3 * work);
+  if (shared < best) best = shared, pl.share = 4;
   const int64_t G = Hq / Hkv;
-  const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  auto most = [&](int64_t QL) { return Nq / QL + (B + 2 < Nq ? B + 2 : Nq); };
-  pl.hpb = G % 2 == 0 ? 2 : 1, pl.QL = 64 / pl.hpb;
-  pl.split = most(pl.QL) * (Hq / pl.hpb) <= 2 * cus;
-  if (!pl.split) {
-    pl.hpb = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
-    pl.QL = kPrefillWaves / pl.hpb * 32;
-  }
+  const int hpb = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1, QL = kPrefillWaves / hpb * 32;
+  const double each = D == 128 ? 2.0 : 1.2, last = D == 128 ? 1.6 : 1.2;
+  const double whole = 7 + larger((double)most(QL) * (Hq / hpb) / cus * (4.5 + each * (mean / 64 + 1)), 4.5 + last * (longest / 64 + 1));
+  if (whole < best) pl.share = 0;
+  pl.hpb = pl.share ? 1 : hpb, pl.QL = pl.share ? 32 : QL;
   pl.most = most(pl.QL);
   return pl;
 }
@@ -127,10 +504,15 @@ static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Hq, int64_t Hkv, in
 
 using namespace tpp;
 
-extern "C" size_t tpp_attn_packed_workspace_size(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D) {
-  if (B < 0 || Nq <= 0 || Hkv <= 0 || Hq <= 0) return 0;
-  const PackedPlan pl = packed_plan(B, Nq, Hq, Hkv, D);
-  return pl.tiles && !pl.split ? (size_t)(kPlanHead + pl.most * kPlanItem) * sizeof(int32_t) : 0;
+// A window that reaches past every key is none (and query + window stays below 2^31).
+static int packed_window(int x, int64_t Nq, int64_t Nk) { return x < 0 || x >= Nq + Nk ? -1 : x; }
+
+extern "C" size_t tpp_attn_packed_workspace_size(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,
+                                                 int causal, int window_left, int window_right, int self) {
+  if (B < 0 || Nq <= 0 || Nk < 0 || Hkv <= 0 || Hq <= 0) return 0;
+  const PackedPlan pl = packed_plan(B, Nq, Nk, Hq, Hkv, D, packed_window(window_left, Nq, Nk),
+                                    causal ? 0 : packed_window(window_right, Nq, Nk), self != 0);
+  return pl.tiles && !pl.share ? (size_t)(kPlanHead + pl.most * kPlanItem) * sizeof(int32_t) : 0;
 }
 
 extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void *o, const int64_t *q_strides,
@@ -158,15 +540,13 @@ extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void
   a.B = (int)B, a.Nq = (int)Nq, a.Nk = (int)Nk, a.Hq = (int)Hq, a.Hkv = (int)Hkv;
   const float sc = softmax_scale > 0.f ? softmax_scale : 1.f / sqrtf((float)D);
   a.scale_log2 = sc * kLog2e;
-  // a window that reaches past every key is none (and query + window stays below 2^31)
-  auto window = [&](int x) { return x < 0 || x >= Nq + Nk ? -1 : x; };
-  a.left = window(window_left), a.right = causal ? 0 : window(window_right);
+  a.left = packed_window(window_left, Nq, Nk), a.right = causal ? 0 : packed_window(window_right, Nq, Nk);
   a.fill = fill;
   hipStream_t st = as_stream(stream);
   // the matrix-core kernels: whole 16-byte rows, a tile's rows by 32-bit byte offsets
   uint64_t low = (uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)k | (uint64_t)(uintptr_t)v | (uint64_t)(uintptr_t)o;
   for (const int64_t x : {a.q_ss, a.q_sh, a.k_ss, a.k_sh, a.v_ss, a.v_sh, a.o_ss, a.o_sh}) low |= (uint64_t)(x * 2);
-  PackedPlan pl = packed_plan(B, Nq, Hq, Hkv, D);
+  const PackedPlan pl = packed_plan(B, Nq, Nk, Hq, Hkv, D, a.left, a.right, !cu_k);
   const bool fits = !(low & 15) && a.k_ss >= 0 && a.v_ss >= 0 && kKvTile * a.k_ss * 2 < (1LL << 31) &&
                     kKvTile * a.v_ss * 2 < (1LL << 31) && pl.most * Hq < (1LL << 31);
   if (!pl.tiles || !fits)
@@ -174,9 +554,12 @@ extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void
       packed_generic_kernel<T><<<dim3((unsigned)Nq, (unsigned)Hq), dim3(64), 0, st>>>(a, (int)D);
       return check_launch(name);
     });
-  const int64_t items = pl.most * (Hq / pl.hpb);
-  if (!pl.split) {
-    if (!workspace || !aligned16(workspace) || ws_bytes < tpp_attn_packed_workspace_size(B, Nq, Nk, Hq, Hkv, D))
+  // packed_wave_kernel without shared keys: blocks of four heads
+  const int nh = pl.share == 1 ? (int)(Hq + 3) / 4 : (int)Hq / pl.hpb;
+  const int64_t items = pl.most * nh;
+  if (!pl.share) {
+    if (!workspace || !aligned16(workspace) ||
+        ws_bytes < tpp_attn_packed_workspace_size(B, Nq, Nk, Hq, Hkv, D, causal, window_left, window_right, !cu_k))
       return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
     a.plan = (const int32_t *)workspace;
     packed_plan_kernel<<<dim3(1), dim3(1024), 0, st>>>(a, pl.QL, (int32_t *)workspace, (int)pl.most);
@@ -184,9 +567,12 @@ extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto dd) {
       constexpr int DD = decltype(dd)::value;
-      if (pl.split) {
-        attn_prefill_split_kernel<T, DD><<<dim3((unsigned)items), dim3(512), 0, st>>>(a, pl.hpb, (int)pl.most, 1, nullptr, nullptr);
-      } else {
+      const dim3 grid((unsigned)items);
+      if (pl.share == 1 && !cu_k) packed_wave_kernel<T, DD, 1, true><<<grid, dim3(256), 0, st>>>(a, nh);
+      else if (pl.share == 1) packed_wave_kernel<T, DD, 1, false><<<grid, dim3(256), 0, st>>>(a, nh);
+      else if (pl.share && !cu_k) packed_wave_kernel<T, DD, 4, true><<<grid, dim3(256), 0, st>>>(a, nh);
+      else if (pl.share) packed_wave_kernel<T, DD, 4, false><<<grid, dim3(256), 0, st>>>(a, nh);
+      else {
         const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
         attn_prefill_kernel<T, DD, kPrefillQG, kPrefillWaves>
             <<<dim3((unsigned)(items < cus ? items : cus)), dim3(64 * kPrefillWaves), 0, st>>>(a, pl.hpb);

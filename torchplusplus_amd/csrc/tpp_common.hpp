@@ -152,6 +152,18 @@ __device__ __forceinline__ float wave_sum(float v) {
          (readlane_f32(v, 32) + readlane_f32(v, 48));
 }
 
+// Sum over lanes 0 .. l, of every lane l.
+__device__ __forceinline__ int wave_scan(int v) {
+  // row_shr 1, 2, 4, 8 inside rows of 16, then row_bcast 15 and 31 (rows 1 and 3, then 2 and 3)
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // Sum over lanes {l, l^16, l^32, l^48} after a row16 reduction: gives each
 // lane the full-wave value without readlane (used where lane groups differ).
 __device__ __forceinline__ float xor_sum(float v, int mask) {
@@ -317,6 +329,10 @@ template <int N, typename V, int M> __device__ __forceinline__ void lds_wait_tie
                  : "n"(n));
   else
     static_assert(M >= 2 && M <= 8 && M != 7, "2 to 6 or 8 registers");
+}
+// LDS byte address of x
+template <typename P> __device__ __forceinline__ unsigned lds_offset(P *x) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)x;
 }
 // f(std::integral_constant<int, i>) for i = 0 .. N-1, in order
 template <typename F, int... I>
