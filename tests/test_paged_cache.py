@@ -57,6 +57,28 @@ def test_tables_and_slots():
     assert c.next_slots(t, torch.tensor([48, 3, -1], dtype=torch.int32)).tolist() == [-1, pb[0] * 16 + 3, -1]
 
 
+def test_steps():
+    c = cache(8)
+    a, b = c.allocate(), c.allocate(3)
+    s = c.prefill_step([a, b], [0, 0], [20, 3])
+    assert s.cu_seqlens.dtype == torch.int32 and s.cu_seqlens.tolist() == [0, 20, 23] and s.key_slots is None
+    assert s.positions.tolist() == [*range(20), 0, 1, 2] and len(set(s.slots.tolist())) == 23
+    assert len(c.pages_of(a)) == 2 and s.block_tables is None
+    t = c.prefill_step([b, a], [3, 20], [1, 13])
+    assert t.cu_seqlens.tolist() == [0, 1, 14] and t.cu_seqlens_k.tolist() == [0, 4, 37]
+    assert t.key_slots[:3].tolist() == s.slots[20:].tolist() and t.key_slots[4:24].tolist() == s.slots[:20].tolist()
+    assert t.slots.tolist() == [t.key_slots[3].item()] + t.key_slots[24:].tolist()
+    before = c.pages_of(a), c.pages_of(b), c.free_pages
+    with pytest.raises(RuntimeError, match="out of pages"):
+        c.prefill_step([a, b], [33, 4], [40, 60])
+    assert before == (c.pages_of(a), c.pages_of(b), c.free_pages)
+    with pytest.raises(ValueError, match="twice"):
+        c.prefill_step([a, a], [33, 34], [1, 1])
+    d = c.decode_step(c.block_tables([a, b]), torch.tensor([33, 4], dtype=torch.int32))
+    assert d.seqlens.tolist() == [34, 5] and d.seqlens.dtype == torch.int32 and d.cu_seqlens is None
+    assert d.slots.tolist() == [c.pages_of(a)[2] * 16 + 1, c.pages_of(b)[0] * 16 + 4]
+
+
 def test_read_gathers_rows():
     c = cache()
     a = c.allocate(20)

@@ -8,7 +8,8 @@ Same constructor and forward signature. Per call the layer runs:
      copies), or split-KV decode attention when a single token is appended
   4. the output projection.
 With a QuantKVCache step 2 rotates in place and appends codes, and step 3 reads
-them (_attend_codes).
+them (_attend_codes). Batches of sequences of different lengths over a
+PagedKVCache go through attend_paged.
 The fused projection weight is built from Wq/Wk/Wv on first use and rebuilt
 whenever one of them changes (load_state_dict, in-place edits), as the
 reference reads its projection weights on every call (gqa.py:82-84).
@@ -23,10 +24,12 @@ import torch.nn as nn
 from torchplusplus_amd._native import ext as _ext
 from torchplusplus_amd.attention._common import norm_rope_qk
 from torchplusplus_amd.attention.flash import flash_attn_func
+from torchplusplus_amd.attention.packed import packed_attention, paged_attention
 from torchplusplus_amd.attention.tree import TREE_MAX_TOKENS, tree_attention
 from torchplusplus_amd.dlops.derived import DerivedWeight, attach
 from torchplusplus_amd.dlops.linear import linear
 from torchplusplus_amd.llmops.kvcache import KVCache, QuantKVCache
+from torchplusplus_amd.llmops.paged import PagedKVCache, PagedStep, qkv_rope_paged
 
 _C = _ext()
 
@@ -168,6 +171,23 @@ class GroupedQueryAttention(nn.Module):
             k, v = cache.read(end, bs)
             o = flash_attn_func(q, k.transpose(1, 2), v.transpose(1, 2), causal=True)
         return o.reshape(bs, seq_len, self.d_out)
+
+    def attend_paged(self, qkv, cos, sin, cache: PagedKVCache, layer: int, step: PagedStep) -> torch.Tensor:
+        """Steps 2-3 on a packed batch's projection [N, (Hq + 2 Hkv) * D] over layer
+        `layer` of a paged cache: norm, rotation and the pages' rows in one launch, then
+        attention over the pages (a decode step), over the batch itself, or, behind cached
+        tokens, over the sequences' rows gathered from the pages. Returns [N, Hq * D]."""
+        kp, vp = cache.k_pages[layer], cache.v_pages[layer]
+        alone = step.cu_seqlens is not None and step.key_slots is None
+        q, k = qkv_rope_paged(qkv, step.positions, step.slots, kp, vp, cos, sin, *self._norms(), with_k=alone)
+        if step.cu_seqlens is None:
+            o = paged_attention(q, kp, vp, step.block_tables, step.seqlens)
+        else:
+            v = qkv[:, -self.n_kv_heads * self.head_dim :].unflatten(1, (-1, self.head_dim))
+            if not alone:
+                k, v = cache.read(layer, step.key_slots)
+            o = packed_attention(q, k, v, step.cu_seqlens, step.cu_seqlens_k)
+        return o.view(-1, self.d_out)
 
     def forward(self, x, cos, sin, kv_cache: Optional[KVCache] = None,
                 cache_pos: Optional[int] = None):

@@ -23,7 +23,7 @@ Execution:
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
@@ -39,6 +39,8 @@ from torchplusplus_amd.dlops.normalization import RmsNormFused
 from torchplusplus_amd.dlops.rope import compute_rope_params
 from torchplusplus_amd.llmops.kvcache import KVCache, QuantKVCache
 from torchplusplus_amd.llmops.llm import LLMInference
+from torchplusplus_amd.llmops.paged import PagedKVCache, PagedStep
+from torchplusplus_amd.llmops.scoring import TokenLogprobs, token_logprobs
 
 _C = _ext()
 
@@ -204,6 +206,62 @@ class FastQwen3(LLMInference):
             _C.ffn_decode(resid, n2.weight, n2.eps, blk.ffn.w_gu(), blk.ffn.linear_layer2.weight)
         return _C.gemv_fused(resid, self.out_head.weight, self.final_rmsnorm.weight,
                              self.final_rmsnorm.eps)
+
+    def forward_paged(self, input_ids: torch.Tensor, cache: PagedKVCache, step: PagedStep,
+                      rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits [N, vocab] of a packed batch's tokens input_ids [N] (or of its `rows`,
+        e.g. each prompt's last), their keys and values written into the cache."""
+        blocks = self.transformer_blocs
+        resid = F.embedding(input_ids, self.tok_embed.weight)
+        attend = lambda i, qkv: blocks[i].attn.attend_paged(qkv, self.cos, self.sin, cache, i, step)  # noqa: E731
+        if 0 < input_ids.numel() <= GEMV_MAX_ROWS:  # as _forward_small
+            for i, blk in enumerate(blocks):
+                qkv = _C.gemv_fused(resid, blk.attn.fused_qkv_weight(), blk.rms_norm1.weight, blk.rms_norm1.eps)
+                _C.gemv_fused(attend(i, qkv), blk.attn.out_projection.weight, None, 1e-6, resid)
+                _C.ffn_decode(resid, blk.rms_norm2.weight, blk.rms_norm2.eps, blk.ffn.w_gu(),
+                              blk.ffn.linear_layer2.weight)
+            resid = resid if rows is None else resid[rows]
+            return _C.gemv_fused(resid, self.out_head.weight, self.final_rmsnorm.weight, self.final_rmsnorm.eps)
+        h = blocks[0].rms_norm1(resid)
+        for i, blk in enumerate(blocks):
+            a = linear(attend(i, linear(h, blk.attn.fused_qkv_weight())), blk.attn.out_projection.weight)
+            h = blk.rms_norm2.forward_add(a, resid)
+            nxt = blocks[i + 1].rms_norm1 if i + 1 < len(blocks) else self.final_rmsnorm
+            h = nxt.forward_add(blk.ffn(h), resid)
+        return linear(h if rows is None else h[rows], self.out_head.weight)
+
+    @torch.inference_mode()
+    def generate_paged(self, prompts: Sequence[torch.Tensor], max_new_token: int, page_size: int = 64,
+                       top_k: int = 0) -> Tuple[torch.Tensor, TokenLogprobs]:
+        """Greedy generation for prompts (1-D token tensors) of different lengths as one
+        batch: the prompts packed without padding, then a token of every sequence a step,
+        over a paged cache. Returns the new tokens [B, max_new_token] and their log
+        probabilities, entropies and top_k alternatives ([B, max_new_token, ...])."""
+        if not prompts or min(len(p) for p in prompts) < 1 or max_new_token < 1:
+            raise ValueError("generate_paged needs prompts of at least one token and at least one new token")
+        dev, bsz = self.out_head.weight.device, len(prompts)
+        lens = [len(p) for p in prompts]
+        if max(lens) + max_new_token > self.cos.shape[0]:
+            raise ValueError(f"{max(lens)} + {max_new_token} tokens exceed the {self.cos.shape[0]} positions of the "
+                             f"rotation's tables")
+        room = [n + max_new_token for n in lens]
+        cache = PagedKVCache(sum(-(-n // page_size) for n in room), page_size, self.get_num_layers(),
+                             self.get_kv_heads(), self.get_head_dim(), self.get_dtype(), dev)
+        seqs = [cache.allocate(n) for n in room]
+        step = cache.prefill_step(seqs, [0] * bsz, lens)
+        tables, positions = cache.block_tables(seqs), torch.tensor(lens, dtype=torch.int32).to(dev)
+        logits = self.forward_paged(torch.cat([p.to(dev) for p in prompts]), cache, step,
+                                    step.cu_seqlens[1:].long() - 1)
+        tokens, scores = [], []
+        for i in range(max_new_token):
+            if i:
+                logits = self.forward_paged(tokens[-1], cache, cache.decode_step(tables, positions))
+                positions = positions + 1
+            tokens.append(_C.argmax_rows(logits))
+            scores.append(token_logprobs(logits, tokens[-1], top_k))
+        self.check_device_errors()
+        return torch.stack(tokens, 1), TokenLogprobs(
+            *(None if x[0] is None else torch.stack(x, 1) for x in zip(*scores)))
 
     @torch.inference_mode()
     def generate_greedy(self, input_ids: torch.Tensor, max_new_token: int,

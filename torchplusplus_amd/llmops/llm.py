@@ -18,6 +18,7 @@ import torch
 import torch.nn as nn
 
 from torchplusplus_amd.llmops.kvcache import KVCache, QuantKVCache
+from torchplusplus_amd.llmops.scoring import TokenLogprobs, token_logprobs
 from torchplusplus_amd.llmops.speculative import verify_draft
 
 
@@ -119,6 +120,20 @@ class LLMInference(nn.Module, ABC):
         if uniforms is None:
             uniforms = torch.rand(probs.shape[:2], device=probs.device)
         return verify_draft(draft_tokens, probs, uniforms, draft_probs, parents)
+
+    @torch.inference_mode()
+    def score(self, input_ids: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+        """Log probabilities of tokens 1 .. S - 1 of input_ids [B, S] given those ahead of
+        them, the entropies of their distributions and the top_k alternatives: [B, S - 1,
+        ...], see llmops.scoring.token_logprobs."""
+        if input_ids.dim() != 2 or input_ids.shape[1] < 2:
+            raise ValueError(f"input_ids must be [B, S] with at least two tokens, got {tuple(input_ids.shape)}")
+        logits = self.forward_impl(input_ids)
+        # (every row of the logits, the last with padding: slicing them would copy them)
+        tokens = torch.cat([input_ids[:, 1:], torch.full_like(input_ids[:, :1], -1)], 1)
+        scores = token_logprobs(logits, tokens, top_k)
+        self.check_device_errors()
+        return TokenLogprobs(*(None if x is None else x[:, :-1] for x in scores))
 
     def sample_greedy(self, logits):
         return torch.argmax(logits, dim=-1, keepdim=True)

@@ -3,6 +3,7 @@ counterpart in the reference, whose cache is one tensor of max_seq_len positions
 sequence, torchpp/llmops/kvcache.py:39-48)."""
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -33,14 +34,32 @@ def qkv_rope_paged(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tens
     return _C.qkv_rope_paged(qkv, positions, slots, k_pages, v_pages, cos, sin, q_norm, k_norm, eps, with_k)
 
 
+@dataclass
+class PagedStep:
+    """What a packed batch's tokens are to a PagedKVCache, the same for every layer.
+    A decode step has one token a sequence and their block_tables and seqlens (the new
+    token counted in). A prefill step has cu_seqlens, and, where tokens follow cached
+    ones, the slots that hold each sequence's positions from 0 on (key_slots) and their
+    cu_seqlens_k."""
+
+    positions: torch.Tensor
+    slots: torch.Tensor
+    cu_seqlens: Optional[torch.Tensor] = None
+    cu_seqlens_k: Optional[torch.Tensor] = None
+    key_slots: Optional[torch.Tensor] = None
+    block_tables: Optional[torch.Tensor] = None
+    seqlens: Optional[torch.Tensor] = None
+
+
 class PagedKVCache:
     """Keys and values of `n_layers` layers in pages of `page_size` rows, dealt to
     sequences as they grow; one table of pages serves every layer. k_pages[i],
     v_pages[i] are layer i's [num_pages, n_kv_heads, page_size, head_dim].
 
     allocate() begins a sequence, grow() deals it pages, free() takes them back;
-    block_tables(), slots() and next_slots() give what the kernels ask for. The
-    table is kept on the host; page contents are not cleared."""
+    prefill_step() and decode_step() give what a model's layers ask for, of
+    block_tables(), slots() and next_slots(). The table is kept on the host; page
+    contents are not cleared."""
 
     def __init__(self, num_pages: int, page_size: int, n_layers: int, n_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.float16, device=torch.device("cuda")):
@@ -128,6 +147,30 @@ class PagedKVCache:
         page = block_tables.long().gather(1, torch.where(inside, entry, 0))
         slot = page * self.page_size + (p % self.page_size).unsqueeze(1)
         return torch.where(inside & (page >= 0), slot, -1).squeeze(1)
+
+    def prefill_step(self, seqs: Sequence[int], starts: Sequence[int], counts: Sequence[int]) -> PagedStep:
+        """counts[i] new tokens of each sequence behind its first starts[i], packed in
+        turn (RuntimeError, and nothing dealt, where there are not enough pages)."""
+        if len(set(seqs)) < len(seqs):
+            raise ValueError("a sequence is given twice")
+        need = [max(-(-(a + n) // self.page_size) - len(self._tables[s]), 0) for s, a, n in zip(seqs, starts, counts)]
+        if sum(need) > len(self._unused):
+            raise RuntimeError(f"out of pages: {sum(need)} needed, {len(self._unused)} of {self.num_pages} unused")
+        for s, a, n in zip(seqs, starts, counts):
+            self.grow(s, a + n)
+        ends = lambda x: torch.tensor([0, *x], dtype=torch.int64).cumsum(0).int().to(self.device)  # noqa: E731
+        step = PagedStep(*self.slots(seqs, starts, counts), cu_seqlens=ends(counts))
+        if any(starts):
+            lengths = [a + n for a, n in zip(starts, counts)]
+            step.key_slots = self.slots(seqs, [0] * len(seqs), lengths)[1]
+            step.cu_seqlens_k = ends(lengths)
+        return step
+
+    def decode_step(self, block_tables: torch.Tensor, positions: torch.Tensor) -> PagedStep:
+        """One new token of every sequence of a table, at positions[b] (int32 [B]; its page
+        is dealt already): on the device alone, as next_slots."""
+        return PagedStep(positions, self.next_slots(block_tables, positions), block_tables=block_tables,
+                         seqlens=positions + 1)
 
     def read(self, layer: int, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """The rows of `slots` (int64 [N]) as packed keys and values [N, n_kv_heads, D]."""
