@@ -62,6 +62,17 @@ def test_long_over_many_splits(dev, page, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b,hq,hk", [(70, 2, 1), (200, 4, 4), (600, 2, 2), (33, 32, 1)])
+def test_many_sequences(dev, b, hq, hk):
+    """Mixed lengths, some 0, more sequences than a wave has lanes, than are dealt splits."""
+    from torchplusplus_amd.attention import paged_attention
+    lens = [(i * i * 37) % 1400 if i % 7 else 0 for i in range(b)]
+    lens[b // 2] = 3000
+    q, kp, vp, table = make(lens, hq, hk, 64, 32, torch.bfloat16, b, dev)
+    check(paged_attention(q, kp, vp, table, i32(lens, dev)), q, kp, vp, table, lens)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128, 48])
 def test_entries_that_are_no_page(dev, d):
     """Holes, entries past the pool and lengths past the table or below 0 read nothing."""

@@ -10,7 +10,6 @@ namespace tpp {
 
 // TreeArgs with one token a sequence, {page, head, row} strides in k_s and v_s, and T = 1.
 struct PagedArgs : TreeArgs {
-  static constexpr bool kPaged = true;
   const int32_t *table;
   int64_t t_sb;
   int pages, lpage, left, lkt; // pages of 2^lpage rows; tiles of 2^lkt keys
@@ -18,6 +17,7 @@ struct PagedArgs : TreeArgs {
   __device__ __forceinline__ int lowest(int len) const { return left >= 0 ? max(len - 1 - left, 0) : 0; }
   __device__ __forceinline__ int begin(int len) const { return lowest(len) >> lkt << lkt; }
   __device__ __forceinline__ int keys(int len) const { return max(len - begin(len), 1); } // (none: one split, of zeros)
+  __device__ __forceinline__ int length(int b) const { return min(max(seqlens[b], 0), Lmax); }
 };
 
 // Any head size up to 256, any alignment: one wave per (sequence, head).
@@ -52,6 +52,8 @@ template <typename T> __global__ __launch_bounds__(64) void paged_generic_kernel
 // a tile ahead, between that tile's K and V (a load into registers was waited for at once, and
 // K with it, where its value is carried around the loop).
 // ---------------------------------------------------------------------------
+constexpr int kPagedDealt = 512; // sequences whose lengths a block looks at
+
 // What tile keys kb .. are shown of: pages that exist, positions from the window's first on.
 struct PagedShown {
   unsigned groups; // bit g: keys 16 g .. of the tile have a page
@@ -64,11 +66,79 @@ struct PagedShown {
   }
 };
 
+// A sequence's splits: runs of `per` batches of 2^(lkt + 2) keys, `n` of them, the first the
+// head's `at`-th.
+struct PagedDeal {
+  int b, at, n, per, batches;
+};
+// The splits are dealt to the sequences by their lengths: all of a head's keys into runs of one
+// length, the least that makes `target` of them or fewer (or nearly: a sequence has one at
+// least, and the search is short), each sequence's as even as its batches allow, and at most
+// `most` of them, for one block to merge. Then every block has about the same to read, where
+// one number of splits for all left the longest sequence's blocks reading when the others were
+// done: 32 sequences of 100 to 4096 keys, 36.6 -> 29.9 us. By a whole wave, for split `e` of a
+// head, or, FIND = false, for sequence `e` (b < 0: there is none).
+// a / n rounded up, for a and n up to 2^20 (a table's positions are limited to so many batches):
+// (a + n - 1/2) / n is 1 / (2 n) off a whole number at least, its error, 2^-22 of it, less.
+// (An integer division is ~30 dependent instructions, and four stood ahead of the first key.)
+__device__ __forceinline__ int div_up(int a, int n) {
+  return (int)(((float)(a + n) - 0.5f) * __builtin_amdgcn_rcpf((float)n));
+}
+__device__ __forceinline__ PagedDeal paged_runs(int b, int at, int batches, int per) {
+  PagedDeal d = {b, at, div_up(batches, per), 0, batches};
+  d.per = div_up(batches, d.n);
+  d.n = div_up(batches, d.per); // (evened out they may be fewer)
+  return d;
+}
+template <bool FIND> __device__ __forceinline__ PagedDeal paged_deal(const PagedArgs &p, int target, int most, int e) {
+  constexpr int U = kPagedDealt / kWave;
+  const int lane = lane_id(), lb = p.lkt + 2;
+  int nb[U], total = 0;
+  float longest = 0.f; // (batches)
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int b = u * kWave + lane;
+    nb[u] = 0;
+    if (b < p.B) nb[u] = (int)(((unsigned)p.keys(p.length(b)) + (1u << lb) - 1) >> lb);
+    longest = fmaxf(longest, (float)nb[u]);
+  }
+  int sum[U], per = 0;
+  auto scan = [&](int div) { // running numbers of runs of `div` batches, their sum
+    int before = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u * kWave >= p.B) break;
+      sum[u] = wave_scan(div_up(nb[u], div)) + before;
+      before = __builtin_amdgcn_readlane(sum[u], kWave - 1);
+    }
+    return before;
+  };
+  total = scan(1);
+  longest = row16_max(longest);
+  const int top = (int)fmaxf(fmaxf(readlane_f32(longest, 0), readlane_f32(longest, 16)),
+                             fmaxf(readlane_f32(longest, 32), readlane_f32(longest, 48)));
+  per = max(min(max((total + target - 1) / target, div_up(top, most)), top), 1);
+  for (int i = 0; scan(per) > target && i < 6; ++i) per += (per + 7) / 8;
+  PagedDeal d = {-1, 0, 0, 1, 0};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (u * kWave >= p.B || d.b >= 0) break;
+    const unsigned long long hit = __ballot(FIND ? sum[u] > e && u * kWave + lane < p.B : u * kWave + lane == e);
+    if (!hit) continue;
+    const int l = __builtin_ctzll(hit);
+    const int batches = __builtin_amdgcn_readlane(nb[u], l), n = div_up(batches, per);
+    d = paged_runs(u * kWave + l, __builtin_amdgcn_readlane(sum[u], l) - n, batches, per);
+  }
+  return d;
+}
+
+// Block (qt, hk) = blockIdx.x, split blockIdx.y of the head, or, undealt (target 0), the whole
+// of sequence blockIdx.y; `slots` splits a head at most.
 template <typename T, int D, int NC>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs p, float *__restrict__ ws_o,
-                                                            float *__restrict__ ws_ml, int nsplit,
-                                                            unsigned nsplit_inv, unsigned hkv_inv, unsigned g_inv,
-                                                            int by_xcd, unsigned *__restrict__ arrived) {
+                                                            float *__restrict__ ws_ml, int target, int most,
+                                                            int slots, unsigned hkv_inv, unsigned g_inv,
+                                                            unsigned *__restrict__ arrived) {
   typedef TreeTile<0, D> TT;
   typedef TreeWave<T, 0, D, NC> W;
   constexpr int KT = TT::KT, NW = 4, STRIDE = NW * KT, NDMA = TT::TILEB / 1024, C4 = D / 4, ROWS = 16 * NC;
@@ -81,21 +151,32 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs p, float *
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int u4 = lane >> 4, l16 = lane & 15;
-  TreeBlock k = tree_block(p, hkv_inv, by_xcd);
+  TreeBlock k = {};
+  k.qt = div_inv(blockIdx.x, hkv_inv), k.hk = blockIdx.x - k.qt * p.Hkv;
+  PagedDeal d = {(int)blockIdx.y, 0, 1, 1 << 30, 1};
+  if (target && p.B > 1) {
+    d = paged_deal<true>(p, target, most, blockIdx.y);
+    if (d.b < 0 || (int)blockIdx.y - d.at >= d.n) return; // (the whole block)
+  } else if (target) {
+    d.b = 0; // its query rows need not wait for its length
+  }
+  k.b = d.b, k.pair = d.b * p.Hkv + k.hk;
   const int rows = p.G;
   W wv;
   int row0[NC], row[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) row0[i] = k.qt * ROWS + i * 16, row[i] = min(row0[i] + l16, rows - 1);
   wv.ask(p, k.b, k.hk, g_inv, row);
-  const int len = min(max(__builtin_amdgcn_readfirstlane(p.seqlens[k.b]), 0), p.Lmax);
+  const int len = __builtin_amdgcn_readfirstlane(p.length(k.b));
   const int lowest = p.lowest(len), begin = p.begin(len);
-  const int nbatch = (int)((unsigned)(p.keys(len) + STRIDE - 1) / (unsigned)STRIDE);
-  const int per = div_inv((unsigned)(nbatch + nsplit - 1), nsplit_inv);
-  k.live = (int)((unsigned)(nbatch + per - 1) / (unsigned)per);
-  if (k.split >= k.live) return;
-  const int c0 = begin + k.split * per * STRIDE; // (below 2^31, as two tiles on: the host's check)
-  const int k_end = (int)min((int64_t)c0 + (int64_t)per * STRIDE, (int64_t)len);
+  if (target && p.B == 1) {
+    const int batches = (int)((unsigned)(p.keys(len) + STRIDE - 1) / (unsigned)STRIDE);
+    d = paged_runs(0, 0, batches, max(div_up(batches, target), div_up(batches, most)));
+    if ((int)blockIdx.y >= d.n) return; // (the whole block)
+  }
+  k.split = target ? blockIdx.y - d.at : 0, k.live = d.n;
+  const int c0 = begin + k.split * d.per * STRIDE; // (below 2^31, as two tiles on)
+  const int k_end = (int)min((int64_t)c0 + (int64_t)d.per * STRIDE, (int64_t)len);
   const int first = c0 + w * KT;
   const int n = first < k_end ? (k_end - first + STRIDE - 1) / STRIDE : 0; // this wave's tiles
 
@@ -234,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs p, float *
       for (int e = 0; e < 4; ++e) ov[e] = from_f32<T>(os[e] * inv);
       *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) = ov;
     } else {
-      const int64_t slot = ((int64_t)k.pair * rows + r) * nsplit + k.split;
+      const int64_t slot = ((int64_t)k.hk * rows + r) * slots + blockIdx.y;
       if (NC == 1 && arrived) {
         store_through(ws_o + slot * D + c * 4, os);
         if (c == 0) {
@@ -248,25 +329,62 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs p, float *
     }
   }
   if constexpr (NC == 1)
-    if (arrived && k.live > 1) tree_merge_here<T, D>(p, k, rows, nsplit, ws_o, ws_ml, g_inv, arrived, smem);
+    if (arrived && k.live > 1)
+      tree_merge_here<T, D>(p, k, rows, (int64_t)k.hk * rows * slots + d.at, slots, ws_o, ws_ml, g_inv, arrived, smem);
 }
 
-// How a call is cut: groups of 16 query rows a block, blocks a pair, splits of the keys.
+// The splits of every row, as tree_merge_kernel, a row block of one sequence and KV head each.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs p, const float *__restrict__ ws_o,
+                                                          const float *__restrict__ ws_ml, int target, int most, int slots) {
+  constexpr int C4 = D / 4, RPB = 256 / (C4 * kMergeParts);
+  __shared__ f32x4 s_o[RPB * kMergeParts * C4];
+  __shared__ float s_ml[RPB * kMergeParts * 2];
+  const int grp = threadIdx.x / C4, q = grp / kMergeParts, g0 = grp % kMergeParts, c = threadIdx.x % C4;
+  const int r = min((int)blockIdx.x * RPB + q, p.G - 1), hk = blockIdx.y, b = blockIdx.z;
+  const PagedDeal d = paged_deal<false>(p, target, most, b);
+  if (d.n == 1) return; // written by the tile kernel
+  const int64_t slot = ((int64_t)hk * p.G + r) * slots + d.at;
+  TreeMerge<1> mg;
+  mg.begin();
+  for (int s0 = 0; s0 < d.n; s0 += kMergeParts * kMergeAhead) {
+    mg.template load<D, false>(ws_o, ws_ml, slot, c, s0, g0, 1, d.n - 1);
+    mg.add(s0, g0, 1, d.n);
+  }
+  s_o[grp * C4 + c] = mg.o[0];
+  if (c == 0) s_ml[grp * 2] = mg.m[0], s_ml[grp * 2 + 1] = mg.l[0];
+  __syncthreads();
+  if (g0 || (int)blockIdx.x * RPB + q >= p.G) return;
+  T *op = (T *)p.o + (int64_t)b * p.o_s[0] + (int64_t)(hk * p.G + r) * p.o_s[2];
+  *reinterpret_cast<typename VecT<T>::v4 *>(op + c * 4) =
+      tree_merge_parts<T>(s_o + q * kMergeParts * C4 + c, C4, s_ml + q * kMergeParts * 2);
+}
+
+// How a call is cut: groups of 16 query rows a block, blocks of them a KV head, splits that a
+// head is to have (0: one a sequence), that one of its sequences, and that there can be.
 struct PagedPlan {
-  int nc, qtiles, nsplit;
+  int nc, qtiles, target, most, slots;
 };
 static PagedPlan paged_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Lmax) {
-  PagedPlan pl = {0, 0, 0};
+  PagedPlan pl = {0, 0, 0, 0, 0};
   if (D != 64 && D != 128) return pl;
-  const int64_t G = Hq / Hkv, kt = D == 128 ? 32 : 64;
+  const int64_t G = Hq / Hkv, stride = 4 * (D == 128 ? 32 : 64);
   pl.nc = G > 16 ? 2 : 1;
   pl.qtiles = (int)((G + 16 * pl.nc - 1) / (16 * pl.nc));
-  // two blocks a CU, as many as are resident at once (tree_plan)
-  const int64_t most = (Lmax + 4 * kt - 1) / (4 * kt);
+  pl.slots = (int)B;
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  int64_t ns = 2 * (int64_t)cus / (B * Hkv * pl.qtiles);
-  if (ns > most) ns = most;
-  pl.nsplit = (int)(ns > 256 ? 256 : ns < 1 ? 1 : ns);
+  // (with four blocks for each that can be resident the card deals them well itself)
+  if (B > kPagedDealt || B * Hkv * pl.qtiles >= 8 * cus || Lmax <= stride) return pl;
+  // Two blocks a CU, as many as are resident at once (tree_plan); two a sequence, where those
+  // are more, for the long ones to be split.
+  int64_t t = 2 * (int64_t)cus / (Hkv * pl.qtiles);
+  if (t < 2 * B) t = 2 * B;
+  const int64_t most = B * ((Lmax + stride - 1) / stride);
+  if (t > most) t = most;
+  pl.target = (int)t;
+  // A block that merges reads rows * splits sums of 4 (D + 2) bytes, ~50 a ns.
+  pl.most = pl.nc == 1 ? (int)(1024 / G) : 1024;
+  pl.slots = (int)(t + B); // (at most t runs of equal length, and a last one each)
   return pl;
 }
 
@@ -277,7 +395,7 @@ using namespace tpp;
 extern "C" size_t tpp_attn_paged_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Lmax) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Lmax <= 0) return 0;
   const PagedPlan pl = paged_plan(B, Hq, Hkv, D, Lmax);
-  return pl.nsplit > 1 ? (size_t)(B * Hq) * pl.nsplit * (D + 2) * sizeof(float) : 0;
+  return pl.target ? (size_t)Hq * pl.slots * (D + 2) * sizeof(float) : 0;
 }
 
 extern "C" int tpp_attn_paged(const void *q, const void *k_pages, const void *v_pages, void *o,
@@ -297,7 +415,7 @@ extern "C" int tpp_attn_paged(const void *q, const void *k_pages, const void *v_
   if ((1 << lpage) != page_size)
     return set_error(TPP_E_UNSUPPORTED, "%s: pages of %lld rows; powers of two from 16 to 1024 are handled", name,
                      (long long)page_size);
-  if (D > 256 || B > 65535 || Hq > 65535 || pages > 0x7fffffffLL || table_pages > (0x7fff0000LL >> lpage))
+  if (D > 256 || B > 65535 || Hq > 65535 || pages > 0x7fffffffLL || table_pages > ((1LL << 27) >> lpage))
     return set_error(TPP_E_UNSUPPORTED, "%s: head_dim above 256, or too many sequences, heads or pages", name);
   if (B == 0) return TPP_OK;
   if (!q || !o || !seqlens || (pages > 0 && (!k_pages || !v_pages)) || (table_pages > 0 && !block_tables))
@@ -321,7 +439,7 @@ extern "C" int tpp_attn_paged(const void *q, const void *k_pages, const void *v_
     low_o |= (uint64_t)(a.o_s[i] * 2);
   }
   bool tiles = (D == 64 || D == 128) && !(low & 15) && !(low_o & 7) && pages > 0 && table_pages > 0 &&
-               B * Hkv <= 65535 && (uint64_t)a.G * (uint64_t)a.G < 1ull << 32;
+               (uint64_t)a.G * (uint64_t)a.G < 1ull << 32;
   for (int64_t r : {a.k_s[2], a.v_s[2]}) tiles = tiles && r >= 0 && r < (1 << 23);
   if (!tiles)
     return TPP_DISPATCH_HALF(dtype, [&] {
@@ -329,28 +447,24 @@ extern "C" int tpp_attn_paged(const void *q, const void *k_pages, const void *v_
       return check_launch(name);
     });
   const PagedPlan pl = paged_plan(B, Hq, Hkv, D, a.Lmax);
-  const int64_t pairs = B * Hkv;
   float *ws_o = (float *)workspace, *ws_ml = nullptr;
-  if (pl.nsplit > 1) {
+  if (pl.target) {
     if (!workspace || ((uintptr_t)workspace & 127) || ws_bytes < tpp_attn_paged_workspace_size(B, Hq, Hkv, D, a.Lmax))
       return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
-    ws_ml = ws_o + (size_t)(pairs * a.G) * pl.nsplit * D;
+    ws_ml = ws_o + (size_t)Hq * pl.slots * D;
   }
-  const bool by_xcd = pairs % 8 == 0;
   // the merge by a pair's last block (one a pair)
-  unsigned *arrived = pl.nsplit > 1 && pl.nc == 1 ? arrival_words(st, pairs) : nullptr;
-  const dim3 grid(by_xcd ? 8 * pl.qtiles : pl.qtiles, pl.nsplit, (unsigned)(by_xcd ? pairs / 8 : pairs));
-  const unsigned ninv = inv_of(pl.nsplit), hinv = inv_of((int)Hkv), ginv = inv_of(a.G);
+  unsigned *arrived = pl.target && pl.nc == 1 ? arrival_words(st, B * Hkv) : nullptr;
+  const dim3 grid((unsigned)(Hkv * pl.qtiles), (unsigned)pl.slots);
+  const unsigned hinv = inv_of((int)Hkv), ginv = inv_of(a.G);
   return TPP_DISPATCH_HALF(dtype, [&] {
     auto go = [&](auto dd) {
       constexpr int DD = decltype(dd)::value;
-      if (pl.nc == 1)
-        paged_tile_kernel<T, DD, 1><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, arrived);
-      else
-        paged_tile_kernel<T, DD, 2><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.nsplit, ninv, hinv, ginv, by_xcd, nullptr);
-      if (pl.nsplit > 1 && !arrived)
-        tree_merge_kernel<T, DD><<<dim3((unsigned)((a.G + 256 / DD - 1) / (256 / DD)), (unsigned)Hkv, (unsigned)B), dim3(256), 0, st>>>(
-            a, ws_o, ws_ml, pl.nsplit, ninv, ginv, a.lkt + 2);
+      if (pl.nc == 1) paged_tile_kernel<T, DD, 1><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.target, pl.most, pl.slots, hinv, ginv, arrived);
+      else paged_tile_kernel<T, DD, 2><<<grid, dim3(256), 0, st>>>(a, ws_o, ws_ml, pl.target, pl.most, pl.slots, hinv, ginv, nullptr);
+      if (pl.target && !arrived)
+        paged_merge_kernel<T, DD><<<dim3((unsigned)((a.G + 256 / DD - 1) / (256 / DD)), (unsigned)Hkv, (unsigned)B), dim3(256), 0, st>>>(
+            a, ws_o, ws_ml, pl.target, pl.most, pl.slots);
     };
     if (D == 128) go(std::integral_constant<int, 128>{});
     else go(std::integral_constant<int, 64>{});

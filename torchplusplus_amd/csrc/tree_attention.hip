@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256, KIND && NC == 1 ? 3 : 2) void tree_tile_kernel
     }
   }
   if constexpr (NC == 1)
-    if (arrived && k.live > 1) tree_merge_here<T, D>(p, k, rows, nsplit, ws_o, ws_ml, g_inv, arrived, smem);
+    if (arrived && k.live > 1) tree_merge_here<T, D>(p, k, rows, (int64_t)k.pair * rows * nsplit, nsplit, ws_o, ws_ml, g_inv, arrived, smem);
 }
 
 // More rows: the four waves share the tiles of the split's keys, each with rows

@@ -9,7 +9,6 @@ namespace tpp {
 constexpr int kTreeMaxT = 64;
 
 struct TreeArgs {
-  static constexpr bool kPaged = false;
   const void *q, *k, *v;
   void *o;
   const uint8_t *ke, *ve; // exponent bytes of coded caches
@@ -711,9 +710,10 @@ template <int D> constexpr int tree_merge_lds = kMergeParts * (256 * 16 + 256 / 
 // of two, 7.8 -> 5.5 us where the sequences are so short that they need no merge. The
 // block counts itself in on an arrival word; what it has summed went past the caches
 // before, and comes so, since the blocks may run on any XCD. Captured calls take the
-// second launch, as do more rows: 32 of 8 sequences took 32.0 us so for 21.4.
+// second launch, as do more rows: 32 of 8 sequences took 32.0 us so for 21.4. Row r's sums
+// are at slots slot0 + r each, one a split.
 template <typename T, int D>
-__device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlock &k, int rows, int nsplit,
+__device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlock &k, int rows, int64_t slot0, int each,
                                                 const float *__restrict__ ws_o, const float *__restrict__ ws_ml,
                                                 unsigned g_inv, unsigned *__restrict__ arrived, char *lds) {
   constexpr int C4 = D / 4, NG = 256 / C4;
@@ -736,7 +736,7 @@ __device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlo
     constexpr int NP = decltype(npc)::value, STEP = kMergeParts / NP, RPB = NG / STEP;
     for (int base = 0; base < rows; base += RPB) {
       const int q = grp / STEP, g0 = grp % STEP, r = min(base + q, rows - 1);
-      const int64_t slot = ((int64_t)k.pair * rows + r) * nsplit;
+      const int64_t slot = slot0 + (int64_t)r * each;
       TreeMerge<NP> mg;
       mg.begin();
       for (int s0 = 0; s0 < k.live; s0 += kMergeParts * kMergeAhead) {
@@ -768,8 +768,8 @@ __device__ __forceinline__ void tree_merge_here(const TreeArgs &p, const TreeBlo
 // group of D / 4 lanes, the first splits' loads before the sequence's length has come
 // (slots that no split wrote are read and not used): a chain of length, maxima and
 // sums would be three trips to memory, twice the launch's time.
-template <typename T, int D, typename A>
-__global__ __launch_bounds__(256) void tree_merge_kernel(A p, const float *__restrict__ ws_o,
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, const float *__restrict__ ws_o,
                                                          const float *__restrict__ ws_ml, int nsplit,
                                                          unsigned nsplit_inv, unsigned g_inv, int lstride) {
   constexpr int C4 = D / 4, RPB = 256 / (C4 * kMergeParts);
@@ -783,10 +783,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(A p, const float *__res
   TreeMerge<1> mg;
   mg.begin();
   mg.template load<D, false>(ws_o, ws_ml, slot, c, 0, g0, 1, nsplit - 1);
-  const int L = min(max(len, 0), p.Lmax);
-  int keys = min(L + p.T, p.Lmax);
-  if constexpr (A::kPaged) keys = p.keys(L);
-  const int nbatch = (int)(((unsigned)keys + (1u << lstride) - 1) >> lstride);
+  const int L = min(max(len, 0), p.Lmax), end = min(L + p.T, p.Lmax);
+  const int nbatch = (int)(((unsigned)end + (1u << lstride) - 1) >> lstride);
   const int per = div_inv((unsigned)(nbatch + nsplit - 1), nsplit_inv);
   const int live = (int)((unsigned)(nbatch + per - 1) / (unsigned)per);
   if (live == 1) return; // written by the tile kernel
