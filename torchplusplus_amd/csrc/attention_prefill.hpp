@@ -24,7 +24,7 @@ struct AttnArgs {
 struct PackedArgs : AttnArgs {
   static constexpr bool kPacked = true;
   const int32_t *cu_q, *cu_k; // [B + 1]
-  const int32_t *plan;        // attn_prefill_kernel's query tiles (packed_plan_kernel)
+  const int32_t *plan;        // attn_prefill_kernel's query tiles (packed_plan_kernel); null: a block a tile
   int Nq, Nk;
   int fill; // rows of no sequence become 0 (else they stay as they were)
 };
@@ -48,6 +48,36 @@ __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs &p, int b) {
 }
 // Sequences with rows to write.
 __device__ __forceinline__ int packed_count(const PackedArgs &p) { return p.fill ? p.B + 2 : p.B; }
+
+// The sequence and the tile in it of query tile `t`, counted over the batch in tiles of QL
+// queries; -1 past the last. By every wave, 256 sequences' lengths in flight at once.
+__device__ __forceinline__ int packed_tile(const PackedArgs &p, int t, int QL, PackedSeq &out) {
+  constexpr int U = 4;
+  const int lane = lane_id(), count = packed_count(p);
+  for (int c0 = 0, before = 0; c0 < count; c0 += U * kWave) {
+    PackedSeq s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = {0, 0, 0, 0};
+      if (c0 + u * kWave + lane < count) s[u] = packed_seq(p, c0 + u * kWave + lane);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int n = (s[u].Sq + QL - 1) / QL;
+      const int sum = wave_scan(n); // tiles up to this lane's sequence
+      const unsigned long long hit = __ballot(before + sum > t);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        out.q0 = __builtin_amdgcn_readlane(s[u].q0, l), out.Sq = __builtin_amdgcn_readlane(s[u].Sq, l);
+        out.k0 = __builtin_amdgcn_readlane(s[u].k0, l), out.Sk = __builtin_amdgcn_readlane(s[u].Sk, l);
+        return t - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
+      }
+      before += __builtin_amdgcn_readlane(sum, kWave - 1);
+      if (c0 + (u + 1) * kWave >= count) return -1;
+    }
+  }
+  return -1;
+}
 
 // Keys lo .. hi - 1 that query i of a sequence sees (none: lo >= hi).
 struct KeyRange {
@@ -187,8 +217,17 @@ __global__ __launch_bounds__(64 * NW) void attn_prefill_kernel(A p, int hpb) {
   int nqt = (Sq + qt_len - 1) / qt_len;
   const int nhg = p.Hq / hpb;
   int npair = p.B * nhg;
-  if constexpr (PACKED) { // one list of query tiles for every head
-    nqt = __builtin_amdgcn_readfirstlane(p.plan[0]), npair = nhg;
+  PackedSeq own = {0, 0, 0, 0}; // packed, no plan: the block's one tile
+  int own_q0 = 0;
+  if constexpr (PACKED) {
+    npair = nhg; // one list of query tiles for every head
+    if (p.plan) {
+      nqt = __builtin_amdgcn_readfirstlane(p.plan[0]);
+    } else {
+      own_q0 = packed_tile(p, (gridDim.x - 1 - blockIdx.x) / nhg, qt_len, own) * qt_len; // (late tiles first)
+      if (own_q0 < 0) return;
+      nqt = gridDim.x / nhg;
+    }
   }
   const int nitems = npair * nqt;
   int off = Sk - Sq;
@@ -200,7 +239,7 @@ __global__ __launch_bounds__(64 * NW) void attn_prefill_kernel(A p, int hpb) {
   // so the K / V tiles its blocks share stay in its L2, and each of its S
   // blocks takes the XCD's items in boustrophedon order (rounds alternate
   // direction), which evens out the heavy and light tiles per block.
-  const bool xcd_split = npair % 8 == 0 && gridDim.x % 8 == 0;
+  const bool xcd_split = npair % 8 == 0 && gridDim.x % 8 == 0 && !(PACKED && gridDim.x == (unsigned)nitems);
   auto next_item = [&](int &k, int &qt, int &rest) -> bool {
     if (xcd_split) {
       const int S = gridDim.x / 8, slot = blockIdx.x / 8, per = npair / 8, ni = nitems / 8;
@@ -230,12 +269,17 @@ __global__ __launch_bounds__(64 * NW) void attn_prefill_kernel(A p, int hpb) {
     hk = (hg * hpb) / G;
     q0 = qt * qt_len;
     if constexpr (PACKED) {
-      const int32_t *it = p.plan + kPlanHead + qt * kPlanItem;
-      int x[5];
+      if (p.plan) {
+        const int32_t *it = p.plan + kPlanHead + qt * kPlanItem;
+        int x[5];
 #pragma unroll
-      for (int i = 0; i < 5; ++i) x[i] = __builtin_amdgcn_readfirstlane(it[i]);
-      seq_q = x[0], q0 = x[1], Sq = x[2], seq_k = x[3], Sk = x[4], off = Sk - Sq;
-    }
+        for (int i = 0; i < 5; ++i) x[i] = __builtin_amdgcn_readfirstlane(it[i]);
+        seq_q = x[0], q0 = x[1], Sq = x[2], seq_k = x[3], Sk = x[4];
+      } else {
+        seq_q = own.q0, q0 = own_q0, Sq = own.Sq, seq_k = own.k0, Sk = own.Sk;
+      }
+      off = Sk - Sq;
+   }
     q_last = (q0 + qt_len < Sq ? q0 + qt_len : Sq) - 1;
     qw = q0 + (w % wph) * 32 * QG; // first query of this wave
     // key band of the whole item

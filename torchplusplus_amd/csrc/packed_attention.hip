@@ -11,9 +11,10 @@
 // sequences have at most N / tile + B query tiles.
 //  * short or few sequences: packed_wave_kernel, tiles of 32 queries of one head, each wave on
 //    its own. A block finds its sequence by a scan of the lengths, so it is one launch.
-//  * else attn_prefill_kernel, one block a CU, 128 queries of two heads (or 64 of four, 256 of
-//    one) a tile. Its static dealing of tiles to blocks wants them from the heaviest to the
-//    lightest: packed_plan_kernel sorts them first.
+//  * else attn_prefill_kernel, 128 queries of two heads (or 64 of four, 256 of one) a tile: a
+//    block each, or, where they are many, one block a CU that loops over its share of them.
+//    That static dealing wants the tiles from the heaviest to the lightest: packed_plan_kernel
+//    sorts them first.
 #include "attention_prefill.hpp"
 
 namespace tpp {
@@ -47,36 +48,6 @@ template <typename T> __global__ __launch_bounds__(64) void packed_generic_kerne
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (c * 64 + lane < D) op[c * 64 + lane] = from_f32<T>(r.out(c));
-}
-
-// The sequence and the tile in it of query tile `t`, counted over the batch in tiles of QL
-// queries; -1 past the last. By every wave, 256 sequences' lengths in flight at once.
-__device__ __forceinline__ int packed_tile(const PackedArgs &p, int t, int QL, PackedSeq &out) {
-  constexpr int U = 4;
-  const int lane = lane_id(), count = packed_count(p);
-  for (int c0 = 0, before = 0; c0 < count; c0 += U * kWave) {
-    PackedSeq s[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      s[u] = {0, 0, 0, 0};
-      if (c0 + u * kWave + lane < count) s[u] = packed_seq(p, c0 + u * kWave + lane);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int n = (s[u].Sq + QL - 1) / QL;
-      const int sum = wave_scan(n); // tiles up to this lane's sequence
-      const unsigned long long hit = __ballot(before + sum > t);
-      if (hit) {
-        const int l = __builtin_ctzll(hit);
-        out.q0 = __builtin_amdgcn_readlane(s[u].q0, l), out.Sq = __builtin_amdgcn_readlane(s[u].Sq, l);
-        out.k0 = __builtin_amdgcn_readlane(s[u].k0, l), out.Sk = __builtin_amdgcn_readlane(s[u].Sk, l);
-        return t - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
-      }
-      before += __builtin_amdgcn_readlane(sum, kWave - 1);
-      if (c0 + (u + 1) * kWave >= count) return -1;
-    }
-  }
-  return -1;
 }
 
 // A query row of a lane: its sequence, its index there and whether it is to be written.
@@ -460,6 +431,7 @@ struct PackedPlan {
   bool tiles;
   int share, hpb, QL;
   int64_t most;
+  bool plan;
 };
 // Estimated times in us, of sequences of the batch's mean lengths (no other is known here),
 // from measurements of 1 to 256 sequences of 17 to 8000 tokens (bf16, 16 / 8 heads of 128, the
@@ -497,6 +469,10 @@ static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int
   if (whole < best) pl.share = 0;
   pl.hpb = pl.share ? 1 : hpb, pl.QL = pl.share ? 32 : QL;
   pl.most = most(pl.QL);
+  // up to two tiles a CU a block each, from the last to the first, and no list of them (its
+  // launch: six turns behind 2500 tokens 46.9 -> 43.0 us; four prompts of 2000, 2.06 tiles a
+  // CU, 90.7 with the list, 118 without)
+  pl.plan = !pl.share && pl.most * (Hq / hpb) > 2 * cus;
   return pl;
 }
 
@@ -512,7 +488,7 @@ extern "C" size_t tpp_attn_packed_workspace_size(int64_t B, int64_t Nq, int64_t 
   if (B < 0 || Nq <= 0 || Nk < 0 || Hkv <= 0 || Hq <= 0) return 0;
   const PackedPlan pl = packed_plan(B, Nq, Nk, Hq, Hkv, D, packed_window(window_left, Nq, Nk),
                                     causal ? 0 : packed_window(window_right, Nq, Nk), self != 0);
-  return pl.tiles && !pl.share ? (size_t)(kPlanHead + pl.most * kPlanItem) * sizeof(int32_t) : 0;
+  return pl.plan ? (size_t)(kPlanHead + pl.most * kPlanItem) * sizeof(int32_t) : 0;
 }
 
 extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void *o, const int64_t *q_strides,
@@ -557,7 +533,7 @@ extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void
   // packed_wave_kernel without shared keys: blocks of four heads
   const int nh = pl.share == 1 ? (int)(Hq + 3) / 4 : (int)Hq / pl.hpb;
   const int64_t items = pl.most * nh;
-  if (!pl.share) {
+  if (pl.plan) {
     if (!workspace || !aligned16(workspace) ||
         ws_bytes < tpp_attn_packed_workspace_size(B, Nq, Nk, Hq, Hkv, D, causal, window_left, window_right, !cu_k))
       return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
@@ -575,7 +551,7 @@ extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void
       else {
         const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
         attn_prefill_kernel<T, DD, kPrefillQG, kPrefillWaves>
-            <<<dim3((unsigned)(items < cus ? items : cus)), dim3(64 * kPrefillWaves), 0, st>>>(a, pl.hpb);
+            <<<dim3((unsigned)(!pl.plan || items < cus ? items : cus)), dim3(64 * kPrefillWaves), 0, st>>>(a, pl.hpb);
       }
     };
     if (D == 128) go(std::integral_constant<int, 128>{});
