@@ -42,7 +42,7 @@ def i32(x, dev):
 
 def check(got, q, k, v, cu, cu_k, **kw):
     o, mean, size = oracle.packed_attention(q, k, v, cu, cu_k, **kw)
-    d, n = q.shape[2], max([b - a for a, b in zip(cu_k, cu_k[1:])], default=0)
+    d, n = q.shape[2], min(max([b - a for a, b in zip(cu_k, cu_k[1:])], default=0), len(k))
     tol = tolerance(o, mean, size, q.dtype, n, d, float(v.abs().max().float()) if v.numel() else 0.0)
     err = (got.double().cpu() - o).abs()
     assert torch.isfinite(got).all()
@@ -131,6 +131,8 @@ def test_rows_of_no_sequence(dev, d):
     assert (out[:2] == 5).all() and (out[cu[-1]:] == 5).all()
     far = cu[:-1] + [1 << 30]
     check(packed_attention(q, k, v, i32(far, dev)), q, k, v, far, far)
+    low = [-2 ** 31] + cu[1:]
+    check(packed_attention(q, k, v, i32(low, dev)), q, k, v, low, low)
     empty = packed_attention(q, k, v, i32([0], dev))
     assert (empty == 0).all()
     assert packed_attention(q[:0], k, v, i32([0, 0], dev), i32([0, 9], dev)).shape == (0, 4, d)

@@ -39,10 +39,10 @@ __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs &p, int b) {
   PackedSeq s = {0, 0, 0, 0};
   const int qa = b > p.B ? 0 : min(max(p.cu_q[b], 0), p.Nq);
   const int qe = b < p.B ? p.cu_q[b + 1] : b == p.B ? p.Nq : p.cu_q[0];
-  s.q0 = qa, s.Sq = max(min(qe, p.Nq) - qa, 0);
+  s.q0 = qa, s.Sq = min(max(qe, qa), p.Nq) - qa;
   if (b < p.B) {
     s.k0 = min(max(p.cu_k[b], 0), p.Nk);
-    s.Sk = max(min(p.cu_k[b + 1], p.Nk) - s.k0, 0);
+    s.Sk = min(max(p.cu_k[b + 1], s.k0), p.Nk) - s.k0;
   }
   return s;
 }
@@ -70,7 +70,8 @@ __device__ __forceinline__ int packed_tile(const PackedArgs &p, int t, int QL, P
         const int l = __builtin_ctzll(hit);
         out.q0 = __builtin_amdgcn_readlane(s[u].q0, l), out.Sq = __builtin_amdgcn_readlane(s[u].Sq, l);
         out.k0 = __builtin_amdgcn_readlane(s[u].k0, l), out.Sk = __builtin_amdgcn_readlane(s[u].Sk, l);
-        return t - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
+        const int own = __builtin_amdgcn_readlane(n, l), at = t - before - (__builtin_amdgcn_readlane(sum, l) - own);
+        return at >= 0 && at < own ? at : -1; // (lengths that do not ascend may add up to anything)
       }
       before += __builtin_amdgcn_readlane(sum, kWave - 1);
       if (c0 + (u + 1) * kWave >= count) return -1;

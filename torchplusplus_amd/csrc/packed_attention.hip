@@ -419,7 +419,7 @@ __global__ __launch_bounds__(1024) void packed_plan_kernel(PackedArgs p, int QL,
   __syncthreads();
   each([&](const PackedSeq &s, int t, int bin) {
     const int at = atomicAdd(&s_at[bin], 1); // (the order inside a bin changes no result)
-    if (at >= room) return;                   // (lengths that do not ascend)
+    if (at < 0 || at >= room) return;         // (lengths that do not ascend)
     int32_t *it = plan + kPlanHead + at * kPlanItem;
     it[0] = s.q0, it[1] = t * QL, it[2] = s.Sq, it[3] = s.k0, it[4] = s.Sk;
   });
@@ -466,7 +466,8 @@ static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int
   const int hpb = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1, QL = kPrefillWaves / hpb * 32;
   const double each = D == 128 ? 2.0 : 1.2, last = D == 128 ? 1.6 : 1.2;
   const double whole = 7 + larger((double)most(QL) * (Hq / hpb) / cus * (4.5 + each * (mean / 64 + 1)), 4.5 + last * (longest / 64 + 1));
-  if (whole < best) pl.share = 0;
+  // (a grid has fewer than 2^32 threads)
+  if (whole < best || most(32) * (pl.share == 1 ? (Hq + 3) / 4 : Hq) > 0xffffff) pl.share = 0;
   pl.hpb = pl.share ? 1 : hpb, pl.QL = pl.share ? 32 : QL;
   pl.most = most(pl.QL);
   // up to two tiles a CU a block each, from the last to the first, and no list of them (its
