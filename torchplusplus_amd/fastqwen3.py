@@ -210,17 +210,22 @@ class FastQwen3(LLMInference):
     def forward_paged(self, input_ids: torch.Tensor, cache: PagedKVCache, step: PagedStep,
                       rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Logits [N, vocab] of a packed batch's tokens input_ids [N] (or of its `rows`,
-        e.g. each prompt's last), their keys and values written into the cache."""
+        e.g. each prompt's last, or none of a part of a prompt), their keys and values written into the cache."""
+        none = self.out_head.weight.new_empty(0, self.out_head.weight.shape[0])
+        if input_ids.numel() == 0:
+            return none
         blocks = self.transformer_blocs
         resid = F.embedding(input_ids, self.tok_embed.weight)
         attend = lambda i, qkv: blocks[i].attn.attend_paged(qkv, self.cos, self.sin, cache, i, step)  # noqa: E731
-        if 0 < input_ids.numel() <= GEMV_MAX_ROWS:  # as _forward_small
+        if input_ids.numel() <= GEMV_MAX_ROWS:  # as _forward_small
             for i, blk in enumerate(blocks):
                 qkv = _C.gemv_fused(resid, blk.attn.fused_qkv_weight(), blk.rms_norm1.weight, blk.rms_norm1.eps)
                 _C.gemv_fused(attend(i, qkv), blk.attn.out_projection.weight, None, 1e-6, resid)
                 _C.ffn_decode(resid, blk.rms_norm2.weight, blk.rms_norm2.eps, blk.ffn.w_gu(),
                               blk.ffn.linear_layer2.weight)
             resid = resid if rows is None else resid[rows]
+            if not len(resid):
+                return none
             return _C.gemv_fused(resid, self.out_head.weight, self.final_rmsnorm.weight, self.final_rmsnorm.eps)
         h = blocks[0].rms_norm1(resid)
         for i, blk in enumerate(blocks):
@@ -228,7 +233,8 @@ class FastQwen3(LLMInference):
             h = blk.rms_norm2.forward_add(a, resid)
             nxt = blocks[i + 1].rms_norm1 if i + 1 < len(blocks) else self.final_rmsnorm
             h = nxt.forward_add(blk.ffn(h), resid)
-        return linear(h if rows is None else h[rows], self.out_head.weight)
+        h = h if rows is None else h[rows]
+        return linear(h, self.out_head.weight) if len(h) else none
 
     @torch.inference_mode()
     def generate_paged(self, prompts: Sequence[torch.Tensor], max_new_token: int, page_size: int = 64,

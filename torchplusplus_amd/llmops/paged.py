@@ -122,14 +122,22 @@ class PagedKVCache:
         flat = [r + [-1] * (width - len(r)) for r in rows]
         return torch.tensor(flat, dtype=torch.int32).view(len(rows), width).to(self.device)
 
+    @staticmethod
+    def _check(seqs, starts, counts) -> None:
+        if not len(seqs) == len(starts) == len(counts):
+            raise ValueError(f"{len(seqs)} sequences need one start and one count each, got {len(starts)} and {len(counts)}")
+        if min([*starts, *counts], default=0) < 0:
+            raise ValueError(f"starts {list(starts)} and counts {list(counts)} must not be below 0")
+
     def slots(self, seqs: Sequence[int], starts: Sequence[int], counts: Sequence[int]
               ) -> Tuple[torch.Tensor, torch.Tensor]:
         """Positions starts[i] .. starts[i] + counts[i] - 1 of every sequence in turn, and
         their slots: int32 and int64 [sum of counts] on the device."""
+        self._check(seqs, starts, counts)
         pos, slots = [], []
         for s, a, n in zip(seqs, starts, counts):
             table = torch.tensor(self._tables[s], dtype=torch.int64)
-            if a < 0 or n < 0 or a + n > len(table) * self.page_size:
+            if a + n > len(table) * self.page_size:
                 raise ValueError(f"positions {a} to {a + n} of a sequence with pages for {len(table) * self.page_size}")
             p = torch.arange(a, a + n)
             pos.append(p)
@@ -141,6 +149,8 @@ class PagedKVCache:
         """The slot of position positions[b] of every sequence of a table: int64 [B],
         -1 where the sequence has no page for it. On the device alone (for a decode
         step, captured or not)."""
+        if block_tables.shape[1] == 0:  # (nothing to gather from)
+            return torch.full_like(positions, -1, dtype=torch.int64)
         p = positions.long()
         entry = torch.div(p, self.page_size, rounding_mode="floor").unsqueeze(1)
         inside = (entry >= 0) & (entry < block_tables.shape[1])
@@ -151,6 +161,7 @@ class PagedKVCache:
     def prefill_step(self, seqs: Sequence[int], starts: Sequence[int], counts: Sequence[int]) -> PagedStep:
         """counts[i] new tokens of each sequence behind its first starts[i], packed in
         turn (RuntimeError, and nothing dealt, where there are not enough pages)."""
+        self._check(seqs, starts, counts)
         if len(set(seqs)) < len(seqs):
             raise ValueError("a sequence is given twice")
         need = [max(-(-(a + n) // self.page_size) - len(self._tables[s]), 0) for s, a, n in zip(seqs, starts, counts)]
