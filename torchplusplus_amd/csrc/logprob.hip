@@ -9,10 +9,13 @@
 //
 // One pass over the row: a thread keeps its running maximum with the two sums, and the
 // place where it met that maximum first. The rows are 2 or 4 V bytes and everything else is
-// small, so HBM bounds the pass. Rows that do not fill the card are cut into chunks, a block
-// each, whose sums and largest logits the row's last block to finish joins: it is found by an
-// arrival word, and the chunks' results go past the caches, since the blocks may run on any
-// XCD. Captured calls, and those of more rows than there are words, join in a second launch.
+// small, so HBM bounds the pass: 1024 bf16 rows of 151936, 311 MB, 58 us (5.4 TB/s). Rows
+// that do not fill the card are cut into chunks, a block each, whose sums and largest logits
+// the row's last block to finish joins: it is found by an arrival word, and the chunks'
+// results go past the caches, since the blocks may run on any XCD. Captured calls, and those
+// of more rows than there are words, join in a second launch. A chain of trips to memory
+// bounds such calls: 8 rows with five alternatives 10.2 us (in two launches 11.2, without
+// alternatives 7.4), 77 fp32 rows of 50257 with 20 alternatives 14.3 (14.9).
 //
 // The largest: of 64 groups of threads the `top`-th largest maximum bounds the `top`-th
 // largest logit from below, so only threads whose maximum reaches it have any of them: those

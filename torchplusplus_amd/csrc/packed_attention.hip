@@ -97,9 +97,10 @@ __device__ __forceinline__ PackedRow packed_row_self(const PackedArgs &p, int t)
 // SH = 1: the four waves of a block are four heads of the same queries. SH = 4: they share one
 // head's keys, every fourth tile each, and are merged through LDS. (Eight waves a row were
 // slower everywhere: the rate at which a CU's LDS-DMA brings tiles, ~80 bytes a ns, bounds
-// both.) The keys that rows see rise with the rows, so the first and last row that see any
-// give the wave's range; keys of a tile that a row does not see, other sequences' among them,
-// are masked.
+// both where sequences are not short. Short ones are the launch and a chain of trips to memory,
+// 7.3 us for one of 230 tokens, 12 for 64 of 3 to 200.) The keys that rows see rise with the
+// rows, so the first and last row that see any give the wave's range; keys of a tile that a row
+// does not see, other sequences' among them, are masked.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int SH, bool SELF>
 __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int nh) {
@@ -441,8 +442,9 @@ struct PackedPlan {
 //    waves 4, 4.2 for each 512 blocks, and the row's share of tiles or 0.93 ns.
 //  * attn_prefill_kernel: 7 with its plan, and 4.5 and 2.0 (1.2) a tile of 64 keys for all tiles
 //    over the CUs, or the longest tile alone, 4.5 and 1.6 (1.2).
-// E.g. one sequence of 230 6.7 (17.8 on the other kernel), of 1000 17 (38), 64 of 3 to 200 15 (34),
-// 16 of 200 16 (21); and back, 16 of 1000 139 (107), eight of 501 to 4001 278 (219).
+// Measured, e.g.: one sequence of 230 7.3 (17.8 on the other kernel), of 1000 17 (38), 64 of 3 to
+// 200 12 (32; fp16, 16 / 16 heads of 64), 16 of 200 17 (21); and back, 16 of 1000 139 (107), eight
+// of 501 to 4001 278 (188: 770 TFLOP/s, 5 us of it the plan's launch).
 static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int left, int right,
                               bool self) {
   PackedPlan pl = {};

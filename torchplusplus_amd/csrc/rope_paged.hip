@@ -9,7 +9,8 @@
 //
 // Bound by HBM: q, k and v are read once, q, k and the two page rows written once. D / 16
 // lanes share a row, each with 8 elements of either half, so a rotation's pair is in one
-// lane and the norm is a DPP sum over the row's lanes.
+// lane and the norm is a DPP sum over the row's lanes. 16000 tokens of 16 + 8 + 8 heads of
+// 128, 295 MB: 48.5 us in the trace, 6.1 TB/s; 32 tokens: 3.1, a launch and one round trip.
 #include "tpp_common.hpp"
 
 namespace tpp {
