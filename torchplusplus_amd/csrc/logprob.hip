@@ -14,20 +14,25 @@
 // the row's last block to finish joins: it is found by an arrival word, and the chunks'
 // results go past the caches, since the blocks may run on any XCD. Captured calls, and those
 // of more rows than there are words, join in a second launch. A chain of trips to memory
-// bounds such calls: 8 rows with five alternatives 10.2 us (in two launches 11.2, without
-// alternatives 7.4), 77 fp32 rows of 50257 with 20 alternatives 14.3 (14.9).
+// bounds such calls: 8 bf16 rows of 151936 with five alternatives 8.3 us, 77 fp32 rows of 50257
+// with 20 alternatives 11.7. Of the first's 7.2 in the kernel the loads are 1.2, the sums of a
+// block 0.4 twice, the selections 1.7 and 1.0, and the exchange 1.5 (the rest waits for the
+// ragged chunk).
 //
 // The largest: of 64 groups of threads the `top`-th largest maximum bounds the `top`-th
-// largest logit from below, so only threads whose maximum reaches it have any of them: those
-// threads' elements are read again (from the caches), the ones that reach the bound kept in
-// LDS and ranked by counting. Order is by (value, index) as one 64-bit key, so equal logits,
-// and rows of one value alone, are bounded like any other.
+// largest logit from below, so only threads whose maximum reaches it have any of them. Those
+// threads' elements that reach the bound go to a list in LDS and are ranked by counting.
+// Every wave finds the bound by itself, bit by bit from ballots; the upper 16 bits of the
+// value do, and all bits of (value, place) where many elements are equal. Up to kLpHeld
+// iterations a thread's elements are loaded at once and stay in registers, and the runs of
+// eight that reach the bound go to LDS; longer ones are read again from the caches.
 #include "tpp_common.hpp"
 
 namespace tpp {
 
 constexpr int kLpThreads = 256, kLpRun = 8, kLpStep = kLpThreads * kLpRun; // elements an iteration
 constexpr int kLpMaxTop = 32, kLpRoom = 1024;
+constexpr int kLpHeld = 8, kLpRuns = kLpMaxTop * kLpHeld;
 
 typedef unsigned long long u64;
 
@@ -88,76 +93,83 @@ struct LpSums { // of elements met so far: maximum, sum of e^(x - m), sum of e^(
   }
 };
 
-// The sums of a block's threads.
-__device__ __forceinline__ LpSums lp_block(const LpSums &a) {
-  __shared__ float s_sum[4][3];
+// A block's exchange.
+struct LpShared {
+  float sum[4][3];
+  u64 max[kLpThreads], cand[kLpRoom + 32], best[4];
+  int active[kLpThreads], n[2];       // threads, or runs, that reach the bound; entries of active and cand
+  float run[kLpRuns][kLpRun];         // values of those runs
+};
+static_assert(kLpRuns <= kLpThreads, "a run's place is in active");
+
+// The sums of a block's threads. Each thread's largest key is in s.max then, for lp_select.
+__device__ __forceinline__ LpSums lp_block(const LpSums &a, u64 mine, LpShared &s) {
   float mx = row16_max(a.m);
   mx = fmaxf(fmaxf(readlane_f32(mx, 0), readlane_f32(mx, 16)), fmaxf(readlane_f32(mx, 32), readlane_f32(mx, 48)));
   LpSums ws = a;
   ws.shift(mx);
   ws.s = wave_sum(ws.s), ws.t = wave_sum(ws.t);
-  if (lane_id() == 0) s_sum[wave_id()][0] = ws.m, s_sum[wave_id()][1] = ws.s, s_sum[wave_id()][2] = ws.t;
+  if (lane_id() == 0) s.sum[wave_id()][0] = ws.m, s.sum[wave_id()][1] = ws.s, s.sum[wave_id()][2] = ws.t;
+  s.max[threadIdx.x] = mine;
+  if (threadIdx.x < 2) s.n[threadIdx.x] = 0;
   __syncthreads();
-  LpSums all = {s_sum[0][0], s_sum[0][1], s_sum[0][2]};
+  LpSums all = {fmaxf(fmaxf(s.sum[0][0], s.sum[1][0]), fmaxf(s.sum[2][0], s.sum[3][0])), 0.f, 0.f};
 #pragma unroll
-  for (int i = 1; i < 4; ++i) all.add(LpSums{s_sum[i][0], s_sum[i][1], s_sum[i][2]});
+  for (int i = 0; i < 4; ++i) {
+    LpSums x = {s.sum[i][0], s.sum[i][1], s.sum[i][2]};
+    x.shift(all.m);
+    all.s += x.s, all.t += x.t;
+  }
   return all;
 }
 
 // The `top` largest of a block's elements, put(rank, key) once for each rank (all of them
-// where there are fewer). `mine`: a bound of this thread's keys that one of them reaches;
-// keys(t, j, bound, f), j < items: f(key) for those of thread t's j-th item that reach the
-// bound.
-template <typename TK, typename PUT>
-__device__ __forceinline__ void lp_select(u64 mine, int top, int items, TK keys, PUT put) {
-  __shared__ u64 s_max[kLpThreads], s_cand[kLpRoom], s_bound, s_best[4];
-  __shared__ int s_active[kLpThreads], s_n[2], s_rank[kWave];
+// where there are fewer), behind lp_block. `mine`, given there: a bound of this thread's keys
+// that one of them reaches. begin(bound), then scan(bound, f) any number of times: f(key) for
+// every key that reaches the bound.
+template <typename BEGIN, typename SCAN, typename PUT>
+__device__ __forceinline__ void lp_select(LpShared &s, int top, BEGIN begin, SCAN scan, PUT put) {
   const int tid = threadIdx.x, lane = lane_id(), w = wave_id();
-  s_max[tid] = mine;
-  if (tid < 2) s_n[tid] = 0;
-  if (tid == 0) s_bound = 0;
-  if (w == 0) s_rank[lane] = 0;
-  __syncthreads();
-  // the top-th largest of 64 groups' (four threads a group); a wave counts a quarter of what is larger
-  u64 g = s_max[lane];
+  // the top-th largest of 64 groups (four threads a group)
+  u64 g = s.max[lane];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) g = max(g, s_max[i * kWave + lane]);
-  int larger = 0;
+  for (int i = 1; i < 4; ++i) g = max(g, s.max[i * kWave + lane]);
+  const unsigned hi = (unsigned)(g >> 32);
+  unsigned b = 0;
 #pragma unroll
-  for (int l = 0; l < kWave / 4; ++l) {
-    const int from = (w * (kWave / 4) + l);
-    const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(g >> 32), from);
-    const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)g, from);
-    larger += (((u64)hi << 32) | lo) > g;
-  }
-  atomicAdd(&s_rank[lane], larger);
-  __syncthreads();
-  if (w == 0 && s_rank[lane] == top - 1) s_bound = g;
-  __syncthreads();
-  const u64 bound = s_bound;
-  if (mine >= bound) s_active[atomicAdd(&s_n[0], 1)] = tid;
-  __syncthreads();
-  // the active threads' items over the block (a wave a thread would wait for memory once for
-  // each of them)
-  const unsigned all = (unsigned)(s_n[0] * items);
-  auto each = [&](auto f) {
-    for (unsigned i = tid; i < all; i += kLpThreads) {
-      const unsigned k = i / (unsigned)items;
-      keys(s_active[k], (int)(i - k * (unsigned)items), bound, f);
-    }
+  for (int bit = 31; bit >= 16; --bit)
+    if (__popcll(__ballot(hi >= (b | 1u << bit))) >= top) b |= 1u << bit;
+  u64 bound = (u64)b << 32;
+  auto list = [&] {
+    begin(bound);
+    scan(bound, [&](u64 key) {
+      const int at = atomicAdd(&s.n[1], 1);
+      if (at < kLpRoom) s.cand[at] = key;
+    });
+    __syncthreads();
   };
-  each([&](u64 key) {
-    const int at = atomicAdd(&s_n[1], 1);
-    if (at < kLpRoom) s_cand[at] = key;
-  });
-  __syncthreads();
-  const int found = s_n[1];
+  list();
+  int found = s.n[1];
+  if (found > kLpRoom || s.n[0] > kLpRuns) { // many equal ones: the bound to the last bit, `top` threads at most
+    for (int bit = 47; bit >= 0; --bit)
+      if (__popcll(__ballot(g >= (bound | 1ull << bit))) >= top) bound |= 1ull << bit;
+    __syncthreads();
+    if (tid < 2) s.n[tid] = 0;
+    __syncthreads();
+    list();
+    found = s.n[1];
+  }
   if (found <= kLpRoom) {
-    for (int c = tid; c < found; c += kLpThreads) {
-      const u64 key = s_cand[c];
+    // four threads a candidate, a quarter of the list each (every wave pads the list with zeros)
+    if (lane < 32) s.cand[found + lane] = 0;
+    for (int c = tid / 4; c < (found + 63) / 64 * 64; c += kLpThreads / 4) {
+      const u64 key = s.cand[min(c, found)];
       int rank = 0;
-      for (int k = 0; k < found; ++k) rank += s_cand[k] > key;
-      if (rank < top) put(rank, key);
+      for (int k = tid % 4; k < found; k += 32)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rank += s.cand[k + 4 * j] > key;
+      rank = (int)group_sum<4>((float)rank);
+      if (tid % 4 == 0 && c < found && rank < top) put(rank, key);
     }
     return;
   }
@@ -166,15 +178,15 @@ __device__ __forceinline__ void lp_select(u64 mine, int top, int items, TK keys,
   u64 last = ~0ull;
   for (int k = 0; k < top; ++k) {
     u64 best = 0;
-    each([&](u64 key) {
+    scan(bound, [&](u64 key) {
       if (key < last) best = max(best, key);
     });
 #pragma unroll
     for (int sh = 1; sh < kWave; sh <<= 1) best = max(best, (u64)__shfl_xor(best, sh, kWave));
     __syncthreads();
-    if (lane == 0) s_best[w] = best;
+    if (lane == 0) s.best[w] = best;
     __syncthreads();
-    last = max(max(s_best[0], s_best[1]), max(s_best[2], s_best[3]));
+    last = max(max(s.best[0], s.best[1]), max(s.best[2], s.best[3]));
     if (tid == 0) put(k, last);
   }
 }
@@ -184,19 +196,13 @@ struct LpRow {
   float m, log_z;
   bool nan; // a NaN, or +inf less +inf
 };
-// The row's token's logit, by thread 0: asked for ahead of everything else.
+// The row's token's logit, asked for behind the first loads of the row: it takes two trips.
 struct LpToken {
   float x;
   bool real;
 };
-template <typename P> __device__ __forceinline__ LpToken lp_token(const LpArgs &p, int64_t r) {
-  LpToken k = {0.f, false};
-  if (threadIdx.x == 0) {
-    const int64_t t = p.tok[r];
-    k.real = t >= 0 && t < p.V;
-    if (k.real) k.x = to_f32(((const P *)p.x)[r * p.x_s + t]);
-  }
-  return k;
+template <typename P> __device__ __forceinline__ LpToken lp_token(const LpArgs &p, int64_t r, int64_t t) {
+  return {to_f32(((const P *)p.x)[r * p.x_s + min(max(t, (int64_t)0), p.V - 1)]), t >= 0 && t < p.V};
 }
 __device__ __forceinline__ LpRow lp_finish(const LpArgs &p, int64_t r, const LpSums &all, const LpToken &k) {
   const LpRow o = {all.m, all.m == -INFINITY ? NAN : logf(all.s), all.s != all.s};
@@ -221,51 +227,80 @@ __device__ __forceinline__ u64 lp_fetch(const u64 *p) {
 }
 
 // The chunks of a row, by one block.
-__device__ __forceinline__ void lp_join(const LpArgs &p, int64_t r, int chunks, const LpToken &k) {
+__device__ __forceinline__ void lp_join(const LpArgs &p, int64_t r, int chunks, const LpToken &k, LpShared &s) {
   constexpr int kKeep = 4; // keys a thread keeps (past them, memory is asked again)
   const int tid = threadIdx.x;
   const u64 *sums = p.sums + r * chunks * 2, *in = p.keys + r * chunks * p.top;
   const int n = chunks * p.top;
   LpSums a = {-INFINITY, 0.f, 0.f};
-  __shared__ u64 s_key[kKeep * kLpThreads];
   u64 key[kKeep], mine = 0;
 #pragma unroll
   for (int j = 0; j < kKeep; ++j) key[j] = j * kLpThreads + tid < n ? lp_fetch(in + j * kLpThreads + tid) : 0;
-#pragma unroll
-  for (int j = 0; j < kKeep; ++j) s_key[j * kLpThreads + tid] = key[j], mine = max(mine, key[j]);
-  for (int c = kKeep * kLpThreads + tid; c < n; c += kLpThreads) mine = max(mine, lp_fetch(in + c));
   for (int c = tid; c < chunks; c += kLpThreads) {
     const u32x2 x = __builtin_bit_cast(u32x2, lp_fetch(sums + c * 2)), y = __builtin_bit_cast(u32x2, lp_fetch(sums + c * 2 + 1));
     a.add(LpSums{__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(y[0])});
   }
-  const LpRow o = lp_finish(p, r, lp_block(a), k);
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) mine = max(mine, key[j]);
+  for (int c = kKeep * kLpThreads + tid; c < n; c += kLpThreads) mine = max(mine, lp_fetch(in + c));
+  const LpRow o = lp_finish(p, r, lp_block(a, mine, s), k);
   if (p.top && !o.nan)
-    lp_select(mine, p.top, (n + kLpThreads - 1) / kLpThreads,
-              [&](int t, int j, u64 bound, auto f) {
-                const int c = j * kLpThreads + t;
-                if (c >= n) return;
-                const u64 x = c < kKeep * kLpThreads ? s_key[c] : lp_fetch(in + c);
-                if (x >= bound) f(x);
+    lp_select(s, p.top, [](u64) {},
+              [&](u64 bound, auto f) {
+#pragma unroll
+                for (int j = 0; j < kKeep; ++j)
+                  if (j * kLpThreads + tid < n && key[j] >= bound) f(key[j]);
+                for (int c = kKeep * kLpThreads + tid; c < n; c += kLpThreads) {
+                  const u64 x = lp_fetch(in + c);
+                  if (x >= bound) f(x);
+                }
               },
               [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
 }
 
-// A row (WHOLE), or chunk blockIdx.y of one: `steps` iterations of the block.
-template <typename P, bool WHOLE> __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LpArgs p, int steps) {
-  constexpr int U = 4; // iterations whose loads are in flight
+// A row (WHOLE), or chunk blockIdx.y of one: `steps` iterations of the block. HELD: at most
+// kLpHeld of them, in registers throughout.
+template <typename P, bool WHOLE, bool HELD> __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LpArgs p, int steps) {
+  constexpr int U = HELD ? kLpHeld : 4; // iterations whose loads are in flight
   typedef typename LpVec<P>::type V;
+  __shared__ LpShared s;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x, base = WHOLE ? 0 : (int64_t)blockIdx.y * steps * kLpStep;
   const P *row = (const P *)p.x + r * p.x_s;
   const int64_t n = WHOLE ? p.V : min(p.V, base + (int64_t)steps * kLpStep);
   const int iters = (int)((n - base + kLpStep - 1) / kLpStep), full = (int)((n - base) / kLpStep);
 
-  const LpToken token = lp_token<P>(p, r);
+  const int64_t tok = p.tok[r];
+  const P *mine_at = row + base + tid * kLpRun;
+  auto at = [&](int i) { return base + (int64_t)i * kLpStep + tid * kLpRun; }; // this thread's elements of iteration i
+  V v[U];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < full) v[u] = __builtin_nontemporal_load((const V *)(mine_at + u * kLpStep));
+    if (full < iters) {
+      V end;
+#pragma unroll
+      for (int e = 0; e < kLpRun; ++e) end[e] = row[min(at(full) + e, n - 1)];
+#pragma unroll
+      for (int e = 0; e < kLpRun; ++e) end[e] = at(full) + e < n ? end[e] : P(-INFINITY);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u == full) v[u] = end;
+    }
+  } else if (full >= U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = __builtin_nontemporal_load((const V *)(mine_at + u * kLpStep));
+  }
+  const LpToken token = lp_token<P>(p, r, tok);
+
   LpSums a = {-INFINITY, 0.f, 0.f};
-  int first = 0; // iteration in which this thread met its maximum
-  auto add = [&](const float (&x)[kLpRun], int i) {
-    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (mx > a.m) a.shift(mx), first = i;
+  int first = 0;    // iteration in which this thread met its maximum
+  float most[U];    // HELD: of every iteration
+  auto largest = [](const float (&x)[kLpRun]) {
+    return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+  };
+  auto add = [&](const float (&x)[kLpRun]) {
     const float mu = a.m == -INFINITY ? 0.f : a.m;
 #pragma unroll
     for (int e = 0; e < kLpRun; ++e) {
@@ -274,45 +309,99 @@ template <typename P, bool WHOLE> __global__ __launch_bounds__(kLpThreads) void 
       a.t = fmaf(f, fmaxf(d, -1e30f), a.t); // (0 times -inf is none)
     }
   };
-  const P *mine_at = row + base + tid * kLpRun;
-  int i = 0;
-  if (full >= U) {
-    V v[U];
+  auto values = [](const V &v, float (&x)[kLpRun]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = __builtin_nontemporal_load((const V *)(mine_at + (int64_t)u * kLpStep));
-    for (; i + U <= full; i += U)
+    for (int e = 0; e < kLpRun; ++e) x[e] = to_f32(v[e]);
+  };
+  float x[kLpRun];
+  if constexpr (HELD) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[kLpRun];
+    for (int u = 0; u < U; ++u) {
+      if (u >= iters) continue;
+      values(v[u], x);
+      most[u] = largest(x);
+      if (most[u] > a.m) a.m = most[u], first = u;
+    }
 #pragma unroll
-        for (int e = 0; e < kLpRun; ++e) x[e] = to_f32(v[u][e]);
-        // (past the last whole round: an iteration that is there, not used)
-        const int next = i + u + U < full / U * U ? i + u + U : i + u;
-        v[u] = __builtin_nontemporal_load((const V *)(mine_at + (int64_t)next * kLpStep));
-        add(x, i + u);
-      }
-  }
-  for (; i < iters; ++i) {
-    float x[kLpRun];
-    lp_load(row, base + (int64_t)i * kLpStep + tid * kLpRun, n, x);
-    add(x, i);
+    for (int u = 0; u < U; ++u) {
+      if (u >= iters) continue;
+      values(v[u], x);
+      add(x);
+    }
+  } else {
+    auto step = [&](int i) {
+      const float mx = largest(x);
+      if (mx > a.m) a.shift(mx), first = i;
+      add(x);
+    };
+    int i = 0;
+    if (full >= U)
+      for (; i + U <= full; i += U)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          values(v[u], x);
+          // (past the last whole round: an iteration that is there, not used)
+          const int next = i + u + U < full / U * U ? i + u + U : i + u;
+          v[u] = __builtin_nontemporal_load((const V *)(mine_at + (int64_t)next * kLpStep));
+          step(i + u);
+        }
+    for (; i < iters; ++i) {
+      lp_load(row, at(i), n, x);
+      step(i);
+    }
   }
 
   const unsigned run0 = (unsigned)(base / kLpRun); // a place is a run of eight, counted over the row
   const u64 mine = lp_key(a.m, run0 + (unsigned)(first * kLpThreads + tid));
-  const LpSums all = lp_block(a);
-  auto keys = [&](int t, int j, u64 bound, auto f) {
-    const unsigned run = run0 + (unsigned)(j * kLpThreads + t);
-    if ((int64_t)run * kLpRun >= n) return;
-    float x[kLpRun];
-    lp_load(row, (int64_t)run * kLpRun, n, x);
+  const LpSums all = lp_block(a, mine, s);
+  auto begin = [&](u64 bound) {
+    if constexpr (HELD) {
+      auto hit = [&](int u) { return u < iters && lp_key(most[u], run0 + (unsigned)(u * kLpThreads + tid)) >= bound; };
+      int hits = 0;
 #pragma unroll
-    for (int e = 0; e < kLpRun; ++e)
-      if ((int64_t)run * kLpRun + e < n && lp_key(x[e], run) >= bound) f(lp_key(x[e], run * kLpRun + e));
+      for (int u = 0; u < U; ++u) hits += hit(u);
+      const int upto = wave_scan(hits), all = __builtin_amdgcn_readlane(upto, kWave - 1);
+      int k = 0;
+      if (lane_id() == 0 && all) k = atomicAdd(&s.n[0], all);
+      k = __builtin_amdgcn_readfirstlane(k) + upto - hits;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!hit(u)) continue;
+        if (k < kLpRuns) {
+          s.active[k] = (int)(run0 + (unsigned)(u * kLpThreads + tid));
+          values(v[u], x);
+#pragma unroll
+          for (int e = 0; e < kLpRun; e += 4) *reinterpret_cast<f32x4 *>(&s.run[k][e]) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+        }
+        ++k;
+      }
+    } else {
+      if (mine >= bound) s.active[atomicAdd(&s.n[0], 1)] = tid;
+    }
+    __syncthreads();
+  };
+  auto reach = [&](float x, unsigned run, int e, u64 bound, auto f) {
+    if (lp_key(x, run) >= bound && (int64_t)run * kLpRun + e < n) f(lp_key(x, run * kLpRun + e));
+  };
+  auto scan = [&](u64 bound, auto f) {
+    if constexpr (HELD) {
+      const int work = min(s.n[0], kLpRuns) * kLpRun;
+      for (int i = tid; i < work; i += kLpThreads) reach(s.run[i / kLpRun][i % kLpRun], s.active[i / kLpRun], i % kLpRun, bound, f);
+    } else {
+      // their iterations over the block (a wave a thread would wait for memory once for each)
+      const unsigned work = (unsigned)(s.n[0] * iters);
+      for (unsigned i = tid; i < work; i += kLpThreads) {
+        const unsigned k = i / (unsigned)iters, run = run0 + (i - k * (unsigned)iters) * kLpThreads + s.active[k];
+        if ((int64_t)run * kLpRun >= n) continue;
+        lp_load(row, (int64_t)run * kLpRun, n, x);
+#pragma unroll
+        for (int e = 0; e < kLpRun; ++e) reach(x[e], run, e, bound, f);
+      }
+    }
   };
   if constexpr (WHOLE) {
     const LpRow o = lp_finish(p, r, all, token);
-    if (p.top && !o.nan) lp_select(mine, p.top, iters, keys, [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
+    if (p.top && !o.nan) lp_select(s, p.top, begin, scan, [&](int rank, u64 key) { lp_put(p, r, o, rank, key); });
   } else {
     const int chunks = gridDim.y;
     const int64_t slot = r * chunks + blockIdx.y;
@@ -323,7 +412,7 @@ template <typename P, bool WHOLE> __global__ __launch_bounds__(kLpThreads) void 
     if (p.top && all.s == all.s) { // (else the row is NaN, no key is used)
       u64 *out = p.keys + slot * p.top;
       if (n - base < p.top && tid >= n - base && tid < p.top) lp_store(out + tid, 0); // fewer elements: below every key
-      lp_select(mine, p.top, iters, keys, [&](int rank, u64 key) { lp_store(out + rank, key); });
+      lp_select(s, p.top, begin, scan, [&](int rank, u64 key) { lp_store(out + rank, key); });
     }
     if (!p.arrived) return;
     __shared__ int s_last;
@@ -336,17 +425,18 @@ template <typename P, bool WHOLE> __global__ __launch_bounds__(kLpThreads) void 
       if (s_last) __hip_atomic_store(p.arrived + r, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (s_last) lp_join(p, r, chunks, token);
+    if (s_last) lp_join(p, r, chunks, token, s);
   }
 }
 
 template <typename P> __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(LpArgs p, int chunks) {
-  lp_join(p, blockIdx.x, chunks, lp_token<P>(p, blockIdx.x));
+  __shared__ LpShared s;
+  lp_join(p, blockIdx.x, chunks, lp_token<P>(p, blockIdx.x, p.tok[blockIdx.x]), s);
 }
 
-// Chunks of a row (1: none), of `steps` iterations: one block a CU. (8 bf16 rows of 151936,
-// five alternatives, one to eight blocks a CU: 10.3, 10.8, 12.2 us; 77 fp32 rows of 50257, 20
-// alternatives: 14.4, 15.2, 15.7: what is selected a chunk costs more than the chunk's loads.)
+// Chunks of a row (1: none), of `steps` iterations: one block a CU. (us in the kernel, one and
+// two: 8 bf16 rows of 151936 with five alternatives 7.2 and 7.6, 4 with 20 7.7 and 10.2, 32 with
+// five 9.5 and 10.2; 77 fp32 rows of 50257 with 20 10.9 and 10.2: more keys to join.)
 struct LpPlan {
   int chunks, steps;
 };
@@ -396,10 +486,14 @@ extern "C" int tpp_token_logprobs(const void *logits, int64_t row_stride, const 
   if (pl.chunks > 1) a.arrived = arrival_words(st, N);
   auto go = [&](auto zero) {
     typedef decltype(zero) P;
+    const dim3 grid((unsigned)N, (unsigned)pl.chunks);
+    const bool held = pl.steps <= kLpHeld;
     if (pl.chunks == 1) {
-      logprob_kernel<P, true><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a, pl.steps);
+      if (held) logprob_kernel<P, true, true><<<grid, dim3(kLpThreads), 0, st>>>(a, pl.steps);
+      else logprob_kernel<P, true, false><<<grid, dim3(kLpThreads), 0, st>>>(a, pl.steps);
     } else {
-      logprob_kernel<P, false><<<dim3((unsigned)N, pl.chunks), dim3(kLpThreads), 0, st>>>(a, pl.steps);
+      if (held) logprob_kernel<P, false, true><<<grid, dim3(kLpThreads), 0, st>>>(a, pl.steps);
+      else logprob_kernel<P, false, false><<<grid, dim3(kLpThreads), 0, st>>>(a, pl.steps);
       if (!a.arrived) logprob_join_kernel<P><<<dim3((unsigned)N), dim3(kLpThreads), 0, st>>>(a, pl.chunks);
     }
     return check_launch(name);
