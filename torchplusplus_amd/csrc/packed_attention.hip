@@ -57,36 +57,40 @@ struct PackedRow {
   bool real;
 };
 // Self-attention: tile `t` is rows 32 t .. 32 t + 31 of the batch, whatever sequences they are
-// of, so that short ones share a tile. The first sequence that ends past the tile's first row
-// is found by a search in 64 parts, each lane's own from there on, 64 sequences at a time.
-__device__ __forceinline__ PackedRow packed_row_self(const PackedArgs &p, int t) {
-  const int lane = lane_id(), first = t * 32, r = min(first + (lane & 31), p.Nq - 1);
+// of, so that short ones share a tile. packed_find searches in 64 parts for the first sequence
+// that ends past the tile's first row, or up to 63 ahead of it; packed_row_self takes it from
+// there, given the begins and ends of the 64 sequences from `lo`, a lane each.
+__device__ __forceinline__ int packed_find(const PackedArgs &p, int t) {
   int lo = 0, hi = p.B; // the sequence is in [lo, hi), or there is none
   while (hi - lo > kWave) {
-    const int step = (hi - lo + kWave - 1) / kWave, at = min(lo + (lane + 1) * step, hi) - 1;
-    const unsigned long long past = __ballot(p.cu_q[at + 1] > first);
+    const int step = (hi - lo + kWave - 1) / kWave, at = min(lo + (lane_id() + 1) * step, hi) - 1;
+    const unsigned long long past = __ballot(p.cu_q[at + 1] > t * 32);
     const int l = past ? __builtin_ctzll(past) : kWave - 1;
     const int next = lo + l * step;
     hi = min(next + step, hi), lo = min(next, hi);
   }
-  PackedRow o = {{r, 0, 0, 0}, 0, first + (lane & 31) < p.Nq && p.fill != 0}; // of no sequence
+  return lo;
+}
+__device__ __forceinline__ PackedRow packed_row_self(const PackedArgs &p, int t, int lo, int begin, int end) {
+  const int first = t * 32, r = min(first + (lane_id() & 31), p.Nq - 1);
+  const bool in = first + (lane_id() & 31) < p.Nq;
+  PackedRow o = {{r, 0, 0, 0}, 0, in && p.fill != 0}; // of no sequence
   bool found = false;
-  for (; lo < p.B; lo += kWave) {
-    const int end = lo + lane < p.B ? p.cu_q[lo + lane + 1] : 0x7fffffff, begin = p.cu_q[lo];
-    const int last = __builtin_amdgcn_readlane(end, kWave - 1);
-    int n = 0; // ends at or ahead of the row: of 64 in order
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1)
-      if (__shfl(end, n + s - 1, kWave) <= r) n += s;
-    const int mine = __shfl(end, n, kWave), ahead = __shfl(end, max(n - 1, 0), kWave);
-    if (!found && (n < kWave - 1 || last > r)) {
-      found = true;
+  auto take = [&](int lo, int begin, int end) { // whether sequences behind these may have rows in the tile
+    if (lo + lane_id() >= p.B) begin = end = 0x7fffffff;
+    // (mostly one or two do)
+    for (unsigned long long hit = __ballot(end > first && begin < first + 32); hit; hit &= hit - 1) {
+      const int l = __builtin_ctzll(hit);
       // (packed_seq's rows, without another trip to memory)
-      const int q0 = min(max(n ? ahead : begin, 0), p.Nq), q1 = min(mine, p.Nq);
-      if (lo + n < p.B && r >= q0 && r < q1) o = {{q0, q1 - q0, q0, q1 - q0}, r - q0, first + (lane & 31) < p.Nq};
+      const int q0 = max(__builtin_amdgcn_readlane(begin, l), 0), q1 = min(__builtin_amdgcn_readlane(end, l), p.Nq);
+      if (!found && r >= q0 && r < q1) found = true, o = {{q0, q1 - q0, q0, q1 - q0}, r - q0, in};
     }
-    if (__all(found)) break;
-  }
+    return __builtin_amdgcn_readlane(end, kWave - 1) < first + 32;
+  };
+  // (the first apart: values loaded in a loop are waited for, with every DMA, where it begins)
+  if (take(lo, begin, end))
+    for (int at = lo + kWave; at < p.B; at += kWave)
+      if (!take(at, p.cu_q[min(at + lane_id(), p.B)], p.cu_q[min(at + lane_id() + 1, p.B)])) break;
   return o;
 }
 
@@ -98,7 +102,7 @@ __device__ __forceinline__ PackedRow packed_row_self(const PackedArgs &p, int t)
 // head's keys, every fourth tile each, and are merged through LDS. (Eight waves a row were
 // slower everywhere: the rate at which a CU's LDS-DMA brings tiles, ~80 bytes a ns, bounds
 // both where sequences are not short. Short ones are the launch and a chain of trips to memory,
-// 7.3 us for one of 230 tokens, 12 for 64 of 3 to 200.) The keys that rows see rise with the
+// 6.8 us for one of 230 tokens, 11.8 for 64 of 3 to 200.) The keys that rows see rise with the
 // rows, so the first and last row that see any give the wave's range; keys of a tile that a row
 // does not see, other sequences' among them, are masked.
 // ---------------------------------------------------------------------------
@@ -115,22 +119,76 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
   __shared__ __attribute__((aligned(16))) char smem[kRing > kMerge ? kRing : kMerge];
   __shared__ float s_m[NW][32], s_l[NW][32];
   __shared__ unsigned s_bad;
+  __shared__ int s_cu[NW][2][kWave];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, ql = lane & 31;
   const int e = blockIdx.x / nh, hb = blockIdx.x - e * nh;
   const int hq = SPLIT ? hb : hb * 4 + w;
   if (hq >= p.Hq) return;
+  const int hk = hq / (p.Hq / p.Hkv);
+  const char *kp = (const char *)((const T *)p.k + (int64_t)hk * p.k_sh);
+  const char *vp = (const char *)((const T *)p.v + (int64_t)hk * p.v_sh);
+  char *const ring = smem + w * (2 * TU * 16);
+  const int dkey = lane / CPR, dslot = lane % CPR;
+  int row_lo = 0, row_hi = p.Nk - 1;
+  // the tile at row kb; keys ahead of row_lo or behind row_hi read those rows (masked)
+  auto issue = [&](const char *head, int64_t ss, int kb, char *dst, auto swizzle) {
+    const int rb = min(max(kb, row_lo), row_hi);
+    const char *tb = head + (int64_t)rb * ss * 2;
+#pragma unroll
+    for (int j = 0; j < NDMA; ++j) {
+      const int key = j * KPI + dkey, rel = min(max(kb + key, row_lo), row_hi) - rb;
+      __builtin_amdgcn_global_load_lds((const void *)(tb + (unsigned)(rel * (int)ss * 2 + ((dslot ^ swizzle(key)) << 4))),
+                                       (__attribute__((address_space(3))) void *)(dst + j * 1024), 16, 0, 0);
+    }
+  };
+  auto issue_k = [&](int kb) { issue(kp, p.k_ss, kb, ring, [](int r) { return r & (CPR - 1); }); };
+  auto issue_v = [&](int kb) { issue(vp, p.v_ss, kb, ring + TU * 16, [](int r) { return vswz<D>(r); }); };
+  V8 qf[KS];
+  auto ask_q = [&](int qrow) {
+    const T *qp = (const T *)p.q + (int64_t)qrow * p.q_ss + (int64_t)hq * p.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const V8 *>(qp + ks * 16 + h * 8);
+  };
+
+  // Tiles go from the keys' end down: a causal tile of self-attention ends with its queries, so
+  // they and the first keys can be asked for ahead of the sequences' lengths. With shared keys,
+  // where there are few waves, that saves a trip to memory (one sequence of 230: 7.3 -> 6.8 us);
+  // without, the loads of all waves at once are what the first tile waits for, and keys that are
+  // of no use add to them (64 of 3 to 200: 11.8 -> 12.8).
   PackedRow row;
+  const bool early = SELF && SPLIT && p.right == 0;
+  const int kearly = min(e * 32 + 32, p.Nq), kw = SPLIT ? w * KT : 0; // (this wave's first tile ends at kend - kw)
+  const bool asked = early && kearly - kw > 0;
   if constexpr (SELF) {
-    row = packed_row_self(p, e);
+    // The lengths come by LDS-DMA, ahead of the query rows: loads return in the order they were
+    // asked for, but for a value in a register the compiler waits for every DMA.
+    const int lo = packed_find(p, e);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      __builtin_amdgcn_global_load_lds((const void *)(p.cu_q + min(lo + lane + i, p.B)),
+                                       (__attribute__((address_space(3))) void *)s_cu[w][i], 4, 0, 0);
+    asm volatile("" ::: "memory");
+    ask_q(min(e * 32 + ql, p.Nq - 1));
+    if (asked) {
+      issue_k(kearly - kw - KT);
+      issue_v(kearly - kw - KT);
+      vm_wait<KS + 2 * NDMA>();
+    } else {
+      vm_wait<KS>();
+    }
+    float begin = lds_read_b32<0>(lds_offset(s_cu[w][0]) + 4 * lane), end = lds_read_b32<0>(lds_offset(s_cu[w][1]) + 4 * lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(begin), "+v"(end)::"memory");
+    row = packed_row_self(p, e, lo, __float_as_int(begin), __float_as_int(end));
   } else {
     PackedSeq seq = {0, 0, 0, 0};
     const int qt = packed_tile(p, e, 32, seq);
     if (qt < 0) return; // (every wave)
     row = {seq, min(qt * 32 + ql, seq.Sq - 1), qt * 32 + ql < seq.Sq};
+    ask_q(row.seq.q0 + row.i);
   }
-  const int hk = hq / (p.Hq / p.Hkv), qrow = row.seq.q0 + row.i;
+  const int qrow = row.seq.q0 + row.i;
   const KeyRange kr = packed_keys(p, row.i, row.seq.Sq, row.seq.Sk);
   const int klo = row.seq.k0 + kr.lo, khi = row.seq.k0 + kr.hi; // rows of k and v that the row sees
   const bool sees = row.real && kr.lo < kr.hi;
@@ -139,31 +197,10 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
   const int kmin = __builtin_amdgcn_readlane(klo, ra), kmax = seeing ? __builtin_amdgcn_readlane(khi, rb) : kmin;
   // keys [all_lo, all_hi) are seen by every row that sees any
   const int all_lo = __builtin_amdgcn_readlane(klo, rb), all_hi = __builtin_amdgcn_readlane(khi, ra);
-  const int k0 = kmin + (SPLIT ? w * KT : 0);
-
-  const char *kp = (const char *)((const T *)p.k + (int64_t)hk * p.k_sh);
-  const char *vp = (const char *)((const T *)p.v + (int64_t)hk * p.v_sh);
-  char *const ring = smem + w * (2 * TU * 16);
-  const int dkey = lane / CPR, dslot = lane % CPR;
-  // (keys past the last that is seen read it, masked)
-  auto issue = [&](const char *head, int64_t ss, int kb, char *dst, auto swizzle) {
-    const char *tb = head + (int64_t)kb * ss * 2;
-    const int most = kmax - 1 - kb;
-#pragma unroll
-    for (int j = 0; j < NDMA; ++j) {
-      const int key = j * KPI + dkey;
-      __builtin_amdgcn_global_load_lds((const void *)(tb + (unsigned)(min(key, most) * (int)ss * 2 + ((dslot ^ swizzle(key)) << 4))),
-                                       (__attribute__((address_space(3))) void *)(dst + j * 1024), 16, 0, 0);
-    }
-  };
-  auto issue_k = [&](int kb) { issue(kp, p.k_ss, kb, ring, [](int r) { return r & (CPR - 1); }); };
-  auto issue_v = [&](int kb) { issue(vp, p.v_ss, kb, ring + TU * 16, [](int r) { return vswz<D>(r); }); };
-
-  const T *qp = (const T *)p.q + (int64_t)qrow * p.q_ss + (int64_t)hq * p.q_sh;
-  V8 qf[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const V8 *>(qp + ks * 16 + h * 8);
-  if (k0 < kmax) {
+  const int kend = early ? kearly : kmax, k0 = kend - kw - KT; // (kmax <= kearly)
+  const bool any = kmin < kmax && k0 + KT > kmin;
+  row_lo = kmin, row_hi = max(kmax - 1, kmin);
+  if (any && !asked) {
     issue_k(k0);
     issue_v(k0);
   }
@@ -186,10 +223,10 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
     vo[tt] = kbase + TU * 16 + kl * D * 2 + (((d0 >> 3) ^ vswz<D>(kl)) << 4) + ((d0 & 7) << 1);
   }
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks])); // here, not in the loop
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks])); // here, not in the loop
 
-  for (int kb = k0; kb < kmax; kb += SH * KT) {
-    const bool more = kb + SH * KT < kmax;
+  for (int kb = k0; any && kb + KT > kmin; kb -= SH * KT) {
+    const bool more = kb - SH * KT + KT > kmin;
     vm_wait<NDMA>(); // this tile's K landed, its V may be in flight
     // S^T = K Q^T: eight fragments, read i is K step i (two blocks of 32 keys: step i / 2)
     V8 kr[4][2];
@@ -207,7 +244,7 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
       lds_wait_tied<(3 - i) * 2>(kr[i]);
       if constexpr (i == 3) { // every K fragment is in registers
         asm volatile("" ::: "memory");
-        if (more) issue_k(kb + SH * KT);
+        if (more) issue_k(kb - SH * KT);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -282,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
       lds_wait_tied<(NC - 1 - c) * R>(vr[c]);
       if constexpr (c == NC - 1) { // every V fragment is in registers
         asm volatile("" ::: "memory");
-        if (more) issue_v(kb + SH * KT);
+        if (more) issue_v(kb - SH * KT);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -294,10 +331,13 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
     });
   }
 
+  if (!any) vm_wait<0>(); // (asked for and not used: the slots are written to below)
   const float l = l_run + __shfl_xor(l_run, 32, kWave);
+  // rows of k and v that the block's tiles had
+  const int had_lo = max(kend - (kend - kmin + KT - 1) / KT * KT, 0), had_hi = min(kend, p.Nk);
   // values that are not finite and not seen (packed_row_again): the rows in `bad`, by `waves`
   auto again = [&](unsigned bad, int w0, int waves) {
-    if (!packed_odd_values<T, D>(p, hk, kmin, all_lo) && !packed_odd_values<T, D>(p, hk, all_hi, kmax)) return;
+    if (!packed_odd_values<T, D>(p, hk, had_lo, all_lo) && !packed_odd_values<T, D>(p, hk, all_hi, had_hi)) return;
     for (int n = 0; bad; bad &= bad - 1, ++n) {
       if (n % waves != w0) continue;
       const int l = __builtin_ctz(bad);
@@ -369,12 +409,12 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += a * x[i];
       }
-      const bool any = seeing >> n & 1;
+      const bool sees = seeing >> n & 1;
       const float inv = 1.f / ls;
       float z = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z = fmaf(v[i], 0.f, z), v[i] = any ? v[i] * inv : 0.f;
-      if (z != z && ls == ls && any) atomicOr(&s_bad, 1u << n);
+      for (int i = 0; i < 8; ++i) z = fmaf(v[i], 0.f, z), v[i] = sees ? v[i] * inv : 0.f;
+      if (z != z && ls == ls && sees) atomicOr(&s_bad, 1u << n);
       store8((T *)p.o + (int64_t)at * p.o_ss + (int64_t)hq * p.o_sh + c * 8, v);
     }
     __syncthreads(); // every row above is written, and what is odd known
@@ -442,7 +482,7 @@ struct PackedPlan {
 //    waves 4, 4.2 for each 512 blocks, and the row's share of tiles or 0.93 ns.
 //  * attn_prefill_kernel: 7 with its plan, and 4.5 and 2.0 (1.2) a tile of 64 keys for all tiles
 //    over the CUs, or the longest tile alone, 4.5 and 1.6 (1.2).
-// Measured, e.g.: one sequence of 230 7.3 (17.8 on the other kernel), of 1000 17 (38), 64 of 3 to
+// Measured, e.g.: one sequence of 230 6.8 (17.8 on the other kernel), of 1000 17 (38), 64 of 3 to
 // 200 12 (32; fp16, 16 / 16 heads of 64), 16 of 200 17 (21); and back, 16 of 1000 139 (107), eight
 // of 501 to 4001 278 (188: 770 TFLOP/s, 5 us of it the plan's launch).
 static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int left, int right,
