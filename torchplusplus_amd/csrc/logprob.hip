@@ -434,19 +434,32 @@ template <typename P> __global__ __launch_bounds__(kLpThreads) void logprob_join
   lp_join(p, blockIdx.x, chunks, lp_token<P>(p, blockIdx.x, p.tok[blockIdx.x]), s);
 }
 
-// Chunks of a row (1: none), of `steps` iterations: one block a CU. (us in the kernel, one and
-// two: 8 bf16 rows of 151936 with five alternatives 7.2 and 7.6, 4 with 20 7.7 and 10.2, 32 with
-// five 9.5 and 10.2; 77 fp32 rows of 50257 with 20 10.9 and 10.2: more keys to join.)
+// Chunks of a row (1: none), of `steps` iterations. As many as fill the CUs k times over, by
+// estimated time in us, from measurements of 1 to 1024 rows: 4; an iteration 0.1 and 0.14 for
+// each of the CU's blocks (16-bit logits, twice that for fp32); 1 a block for what it selects; 3
+// for the join; 2.5 where elements are not held. Measured, bf16 rows of 151936, k = 1 and 2: 8
+// with five alternatives 7.2 and 7.6 (in the kernel), 4 with 20 7.7 and 10.2. A few blocks more
+// than CUs are the worst: 130 rows with 32 alternatives, 260 chunks 27.6, 1040 20.9, 300 rows
+// with five, whole 30.7, halves 26.5.
 struct LpPlan {
   int chunks, steps;
 };
-static LpPlan lp_plan(int64_t N, int64_t V) {
+static LpPlan lp_plan(int64_t N, int64_t V, int dtype) {
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
   const int64_t iters = (V + kLpStep - 1) / kLpStep;
-  int64_t c = (cus + N - 1) / N;
-  if (c > iters) c = iters;
-  const int64_t steps = (iters + c - 1) / c;
-  return {(int)((iters + steps - 1) / steps), (int)steps};
+  LpPlan best = {1, (int)iters};
+  double least = 0;
+  for (int k = 1; k <= 6; ++k) {
+    int64_t c = k * cus / N;
+    if (c < 1) c = 1;
+    if (c > iters) c = iters;
+    const int64_t steps = (iters + c - 1) / c;
+    c = (iters + steps - 1) / steps;
+    const double blocks = (double)((N * c + cus - 1) / cus);
+    const double us = 4 + steps * (0.1 + (dtype == TPP_F32 ? 0.28 : 0.14) * blocks) + blocks + (c > 1 ? 3 : 0) + (steps > kLpHeld ? 2.5 : 0);
+    if (k == 1 || us < least) least = us, best = {(int)c, (int)steps};
+  }
+  return best;
 }
 
 } // namespace tpp
@@ -455,7 +468,7 @@ using namespace tpp;
 
 extern "C" size_t tpp_token_logprobs_workspace_size(int64_t N, int64_t V, int64_t top, int dtype) {
   if (N <= 0 || V <= 0 || top < 0) return 0;
-  const LpPlan pl = lp_plan(N, V);
+  const LpPlan pl = lp_plan(N, V, dtype);
   return pl.chunks > 1 ? (size_t)N * pl.chunks * (2 + (size_t)top) * sizeof(u64) : 0;
 }
 
@@ -476,7 +489,7 @@ extern "C" int tpp_token_logprobs(const void *logits, int64_t row_stride, const 
   LpArgs a = {};
   a.x = logits, a.tok = tokens, a.lp = logprobs, a.ent = entropy, a.top_lp = top_logprobs, a.top_id = top_tokens;
   a.x_s = row_stride, a.V = V, a.top = (int)top;
-  const LpPlan pl = lp_plan(N, V);
+  const LpPlan pl = lp_plan(N, V, dtype);
   if (pl.chunks > 1) {
     if (!workspace || !aligned16(workspace) || ws_bytes < tpp_token_logprobs_workspace_size(N, V, top, dtype))
       return set_error(TPP_E_WORKSPACE, "%s: workspace missing, unaligned or too small", name);
