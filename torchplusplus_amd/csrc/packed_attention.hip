@@ -9,8 +9,8 @@
 // attention_prefill.hpp with each query tile's sequence in place of the batch index. Grids are
 // sized by what is known on the host, the number of tokens and of sequences: N tokens in B
 // sequences have at most N / tile + B query tiles.
-//  * short or few sequences: packed_wave_kernel, tiles of 32 queries of one head, each wave on
-//    its own. A block finds its sequence by a scan of the lengths, so it is one launch.
+//  * short or few sequences: packed_wave_kernel, tiles of 32 queries of one head (of a few
+//    queries behind cached keys: of as many heads as fill the tile), each wave on its own. A block finds its sequence by a scan of the lengths, so it is one launch.
 //  * else attn_prefill_kernel, 128 queries of two heads (or 64 of four, 256 of one) a tile: a
 //    block each, or, where they are many, one block a CU that loops over its share of them.
 //    That static dealing wants the tiles from the heaviest to the lightest: packed_plan_kernel
@@ -107,7 +107,7 @@ __device__ __forceinline__ PackedRow packed_row_self(const PackedArgs &p, int t,
 // does not see, other sequences' among them, are masked.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int SH, bool SELF>
-__global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int nh) {
+__global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int nh, int lg) {
   constexpr bool SPLIT = SH > 1;
   typedef typename VecT<T>::v8 V8;
   typedef typename VecT<T>::v4 V4;
@@ -124,7 +124,8 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, ql = lane & 31;
   const int e = blockIdx.x / nh, hb = blockIdx.x - e * nh;
-  const int hq = SPLIT ? hb : hb * 4 + w;
+  // rows: 32 >> lg queries of 1 << lg heads that share their keys, a query's heads side by side
+  const int hq = (SPLIT ? hb : hb * 4 + w) << lg, heads = (1 << lg) - 1;
   if (hq >= p.Hq) return;
   const int hk = hq / (p.Hq / p.Hkv);
   const char *kp = (const char *)((const T *)p.k + (int64_t)hk * p.k_sh);
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
   auto issue_v = [&](int kb) { issue(vp, p.v_ss, kb, ring + TU * 16, [](int r) { return vswz<D>(r); }); };
   V8 qf[KS];
   auto ask_q = [&](int qrow) {
-    const T *qp = (const T *)p.q + (int64_t)qrow * p.q_ss + (int64_t)hq * p.q_sh;
+    const T *qp = (const T *)p.q + (int64_t)qrow * p.q_ss + (int64_t)(hq + (ql & heads)) * p.q_sh;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const V8 *>(qp + ks * 16 + h * 8);
   };
@@ -183,9 +184,10 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
     row = packed_row_self(p, e, lo, __float_as_int(begin), __float_as_int(end));
   } else {
     PackedSeq seq = {0, 0, 0, 0};
-    const int qt = packed_tile(p, e, 32, seq);
+    const int qt = packed_tile(p, e, 32 >> lg, seq);
     if (qt < 0) return; // (every wave)
-    row = {seq, min(qt * 32 + ql, seq.Sq - 1), qt * 32 + ql < seq.Sq};
+    const int i = (qt * 32 + ql) >> lg;
+    row = {seq, min(i, seq.Sq - 1), i < seq.Sq};
     ask_q(row.seq.q0 + row.i);
   }
   const int qrow = row.seq.q0 + row.i;
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
       if (n % waves != w0) continue;
       const int l = __builtin_ctz(bad);
       packed_row_again<T, D>(p, __builtin_amdgcn_readlane(qrow, l), __builtin_amdgcn_readlane(klo, l),
-                             __builtin_amdgcn_readlane(khi, l), hq, hk);
+                             __builtin_amdgcn_readlane(khi, l), hq + (l & heads), hk);
     }
   };
   if constexpr (!SPLIT) {
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
       const int n = r * ORPI + lane / CPR, c = lane % CPR;
       const V8 x = *reinterpret_cast<const V8 *>(ring + n * RBY + ((c ^ (n % CPR)) * 16));
       const int at = __shfl(qrow, n, kWave);
-      if (reals >> n & 1) *reinterpret_cast<V8 *>(op + (int64_t)at * p.o_ss + c * 8) = x;
+      if (reals >> n & 1) *reinterpret_cast<V8 *>(op + (int64_t)at * p.o_ss + (int64_t)(n & heads) * p.o_sh + c * 8) = x;
     }
     unsigned long long bad = __ballot(z != z && l == l && sees);
     if (bad) {
@@ -415,7 +417,7 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
 #pragma unroll
       for (int i = 0; i < 8; ++i) z = fmaf(v[i], 0.f, z), v[i] = sees ? v[i] * inv : 0.f;
       if (z != z && ls == ls && sees) atomicOr(&s_bad, 1u << n);
-      store8((T *)p.o + (int64_t)at * p.o_ss + (int64_t)hq * p.o_sh + c * 8, v);
+      store8((T *)p.o + (int64_t)at * p.o_ss + (int64_t)(hq + (n & heads)) * p.o_sh + c * 8, v);
     }
     __syncthreads(); // every row above is written, and what is odd known
     if (s_bad) again(s_bad, w, NW);
@@ -467,10 +469,11 @@ __global__ __launch_bounds__(1024) void packed_plan_kernel(PackedArgs p, int QL,
 }
 
 // How a call is cut: the kernel (share: packed_wave_kernel's waves a row, 0: attn_prefill_kernel),
-// query heads and queries of a tile, the most tiles there can be.
+// query heads (packed_wave_kernel: their logarithm too) and queries of a tile, the most tiles
+// there can be.
 struct PackedPlan {
   bool tiles;
-  int share, hpb, QL;
+  int share, lg, hpb, QL;
   int64_t most;
   bool plan;
 };
@@ -497,7 +500,12 @@ static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int
   double longest = lk, mean = right >= 0 && lq <= lk ? lk - lq / 2 : lk;
   if (left >= 0 && right >= 0 && left + right + 33.0 < longest) longest = left + right + 33.0;
   if (mean > longest) mean = longest;
-  const double items = (double)most(32) * Hq, work = items * (mean / kt + 0.5), chain = longest / kt + 1;
+  // few queries a sequence: the heads of a group fill the tile, which reads their keys once (17
+  // sequences of one query behind 2410 keys, 16 / 2 heads, 61 -> 23 us; 11 of 4 behind 3865, 32 / 4
+  // heads of 64, 57 -> 22; 32 of 16 behind 2000, 16 / 8 heads, 80 -> 50)
+  int lg = 0;
+  while (!self && lg < 5 && (Hq / Hkv) % (2 << lg) == 0 && lq * (2 << lg) <= 32) ++lg;
+  const double items = (double)most(32 >> lg) * (Hq >> lg), work = items * (mean / kt + 0.5), chain = longest / kt + 1;
   auto larger = [](double a, double b) { return a > b ? a : b; };
   const double alone = 2.5 + 4.5 * larger(1, items / (8 * cus)) + larger(0.8 * chain, 1.1e-3 * work);
   double best = alone;
@@ -509,8 +517,8 @@ static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int
   const double each = D == 128 ? 2.0 : 1.2, last = D == 128 ? 1.6 : 1.2;
   const double whole = 7 + larger((double)most(QL) * (Hq / hpb) / cus * (4.5 + each * (mean / 64 + 1)), 4.5 + last * (longest / 64 + 1));
   // (a grid has fewer than 2^32 threads)
-  if (whole < best || most(32) * (pl.share == 1 ? (Hq + 3) / 4 : Hq) > 0xffffff) pl.share = 0;
-  pl.hpb = pl.share ? 1 : hpb, pl.QL = pl.share ? 32 : QL;
+  if (whole < best || most(32 >> lg) * (pl.share == 1 ? ((Hq >> lg) + 3) / 4 : Hq >> lg) > 0xffffff) pl.share = 0;
+  pl.lg = lg, pl.hpb = pl.share ? 1 << lg : hpb, pl.QL = pl.share ? 32 >> lg : QL;
   pl.most = most(pl.QL);
   // up to two tiles a CU a block each, from the last to the first, and no list of them (its
   // launch: six turns behind 2500 tokens 46.9 -> 43.0 us; four prompts of 2000, 2.06 tiles a
@@ -574,7 +582,7 @@ extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void
       return check_launch(name);
     });
   // packed_wave_kernel without shared keys: blocks of four heads
-  const int nh = pl.share == 1 ? (int)(Hq + 3) / 4 : (int)Hq / pl.hpb;
+  const int nh = pl.share == 1 ? ((int)Hq / pl.hpb + 3) / 4 : (int)Hq / pl.hpb;
   const int64_t items = pl.most * nh;
   if (pl.plan) {
     if (!workspace || !aligned16(workspace) ||
@@ -587,10 +595,10 @@ extern "C" int tpp_attn_packed(const void *q, const void *k, const void *v, void
     auto go = [&](auto dd) {
       constexpr int DD = decltype(dd)::value;
       const dim3 grid((unsigned)items);
-      if (pl.share == 1 && !cu_k) packed_wave_kernel<T, DD, 1, true><<<grid, dim3(256), 0, st>>>(a, nh);
-      else if (pl.share == 1) packed_wave_kernel<T, DD, 1, false><<<grid, dim3(256), 0, st>>>(a, nh);
-      else if (pl.share && !cu_k) packed_wave_kernel<T, DD, 4, true><<<grid, dim3(256), 0, st>>>(a, nh);
-      else if (pl.share) packed_wave_kernel<T, DD, 4, false><<<grid, dim3(256), 0, st>>>(a, nh);
+      if (pl.share == 1 && !cu_k) packed_wave_kernel<T, DD, 1, true><<<grid, dim3(256), 0, st>>>(a, nh, pl.lg);
+      else if (pl.share == 1) packed_wave_kernel<T, DD, 1, false><<<grid, dim3(256), 0, st>>>(a, nh, pl.lg);
+      else if (pl.share && !cu_k) packed_wave_kernel<T, DD, 4, true><<<grid, dim3(256), 0, st>>>(a, nh, pl.lg);
+      else if (pl.share) packed_wave_kernel<T, DD, 4, false><<<grid, dim3(256), 0, st>>>(a, nh, pl.lg);
       else {
         const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
         attn_prefill_kernel<T, DD, kPrefillQG, kPrefillWaves>
