@@ -10,7 +10,8 @@
 // sized by what is known on the host, the number of tokens and of sequences: N tokens in B
 // sequences have at most N / tile + B query tiles.
 //  * short or few sequences: packed_wave_kernel, tiles of 32 queries of one head (of a few
-//    queries behind cached keys: of as many heads as fill the tile), each wave on its own. A block finds its sequence by a scan of the lengths, so it is one launch.
+//    queries behind cached keys: of as many heads as fill the tile), each wave on its own. A
+//    block finds its sequence by a scan of the lengths, so it is one launch.
 //  * else attn_prefill_kernel, 128 queries of two heads (or 64 of four, 256 of one) a tile: a
 //    block each, or, where they are many, one block a CU that loops over its share of them.
 //    That static dealing wants the tiles from the heaviest to the lightest: packed_plan_kernel

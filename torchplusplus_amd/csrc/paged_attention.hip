@@ -53,7 +53,7 @@ template <typename T> __global__ __launch_bounds__(64) void paged_generic_kernel
 // K with it, where its value is carried around the loop).
 //
 // HBM bounds it where the cache is long: 32 sequences of 100 to 4096 positions, 146 MB, 30.0 us
-// (4.9 TB/s), two of 60000 to 100000, 328 MB, 66 us (5.0); one of 700, 2.9 MB, is its launch and
+// (4.9 TB/s), two of 60000 to 100000, 328 MB, 57 us (5.8); one of 700, 2.9 MB, is its launch and
 // trips to memory, 6.9 us.
 // ---------------------------------------------------------------------------
 constexpr int kPagedDealt = 512; // sequences whose lengths a block looks at
@@ -379,15 +379,21 @@ static PagedPlan paged_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
   // (with four blocks for each that can be resident the card deals them well itself)
   if (B > kPagedDealt || B * Hkv * pl.qtiles >= 8 * cus || Lmax <= stride) return pl;
-  // Two blocks a CU, as many as are resident at once (tree_plan); two a sequence, where those
-  // are more, for the long ones to be split.
-  int64_t t = 2 * (int64_t)cus / (Hkv * pl.qtiles);
+  // A block for three quarters of the CUs: four waves' tiles in flight are what a CU reads at
+  // its best, a second block only has it read for two (bf16, us at 3/4, 1, 1.5 and 2 a CU: 100000
+  // and 60000 keys, 32 / 4 heads, 57, 60, 72, 65; one of 60000, 16 / 8, 41, 42, 46, 44; eight of
+  // 8000, 32 / 8, 44, 45, 51, 46; three of 300 to 9000, 16 / 8, 15.5, 16.1, 17.9, 17.4). Two a
+  // sequence, where those are more, for the long ones to be split.
+  int64_t t = 3 * (int64_t)cus / 4 / (Hkv * pl.qtiles);
+  if (t < 1) t = 1;
   if (t < 2 * B) t = 2 * B;
   const int64_t most = B * ((Lmax + stride - 1) / stride);
   if (t > most) t = most;
   pl.target = (int)t;
-  // A block that merges reads rows * splits sums of 4 (D + 2) bytes, ~50 a ns.
-  pl.most = pl.nc == 1 ? (int)(1024 / G) : 1024;
+  // A block that merges reads rows * splits sums of 4 (D + 2) bytes (one of 15741 keys, 32 / 4
+  // heads: 16 with 32 splits, 17 with 48, 19 with 96, 30 with 123; of 40000, 8 / 1: 22 with 32, 20
+  // with 48, 24 with 128).
+  pl.most = pl.nc == 1 ? (int)(384 / G) : 1024;
   pl.slots = (int)(t + B); // (at most t runs of equal length, and a last one each)
   return pl;
 }
