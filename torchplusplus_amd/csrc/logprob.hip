@@ -23,16 +23,19 @@
 // largest logit from below, so only threads whose maximum reaches it have any of them. Those
 // threads' elements that reach the bound go to a list in LDS and are ranked by counting.
 // Every wave finds the bound by itself, bit by bit from ballots; the upper 16 bits of the
-// value do, and all bits of (value, place) where many elements are equal. Up to kLpHeld
-// iterations a thread's elements are loaded at once and stay in registers, and the runs of
-// eight that reach the bound go to LDS; longer ones are read again from the caches.
+// value do. Where more elements reach it than there is room for (many equal ones, or the
+// largest in fewer groups than `top`), the bound is the `top`-th largest maximum of all threads
+// to the last bit of (value, place): no two are equal, so `top` threads reach it and no more.
+// Up to kLpHeld iterations a thread's elements are loaded at once and stay in registers, and
+// the runs of eight that reach the bound go to LDS, kLpHeld of each such thread at most; longer
+// ones are read again from the caches.
 #include "tpp_common.hpp"
 
 namespace tpp {
 
 constexpr int kLpThreads = 256, kLpRun = 8, kLpStep = kLpThreads * kLpRun; // elements an iteration
 constexpr int kLpMaxTop = 32, kLpRoom = 1024;
-constexpr int kLpHeld = 8, kLpRuns = kLpMaxTop * kLpHeld;
+constexpr int kLpHeld = 8, kLpRuns = kLpMaxTop * kLpHeld; // (runs of kLpMaxTop threads)
 
 typedef unsigned long long u64;
 
@@ -150,9 +153,18 @@ __device__ __forceinline__ void lp_select(LpShared &s, int top, BEGIN begin, SCA
   };
   list();
   int found = s.n[1];
-  if (found > kLpRoom || s.n[0] > kLpRuns) { // many equal ones: the bound to the last bit, `top` threads at most
-    for (int bit = 47; bit >= 0; --bit)
-      if (__popcll(__ballot(g >= (bound | 1ull << bit))) >= top) bound |= 1ull << bit;
+  if (found > kLpRoom || s.n[0] > kLpRuns) { // the top-th largest of the threads
+    u64 each[kLpThreads / kWave];
+#pragma unroll
+    for (int i = 0; i < kLpThreads / kWave; ++i) each[i] = s.max[i * kWave + lane];
+    bound = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const u64 higher = bound | 1ull << bit;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kLpThreads / kWave; ++i) n += __popcll(__ballot(each[i] >= higher));
+      if (n >= top) bound = higher;
+    }
     __syncthreads();
     if (tid < 2) s.n[tid] = 0;
     __syncthreads();
