@@ -130,7 +130,7 @@ class LLMInference(nn.Module, ABC):
             raise ValueError(f"input_ids must be [B, S] with at least two tokens, got {tuple(input_ids.shape)}")
         logits = self.forward_impl(input_ids)
         # (every row of the logits, the last with padding: slicing them would copy them)
-        tokens = torch.cat([input_ids[:, 1:], torch.full_like(input_ids[:, :1], -1)], 1)
+        tokens = torch.cat([input_ids[:, 1:], torch.full_like(input_ids[:, :1], -1)], 1).long()
         scores = token_logprobs(logits, tokens, top_k)
         self.check_device_errors()
         return TokenLogprobs(*(None if x is None else x[:, :-1] for x in scores))
