@@ -149,6 +149,8 @@ class PagedKVCache:
         """The slot of position positions[b] of every sequence of a table: int64 [B],
         -1 where the sequence has no page for it. On the device alone (for a decode
         step, captured or not)."""
+        if positions.shape != block_tables.shape[:1]:
+            raise ValueError(f"a table of {block_tables.shape[0]} sequences needs one position each, got {tuple(positions.shape)}")
         if block_tables.shape[1] == 0:  # (nothing to gather from)
             return torch.full_like(positions, -1, dtype=torch.int64)
         p = positions.long()
