@@ -37,7 +37,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     NaN. Rows of no sequence (behind the last one, in a padded batch) stay as they
     were in a given `out`, and are 0 in a new one. softmax_scale is above 0, by
     default 1/sqrt(D). head_dim 64 and 128 with 16-byte rows run on the matrix
-    cores, others up to 256 on a slow kernel. Returns o [Nq, Hq, D]."""
+    cores, with weights rounded to the type of v (fp16: those below 2^-32 of the
+    row's largest may count as 0); others up to 256 on a slow kernel, a wave a row.
+    Returns o [Nq, Hq, D]."""
     left, right = window_size
     return _C.packed_attention(q, k, v, cu_seqlens, cu_seqlens_k, _scale(softmax_scale), bool(causal), int(left),
                                int(right), out)

@@ -299,7 +299,11 @@ __global__ __launch_bounds__(256, 2) void packed_wave_kernel(PackedArgs p, int n
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[tt][i] *= alpha;
     }
-    V8 pb[2 * NB]; // the one rounding of the weights, to the type of V (l has them unrounded)
+    // The one rounding of the weights, to the type of V, as attn_prefill_kernel's (l has them
+    // unrounded): what a second product with the rest of them would keep is half the matrix work
+    // again. Off the 64-bit form by 0.0019-0.0023 (bf16) and 0.00022-0.00027 (fp16) relative,
+    // outputs rounded alone by 0.0016-0.0017 and 0.00019-0.00021.
+    V8 pb[2 * NB];
 #pragma unroll
     for (int c = 0; c < 2 * NB; ++c)
 #pragma unroll
@@ -489,6 +493,11 @@ struct PackedPlan {
 // Measured, e.g.: one sequence of 230 6.8 (17.8 on the other kernel), of 1000 17 (38), 64 of 3 to
 // 200 12 (32; fp16, 16 / 16 heads of 64), 16 of 200 17 (21); and back, 16 of 1000 139 (107), eight
 // of 501 to 4001 278 (188: 770 TFLOP/s, 5 us of it the plan's launch).
+// What the mean does not show: long and short sequences in one batch take the kernel that suits
+// their mean (eight of 2000 171 us, with 200 of 8, 7 on their own, 233), and one part of a prompt
+// of 512 behind 4000 keys beside 31 single tokens there, 59 and 44 on their own, 230: the tokens'
+// heads do not share tiles. Keys are not split over blocks: 33 behind 8000 keys 53-60 us, 32
+// behind 30000 209, 6.5 and 24 at the copy's rate.
 static PackedPlan packed_plan(int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D, int left, int right,
                               bool self) {
   PackedPlan pl = {};

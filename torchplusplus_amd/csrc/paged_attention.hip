@@ -377,7 +377,10 @@ static PagedPlan paged_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
   pl.qtiles = (int)((G + 16 * pl.nc - 1) / (16 * pl.nc));
   pl.slots = (int)B;
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  // (with four blocks for each that can be resident the card deals them well itself)
+  // With four blocks for each that can be resident the card deals sequences of like lengths well
+  // itself (300 of 500 keys, 16 / 8 heads: 95 us, 120 at the copy's rate). A long one among so
+  // many is one block a KV head, and the call waits for it: of 60000 beside 254 of 500, dealt,
+  // 140 us (150), beside 299, undealt, 608 (168).
   if (B > kPagedDealt || B * Hkv * pl.qtiles >= 8 * cus || Lmax <= stride) return pl;
   // A block for three quarters of the CUs: four waves' tiles in flight are what a CU reads at
   // its best, a second block only has it read for two (bf16, us at 3/4, 1, 1.5 and 2 a CU: 100000
